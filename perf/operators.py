@@ -224,30 +224,37 @@ def _framework():
     return _modules[0]
 
 
+def _handle(s):
+    """The cache's handle, which a program has from its cache and keeps: made once a state."""
+    if "handle" not in s:
+        cache, _ = _framework()
+        kind = cache.E4M3Storage if s["k"].dim() == 5 else cache.E4M3KVView
+        s["handle"] = kind(s["k"], s["v"], s["scales"], s["block_table"], window=s["case"].get("window") or None, weights=s["weights"],
+                           dropped=s.get("dropped"))
+    return s["handle"]
+
+
 def run(s):
     c = s["case"]
     if c["op"] == "store":
         if own:
-            cache, ops = _framework()
-            kv = cache.E4M3KVView(s["k"], s["v"], s["scales"], s["block_table"], weights=s["weights"])
-            ops.kv_store_e4m3(s["qkv"], s["cos_sin"], c["heads"], c["kv_heads"], kv, s["cu_seqlens"], s["slots"], s["start_pos"], s["max_q_len"], s["q"],
-                              pairing=c["pairing"], rotary_dim=c["rot"])
+            _, ops = _framework()
+            ops.kv_store_e4m3(s["qkv"], s["cos_sin"], c["heads"], c["kv_heads"], _handle(s), s["cu_seqlens"], s["slots"], s["start_pos"],
+                              s["max_q_len"], s["q"], pairing=c["pairing"], rotary_dim=c["rot"])
         else:
             _plain_store(s, c)
         return {"q": s["q"], "k": s["k"], "v": s["v"], "scales": s["scales"], "weights": s["weights"]}
     if c["op"] == "attend":
         if own:
-            cache, ops = _framework()
-            kv = cache.E4M3KVView(s["k"], s["v"], s["scales"], s["block_table"], window=c["window"] or None, weights=s["weights"])
-            ops.attention_e4m3(s["q"], s["out"], kv, s["cu_seqlens"], s["slots"], s["start_pos"], s["max_q_len"], c["heads"], s["scale"],
+            _, ops = _framework()
+            ops.attention_e4m3(s["q"], s["out"], _handle(s), s["cu_seqlens"], s["slots"], s["start_pos"], s["max_q_len"], c["heads"], s["scale"],
                                max_kv_len=s["max_kv_len"], total_kv_len=s["total_kv_len"])
         else:
             _plain_attend(s, c)
         return {"out": s["out"], "weights": s["weights"]}
     if own:
-        cache, ops = _framework()
-        store = cache.E4M3Storage(s["k"], s["v"], s["scales"], s["block_table"], weights=s["weights"], dropped=s["dropped"])
-        ops.kv_evict_e4m3(store, s["slots"], s["lengths"], s["max_length"], c["budget"], c["recent"], kept=s["kept"])
+        _, ops = _framework()
+        ops.kv_evict_e4m3(_handle(s), s["slots"], s["lengths"], s["max_length"], c["budget"], c["recent"], kept=s["kept"])
     else:
         _plain_evict(s, c)
     return {"k": s["k"], "v": s["v"], "scales": s["scales"], "weights": s["weights"], "dropped": s["dropped"], "kept": s["kept"]}
