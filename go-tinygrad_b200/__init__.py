@@ -6,6 +6,7 @@ The package directory carries a hyphen; import it as ``go_tinygrad_b200`` (the
 module of that name beside it loads this package).
 """
 from . import config, weights, cache, parts, models  # noqa: F401  (models registers architectures)
+from .cache import KeepRule
 from .config import ConfigError, LlamaConfig, read_model_config, registered_architectures
 from .engine import Model, StepEntry, StepError, step
 from .engine.generate import GenerationResult, generate
@@ -14,4 +15,4 @@ from .weights import WeightError, write_random_model
 
 __all__ = ["ConfigError", "LlamaConfig", "read_model_config", "registered_architectures", "Model",
            "StepEntry", "StepError", "step", "WeightError", "write_random_model", "GenerationResult",
-           "generate", "Sampler"]
+           "generate", "Sampler", "KeepRule"]

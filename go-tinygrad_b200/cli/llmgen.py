@@ -7,12 +7,15 @@ random weights.
 
     llmgen -model DIR [-prompt TEXT | -ids 1,2,3 [-ids ...] | -ids-file F] [-tokens N]
            [-temp T] [-seed S] [-stop 2,7] [-dtype bfloat16|float32] [-random-weights]
-           [-max-len N] [-slots N]
+           [-max-len N] [-slots N] [-kv-format e4m3 [-keep N [-keep-recent M]]]
 
 ``-slots`` is how many sequences run together (the cache's slots; more prompts
 than that run batch after batch) and ``-max-len`` the longest sequence, prompt
 and new tokens together, a slot holds: the cache is sized for ``slots`` sequences
 of ``max-len`` tokens, and a sequence that reaches it ends there.
+``-kv-format e4m3`` holds the cache's keys and values in 8 bits; ``-keep N`` beside it
+cuts a sequence that holds 64 rows more than N back to N: its ``-keep-recent`` newest
+(default: a quarter of N) and of the others those that gathered most attention weight.
 
 This library runs on the GPU only: ``-gpu`` is accepted and changes nothing,
 ``-gpu-layers`` must be 0 (all layers).  The reference's ``-turbo-quant``,
@@ -56,6 +59,10 @@ def parser() -> argparse.ArgumentParser:
                     help="sequences that run together: the cache's slots")
     ap.add_argument("-max-len", "--max-len", type=int, default=0,
                     help="longest sequence (prompt + new tokens) a slot holds; 0: what the prompts need")
+    ap.add_argument("-kv-format", "--kv-format", default=None, choices=["e4m3"],
+                    help="hold the cache's keys and values in 8 bits")
+    ap.add_argument("-keep", "--keep", type=int, default=0, help="rows a sequence keeps in the cache; 0: all")
+    ap.add_argument("-keep-recent", "--keep-recent", type=int, default=None, help="newest rows among them (default: a quarter)")
     for flag in ("turbo-quant", "speculative", "eager-load"):
         ap.add_argument(f"-{flag}", f"--{flag}", action="store_true", help=argparse.SUPPRESS)
     return ap
@@ -76,12 +83,19 @@ def main(argv: Optional[List[str]] = None) -> int:
     if args.slots <= 0 or args.max_len < 0:
         print("-slots must be positive and -max-len non-negative", file=sys.stderr)
         return 1
+    if args.keep and not args.kv_format:
+        print("-keep needs -kv-format e4m3", file=sys.stderr)
+        return 1
+    if args.keep < 0 or (args.keep_recent is not None and not 0 <= args.keep_recent <= args.keep):
+        print("-keep must be non-negative and -keep-recent between 0 and it", file=sys.stderr)
+        return 1
     if args.gpu_layers != 0:
         print("-gpu-layers: all layers run on the GPU; only 0 is supported", file=sys.stderr)
         return 1
 
     import torch
     from .. import Model, write_random_model
+    from ..cache import KeepRule
     from ..config import ConfigError, read_config_json
     from ..engine.generate import generate
     from ..weights import WeightError
@@ -131,12 +145,17 @@ def main(argv: Optional[List[str]] = None) -> int:
     start = time.time()
     try:
         cache = None
+        keep = None
+        if args.keep:
+            keep = KeepRule(args.keep, args.keep // 4 if args.keep_recent is None else args.keep_recent)
         if args.max_len:
             slots = min(args.slots, len(prompts))
-            cache = model.new_cache(max_tokens=slots * ((args.max_len + 63) // 64 * 64), max_slots=slots)
+            cache = model.new_cache(max_tokens=slots * ((args.max_len + 63) // 64 * 64), max_slots=slots,
+                                    kv_format=args.kv_format, keep=keep)
         results = generate(model, prompts, args.tokens, temperature=args.temp, seed=args.seed,
                            stop=args.stop, max_batch=args.slots, cache=cache,
-                           max_sequence=args.max_len or None)
+                           max_sequence=args.max_len or None, **({} if cache is not None else
+                                                                 {"kv_format": args.kv_format, "keep": keep}))
     except ValueError as e:
         print(f"generate: {e}", file=sys.stderr)
         return 1

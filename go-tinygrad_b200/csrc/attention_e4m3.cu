@@ -1,0 +1,218 @@
+// Attention over the 8-bit key/value cache (layout and codes: e4m3.cuh).
+//
+// o = sum_j p_j v_j with p = softmax_j(scale q . k_j) over the rows j of the sequence up to the query's own (within a window,
+// where there is one).  Where the cache gathers weights, row j's weight grows by the sum of p_j over the step's queries and
+// the query heads of its key/value head.
+//
+//   attention_rows:   any head size and type, one block per (token, query head); scores, softmax and sums in float.
+//   row_weights:      the weights, once every row's maximum and sum are known: a block per (cache page, head, sequence).
+#include "e4m3.cuh"
+
+namespace {
+
+// ============================================================== any head size, float or bfloat16
+constexpr int kRowThreads = 128;
+constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kMaxChannels = 256;
+
+// 32 rows at a time a warp: a lane scores one row and then adds up the channels lane, lane + 32, ... of all 32.
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads)
+attention_rows_kernel(const T* __restrict__ q, int ldq, T* __restrict__ out, int ldo, const E4M3Pages kv, const int* __restrict__ cu_seqlens,
+                      const int* __restrict__ slots, const int* __restrict__ start_pos, int B, int n_heads, float scale, int window,
+                      float2* __restrict__ stats) {
+    chain_release();
+    chain_wait();
+    __shared__ float qs[kMaxChannels];
+    __shared__ float ps[kRowWarps][32];
+    __shared__ float wm[kRowWarps], wl[kRowWarps];
+    __shared__ float wo[kRowWarps][kMaxChannels];
+    const int token = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (token < cu_seqlens[0] || token >= cu_seqlens[B]) return;
+    int b = 0;
+    for (int lo = 0, hi = B; lo < hi;) {                                        // the last sequence that begins at or before the token
+        const int mid = (lo + hi) >> 1;
+        if (cu_seqlens[mid] <= token) { b = mid; lo = mid + 1; } else hi = mid;
+    }
+    const int slot = slots[b], hd = kv.hd, h = head / (n_heads / kv.n_kv);
+    const int* table = kv.block_table + (size_t)slot * kv.table_stride;
+    const int row = start_pos[b] - (kv.dropped ? kv.dropped[slot] : 0) + token - cu_seqlens[b];
+    const int first = window > 0 ? max(0, row - window + 1) : 0;
+    for (int d = tid; d < hd; d += kRowThreads) qs[d] = to_f32(q[(size_t)token * ldq + head * hd + d]) * scale;
+    __syncthreads();
+    float m = -INFINITY, l = 0.f;
+    float o[kMaxChannels / 32];
+#pragma unroll
+    for (int i = 0; i < kMaxChannels / 32; ++i) o[i] = 0.f;
+    for (int c = first / 32 + warp; c * 32 <= row; c += kRowWarps) {
+        const size_t page = table[c / (kPageTokens / 32)];
+        const int t0 = c % (kPageTokens / 32) * 32, t = t0 + lane, j = c * 32 + lane;
+        const float k_scale = kv.scales[page * kv.scale_stride + h], v_scale = kv.scales[page * kv.scale_stride + kv.n_kv + h];
+        const uint8_t* kr = kv.k + page * kv.k_stride + ((size_t)h * kPageTokens + t) * hd;
+        const bool seen = j >= first && j <= row;
+        float s = 0.f;
+        if (seen) {
+            if (hd % 16 == 0) {
+                for (int d = 0; d < hd; d += 16) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(kr + d);
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t pair = e4m3_pair_f16(w[e >> 1] >> (16 * (e & 1)));
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+                        s = fmaf(qs[d + 2 * e], f.x, s);
+                        s = fmaf(qs[d + 2 * e + 1], f.y, s);
+                    }
+                }
+            } else {
+                for (int d = 0; d < hd; ++d) s = fmaf(qs[d], e4m3_value(kr[d]), s);
+            }
+        }
+        s = seen ? s * k_scale : -INFINITY;
+        const float m_new = fmaxf(m, warp_max(s));
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float p = seen ? expf(s - m_use) : 0.f, corr = expf(m - m_use);
+        m = m_new;
+        l = l * corr + p;
+        __syncwarp();
+        ps[warp][lane] = p * v_scale;
+        __syncwarp();
+        // rows that no query of this token sees may hold anything (a row nobody has written yet: the NaN code)
+        const int from = max(first - c * 32, 0), to = min(row - c * 32, 31);
+        const uint8_t* vr = kv.v + page * kv.v_stride + (size_t)h * hd * kPageTokens + t0;
+#pragma unroll
+        for (int i = 0; i < kMaxChannels / 32; ++i) {
+            const int d = lane + 32 * i;
+            if (d >= hd) break;
+            const uint4 u[2] = {*reinterpret_cast<const uint4*>(vr + d * kPageTokens), *reinterpret_cast<const uint4*>(vr + d * kPageTokens + 16)};
+            const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
+            float acc = o[i] * corr;
+            if (from == 0 && to == 31) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const uint32_t pair = e4m3_pair_f16(w[e >> 1] >> (16 * (e & 1)));
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+                    acc = fmaf(ps[warp][2 * e], f.x, acc);
+                    acc = fmaf(ps[warp][2 * e + 1], f.y, acc);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (e >= from && e <= to) acc = fmaf(ps[warp][e], e4m3_value((uint8_t)(w[e >> 2] >> (8 * (e & 3)))), acc);
+            }
+            o[i] = acc;
+        }
+    }
+    l = warp_sum(l);
+    if (lane == 0) { wm[warp] = m; wl[warp] = l; }
+#pragma unroll
+    for (int i = 0; i < kMaxChannels / 32; ++i)
+        if (lane + 32 * i < hd) wo[warp][lane + 32 * i] = o[i];
+    __syncthreads();
+    float M = wm[0];
+    for (int w = 1; w < kRowWarps; ++w) M = fmaxf(M, wm[w]);
+    const float M_use = M == -INFINITY ? 0.f : M;
+    float f[kRowWarps], L = 0.f;
+    for (int w = 0; w < kRowWarps; ++w) { f[w] = expf(wm[w] - M_use); L += f[w] * wl[w]; }
+    for (int d = tid; d < hd; d += kRowThreads) {
+        float acc = 0.f;
+        for (int w = 0; w < kRowWarps; ++w) acc += f[w] * wo[w][d];
+        out[(size_t)token * ldo + head * hd + d] = from_f32<T>(acc / L);
+    }
+    if (stats && tid == 0) stats[(size_t)token * n_heads + head] = make_float2(M, L);
+}
+
+// A block per (page of the sequence, key/value head, sequence): 64 rows by two halves of the (query, head) pairs that may
+// see them; the halves are added in order, so the sum does not depend on what else runs.
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads)
+row_weights_kernel(const T* __restrict__ q, int ldq, const E4M3Pages kv, const int* __restrict__ cu_seqlens, const int* __restrict__ slots,
+                   const int* __restrict__ start_pos, int n_heads, float scale, int window, const float2* __restrict__ stats) {
+    chain_release();
+    chain_wait();
+    constexpr int kAtOnce = 8;
+    extern __shared__ float smem[];
+    const int hd = kv.hd, ld = hd + 1;
+    float* ks = smem;                                                           // [64][hd + 1]
+    float* qs = ks + kPageTokens * ld;                                          // [kAtOnce][hd]
+    __shared__ float2 st[kAtOnce];
+    __shared__ float half_sum[kPageTokens];
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+    const int first = cu_seqlens[b], n_new = cu_seqlens[b + 1] - first, slot = slots[b];
+    if (n_new <= 0) return;
+    const int start = start_pos[b] - (kv.dropped ? kv.dropped[slot] : 0);
+    const int group = n_heads / kv.n_kv, t = tid & 63, part = tid >> 6;
+    for (int block = blockIdx.x; block * kPageTokens < start + n_new; block += gridDim.x) {
+        const size_t page = kv.block_table[(size_t)slot * kv.table_stride + block];
+        const uint8_t* kr = kv.k + page * kv.k_stride + (size_t)h * kPageTokens * hd;
+        __syncthreads();
+        for (int i = tid; i < kPageTokens * hd; i += kRowThreads) ks[i / hd * ld + i % hd] = e4m3_value(kr[i]);
+        const float k_scale = kv.scales[page * kv.scale_stride + h];
+        const int row = block * kPageTokens + t;
+        const int from = max(0, block * kPageTokens - start);                   // queries before that one see none of these rows
+        const int pairs = (n_new - from) * group;
+        float sum = 0.f;
+        for (int p0 = 0; p0 < pairs; p0 += kAtOnce) {
+            __syncthreads();
+            const int here = min(kAtOnce, pairs - p0);
+            for (int i = tid; i < here * hd; i += kRowThreads) {
+                const int pair = p0 + i / hd;
+                qs[i] = to_f32(q[(size_t)(first + from + pair / group) * ldq + (h * group + pair % group) * hd + i % hd]) * scale;
+            }
+            if (tid < here) st[tid] = stats[(size_t)(first + from + (p0 + tid) / group) * n_heads + h * group + (p0 + tid) % group];
+            __syncthreads();
+            for (int i = part; i < here; i += 2) {
+                const int at = start + from + (p0 + i) / group;
+                if (row > at || (window > 0 && row <= at - window)) continue;
+                float s = 0.f;
+                for (int d = 0; d < hd; ++d) s = fmaf(qs[i * hd + d], ks[t * ld + d], s);
+                sum += expf(s * k_scale - st[i].x) / st[i].y;
+            }
+        }
+        if (part) half_sum[t] = sum;
+        __syncthreads();
+        if (!part && row < start + n_new) {
+            float* w = kv.weights + page * kv.weight_stride + h * kPageTokens + t;
+            *w += sum + half_sum[t];
+        }
+    }
+}
+
+template <typename T>
+int launch_rows(const void* q, int ldq, void* out, int ldo, const E4M3Pages& kv, const int* cu_seqlens, const int* slots, const int* start_pos,
+                int B, int max_q_len, int max_kv_len, int N, int n_heads, float scale, int window, float* scratch, cudaStream_t stream) {
+    float2* stats = kv.weights ? (float2*)scratch : nullptr;
+    int st = launch_chained(attention_rows_kernel<T>, dim3(N, n_heads), dim3(kRowThreads), 0, stream, (const T*)q, ldq, (T*)out, ldo, kv,
+                            cu_seqlens, slots, start_pos, B, n_heads, scale, window, stats);
+    if (st != 0 || !kv.weights) return st;
+    const size_t smem = ((size_t)kPageTokens * (kv.hd + 1) + 8 * (size_t)kv.hd) * sizeof(float);
+    cudaError_t e = cudaFuncSetAttribute(row_weights_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    return launch_chained(row_weights_kernel<T>, dim3((max_kv_len + kPageTokens - 1) / kPageTokens, kv.n_kv, B), dim3(kRowThreads), smem, stream,
+                          (const T*)q, ldq, kv, cu_seqlens, slots, start_pos, n_heads, scale, window, (const float2*)stats);
+}
+}  // namespace
+
+// Floats of scratch that gtg_attention_e4m3 needs for the same numbers.
+GTG_API long long gtg_attention_e4m3_scratch_floats(int dtype, int B, int N, int max_q_len, int n_heads, int n_kv, int hd, int max_kv_len,
+                                                    long long total_kv_len, int window, int weigh) {
+    (void)dtype; (void)B; (void)max_q_len; (void)n_kv; (void)hd; (void)max_kv_len; (void)total_kv_len; (void)window;
+    return weigh ? 2LL * N * n_heads : 0;
+}
+
+// dtype: of q and out (0 float, 1 bfloat16).  max_kv_len: rows of the longest sequence after this step; total_kv_len: of all
+// (0: not known); they decide how the work is cut and how many blocks look for weights.
+GTG_API int gtg_attention_e4m3(int dtype, const void* q, int ldq, void* out, int ldo, void* k, long long k_stride, void* v, long long v_stride,
+                               float* scales, long long scale_stride, float* weights, long long weight_stride, const int* block_table,
+                               int table_stride, const int* dropped, const int* cu_seqlens, const int* slots, const int* start_pos, int B,
+                               int max_q_len, int max_kv_len, long long total_kv_len, int N, int n_heads, int n_kv, int hd, float scale,
+                               int window, float* scratch, cudaStream_t stream) {
+    if (B <= 0 || N <= 0 || max_q_len <= 0) return 0;
+    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || hd <= 0 || max_kv_len <= 0 || window < 0) return kErrBadArgument;
+    if (hd > kMaxChannels || B > 65535 || n_heads > 65535) return kErrUnsupported;
+    const E4M3Pages kv = {(uint8_t*)k, (uint8_t*)v, k_stride, v_stride, scales, scale_stride, weights, weight_stride, block_table, table_stride,
+                          dropped, n_kv, hd};
+    (void)total_kv_len;
+    if (dtype == 0) return launch_rows<float>(q, ldq, out, ldo, kv, cu_seqlens, slots, start_pos, B, max_q_len, max_kv_len, N, n_heads, scale, window, scratch, stream);
+    return launch_rows<bf16>(q, ldq, out, ldo, kv, cu_seqlens, slots, start_pos, B, max_q_len, max_kv_len, N, n_heads, scale, window, scratch, stream);
+}

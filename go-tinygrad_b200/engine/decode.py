@@ -110,7 +110,7 @@ class DecodeBatch:
         """Run the step for the state now on the device; grows every sequence by one."""
         self.cache.reserve_many([(s, self.cache.length(s) + 1) for s in self.slots])
         self.cache.flush_tables()
-        lengths = [self.cache.length(s) + 1 for s in self.slots]
+        lengths = [self.cache.held(s) + 1 for s in self.slots]
         longest = max(lengths)
         if self.model.op_hook is not None or self.model.rt.check_access:   # a hook listens or checks run: in the open
             self.graph = None
@@ -141,6 +141,7 @@ class DecodeBatch:
         self.model.steps_run += 1
         for s in self.slots:
             self.cache.advance(s, 1)
+        self.cache.evict_due(self.slots)
 
     def _record(self) -> "torch.cuda.CUDAGraph":
         """Capture one step on a side stream.  Done by hand rather than with
@@ -195,6 +196,8 @@ class DecodeBatch:
 
     def reserve_ahead(self, n_steps: int) -> None:
         """Take the pages `n_steps` more steps will need now, so that the steps
-        themselves touch no block table."""
-        self.cache.reserve_many([(s, self.cache.length(s) + n_steps) for s in self.slots])
+        themselves touch no block table (a cache that evicts: up to its next eviction)."""
+        cache = self.cache
+        ahead = {s: n_steps if cache.keep is None else min(n_steps, max(1, cache.keep.most - cache.held(s))) for s in self.slots}
+        self.cache.reserve_many([(s, self.cache.length(s) + ahead[s]) for s in self.slots])
         self.cache.flush_tables()

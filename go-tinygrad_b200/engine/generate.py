@@ -19,7 +19,7 @@ from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
-from ..cache import Cache
+from ..cache import Cache, KeepRule
 from ..sampling import Sampler
 from .decode import DecodeBatch
 from .model import Model
@@ -44,13 +44,15 @@ def generate(model: Model, prompts: Sequence[Sequence[int]],
              max_new_tokens: Union[int, Sequence[int]] = 50, *, temperature: float = 0.0,
              seed: int = 0, stop: Optional[Sequence[int]] = None, cache: Optional[Cache] = None,
              max_batch: Optional[int] = None, max_tokens: Optional[int] = None,
-             max_sequence: Optional[int] = None, use_graph: bool = True) -> List[GenerationResult]:
+             max_sequence: Optional[int] = None, use_graph: bool = True, kv_format: Optional[str] = None,
+             keep: Optional[KeepRule] = None) -> List[GenerationResult]:
     """Generate for every prompt (lists of token ids).  `stop` defaults to the
     model's own end tokens (config.json's eos_token_id).  With no `cache` one
     is made that holds `max_tokens` tokens (default: what the largest batch
     needs, up to `max_batch` requests at a time, default 64).  `max_sequence`
     caps a sequence's length (prompt and new tokens) below the model's own longest
-    position: a request that reaches it ends with "capacity".  Decode steps of a
+    position: a request that reaches it ends with "capacity".  `kv_format` and `keep` as in
+    `Model.new_cache`, for the cache made here (one that is passed has its own).  Decode steps of a
     batch whose membership does not change are replayed as a CUDA graph (one
     recording per batch size, kept with a `cache` the caller passes, so that
     later calls with the same cache, temperature and seed record nothing) unless
@@ -61,6 +63,8 @@ def generate(model: Model, prompts: Sequence[Sequence[int]],
     if len(limits) != n:
         raise ValueError("max_new_tokens must be one number or one per prompt")
     stop_set = set(model.plan.stop_tokens if stop is None else stop)
+    if cache is not None and (kv_format is not None or keep is not None):
+        raise ValueError("kv_format and keep are for the cache made here; the one passed has its own")
     max_seq = model.plan.max_position
     if max_sequence is not None:
         if max_sequence <= 0:
@@ -74,13 +78,16 @@ def generate(model: Model, prompts: Sequence[Sequence[int]],
         max_batch = max_batch or 64
         if max_tokens is None:
             longest = max_seq if max_seq is not None else max(l + m for l, m in zip(lengths, limits))
-            need = sorted(((min(l + max(0, m - 1), longest) + 63) // 64 * 64 for l, m in zip(lengths, limits)),
+            most = longest if keep is None else keep.most      # rows held at once, or the whole prompt if that is more
+            need = sorted(((max(min(l, longest), min(l + max(0, m - 1), longest, most)) + 63) // 64 * 64 for l, m in zip(lengths, limits)),
                           reverse=True)
             max_tokens = max(64, sum(need[:max_batch]))
-        cache = model.new_cache(max_tokens=max_tokens, max_slots=max_batch)
+            if keep is not None:
+                max_tokens = max(max_tokens, (keep.most + 63) // 64 * 64)
+        cache = model.new_cache(max_tokens=max_tokens, max_slots=max_batch, kv_format=kv_format, keep=keep)
     max_batch = min(max_batch or cache.n_slots, cache.n_slots)
     batches = plan_batches(lengths, limits, max_tokens=cache.max_tokens, max_batch=max_batch,
-                           max_sequence=max_seq)
+                           max_sequence=max_seq, max_held=cache.keep.most if cache.keep is not None else None)
     sampler = Sampler(temperature, seed)
     results: List[Optional[GenerationResult]] = [None] * n
     # batch size (and what else a recording fixes) -> DecodeBatch

@@ -13,7 +13,7 @@ from typing import Any, List, Mapping, Optional, Sequence, Union
 
 import torch
 
-from ..cache import Cache, StateRequest
+from ..cache import Cache, KeepRule, StateRequest
 from ..config.registry import Architecture, find_architecture, read_config_json
 from ..parts.base import Block, Runtime, build_part, walk
 from ..parts.plan import ModelPlan, plan_weight_specs
@@ -112,9 +112,12 @@ class Model:
                                                  device=str(model.rt.device)))
 
     # ------------------------------------------------------------------ cache
-    def new_cache(self, max_tokens: int, max_slots: Optional[int] = None) -> Cache:
+    def new_cache(self, max_tokens: int, max_slots: Optional[int] = None, kv_format: Optional[str] = None,
+                  keep: Optional[KeepRule] = None) -> Cache:
         """A cache for up to `max_tokens` tokens held by live sequences, each
-        sequence's count rounded up to a multiple of 64."""
+        sequence's count rounded up to a multiple of 64.  `kv_format` "e4m3" holds keys and
+        values in 8 bits (refused for a model with a mixer that reads no such cache); `keep`
+        beside it bounds the rows a sequence holds by evicting those of least attention weight."""
         requests, shared = [], []
         for i, entry in enumerate(self.plan.schedule):
             if entry.cache is None:
@@ -125,7 +128,8 @@ class Model:
                 requests.append([r for r in self.blocks[entry.layer].cache_requests() if isinstance(r, StateRequest)])
                 shared.append(entry.cache)
         return Cache(requests, shared, max_tokens=max_tokens, max_slots=max_slots,
-                     max_position=self.plan.max_position, dtype=self.rt.dtype, device=self.rt.device)
+                     max_position=self.plan.max_position, dtype=self.rt.dtype, device=self.rt.device,
+                     kv_format=kv_format, keep=keep)
 
     def generate(self, prompts, max_new_tokens=50, **options):
         """Generate for a list of prompts (token ids); see engine/generate.py."""

@@ -24,12 +24,13 @@ class RequestTooLarge(ValueError):
 
 
 def plan_batches(prompt_lengths: Sequence[int], max_new_tokens: Sequence[int], *, max_tokens: int,
-                 max_batch: int, max_sequence: Optional[int] = None) -> List[List[int]]:
+                 max_batch: int, max_sequence: Optional[int] = None, max_held: Optional[int] = None) -> List[List[int]]:
     """Split requests, in order, into batches that start together.  A batch holds
     at most `max_batch` requests and its requests' worst-case footprints
     (prompt + new tokens, each rounded up to a page) fit `max_tokens`.  A
     request whose worst case exceeds `max_sequence` positions is still taken:
-    it ends when it reaches that length."""
+    it ends when it reaches that length.  `max_held`: rows a sequence holds at most
+    while single tokens join it (a cache that evicts); its prompt is held whole once."""
     if max_batch <= 0:
         raise ValueError("max_batch must be positive")
     batches: List[List[int]] = []
@@ -46,6 +47,8 @@ def plan_batches(prompt_lengths: Sequence[int], max_new_tokens: Sequence[int], *
                 raise RequestTooLarge(f"request {i}: a prompt of {p} tokens exceeds the longest "
                                       f"sequence the model takes ({max_sequence})")
             total = min(total, max_sequence)
+        if max_held is not None:
+            total = max(p, min(total, max_held))
         need = _rounded(total)
         if need > max_tokens:
             raise RequestTooLarge(f"request {i} needs room for {need} tokens; the cache holds {max_tokens}")

@@ -86,6 +86,7 @@ def build_context(model: Model, cache: Cache, entries: Sequence[StepEntry]):
     cu = [0]
     slots: List[int] = []
     start: List[int] = []
+    held: List[int] = []                                 # rows of each sequence after the step
     seen = set()
     for b, e in enumerate(entries):
         toks = np.asarray(e.tokens, dtype=np.int64).reshape(-1)
@@ -113,6 +114,7 @@ def build_context(model: Model, cache: Cache, entries: Sequence[StepEntry]):
         cu.append(cu[-1] + n)
         slots.append(e.slot)
         start.append(s0)
+        held.append(cache.held(e.slot) + n)
     cache.reserve_many([(e.slot, s + len(e.tokens)) for e, s in zip(entries, start)])
     cache.flush_tables()
 
@@ -133,9 +135,9 @@ def build_context(model: Model, cache: Cache, entries: Sequence[StepEntry]):
         tokens=take(n_tok), positions=take(n_tok), token_seq=take(n_tok),
         cu_seqlens=take(n_seq + 1), slots=take(n_seq), start_pos=take(n_seq),
         max_q_len=max(len(e.tokens) for e in entries),
-        max_kv_len=max(s + len(e.tokens) for s, e in zip(start, entries)),
+        max_kv_len=max(held),
         is_decode=all(len(e.tokens) == 1 for e in entries),
-        total_kv_len=sum(s + len(e.tokens) for s, e in zip(start, entries)),
+        total_kv_len=sum(held),
         step=model.steps_run, op_hook=model.op_hook,
     )
     rows = take(n_want) if n_want else None
@@ -177,5 +179,6 @@ def step(model: Model, cache: Cache, entries: Sequence[StepEntry]) -> torch.Tens
         logits = logits_at(model, stream, ctx, rows)
     for e in entries:
         cache.advance(e.slot, len(e.tokens))
+    cache.evict_due([e.slot for e in entries])
     model.steps_run += 1
     return logits

@@ -133,6 +133,12 @@ _SIGNATURES = {
     "gtg_attention_tcgen05_status": ("attention_tcgen05", []),
     "gtg_attention_prefill_tcgen05": ("attention_tcgen05", [_P, _I, _I, _P, _I, _P, _P, _L, _I, _P, _I, _P, _P, _P,
                                                             _I, _I, _I, _I, _I, _F, _I, _I, _P, _F, _I, _P, _P]),
+    "gtg_kv_store_e4m3": ("kv_e4m3", [_I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P,
+                                      _I, _I, _I, _P, _I, _P]),
+    "gtg_kv_evict_e4m3": ("kv_e4m3", [_I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _I, _P, _I, _I, _P, _P, _I, _I, _I, _P, _P]),
+    "gtg_attention_e4m3_scratch_floats": ("attention_e4m3", [_I, _I, _I, _I, _I, _I, _I, _I, _L, _I, _I]),
+    "gtg_attention_e4m3": ("attention_e4m3", [_I, _P, _I, _P, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P,
+                                              _I, _I, _I, _L, _I, _I, _I, _I, _F, _I, _P, _P]),
     "gtg_argmax": ("sampling", [_P, _I, _I, _I, _P, _P]),
     "gtg_sample_temperature": ("sampling", [_P, _I, _I, _I, _F, _U, _P, _P, _P, _P]),
 }
@@ -140,6 +146,7 @@ _RESTYPES = {"gtg_attention_decode_scratch_floats": c_longlong,
              "gtg_attention_masked_scratch_floats": c_longlong,
              "gtg_attention_diff_scratch_floats": c_longlong,
              "gtg_lightning_chunk_values": c_longlong,
+             "gtg_attention_e4m3_scratch_floats": c_longlong,
              "gtg_gemm_bf16_swapab_scratch_floats": c_longlong}
 
 _FUNCS = {}
@@ -1671,6 +1678,165 @@ def attention_decode_bf16(q, out, kv, slots, positions, n_heads: int, scale: flo
                                             int(n_splits), _ptr(scratch), int(chunk_pages), int(ring_pages),
                                             _stream()),
            "attention_decode_bf16")
+
+
+# ------------------------------------------------------------ the 8-bit key/value cache
+E4M3_MAX_CHANNELS = 256       # of a head
+
+
+def _need_e4m3(kv, what: str, q, slots, start_pos, cu_seqlens) -> None:
+    """What both kernels ask of an `E4M3KVView` and a step's index tensors."""
+    _need(getattr(kv, "format", None) == "e4m3", f"{what}: needs a view of an e4m3 cache")
+    for t in (slots, start_pos, cu_seqlens):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise KernelError(f"{what}: slots, start_pos and cu_seqlens must be contiguous int32")
+    n = slots.numel()
+    if start_pos.numel() != n or cu_seqlens.numel() != n + 1:
+        raise KernelError(f"{what}: {n} slots need {n} start positions and {n + 1} cumulative lengths")
+    device = kv.k.device
+    if slots.device != device or start_pos.device != device or cu_seqlens.device != device or q.device != device:
+        raise KernelError(f"{what}: the step's tensors must be on the cache's device")
+    if device.type == "cuda" and device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: the cache is on {device}, which is not the current device")
+
+
+def _check_access_e4m3(what: str, kv, slots, start_pos, cu_seqlens) -> None:
+    """The debug pass over a view whose rows are positions less what has been evicted."""
+    if not _checked:
+        return
+    if kv.dropped is not None:
+        start_pos = start_pos - kv.dropped[slots.long().clamp(0, kv.dropped.numel() - 1)]
+    _check_access(what, 2, kv, slots, start_pos=start_pos, cu_seqlens=cu_seqlens)
+
+
+def kv_store_e4m3(qkv: torch.Tensor, cos_sin: Optional[torch.Tensor], n_heads: int, n_kv_store: int, kv, cu_seqlens: torch.Tensor,
+                  slots: torch.Tensor, start_pos: torch.Tensor, max_q_len: int, q_out: Optional[torch.Tensor], pairing: str = "half",
+                  rotary_dim: Optional[int] = None, values_from_keys: bool = False) -> None:
+    """A step's queries, keys and values between projection and attention, for a cache in e4m3 (`kv`, an
+    `E4M3KVView`): the rotated query heads of qkv [N, heads * head_dim] go to q_out [N, n_heads * head_dim] (None: they are not
+    wanted), the rotated key heads and the value heads into the cache, at the rows of each sequence's new tokens (sequence b owns
+    qkv's rows cu_seqlens[b]..cu_seqlens[b+1], `max_q_len` of them at most, at positions start_pos[b], ...).  qkv is left as it
+    is.  With n_kv_store == 0 nothing is stored.  Rotation as in `rope_kv_store`, in float; a key is rounded once, to its code.
+
+    The block of 64 rows a token falls into has one scale for keys and one for values, the least power of two that its largest
+    finite value divided by 448 does not exceed; a token that needs a larger one than the block's older rows raises it, and
+    their codes are rounded to it.  Values that are not finite become NaN and count for no scale.  The gathered weights of the
+    new rows (a cache that evicts) become 0.  A slot must not appear twice."""
+    _rows2d(qkv, "kv_store_e4m3: qkv")
+    _need_e4m3(kv, "kv_store_e4m3", qkv, slots, start_pos, cu_seqlens)
+    dt, hd, N = _dt(qkv), kv.head_dim, qkv.shape[0]
+    if pairing not in ROTARY_PAIRINGS:
+        raise KernelError(f"kv_store_e4m3: pairing {pairing!r} is not supported; supported: {sorted(ROTARY_PAIRINGS)}")
+    rot = hd if rotary_dim is None else int(rotary_dim)
+    if n_kv_store not in (0, kv.n_kv_heads):
+        raise KernelError(f"kv_store_e4m3: the cache holds {kv.n_kv_heads} heads, not {n_kv_store}")
+    if qkv.shape[1] < (n_heads + (1 if values_from_keys else 2) * n_kv_store) * hd:
+        raise KernelError("kv_store_e4m3: qkv is too narrow")
+    if max_q_len < 1 and N:
+        raise KernelError("kv_store_e4m3: max_q_len must be the longest run of new tokens")
+    if cos_sin is not None:
+        if rot % 2 or not 0 < rot <= hd:
+            raise KernelError(f"kv_store_e4m3: rotary_dim {rot} must be even and between 2 and head_dim {hd}")
+        if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or tuple(cos_sin.shape) != (N, rot // 2, 2):
+            raise KernelError("kv_store_e4m3: cos_sin must be contiguous float32 [N, rotary_dim/2, 2]")
+    else:
+        rot = 0
+    if q_out is not None:
+        _rows2d(q_out, "kv_store_e4m3: q_out")
+        if q_out.dtype != qkv.dtype or tuple(q_out.shape) != (N, n_heads * hd):
+            raise KernelError("kv_store_e4m3: q_out must be [N, n_heads * head_dim] of qkv's dtype")
+    if n_kv_store:
+        _check_access_e4m3("kv_store_e4m3", kv, slots, start_pos, cu_seqlens)
+    _check(_fn("gtg_kv_store_e4m3")(dt, qkv.data_ptr(), qkv.stride(0), _ptr(cos_sin), n_heads, kv.n_kv_heads, hd, rot, ROTARY_PAIRINGS[pairing],
+                                    1 if values_from_keys else 0, 1 if n_kv_store else 0, *kv.address(), cu_seqlens.data_ptr(), slots.data_ptr(),
+                                    start_pos.data_ptr(), slots.numel(), int(max_q_len), N, _ptr(q_out), q_out.stride(0) if q_out is not None else 0,
+                                    _stream()), "kv_store_e4m3")
+
+
+def attention_e4m3_scratch_floats(dtype: torch.dtype, n_seqs: int, n_tokens: int, max_q_len: int, n_heads: int, kv, max_kv_len: int,
+                                  total_kv_len: int = 0, window: Optional[int] = None) -> int:
+    """Floats of scratch `attention_e4m3` needs for the same arguments (0: none)."""
+    window = kv.window if window is None else window
+    return int(_fn("gtg_attention_e4m3_scratch_floats")(0 if dtype == torch.float32 else 1, n_seqs, n_tokens, int(max_q_len), n_heads, kv.n_kv_heads,
+                                                        kv.head_dim, int(max_kv_len), int(total_kv_len), int(window or 0),
+                                                        1 if kv.weights is not None else 0))
+
+
+def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Tensor, slots: torch.Tensor, start_pos: torch.Tensor, max_q_len: int,
+                   n_heads: int, scale: float, *, max_kv_len: int, total_kv_len: int = 0, window: Optional[int] = None,
+                   scratch: Optional[torch.Tensor] = None) -> None:
+    """Causal grouped-query attention over a cache in e4m3 (`kv`, an `E4M3KVView`), for decode steps, prompts and anything in
+    between: q [N, n_heads * head_dim] rotated, its keys and values in the cache (`kv_store_e4m3`), out like q (float32 or
+    bfloat16).  Sequence b owns q's rows cu_seqlens[b]..cu_seqlens[b+1] (`max_q_len` of them at most) at positions start_pos[b], ...;
+    a query sees the rows at and before its own, the last `window` of them where a window is given (default: the view's).
+    `max_kv_len`: rows of the longest sequence after this step; `total_kv_len`: of all (0: not known).  Both decide only how the work
+    is cut: a sequence that has outgrown them is still computed right.  Where the view gathers weights, every row's grows by the
+    sum of its probabilities over the step's queries and the heads that share it.  Rows of q and out behind the last sequence
+    are left alone.  `scratch`: float32, at least `attention_e4m3_scratch_floats` (None: taken from the allocator)."""
+    _rows2d(q, "attention_e4m3: q")
+    _rows2d(out, "attention_e4m3: out")
+    _need_e4m3(kv, "attention_e4m3", q, slots, start_pos, cu_seqlens)
+    dt, hd, N = _dt(q), kv.head_dim, q.shape[0]
+    if out.dtype != q.dtype or q.shape[1] != n_heads * hd or out.shape[1] != n_heads * hd or out.shape[0] < N:
+        raise KernelError("attention_e4m3: q and out must be [N, n_heads * head_dim] of one dtype")
+    if n_heads <= 0 or n_heads % kv.n_kv_heads:
+        raise KernelError(f"attention_e4m3: {n_heads} query heads cannot share {kv.n_kv_heads} key/value heads")
+    if N and (max_q_len < 1 or max_kv_len < 1):
+        raise KernelError("attention_e4m3: max_q_len and max_kv_len must be positive")
+    window = kv.window if window is None else window
+    if window is not None and window < 0:
+        raise KernelError("attention_e4m3: the window must not be negative")
+    B = slots.numel()
+    _check_access_e4m3("attention_e4m3", kv, slots, start_pos, cu_seqlens)
+    if N == 0 or B == 0:
+        return
+    need = int(_fn("gtg_attention_e4m3_scratch_floats")(dt, B, N, int(max_q_len), n_heads, kv.n_kv_heads, hd, int(max_kv_len), int(total_kv_len),
+                                                        int(window or 0), 1 if kv.weights is not None else 0))
+    if need:
+        if scratch is None:
+            scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+        elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need or scratch.data_ptr() % 16:
+            raise KernelError(f"attention_e4m3: scratch needs {need} contiguous floats on a 16-byte boundary")
+    _check(_fn("gtg_attention_e4m3")(dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *kv.address(), cu_seqlens.data_ptr(),
+                                     slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), int(total_kv_len), N, n_heads,
+                                     kv.n_kv_heads, hd, float(scale), int(window or 0), _ptr(scratch) if need else None, _stream()), "attention_e4m3")
+
+
+def kv_evict_e4m3(storage, slots: torch.Tensor, lengths: torch.Tensor, max_length: int, budget: int, recent: int,
+                  kept: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Cut sequences of an e4m3 cache (`storage`, an `E4M3Storage` that gathers weights) back to `budget` rows, in place: of the
+    lengths[i] rows (at most `max_length`) that the sequence in slots[i] holds, each layer run and key/value head keeps its
+    `recent` newest and of the others the budget - recent of largest gathered weight (the lower row on a tie), in their order, at
+    rows 0..budget-1.  Blocks all of whose rows stay in place are left as they were; any other gets the least scale that holds
+    its rows, and their codes are rounded to it (which changes only codes that need the smallest steps).  A sequence of at
+    most `budget` rows is left alone.  storage.dropped[slot], where given, grows by the rows cut.  Returns `kept` (int32
+    [entries, n, n_kv_heads, budget], made if None): the former row of each row kept, -1 behind a shorter sequence's last.
+    A slot must not appear twice."""
+    _need(getattr(storage, "format", None) == "e4m3" and storage.k.dim() == 5, "kv_evict_e4m3: needs the storage of an e4m3 cache")
+    _need(storage.weights is not None, "kv_evict_e4m3: this cache gathers no attention weights")
+    n, device = slots.numel(), storage.k.device
+    for t in (slots, lengths):
+        _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n and t.device == device,
+              "kv_evict_e4m3: slots and lengths must be contiguous int32 of one size on the cache's device")
+    _need(budget >= 1 and 0 <= recent <= budget, f"kv_evict_e4m3: budget {budget} must be positive and recent {recent} between 0 and it")
+    _need(0 <= max_length <= storage.block_table.shape[1] * PAGE_TOKENS, f"kv_evict_e4m3: the block table holds no {max_length} rows of a sequence")
+    E, KV = storage.k.shape[0], storage.n_kv_heads
+    if kept is None:
+        kept = torch.empty(E, n, KV, budget, dtype=torch.int32, device=device)
+    else:
+        _need(kept.dtype == torch.int32 and kept.is_contiguous() and tuple(kept.shape) == (E, n, KV, budget) and kept.device == device,
+              "kv_evict_e4m3: kept must be contiguous int32 [entries, n, n_kv_heads, budget]")
+    if n == 0:
+        return kept
+    k, v, s, w = storage.k, storage.v, storage.scales, storage.weights
+    if _checked:
+        start = (lengths - 1).clamp(min=0)
+        _check_access("kv_evict_e4m3", 2, storage.entry(0), slots, start_pos=start, cu_seqlens=torch.arange(n + 1, dtype=torch.int32, device=device))
+    _check(_fn("gtg_kv_evict_e4m3")(E, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), s.data_ptr(), s.stride(0),
+                                    s.stride(1), w.data_ptr(), w.stride(0), w.stride(1), storage.block_table.data_ptr(), storage.block_table.stride(0),
+                                    _ptr(storage.dropped), KV, storage.head_dim, slots.data_ptr(), lengths.data_ptr(), n, int(budget), int(recent),
+                                    kept.data_ptr(), _stream()), "kv_evict_e4m3")
+    return kept
 
 
 # ---------------------------------------------------------- attention through a latent

@@ -232,7 +232,7 @@ class GQAttention(Mixer):
             return [KVRequest(self.n_kv, 2 * self.head_dim, self.cache_window, value_dim=self.value_dim)]
         if self.general:
             return [KVRequest(self.n_kv, self.head_dim, self.cache_window, value_dim=self.value_dim, chunk=self.chunk)]
-        return [KVRequest(self.n_kv, self.head_dim, self.cache_window)]
+        return [KVRequest(self.n_kv, self.head_dim, self.cache_window, e4m3=not self.rows_route)]
 
     def load(self, tensors: Mapping[str, torch.Tensor], rt: Runtime) -> None:
         parts = [tensors[self.names["q"]]]
@@ -371,11 +371,40 @@ class GQAttention(Mixer):
         ctx.trace("attn", mixed)
         return emit_update(mixed, self.w_o, ctx)
 
+    def _forward_e4m3(self, x: torch.Tensor, ctx: StepContext, cache: CacheHandle) -> torch.Tensor:
+        """The plain route over a cache in 8 bits: projection; rotation and store; attention."""
+        rt, kv, n = ctx.rt, cache.kv, x.shape[0]
+        qkv = rt.empty(n, self.w_qkv.shape[0])
+        rotation = self.position.rotation(ctx)
+        ops.linear(x, self.w_qkv, qkv)
+        if ctx.op_hook is not None:
+            ctx.trace("q", qkv[:, : self.q_dim].clone())
+            if self.own_kv:
+                ctx.trace("k", qkv[:, self.q_dim: self.q_dim + self.kv_dim])
+                ctx.trace("v", qkv[:, self.q_dim + (0 if self.v_from_k else self.kv_dim):][:, : self.kv_dim])
+        q = rt.empty(n, self.q_dim)
+        ops.kv_store_e4m3(qkv, rotation, self.n_heads, self.n_kv if cache.writes and self.own_kv else 0, kv, ctx.cu_seqlens, ctx.slots,
+                          ctx.start_pos, ctx.max_q_len, q, pairing=self.position.pairing, rotary_dim=self.position.rotary_dim,
+                          values_from_keys=self.v_from_k)
+        ctx.trace("q_attn", q)
+        mixed = rt.empty(n, self.q_dim)
+        need = ops.attention_e4m3_scratch_floats(rt.dtype, ctx.n_seqs, n, ctx.max_q_len, self.n_heads, kv, ctx.max_kv_len, ctx.total_kv_len,
+                                                 self.window or 0)
+        ops.attention_e4m3(q, mixed, kv, ctx.cu_seqlens, ctx.slots, ctx.start_pos, ctx.max_q_len, self.n_heads, self.scale,
+                           max_kv_len=ctx.max_kv_len, total_kv_len=ctx.total_kv_len, window=self.window or 0,
+                           scratch=rt.empty(need, dtype=torch.float32) if need else None)
+        ctx.trace("attn", mixed)
+        return emit_update(mixed, self.w_o, ctx)
+
     def forward(self, x: torch.Tensor, ctx: StepContext, cache: CacheHandle) -> torch.Tensor:
         rt = ctx.rt
         kv = cache.kv
         if kv is None or kv.n_kv_heads != self.n_kv or kv.head_dim != self.maps * self.head_dim or kv.value_dim != self.value_dim:
             raise ValueError("attention was given a cache entry that does not match its heads")
+        if kv.format == "e4m3":
+            if self.differential or self.rows_route or self.conv_route or self.general:
+                raise ValueError("this attention mixer's options are not built over an e4m3 cache")
+            return self._forward_e4m3(x, ctx, cache)
         if self.differential:
             return self._forward_differential(x, ctx, cache)
         if self.rows_route:

@@ -196,7 +196,7 @@ class StepContext:
     slots: torch.Tensor         # [n_seqs] cache slot of each sequence
     start_pos: torch.Tensor     # [n_seqs] tokens already in the cache before this step
     max_q_len: int              # longest run of new tokens in the batch
-    max_kv_len: int             # longest sequence after this step
+    max_kv_len: int             # longest sequence after this step (in rows that the cache holds of it)
     is_decode: bool             # every sequence brings exactly one token
     total_kv_len: int = 0       # all sequences' lengths after this step, added up (0: not known)
     shared: Dict[Any, Any] = field(default_factory=dict)   # per-step values parts share (rotary tables)
