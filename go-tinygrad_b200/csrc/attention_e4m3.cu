@@ -4,9 +4,10 @@
 // where there is one).  Where the cache gathers weights, row j's weight grows by the sum of p_j over the step's queries and
 // the query heads of its key/value head.
 //
+//   few_queries:      bfloat16, heads of up to 128 channels in steps of 16, few queries a sequence (attention_e4m3_few.cuh);
 //   attention_rows:   any head size and type, one block per (token, query head); scores, softmax and sums in float.
 //   row_weights:      the weights, once every row's maximum and sum are known: a block per (cache page, head, sequence).
-#include "e4m3.cuh"
+#include "attention_e4m3_few.cuh"
 
 namespace {
 
@@ -131,9 +132,9 @@ row_weights_kernel(const T* __restrict__ q, int ldq, const E4M3Pages kv, const i
     chain_release();
     chain_wait();
     constexpr int kAtOnce = 8;
-    extern __shared__ float smem[];
+    extern __shared__ float row_smem[];
     const int hd = kv.hd, ld = hd + 1;
-    float* ks = smem;                                                           // [64][hd + 1]
+    float* ks = row_smem;                                                           // [64][hd + 1]
     float* qs = ks + kPageTokens * ld;                                          // [kAtOnce][hd]
     __shared__ float2 st[kAtOnce];
     __shared__ float half_sum[kPageTokens];
@@ -193,10 +194,18 @@ int launch_rows(const void* q, int ldq, void* out, int ldo, const E4M3Pages& kv,
 }
 }  // namespace
 
+static FewPlan few_plan(int B, int max_q_len, int n_heads, int n_kv, int hd, int max_kv_len, long long total_kv_len, int window, int weigh) {
+#define GTG_FEW(HD) case HD: return few_plan_for<HD>(B, max_q_len, n_heads, n_kv, max_kv_len, total_kv_len, window, weigh);
+    switch (hd) { GTG_FEW(16) GTG_FEW(32) GTG_FEW(48) GTG_FEW(64) GTG_FEW(80) GTG_FEW(96) GTG_FEW(112) default: GTG_FEW(128) }
+#undef GTG_FEW
+}
+
 // Floats of scratch that gtg_attention_e4m3 needs for the same numbers.
 GTG_API long long gtg_attention_e4m3_scratch_floats(int dtype, int B, int N, int max_q_len, int n_heads, int n_kv, int hd, int max_kv_len,
                                                     long long total_kv_len, int window, int weigh) {
-    (void)dtype; (void)B; (void)max_q_len; (void)n_kv; (void)hd; (void)max_kv_len; (void)total_kv_len; (void)window;
+    if (B <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || max_q_len <= 0 || max_kv_len <= 0) return 0;
+    if (few_takes(dtype, max_q_len, n_heads, n_kv, hd))
+        return few_plan(B, max_q_len, n_heads, n_kv, hd, max_kv_len, total_kv_len, window, weigh).floats();
     return weigh ? 2LL * N * n_heads : 0;
 }
 
@@ -212,7 +221,18 @@ GTG_API int gtg_attention_e4m3(int dtype, const void* q, int ldq, void* out, int
     if (hd > kMaxChannels || B > 65535 || n_heads > 65535) return kErrUnsupported;
     const E4M3Pages kv = {(uint8_t*)k, (uint8_t*)v, k_stride, v_stride, scales, scale_stride, weights, weight_stride, block_table, table_stride,
                           dropped, n_kv, hd};
-    (void)total_kv_len;
+    if (few_takes(dtype, max_q_len, n_heads, n_kv, hd)) {
+        const FewPlan plan = few_plan(B, max_q_len, n_heads, n_kv, hd, max_kv_len, total_kv_len, window, weights != nullptr);
+        if (plan.floats() && !scratch) return kErrBadArgument;
+        FewArgs a = {};
+        a.q = (const bf16*)q; a.ldq = ldq; a.out = (bf16*)out; a.ldo = ldo;
+        a.cu_seqlens = cu_seqlens; a.slots = slots; a.start_pos = start_pos;
+        a.n_heads = n_heads; a.group = n_heads / n_kv; a.scale = scale; a.window = window;
+#define GTG_FEW(HD) case HD: return launch_few<HD>(a, kv, plan, B, scratch, stream);
+        switch (hd) { GTG_FEW(16) GTG_FEW(32) GTG_FEW(48) GTG_FEW(64) GTG_FEW(80) GTG_FEW(96) GTG_FEW(112) GTG_FEW(128) }
+#undef GTG_FEW
+    }
+    if (weights && !scratch) return kErrBadArgument;
     if (dtype == 0) return launch_rows<float>(q, ldq, out, ldo, kv, cu_seqlens, slots, start_pos, B, max_q_len, max_kv_len, N, n_heads, scale, window, scratch, stream);
     return launch_rows<bf16>(q, ldq, out, ldo, kv, cu_seqlens, slots, start_pos, B, max_q_len, max_kv_len, N, n_heads, scale, window, scratch, stream);
 }

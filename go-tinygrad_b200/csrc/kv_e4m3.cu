@@ -38,8 +38,8 @@ template <typename T>
 __global__ void __launch_bounds__(kStoreThreads)
 kv_store_kernel(const StoreInput<T> in, const E4M3Pages kv, const int* __restrict__ cu_seqlens, const int* __restrict__ slots,
                 const int* __restrict__ start_pos, int blocks_per_seq, long long blocks_kv, int N, T* __restrict__ q_out, int ldq) {
-    chain_release();
     chain_wait();
+    chain_release();                  // only now: what comes next may read older pages at once (all before this kernel is complete)
     __shared__ float scratch[33];
     const int tid = threadIdx.x;
     if ((long long)blockIdx.x >= blocks_kv) {

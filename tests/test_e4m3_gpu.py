@@ -384,6 +384,25 @@ def test_what_is_not_finite_stays_with_who_sees_it(dtype, new):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128, 48, 20])
+@pytest.mark.parametrize("new,window", [(2, 0), (5, 0), (60, 0), (130, 0), (3, 40), (100, 40)])
+def test_nan_values_spoil_the_queries_that_see_their_rows(dtype, hd, new, window):
+    """One channel of one value row is NaN: queries before it are untouched, those at or behind it have NaN in that channel of
+    its head (until it is behind the window), and nowhere else."""
+    held, row, channel = 200, 199 - new // 2, 11
+    p = Pages([held], 2, hd, seed=18)
+    p.v.view(torch.uint8)[p.pages[0][row // 64], 1, channel, row % 64] = NAN
+    q = torch.randn(new, 4 * hd, device=DEV).to(dtype)
+    out = torch.empty_like(q)
+    ops.attention_e4m3(q, out, p.view(), cut([new]), ints(p.slots), ints([held - new]), new, 4, hd ** -0.5, max_kv_len=held, window=window)
+    at = held - new + torch.arange(new, device=DEV)
+    sees = (at >= row) & ((at - row < window) if window else True)
+    want = torch.zeros(new, 2, 2, hd, dtype=torch.bool, device=DEV)
+    want[sees, 1, :, channel] = True
+    assert torch.equal(out.isnan().reshape(want.shape), want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("held,new", [([3000, 70, 1], [1, 1, 1]), ([500, 333], [257, 40])])
 def test_the_same_twice_and_alone(dtype, held, new):
     """The same inputs give the same bits; a sequence's result does not depend on another's rows; two calls over one another on
