@@ -120,7 +120,7 @@ attention_rows_kernel(const T* __restrict__ q, int ldq, T* __restrict__ out, int
         for (int w = 0; w < kRowWarps; ++w) acc += f[w] * wo[w][d];
         out[(size_t)token * ldo + head * hd + d] = from_f32<T>(acc / L);
     }
-    if (stats && tid == 0) stats[(size_t)token * n_heads + head] = make_float2(M, L);
+    if (stats && tid == 0) stats[(size_t)token * n_heads + head] = make_float2(M_use * kLog2e, L);
 }
 
 // A block per (page of the sequence, key/value head, sequence): 64 rows by two halves of the (query, head) pairs that may
@@ -148,7 +148,7 @@ row_weights_kernel(const T* __restrict__ q, int ldq, const E4M3Pages kv, const i
         const uint8_t* kr = kv.k + page * kv.k_stride + (size_t)h * kPageTokens * hd;
         __syncthreads();
         for (int i = tid; i < kPageTokens * hd; i += kRowThreads) ks[i / hd * ld + i % hd] = e4m3_value(kr[i]);
-        const float k_scale = kv.scales[page * kv.scale_stride + h];
+        const float k_scale = kv.scales[page * kv.scale_stride + h] * kLog2e;
         const int row = block * kPageTokens + t;
         const int from = max(0, block * kPageTokens - start);                   // queries before that one see none of these rows
         const int pairs = (n_new - from) * group;
@@ -167,7 +167,7 @@ row_weights_kernel(const T* __restrict__ q, int ldq, const E4M3Pages kv, const i
                 if (row > at || (window > 0 && row <= at - window)) continue;
                 float s = 0.f;
                 for (int d = 0; d < hd; ++d) s = fmaf(qs[i * hd + d], ks[t * ld + d], s);
-                sum += expf(s * k_scale - st[i].x) / st[i].y;
+                sum += exp2f(fmaf(s, k_scale, -st[i].x)) / st[i].y;
             }
         }
         if (part) half_sum[t] = sum;
@@ -180,22 +180,28 @@ row_weights_kernel(const T* __restrict__ q, int ldq, const E4M3Pages kv, const i
 }
 
 template <typename T>
-int launch_rows(const void* q, int ldq, void* out, int ldo, const E4M3Pages& kv, const int* cu_seqlens, const int* slots, const int* start_pos,
-                int B, int max_q_len, int max_kv_len, int N, int n_heads, float scale, int window, float* scratch, cudaStream_t stream) {
-    float2* stats = kv.weights ? (float2*)scratch : nullptr;
-    int st = launch_chained(attention_rows_kernel<T>, dim3(N, n_heads), dim3(kRowThreads), 0, stream, (const T*)q, ldq, (T*)out, ldo, kv,
-                            cu_seqlens, slots, start_pos, B, n_heads, scale, window, stats);
-    if (st != 0 || !kv.weights) return st;
+int launch_row_weights(const void* q, int ldq, const E4M3Pages& kv, const int* cu_seqlens, const int* slots, const int* start_pos, int B,
+                       int max_kv_len, int n_heads, float scale, int window, const float2* stats, cudaStream_t stream) {
     const size_t smem = ((size_t)kPageTokens * (kv.hd + 1) + 8 * (size_t)kv.hd) * sizeof(float);
     cudaError_t e = cudaFuncSetAttribute(row_weights_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
     return launch_chained(row_weights_kernel<T>, dim3((max_kv_len + kPageTokens - 1) / kPageTokens, kv.n_kv, B), dim3(kRowThreads), smem, stream,
-                          (const T*)q, ldq, kv, cu_seqlens, slots, start_pos, n_heads, scale, window, (const float2*)stats);
+                          (const T*)q, ldq, kv, cu_seqlens, slots, start_pos, n_heads, scale, window, stats);
+}
+
+template <typename T>
+int launch_rows(const void* q, int ldq, void* out, int ldo, const E4M3Pages& kv, const int* cu_seqlens, const int* slots, const int* start_pos,
+                int B, int max_kv_len, int N, int n_heads, float scale, int window, float* scratch, cudaStream_t stream) {
+    float2* stats = kv.weights ? (float2*)scratch : nullptr;
+    const int st = launch_chained(attention_rows_kernel<T>, dim3(N, n_heads), dim3(kRowThreads), 0, stream, (const T*)q, ldq, (T*)out, ldo, kv,
+                                  cu_seqlens, slots, start_pos, B, n_heads, scale, window, stats);
+    if (st != 0 || !kv.weights) return st;
+    return launch_row_weights<T>(q, ldq, kv, cu_seqlens, slots, start_pos, B, max_kv_len, n_heads, scale, window, stats, stream);
 }
 }  // namespace
 
-static FewPlan few_plan(int B, int max_q_len, int n_heads, int n_kv, int hd, int max_kv_len, long long total_kv_len, int window, int weigh) {
-#define GTG_FEW(HD) case HD: return few_plan_for<HD>(B, max_q_len, n_heads, n_kv, max_kv_len, total_kv_len, window, weigh);
+static FewPlan few_plan(int B, int max_q_len, int n_heads, int n_kv, int hd, int max_kv_len, int weigh) {
+#define GTG_FEW(HD) case HD: return few_plan_for<HD>(B, max_q_len, n_heads, n_kv, max_kv_len, weigh);
     switch (hd) { GTG_FEW(16) GTG_FEW(32) GTG_FEW(48) GTG_FEW(64) GTG_FEW(80) GTG_FEW(96) GTG_FEW(112) default: GTG_FEW(128) }
 #undef GTG_FEW
 }
@@ -203,9 +209,10 @@ static FewPlan few_plan(int B, int max_q_len, int n_heads, int n_kv, int hd, int
 // Floats of scratch that gtg_attention_e4m3 needs for the same numbers.
 GTG_API long long gtg_attention_e4m3_scratch_floats(int dtype, int B, int N, int max_q_len, int n_heads, int n_kv, int hd, int max_kv_len,
                                                     long long total_kv_len, int window, int weigh) {
+    (void)total_kv_len; (void)window;
     if (B <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || max_q_len <= 0 || max_kv_len <= 0) return 0;
     if (few_takes(dtype, max_q_len, n_heads, n_kv, hd))
-        return few_plan(B, max_q_len, n_heads, n_kv, hd, max_kv_len, total_kv_len, window, weigh).floats();
+        return few_plan(B, max_q_len, n_heads, n_kv, hd, max_kv_len, weigh).floats();
     return weigh ? 2LL * N * n_heads : 0;
 }
 
@@ -222,17 +229,30 @@ GTG_API int gtg_attention_e4m3(int dtype, const void* q, int ldq, void* out, int
     const E4M3Pages kv = {(uint8_t*)k, (uint8_t*)v, k_stride, v_stride, scales, scale_stride, weights, weight_stride, block_table, table_stride,
                           dropped, n_kv, hd};
     if (few_takes(dtype, max_q_len, n_heads, n_kv, hd)) {
-        const FewPlan plan = few_plan(B, max_q_len, n_heads, n_kv, hd, max_kv_len, total_kv_len, window, weights != nullptr);
+        const FewPlan plan = few_plan(B, max_q_len, n_heads, n_kv, hd, max_kv_len, weights != nullptr);
         if (plan.floats() && !scratch) return kErrBadArgument;
         FewArgs a = {};
         a.q = (const bf16*)q; a.ldq = ldq; a.out = (bf16*)out; a.ldo = ldo;
         a.cu_seqlens = cu_seqlens; a.slots = slots; a.start_pos = start_pos;
-        a.n_heads = n_heads; a.group = n_heads / n_kv; a.scale = scale; a.window = window;
-#define GTG_FEW(HD) case HD: return launch_few<HD>(a, kv, plan, B, scratch, stream);
+        a.B = B; a.n_heads = n_heads; a.group = n_heads / n_kv; a.scale = scale; a.window = window;
+#define GTG_FEW(HD) case HD: return launch_few<HD>(a, kv, plan, scratch, stream);
         switch (hd) { GTG_FEW(16) GTG_FEW(32) GTG_FEW(48) GTG_FEW(64) GTG_FEW(80) GTG_FEW(96) GTG_FEW(112) GTG_FEW(128) }
 #undef GTG_FEW
     }
     if (weights && !scratch) return kErrBadArgument;
-    if (dtype == 0) return launch_rows<float>(q, ldq, out, ldo, kv, cu_seqlens, slots, start_pos, B, max_q_len, max_kv_len, N, n_heads, scale, window, scratch, stream);
-    return launch_rows<bf16>(q, ldq, out, ldo, kv, cu_seqlens, slots, start_pos, B, max_q_len, max_kv_len, N, n_heads, scale, window, scratch, stream);
+    if (dtype == 0) return launch_rows<float>(q, ldq, out, ldo, kv, cu_seqlens, slots, start_pos, B, max_kv_len, N, n_heads, scale, window, scratch, stream);
+    return launch_rows<bf16>(q, ldq, out, ldo, kv, cu_seqlens, slots, start_pos, B, max_kv_len, N, n_heads, scale, window, scratch, stream);
+}
+
+// The weights alone: stats float2 [N][n_heads], per query what its scores (in powers of two) are compared with and its sum.
+GTG_API int gtg_row_weights_e4m3(int dtype, const void* q, int ldq, void* k, long long k_stride, float* scales, long long scale_stride,
+                                 float* weights, long long weight_stride, const int* block_table, int table_stride, const int* dropped,
+                                 const int* cu_seqlens, const int* slots, const int* start_pos, int B, int max_kv_len, int n_heads, int n_kv,
+                                 int hd, float scale, int window, const float* stats, cudaStream_t stream) {
+    if (B <= 0) return 0;
+    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || hd <= 0 || max_kv_len <= 0 || window < 0 || !weights || !stats) return kErrBadArgument;
+    if (hd > kMaxChannels || B > 65535 || n_kv > 65535) return kErrUnsupported;
+    const E4M3Pages kv = {(uint8_t*)k, nullptr, k_stride, 0, scales, scale_stride, weights, weight_stride, block_table, table_stride, dropped, n_kv, hd};
+    if (dtype == 0) return launch_row_weights<float>(q, ldq, kv, cu_seqlens, slots, start_pos, B, max_kv_len, n_heads, scale, window, (const float2*)stats, stream);
+    return launch_row_weights<bf16>(q, ldq, kv, cu_seqlens, slots, start_pos, B, max_kv_len, n_heads, scale, window, (const float2*)stats, stream);
 }

@@ -54,6 +54,7 @@ LIBRARIES: Dict[str, str] = {
     "mlstm": "mlstm.cu",
     "kv_e4m3": "kv_e4m3.cu",
     "attention_e4m3": "attention_e4m3.cu",
+    "attention_e4m3_tcgen05": "attention_e4m3_tcgen05.cu",
 }
 # sources a library's file includes textually (they count for staleness)
 INCLUDED_SOURCES: Dict[str, List[str]] = {"attention_decode_static.cu": ["attention_bf16.cu"]}

@@ -139,6 +139,11 @@ _SIGNATURES = {
     "gtg_attention_e4m3_scratch_floats": ("attention_e4m3", [_I, _I, _I, _I, _I, _I, _I, _I, _L, _I, _I]),
     "gtg_attention_e4m3": ("attention_e4m3", [_I, _P, _I, _P, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P,
                                               _I, _I, _I, _L, _I, _I, _I, _I, _F, _I, _P, _P]),
+    "gtg_row_weights_e4m3": ("attention_e4m3", [_I, _P, _I, _P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _P, _P]),
+    "gtg_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", [_P, _I, _P, _I, _P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I,
+                                                              _F, _I, _P, _P]),
+    "gtg_attention_e4m3_tcgen05_status": ("attention_e4m3_tcgen05", []),
+    "gtg_attention_e4m3_tcgen05_test_hooks": ("attention_e4m3_tcgen05", [_I]),
     "gtg_argmax": ("sampling", [_P, _I, _I, _I, _P, _P]),
     "gtg_sample_temperature": ("sampling", [_P, _I, _I, _I, _F, _U, _P, _P, _P, _P]),
 }
@@ -1291,13 +1296,15 @@ def bounded_wait_failures() -> int:
     copies (it then returned without a result).  Reading it synchronises."""
     total = 0
     for symbol in ("gtg_gemm_bf16_skinny_status", "gtg_gemm_bf16_tcgen05_status", "gtg_gemm_bf16_swapab_status",
-                   "gtg_attention_tcgen05_status", "gtg_attention_diff_tcgen05_status", "gtg_latent_status"):
+                   "gtg_attention_tcgen05_status", "gtg_attention_diff_tcgen05_status", "gtg_latent_status",
+                   "gtg_attention_e4m3_tcgen05_status"):
         if _SIGNATURES[symbol][0] in build._LOADED:        # only libraries that have run can have failed
             total += int(_fn(symbol)())
     return total
 
 
-WAITING_LIBRARIES = ("gemm_bf16_skinny", "gemm_bf16_tcgen05", "gemm_bf16_swapab", "attention_tcgen05", "attention_diff_tcgen05", "latent")
+WAITING_LIBRARIES = ("gemm_bf16_skinny", "gemm_bf16_tcgen05", "gemm_bf16_swapab", "attention_tcgen05", "attention_diff_tcgen05", "latent",
+                     "attention_e4m3_tcgen05")
 
 
 def wait_test_hooks(library: str, test_waits: bool) -> None:
@@ -1753,10 +1760,20 @@ def kv_store_e4m3(qkv: torch.Tensor, cos_sin: Optional[torch.Tensor], n_heads: i
                                     _stream()), "kv_store_e4m3")
 
 
+E4M3_FEW_QUERIES = 32         # tokens of a step times the heads of a group, up to which a cache's rows are read for few queries
+
+
+def _e4m3_prompt_form(dt: int, max_q_len: int, n_heads: int, n_kv: int, hd: int) -> bool:
+    """Whether the tcgen05 form serves (if rows of q and out also start on 16-byte boundaries)."""
+    return dt == 1 and (hd == 64 or hd == 128) and max_q_len * (n_heads // n_kv) > E4M3_FEW_QUERIES
+
+
 def attention_e4m3_scratch_floats(dtype: torch.dtype, n_seqs: int, n_tokens: int, max_q_len: int, n_heads: int, kv, max_kv_len: int,
                                   total_kv_len: int = 0, window: Optional[int] = None) -> int:
     """Floats of scratch `attention_e4m3` needs for the same arguments (0: none)."""
     window = kv.window if window is None else window
+    if _e4m3_prompt_form(0 if dtype == torch.float32 else 1, max_q_len, n_heads, kv.n_kv_heads, kv.head_dim):
+        return 2 * n_tokens * n_heads if kv.weights is not None else 0
     return int(_fn("gtg_attention_e4m3_scratch_floats")(0 if dtype == torch.float32 else 1, n_seqs, n_tokens, int(max_q_len), n_heads, kv.n_kv_heads,
                                                         kv.head_dim, int(max_kv_len), int(total_kv_len), int(window or 0),
                                                         1 if kv.weights is not None else 0))
@@ -1790,13 +1807,27 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
     _check_access_e4m3("attention_e4m3", kv, slots, start_pos, cu_seqlens)
     if N == 0 or B == 0:
         return
-    need = int(_fn("gtg_attention_e4m3_scratch_floats")(dt, B, N, int(max_q_len), n_heads, kv.n_kv_heads, hd, int(max_kv_len), int(total_kv_len),
-                                                        int(window or 0), 1 if kv.weights is not None else 0))
+    prompt = _e4m3_prompt_form(dt, max_q_len, n_heads, kv.n_kv_heads, hd)
+    if prompt:
+        need = 2 * N * n_heads if kv.weights is not None else 0
+    else:
+        need = int(_fn("gtg_attention_e4m3_scratch_floats")(dt, B, N, int(max_q_len), n_heads, kv.n_kv_heads, hd, int(max_kv_len), int(total_kv_len),
+                                                            int(window or 0), 1 if kv.weights is not None else 0))
     if need:
         if scratch is None:
             scratch = torch.empty(need, dtype=torch.float32, device=q.device)
         elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need or scratch.data_ptr() % 16:
             raise KernelError(f"attention_e4m3: scratch needs {need} contiguous floats on a 16-byte boundary")
+    if prompt and not (q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16):
+        a = kv.address()
+        stats = scratch.data_ptr() if need else None
+        index = (a[8], a[9], a[10], cu_seqlens.data_ptr(), slots.data_ptr(), start_pos.data_ptr())
+        _check(_fn("gtg_attention_e4m3_tcgen05")(q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *a[:6], *index, B, int(max_q_len), n_heads,
+                                                 kv.n_kv_heads, hd, float(scale), int(window or 0), stats, _stream()), "attention_e4m3")
+        if need:
+            _check(_fn("gtg_row_weights_e4m3")(dt, q.data_ptr(), q.stride(0), a[0], a[1], *a[4:8], *index, B, int(max_kv_len), n_heads, kv.n_kv_heads,
+                                               hd, float(scale), int(window or 0), stats, _stream()), "attention_e4m3: weights")
+        return
     _check(_fn("gtg_attention_e4m3")(dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *kv.address(), cu_seqlens.data_ptr(),
                                      slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), int(total_kv_len), N, n_heads,
                                      kv.n_kv_heads, hd, float(scale), int(window or 0), _ptr(scratch) if need else None, _stream()), "attention_e4m3")

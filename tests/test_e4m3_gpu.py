@@ -466,6 +466,46 @@ def test_captured(dtype):
             assert torch.equal(bufs[0][1], bufs[i][1]) and all(torch.equal(x, y) for x, y in zip(results[0], results[i]))
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [1, 9, 200])
+def test_rows_of_any_stride(hd, new):
+    """Rows of q and out that start nowhere in particular give what aligned ones give, as far as bfloat16 can tell."""
+    p = Pages([300], 2, hd, seed=19)
+    q = torch.randn(new, 4 * hd, device=DEV).bfloat16()
+    outs = []
+    for pad in (0, 1, 8):
+        wide_q, wide_out = (torch.zeros(new, 4 * hd + pad, dtype=BF16, device=DEV) for _ in range(2))
+        rows, out = wide_q[:, pad:], wide_out[:, pad:]
+        rows.copy_(q)
+        ops.attention_e4m3(rows, out, p.view(), cut([new]), ints(p.slots), ints([300 - new]), new, 4, hd ** -0.5, max_kv_len=300)
+        outs.append(out.double())
+        assert (wide_out[:, :pad] == 0).all()
+    # two results that are each within half a step (2^-8) and the products' rounding of the same value
+    assert ((outs[0] - outs[1]).abs() <= outs[0].abs() * 2.0 ** -7 + 2.0 ** -9).all() and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_waits_that_run_out(hd):
+    """The tcgen05 form's give-up path: tiles that never arrive.  The kernel returns, says so, and works again afterwards."""
+    p = Pages([300, 70], 2, hd, seed=23)
+    q = torch.randn(270, 4 * hd, device=DEV).bfloat16()
+
+    def run():
+        out = torch.full_like(q, 7.0)
+        ops.attention_e4m3(q, out, p.view(), cut([200, 70]), ints(p.slots), ints([100, 0]), 200, 4, hd ** -0.5, max_kv_len=300)
+        return out
+    want = run()
+    assert ops.bounded_wait_failures() == 0
+    try:
+        ops.wait_test_hooks("attention_e4m3_tcgen05", True)
+        run()
+        torch.cuda.synchronize()
+        assert ops.bounded_wait_failures() != 0
+    finally:
+        ops.wait_test_hooks("attention_e4m3_tcgen05", False)
+    assert ops.bounded_wait_failures() == 0 and torch.equal(run(), want) and ops.bounded_wait_failures() == 0
+
+
 def test_other_streams_and_devices_are_checked():
     p = Pages([70], 1, 64, seed=16)
     q = torch.randn(1, 64, device=DEV)
