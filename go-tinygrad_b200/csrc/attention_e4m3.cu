@@ -243,16 +243,3 @@ GTG_API int gtg_attention_e4m3(int dtype, const void* q, int ldq, void* out, int
     if (dtype == 0) return launch_rows<float>(q, ldq, out, ldo, kv, cu_seqlens, slots, start_pos, B, max_kv_len, N, n_heads, scale, window, scratch, stream);
     return launch_rows<bf16>(q, ldq, out, ldo, kv, cu_seqlens, slots, start_pos, B, max_kv_len, N, n_heads, scale, window, scratch, stream);
 }
-
-// The weights alone: stats float2 [N][n_heads], per query what its scores (in powers of two) are compared with and its sum.
-GTG_API int gtg_row_weights_e4m3(int dtype, const void* q, int ldq, void* k, long long k_stride, float* scales, long long scale_stride,
-                                 float* weights, long long weight_stride, const int* block_table, int table_stride, const int* dropped,
-                                 const int* cu_seqlens, const int* slots, const int* start_pos, int B, int max_kv_len, int n_heads, int n_kv,
-                                 int hd, float scale, int window, const float* stats, cudaStream_t stream) {
-    if (B <= 0) return 0;
-    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || hd <= 0 || max_kv_len <= 0 || window < 0 || !weights || !stats) return kErrBadArgument;
-    if (hd > kMaxChannels || B > 65535 || n_kv > 65535) return kErrUnsupported;
-    const E4M3Pages kv = {(uint8_t*)k, nullptr, k_stride, 0, scales, scale_stride, weights, weight_stride, block_table, table_stride, dropped, n_kv, hd};
-    if (dtype == 0) return launch_row_weights<float>(q, ldq, kv, cu_seqlens, slots, start_pos, B, max_kv_len, n_heads, scale, window, (const float2*)stats, stream);
-    return launch_row_weights<bf16>(q, ldq, kv, cu_seqlens, slots, start_pos, B, max_kv_len, n_heads, scale, window, (const float2*)stats, stream);
-}

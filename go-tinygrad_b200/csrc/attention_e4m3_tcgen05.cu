@@ -463,6 +463,232 @@ int launch(const PromptArgs& a, const E4M3Pages& kv, int B, int max_q_len, cudaS
     return launch_chained(attention_e4m3_prompt_kernel<HD, kTest>, dim3(kv.n_kv, B, (unsigned)((rows + BQ - 1) / BQ)), dim3(kThreads),
                           (size_t)Shape<HD>::kSmemBytes, stream, a, kv);
 }
+// ============================================================== gathered weights of prompts and chunks
+// weight_j += sum over the queries that see row j, of all heads of the group, of 2^(score - x) / l, x and l the query's
+// statistics that the attention left.  The products again, the other way round: one block per (128 rows of the cache, key/value
+// head, sequence), the rows as the tile's rows, so that a thread owns a row and its sum:
+//   K      converted once to bfloat16 (exact) into shared memory, S = K Q^T by tcgen05.mma 128 x 128 x head size;
+//   Q      128 tokens of one head at a time by tensor copies through a ring, as they are (bfloat16);
+//   sums   four warps, S from tensor memory, 1 / l folded into the exponent: one multiply-add, one exponential and one add a
+//          score.  The exponentials bound it (16 a cycle).
+// Nothing is shared between blocks, so a weight does not depend on what else runs.
+constexpr int kWeightThreads = 192;                      // sums 0-3, copies 4, products 5
+template <int HD> struct WeightShape {
+    static constexpr int kStages = HD == 64 ? 3 : 2;
+    static constexpr int kTileBytes = 128 * HD * 2;      // 128 rows of keys, or of queries
+    static constexpr int kOffQ = kTileBytes, kOffY = kOffQ + kStages * kTileBytes, kOffBar = kOffY + 2 * 128 * 4;
+    static constexpr int kSmemBytes = kOffBar + 256;
+};
+
+// Four codes as four bfloat16.
+__device__ __forceinline__ void bf16_of_codes(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    const uint32_t a = e4m3_pair_f16(w), b = e4m3_pair_f16(w >> 16);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    const __nv_bfloat162 p = __floats2bfloat162_rn(x.x, x.y), r = __floats2bfloat162_rn(y.x, y.y);
+    lo = *reinterpret_cast<const uint32_t*>(&p);
+    hi = *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <int HD, bool kTest>
+__global__ void __launch_bounds__(kWeightThreads, 2)
+e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs a, const E4M3Pages kv) {
+    using S = WeightShape<HD>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const int h = blockIdx.y, b = blockIdx.z;
+    const int q_begin = a.cu_seqlens[b];
+    const int q_len = a.cu_seqlens[b + 1] - q_begin;
+    const int slot = a.slots[b];
+    const int start = a.start_pos[b] - (kv.dropped ? kv.dropped[slot] : 0);
+    if (q_len <= 0 || (int)blockIdx.x * 128 >= start + q_len) return;
+    const uint32_t base = smem_addr(smem);
+    if (base & 1023u) {
+        if (threadIdx.x == 0) atomicExch(&g_status, 2);
+        return;
+    }
+    const uint32_t bars = base + S::kOffBar;
+    const uint32_t k_full = bars;
+    auto q_full = [&](int s) { return bars + 8u + 8u * s; };
+    auto q_free = [&](int s) { return bars + 32u + 8u * s; };
+    auto s_full = [&](int s) { return bars + 56u + 8u * s; };
+    auto s_free = [&](int s) { return bars + 72u + 8u * s; };
+    auto y_full = [&](int s) { return bars + 88u + 8u * s; };
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + S::kOffBar + 128);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kOffBar + 136);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int* table = kv.block_table + (size_t)slot * kv.table_stride;
+    if (threadIdx.x == 0) {
+        mbar_init(k_full, 4);
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(q_full(s), 1); mbar_init(q_free(s), 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(s_full(s), 1); mbar_init(s_free(s), 4); mbar_init(y_full(s), 4); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::);
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n"
+                     ::"r"(smem_addr(tmem_holder)), "r"(kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
+    const uint32_t tmem = *tmem_holder;
+    chain_wait();
+    chain_release();
+
+    // the tokens that see any of rows 128 kt .. 128 kt + 127: [t_lo, t_hi), cut into tiles for each head of the group
+    struct Span { int t_lo, t_hi, per_head; };
+    auto span_of = [&](int kt) {
+        Span s;
+        s.t_lo = max(0, kt * 128 - start);
+        s.t_hi = a.window > 0 ? min((long long)q_len, (long long)kt * 128 + 127 + a.window - start) : q_len;
+        s.per_head = s.t_hi > s.t_lo ? (s.t_hi - s.t_lo + 127) / 128 : 0;
+        return s;
+    };
+    int n = 0;                                                   // tiles so far, of all turns
+    if (warp == 4) {
+        if (lane == 0) {
+            bool ok = true;
+            for (int kt = blockIdx.x; kt * 128 < start + q_len && ok; kt += gridDim.x) {
+                const Span sp = span_of(kt);
+                for (int i = 0; i < sp.per_head * a.group; ++i, ++n) {
+                    const int s = n % S::kStages;
+                    ok = mbar_wait<kTest>(q_free(s), (((uint32_t)n / S::kStages) & 1u) ^ 1u, abort_flag);
+                    if (!ok) break;
+                    mbar_expect_tx(q_full(s), S::kTileBytes);
+                    for (int hh = 0; hh < HD / 64; ++hh)
+                        tma_load_2d<kTest>(base + S::kOffQ + s * S::kTileBytes + hh * (128 * 128), &map_q, (h * a.group + i / sp.per_head) * HD + 64 * hh,
+                                           q_begin + sp.t_lo + i % sp.per_head * 128, q_full(s));
+                }
+            }
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            const uint32_t idesc = umma_idesc(128, 128, 0);
+            bool ok = true;
+            for (int kt = blockIdx.x, turn = 0; kt * 128 < start + q_len && ok; kt += gridDim.x) {
+                const Span sp = span_of(kt);
+                if (sp.per_head == 0) continue;                  // (rows that no query sees: no role takes a turn for them)
+                ok = mbar_wait<kTest>(k_full, (uint32_t)turn++ & 1u, abort_flag);
+                for (int i = 0; i < sp.per_head * a.group && ok; ++i, ++n) {
+                    const int s = n % S::kStages, buf = n & 1;
+                    ok = mbar_wait<kTest>(q_full(s), ((uint32_t)n / S::kStages) & 1u, abort_flag) &&
+                         mbar_wait<kTest>(s_free(buf), (((uint32_t)n >> 1) & 1u) ^ 1u, abort_flag);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
+                    const uint32_t qbase = base + S::kOffQ + s * S::kTileBytes;
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        const uint64_t dk = umma_desc(base + (kk / 4) * (128 * 128)) + 2 * (kk % 4);
+                        const uint64_t dq = umma_desc(qbase + (kk / 4) * (128 * 128)) + 2 * (kk % 4);
+                        umma_ss(tmem + 128 * buf, dk, dq, idesc, kk > 0 ? 1u : 0u);
+                    }
+                    umma_commit(q_free(s));
+                    umma_commit(s_full(buf));
+                }
+            }
+        }
+    } else {
+        const unsigned full = 0xffffffffu;
+        const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+        float* y = reinterpret_cast<float*>(smem + S::kOffY);
+        const int r = threadIdx.x;                               // row of the tile; also a column of the next tile's statistics
+        bool ok = true;
+        for (int kt = blockIdx.x; kt * 128 < start + q_len && ok; kt += gridDim.x) {
+            const Span sp = span_of(kt);
+            const int tiles = sp.per_head * a.group;
+            if (tiles == 0) continue;
+            const int row = kt * 128 + r;
+            const bool there = row < start + q_len;
+            // ---- the tile's keys (all products of the turn before are complete: this warp has seen the last one's barrier)
+#pragma unroll
+            for (int m = 0; m < HD / 16; ++m) {
+                const int id = r + 128 * m, key = id / (HD / 16), piece = id % (HD / 16);
+                const int j = kt * 2 + key / 64;
+                uint4 u = make_uint4(0, 0, 0, 0);
+                if (j * kPageTokens < start + q_len)
+                    u = *reinterpret_cast<const uint4*>(kv.k + (size_t)table[j] * kv.k_stride + ((size_t)h * kPageTokens + key % 64) * HD + piece * 16);
+                uint32_t o[8];
+                bf16_of_codes(u.x, o[0], o[1]);
+                bf16_of_codes(u.y, o[2], o[3]);
+                bf16_of_codes(u.z, o[4], o[5]);
+                bf16_of_codes(u.w, o[6], o[7]);
+                const uint32_t at = base + (piece / 4) * (128 * 128) + key * 128;
+                store_shared16(at + (((piece % 4 * 2) ^ (key & 7)) << 4), o[0], o[1], o[2], o[3]);
+                store_shared16(at + (((piece % 4 * 2 + 1) ^ (key & 7)) << 4), o[4], o[5], o[6], o[7]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(k_full);
+            const size_t page = there ? table[row / kPageTokens] : 0;
+            const float f = there ? a.scale * kLog2e * kv.scales[page * kv.scale_stride + h] : 0.f;
+            auto statistic = [&](int i) {                        // of tile i's column r: what takes a score to its probability's exponent
+                const int token = sp.t_lo + i % sp.per_head * 128 + r;
+                if (i >= tiles || token >= sp.t_hi) return 0.f;
+                const float2 st = a.stats[(size_t)(q_begin + token) * a.n_heads + h * a.group + i / sp.per_head];
+                return -(st.x + log2f(st.y));
+            };
+            float mine = statistic(0), total = 0.f;
+            for (int i = 0; i < tiles; ++i, ++n) {
+                const int buf = n & 1;
+                y[128 * buf + r] = mine;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(y_full(buf));
+                mine = statistic(i + 1);
+                ok = __all_sync(full, mbar_wait<kTest>(y_full(buf), ((uint32_t)n >> 1) & 1u, abort_flag) &&
+                                          mbar_wait<kTest>(s_full(buf), ((uint32_t)n >> 1) & 1u, abort_flag));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
+                const int t0 = sp.t_lo + i % sp.per_head * 128;
+                // columns [lo, hi) of the tile are tokens that see this row
+                const int lo = max(row - start - t0, 0);
+                const long long past = min((long long)sp.t_hi, a.window > 0 ? (long long)row + a.window - start : (long long)sp.t_hi) - t0;
+                const int hi = (int)min(past, 128LL);
+                const bool whole = __all_sync(full, lo == 0 && hi == 128);
+                const float* yt = y + 128 * buf;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+                for (int c = 0; c < 128; c += 32) {
+                    uint32_t sv[32];
+                    tmem_ld32(tmem + 128 * buf + lane_off + c, sv);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4*>(yt + c + e);
+                        const float ys[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const float p = fast_exp2(fmaf(__uint_as_float(sv[e + x]), f, ys[x]));
+                            sum[x] += whole || (c + e + x >= lo && c + e + x < hi) ? p : 0.f;
+                        }
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_free(buf));
+                total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+            if (ok && there) kv.weights[page * kv.weight_stride + (size_t)h * kPageTokens + row % kPageTokens] += total;
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
+    __syncthreads();
+    if (warp == 5) {
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols));
+    }
+}
+
+template <int HD, bool kTest>
+int launch_weights(const PromptArgs& a, const E4M3Pages& kv, const CUtensorMap& map_q, int B, int max_kv_len, cudaStream_t stream) {
+    static bool configured = false;
+    if (!configured) {
+        const cudaError_t e = cudaFuncSetAttribute(e4m3_weights_kernel<HD, kTest>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightShape<HD>::kSmemBytes);
+        if (e != cudaSuccess) return (int)e;
+        configured = true;
+    }
+    return launch_chained(e4m3_weights_kernel<HD, kTest>, dim3((max_kv_len + 127) / 128, kv.n_kv, B), dim3(kWeightThreads),
+                          (size_t)WeightShape<HD>::kSmemBytes, stream, map_q, a, kv);
+}
 }  // namespace
 
 GTG_API int gtg_attention_e4m3_tcgen05_status() {
@@ -471,22 +697,33 @@ GTG_API int gtg_attention_e4m3_tcgen05_status() {
     return v;
 }
 
-// Heads of 64 or 128 channels, bfloat16 rows of q and out on 16-byte boundaries.  stats: float2 [N][n_heads] or null.
+// Heads of 64 or 128 channels, bfloat16 rows of q and out on 16-byte boundaries.  weights (or null) gather what the rows get;
+// stats: float2 [N][n_heads] of scratch for that.
 GTG_API int gtg_attention_e4m3_tcgen05(const void* q, int ldq, void* out, int ldo, void* k, long long k_stride, void* v, long long v_stride,
-                                       float* scales, long long scale_stride, const int* block_table, int table_stride, const int* dropped,
-                                       const int* cu_seqlens, const int* slots, const int* start_pos, int B, int max_q_len, int n_heads, int n_kv,
-                                       int hd, float scale, int window, float* stats, cudaStream_t stream) {
-    if (B <= 0 || max_q_len <= 0) return 0;
-    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || window < 0) return kErrBadArgument;
+                                       float* scales, long long scale_stride, float* weights, long long weight_stride, const int* block_table,
+                                       int table_stride, const int* dropped, const int* cu_seqlens, const int* slots, const int* start_pos, int B,
+                                       int max_q_len, int max_kv_len, int N, int n_heads, int n_kv, int hd, float scale, int window, float* stats,
+                                       cudaStream_t stream) {
+    if (B <= 0 || max_q_len <= 0 || N <= 0) return 0;
+    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || window < 0 || max_kv_len <= 0 || (weights && !stats)) return kErrBadArgument;
+    if (n_kv > 65535) return kErrUnsupported;
     if ((hd != 64 && hd != 128) || ldq % 8 || ldo % 8 || (uintptr_t)q % 16 || (uintptr_t)out % 16) return kErrUnsupported;
     if (B > 65535 || ((long long)max_q_len * (n_heads / n_kv) + BQ - 1) / BQ > 65535) return kErrUnsupported;
-    const E4M3Pages kv = {(uint8_t*)k, (uint8_t*)v, k_stride, v_stride, scales, scale_stride, nullptr, 0, block_table, table_stride, dropped, n_kv, hd};
+    const E4M3Pages kv = {(uint8_t*)k, (uint8_t*)v, k_stride, v_stride, scales, scale_stride, weights, weight_stride, block_table, table_stride, dropped, n_kv, hd};
     PromptArgs a = {};
     a.q = (const bf16*)q; a.ldq = ldq; a.out = (bf16*)out; a.ldo = ldo;
     a.cu_seqlens = cu_seqlens; a.slots = slots; a.start_pos = start_pos;
-    a.n_heads = n_heads; a.group = n_heads / n_kv; a.scale = scale; a.window = window; a.stats = (float2*)stats;
-    if (g_test_waits) return hd == 64 ? launch<64, true>(a, kv, B, max_q_len, stream) : launch<128, true>(a, kv, B, max_q_len, stream);
-    return hd == 64 ? launch<64, false>(a, kv, B, max_q_len, stream) : launch<128, false>(a, kv, B, max_q_len, stream);
+    a.n_heads = n_heads; a.group = n_heads / n_kv; a.scale = scale; a.window = window;
+    a.stats = weights ? (float2*)stats : nullptr;
+    const bool test = g_test_waits;
+    const int st = hd == 64 ? (test ? launch<64, true>(a, kv, B, max_q_len, stream) : launch<64, false>(a, kv, B, max_q_len, stream))
+                            : (test ? launch<128, true>(a, kv, B, max_q_len, stream) : launch<128, false>(a, kv, B, max_q_len, stream));
+    if (st != 0 || !weights) return st;
+    CUtensorMap map_q;
+    const int mt = make_map(&map_q, q, N, n_heads * hd, ldq, 128);
+    if (mt != 0) return mt;
+    return hd == 64 ? (test ? launch_weights<64, true>(a, kv, map_q, B, max_kv_len, stream) : launch_weights<64, false>(a, kv, map_q, B, max_kv_len, stream))
+                    : (test ? launch_weights<128, true>(a, kv, map_q, B, max_kv_len, stream) : launch_weights<128, false>(a, kv, map_q, B, max_kv_len, stream));
 }
 
 // For the test of the give-up path: while set, launches take the kTest form, in which the conversion's warps never say that a

@@ -139,9 +139,8 @@ _SIGNATURES = {
     "gtg_attention_e4m3_scratch_floats": ("attention_e4m3", [_I, _I, _I, _I, _I, _I, _I, _I, _L, _I, _I]),
     "gtg_attention_e4m3": ("attention_e4m3", [_I, _P, _I, _P, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P,
                                               _I, _I, _I, _L, _I, _I, _I, _I, _F, _I, _P, _P]),
-    "gtg_row_weights_e4m3": ("attention_e4m3", [_I, _P, _I, _P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _P, _P]),
-    "gtg_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", [_P, _I, _P, _I, _P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I,
-                                                              _F, _I, _P, _P]),
+    "gtg_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", [_P, _I, _P, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P,
+                                                              _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P]),
     "gtg_attention_e4m3_tcgen05_status": ("attention_e4m3_tcgen05", []),
     "gtg_attention_e4m3_tcgen05_test_hooks": ("attention_e4m3_tcgen05", [_I]),
     "gtg_argmax": ("sampling", [_P, _I, _I, _I, _P, _P]),
@@ -1819,14 +1818,9 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
         elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need or scratch.data_ptr() % 16:
             raise KernelError(f"attention_e4m3: scratch needs {need} contiguous floats on a 16-byte boundary")
     if prompt and not (q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16):
-        a = kv.address()
-        stats = scratch.data_ptr() if need else None
-        index = (a[8], a[9], a[10], cu_seqlens.data_ptr(), slots.data_ptr(), start_pos.data_ptr())
-        _check(_fn("gtg_attention_e4m3_tcgen05")(q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *a[:6], *index, B, int(max_q_len), n_heads,
-                                                 kv.n_kv_heads, hd, float(scale), int(window or 0), stats, _stream()), "attention_e4m3")
-        if need:
-            _check(_fn("gtg_row_weights_e4m3")(dt, q.data_ptr(), q.stride(0), a[0], a[1], *a[4:8], *index, B, int(max_kv_len), n_heads, kv.n_kv_heads,
-                                               hd, float(scale), int(window or 0), stats, _stream()), "attention_e4m3: weights")
+        _check(_fn("gtg_attention_e4m3_tcgen05")(q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *kv.address(), cu_seqlens.data_ptr(),
+                                                 slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), N, n_heads, kv.n_kv_heads,
+                                                 hd, float(scale), int(window or 0), scratch.data_ptr() if need else None, _stream()), "attention_e4m3")
         return
     _check(_fn("gtg_attention_e4m3")(dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *kv.address(), cu_seqlens.data_ptr(),
                                      slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), int(total_kv_len), N, n_heads,

@@ -327,6 +327,15 @@ def test_a_plan_the_sequences_have_outgrown(dtype, new):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128, 32])
+@pytest.mark.parametrize("new,window,loose", [(1, 100, True), (6, 700, False), (200, 100, True), (200, 100, False), (150, 1, False)])
+def test_weights_of_a_window(dtype, hd, new, window, loose):
+    """Rows behind the window gather nothing, whether the plan has room for them or not."""
+    worst, worst_w = attention_case(dtype, [1300, 300], [new, 1], 4, 2, hd, window=window, weights=True, loose=loose)
+    assert worst <= 1 and worst_w <= 1, (worst, worst_w)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("new", [1, 90])
 def test_peaked_scores(dtype, new):
     """Scores of hundreds: one row takes all; and queries of zero: every row the same."""
@@ -487,13 +496,15 @@ def test_rows_of_any_stride(hd, new):
 @pytest.mark.parametrize("hd", [64, 128])
 def test_prompt_waits_that_run_out(hd):
     """The tcgen05 form's give-up path: tiles that never arrive.  The kernel returns, says so, and works again afterwards."""
-    p = Pages([300, 70], 2, hd, seed=23)
+    p = Pages([300, 70], 2, hd, seed=23, weights=True)
     q = torch.randn(270, 4 * hd, device=DEV).bfloat16()
+    before = p.weights.clone()
 
     def run():
         out = torch.full_like(q, 7.0)
+        p.weights.copy_(before)
         ops.attention_e4m3(q, out, p.view(), cut([200, 70]), ints(p.slots), ints([100, 0]), 200, 4, hd ** -0.5, max_kv_len=300)
-        return out
+        return torch.cat([out.float().flatten(), p.weights.flatten()])
     want = run()
     assert ops.bounded_wait_failures() == 0
     try:
