@@ -249,6 +249,313 @@ kv_evict_kernel(const E4M3Pages pages, const EvictStrides strides, int* __restri
     }
 }
 
+// ---- the same for heads of a multiple of 16 channels, with the sequence's weights, pages and scales in shared memory.
+// Choosing: the weights are read once; the need-th largest is found eight bits a pass (equal digits of a warp counted by one
+// lane, the digit found by one warp), then every warp places a stretch of the rows by itself, after one exchange of counts.
+// Moving: eight warps move the keys and eight the values, tile by tile of 64 rows from the first that changes, the next
+// tile's codes on their way while one is worked on (what a tile overwrites no later one reads).  A value tile is gathered byte by
+// byte from its source pages' rows in shared memory, since the rows of the cache are innermost there.
+constexpr int kMoveThreads = 512, kMoveWarps = kMoveThreads / 32, kPlaneThreads = kMoveThreads / 2;
+constexpr int kVRow = 80;                  // bytes between channels of a staged value page: 16-byte pieces of 8 channels in 8 places
+template <int HD> struct Move {
+    static constexpr int MINE = (4 * HD + kPlaneThreads - 1) / kPlaneThreads;    // 16-byte pieces of a page a thread has
+    static constexpr int V_BYTES = 2 * HD * kVRow;
+};
+
+__device__ __forceinline__ void plane_sync(int plane) { asm volatile("bar.sync %0, %1;\n" ::"r"(1 + plane), "n"(kPlaneThreads) : "memory"); }
+
+// 16 codes times a power of two each word's pair shares: x[e] is codes 2 e, 2 e + 1, r[e] the factors (in half: clamped to what
+// half holds, beyond which codes are all zero, or all become zero).
+__device__ __forceinline__ __half2 times_ratio(uint32_t two_codes, float a, float b) {
+    const uint32_t h = e4m3_pair_f16(two_codes);
+    const float lo = 5.9604645e-8f, hi = 32768.f;
+    return __hmul2(*reinterpret_cast<const __half2*>(&h), __floats2half2_rn(fminf(fmaxf(a, lo), hi), fminf(fmaxf(b, lo), hi)));
+}
+__device__ __forceinline__ uint32_t pair_codes(__half2 x) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;\n" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&x)));
+    return r;
+}
+// The largest |code| of a word that is not NaN, as a float.
+__device__ __forceinline__ float largest_code(uint32_t w) {
+    w &= 0x7f7f7f7fu;
+    w &= ~__vcmpeq4(w, 0x7f7f7f7fu);
+    const uint32_t a = __vmaxu4(w, w >> 16);
+    return e4m3_value((uint8_t)max(a & 0xffu, (a >> 8) & 0xffu));
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kMoveThreads)
+kv_evict_move_kernel(const E4M3Pages pages, const EvictStrides strides, int* __restrict__ dropped, const int* __restrict__ slots,
+                     const int* __restrict__ lengths, int max_length, int budget, int recent, int* __restrict__ kept_out) {
+    using M = Move<HD>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ int histogram[256];
+    __shared__ int greater[kMoveWarps], equal[kMoveWarps];
+    __shared__ float warp_most[kMoveWarps];
+    __shared__ int choice[2], first_gone;
+    const int h = blockIdx.x, b = blockIdx.y, entry = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int length = lengths[b], slot = slots[b];
+    int* kept_at = kept_out + (((size_t)entry * gridDim.y + b) * pages.n_kv + h) * budget;
+    if (length <= budget || length > max_length) {
+        for (int i = tid; i < budget; i += kMoveThreads) kept_at[i] = i < length && length <= budget ? i : -1;
+        return;
+    }
+    if (h == 0 && entry == 0 && tid == 0 && dropped) dropped[slot] += length - budget;
+    const int max_pages = (max_length + kPageTokens - 1) / kPageTokens, n_pages = (length + kPageTokens - 1) / kPageTokens;
+    unsigned char* staged = smem;                                               // two value pages
+    float* w = reinterpret_cast<float*>(smem + M::V_BYTES);                     // [max_pages * 64]
+    int* kept = reinterpret_cast<int*>(w + max_pages * kPageTokens);            // [budget rounded up to 64]
+    int* page_id = kept + (budget + 63) / 64 * 64;                              // [max_pages]
+    float* page_scale = reinterpret_cast<float*>(page_id + max_pages);          // [2][max_pages]
+    const int* table = pages.block_table + (size_t)slot * pages.table_stride;
+    uint8_t* kc = pages.k + entry * strides.k + (size_t)h * kPageTokens * HD;
+    uint8_t* vc = pages.v + entry * strides.v + (size_t)h * kPageTokens * HD;
+    float* scales = pages.scales + entry * strides.scales + h;
+    float* weights = pages.weights + entry * strides.weights + h * kPageTokens;
+    for (int i = tid; i < n_pages * (kPageTokens / 4); i += kMoveThreads) {
+        const int p = i / (kPageTokens / 4), page = table[p];
+        reinterpret_cast<float4*>(w)[i] = reinterpret_cast<const float4*>(weights + (size_t)page * pages.weight_stride)[i % (kPageTokens / 4)];
+        if (i % (kPageTokens / 4) == 0) page_id[p] = page;
+        if (i % (kPageTokens / 4) < 2) page_scale[i % 2 * max_pages + p] = scales[(size_t)page * pages.scale_stride + i % 2 * pages.n_kv];
+    }
+    if (tid < 256) histogram[tid] = 0;
+    if (tid == 0) first_gone = 0x7fffffff;
+    __syncthreads();
+    const int n = length - recent, need = budget - recent;
+
+    // ---- the need-th largest of the first n weights
+    uint32_t threshold = 0;
+    int left = need;
+    for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
+        const uint32_t above = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
+        for (int i0 = warp * 32; i0 < n; i0 += kMoveThreads) {
+            const uint32_t u = i0 + lane < n ? ordered_bits(w[i0 + lane]) : 0u;
+            const bool counts = i0 + lane < n && (u & above) == (threshold & above);
+            const int digit = counts ? (int)((u >> shift) & 255u) : 256;
+            const unsigned like = __match_any_sync(0xffffffffu, digit);
+            if (counts && lane == __ffs(like) - 1) atomicAdd(&histogram[digit], __popc(like));
+        }
+        __syncthreads();
+        if (warp == 0) {                                                        // lane l: digits 255 - 8 l down to 248 - 8 l
+            int mine[8], sum = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum += mine[e] = histogram[255 - 8 * lane - e];
+            int incl = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += up;
+            }
+            const unsigned enough = __ballot_sync(0xffffffffu, incl >= left);
+            if (lane == __ffs(enough) - 1) {
+                int more = incl - sum, digit = 255 - 8 * lane;
+                bool found = false;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    found = found || more + mine[e] >= left;
+                    if (!found) { more += mine[e]; --digit; }
+                }
+                choice[0] = digit;
+                choice[1] = more;
+            }
+        }
+        __syncthreads();
+        threshold |= (uint32_t)choice[0] << shift;
+        left -= choice[1];
+        if (tid < 256) histogram[tid] = 0;
+        __syncthreads();
+    }
+    // ---- the rows that stay, in order
+    {
+        const int stretch = (n + kMoveThreads - 1) / kMoveThreads * 32;         // of a warp
+        const int begin = min(n, warp * stretch), end = min(n, begin + stretch);
+        int more = 0, same = 0;
+        for (int i0 = begin; i0 < end; i0 += 32) {
+            const uint32_t u = i0 + lane < end ? ordered_bits(w[i0 + lane]) : 0u;
+            more += __popc(__ballot_sync(0xffffffffu, i0 + lane < end && u > threshold));
+            same += __popc(__ballot_sync(0xffffffffu, i0 + lane < end && u == threshold));
+        }
+        if (lane == 0) { greater[warp] = more; equal[warp] = same; }
+        __syncthreads();
+        int place = 0, rank = 0;
+        for (int x = 0; x < warp; ++x) { place += greater[x]; rank += equal[x]; }
+        const int taken = need > 0 ? left : 0;                                  // of those equal to the threshold
+        place += min(taken, rank);
+        int gone = 0x7fffffff;
+        for (int i0 = begin; i0 < end; i0 += 32) {
+            const uint32_t u = i0 + lane < end ? ordered_bits(w[i0 + lane]) : 0u;
+            const bool even = i0 + lane < end && u == threshold;
+            const unsigned evens = __ballot_sync(0xffffffffu, even), below = (1u << lane) - 1u;
+            const bool stays = need > 0 && i0 + lane < end && (u > threshold || (even && rank + __popc(evens & below) < taken));
+            const unsigned all = __ballot_sync(0xffffffffu, stays);
+            if (stays) kept[place + __popc(all & below)] = i0 + lane;
+            if (gone == 0x7fffffff) {
+                const unsigned lost = __ballot_sync(0xffffffffu, i0 + lane < end && !stays);
+                if (lost) gone = i0 + __ffs(lost) - 1;
+            }
+            place += __popc(all);
+            rank += __popc(evens);
+        }
+        if (lane == 0 && gone != 0x7fffffff) atomicMin(&first_gone, gone);
+        for (int i = tid; i < recent; i += kMoveThreads) kept[need + i] = n + i;
+    }
+    __syncthreads();
+    for (int i = tid; i < budget; i += kMoveThreads) kept_at[i] = kept[i];
+    const int tiles = (budget + kPageTokens - 1) / kPageTokens;
+    const int first_tile = first_gone < budget ? first_gone / kPageTokens : tiles;        // all rows before it stay where they are
+    for (int r = first_tile * kPageTokens + tid; r < budget; r += kMoveThreads)
+        weights[(size_t)page_id[r / kPageTokens] * pages.weight_stride + r % kPageTokens] = w[kept[r]];
+
+    // ---- tiles to the front
+    const int plane = tid / kPlaneThreads, t = tid % kPlaneThreads;
+    const float* old_scale = page_scale + plane * max_pages;
+    uint4 ahead[2][M::MINE];
+    auto rows_of = [&](int to) { return min(kPageTokens, budget - to * kPageTokens); };
+    // keys: the tile's rows; values: two pages from source page `p` on
+    auto fetch = [&](int to, int p) {
+#pragma unroll
+        for (int m = 0; m < M::MINE; ++m) {
+            const int id = t + kPlaneThreads * m;
+            if (plane == 0) {
+                const int r = id / (HD / 16);
+                if (r < rows_of(to)) {
+                    const int src = kept[to * kPageTokens + r];
+                    ahead[0][m] = *reinterpret_cast<const uint4*>(kc + (size_t)page_id[src / kPageTokens] * pages.k_stride + src % kPageTokens * HD + id % (HD / 16) * 16);
+                }
+            } else if (id < 4 * HD) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    if (p + x < n_pages) ahead[x][m] = *reinterpret_cast<const uint4*>(vc + (size_t)page_id[p + x] * pages.v_stride + id * 16);
+            }
+        }
+    };
+    auto first_page = [&](int to) { return kept[to * kPageTokens] / kPageTokens; };
+    auto block_most = [&](float most) {
+        most = warp_max(most);
+        if (lane == 0) warp_most[warp] = most;
+        plane_sync(plane);
+        most = 0.f;
+#pragma unroll
+        for (int x = 0; x < kMoveWarps / 2; ++x) most = fmaxf(most, warp_most[plane * (kMoveWarps / 2) + x]);
+        return most;
+    };
+    if (first_tile < tiles) fetch(first_tile, first_page(first_tile));
+    for (int to = first_tile; to < tiles; ++to) {
+        const int rows = rows_of(to);
+        const int* source = kept + to * kPageTokens;
+        uint4 mine[M::MINE];
+        float most = 0.f;
+        if (plane == 0) {
+#pragma unroll
+            for (int m = 0; m < M::MINE; ++m) {
+                const int r = (t + kPlaneThreads * m) / (HD / 16);
+                mine[m] = ahead[0][m];
+                if (r < rows) {
+                    const float c = fmaxf(fmaxf(largest_code(mine[m].x), largest_code(mine[m].y)), fmaxf(largest_code(mine[m].z), largest_code(mine[m].w)));
+                    most = fmaxf(most, c * old_scale[source[r] / kPageTokens]);
+                }
+            }
+        } else {
+            const int last = source[rows - 1] / kPageTokens;
+            int p = source[0] / kPageTokens;
+#pragma unroll
+            for (int m = 0; m < M::MINE; ++m) mine[m] = make_uint4(0, 0, 0, 0);
+            for (;; p += 2) {
+                plane_sync(plane);                                              // the pages before have been read
+#pragma unroll
+                for (int m = 0; m < M::MINE; ++m) {
+                    const int id = t + kPlaneThreads * m;
+                    if (id < 4 * HD) {
+                        *reinterpret_cast<uint4*>(staged + id / 4 * kVRow + id % 4 * 16) = ahead[0][m];
+                        *reinterpret_cast<uint4*>(staged + (HD + id / 4) * kVRow + id % 4 * 16) = ahead[1][m];
+                    }
+                }
+                plane_sync(plane);
+                if (p + 2 <= last) fetch(to, p + 2);
+#pragma unroll
+                for (int m = 0; m < M::MINE; ++m) {
+                    const int id = t + kPlaneThreads * m;                       // channel id / 4, rows 16 (id % 4) ..
+                    if (id >= 4 * HD) continue;
+                    uint32_t word[4] = {mine[m].x, mine[m].y, mine[m].z, mine[m].w};
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int r = id % 4 * 16 + e;
+                        if (r >= rows) continue;
+                        const int src = source[r], x = src / kPageTokens - p;
+                        if (x < 0 || x > 1) continue;
+                        const uint32_t c = staged[(x * HD + id / 4) * kVRow + src % kPageTokens];
+                        word[e >> 2] |= c << (8 * (e & 3));
+                        const uint32_t size = c & 0x7fu;
+                        most = fmaxf(most, e4m3_value((uint8_t)(size == 0x7fu ? 0u : size)) * old_scale[p + x]);
+                    }
+                    mine[m] = make_uint4(word[0], word[1], word[2], word[3]);
+                }
+                if (p + 2 > last) break;
+            }
+        }
+        const float scale = e4m3_needed_scale(block_most(most)), inverse = pow2_inverse(scale);
+        if (to + 1 < tiles) fetch(to + 1, first_page(to + 1));
+        const size_t page = page_id[to];
+#pragma unroll
+        for (int m = 0; m < M::MINE; ++m) {
+            const int id = t + kPlaneThreads * m;
+            uint32_t word[4] = {mine[m].x, mine[m].y, mine[m].z, mine[m].w};
+            if (plane == 0) {
+                const int r = id / (HD / 16);
+                if (r >= rows) continue;
+                const float ratio = old_scale[source[r] / kPageTokens] * inverse;
+                if (ratio != 1.f) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        word[x] = pair_codes(times_ratio(word[x], ratio, ratio)) | pair_codes(times_ratio(word[x] >> 16, ratio, ratio)) << 16;
+                }
+                *reinterpret_cast<uint4*>(kc + page * pages.k_stride + r * HD + id % (HD / 16) * 16) = make_uint4(word[0], word[1], word[2], word[3]);
+            } else if (id < 4 * HD) {
+                const int r0 = id % 4 * 16;
+                if (r0 >= rows) continue;
+                const float first = old_scale[source[r0] / kPageTokens] * inverse, last = old_scale[source[min(r0 + 15, rows - 1)] / kPageTokens] * inverse;
+                // (a piece whose rows come from two pages or fewer has the scales of its first and last row)
+                const bool two = source[min(r0 + 15, rows - 1)] / kPageTokens - source[r0] / kPageTokens <= 1;
+                if (!(two && first == 1.f && last == 1.f)) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        float f[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f[e] = old_scale[source[min(r0 + 4 * x + e, rows - 1)] / kPageTokens] * inverse;
+                        word[x] = pair_codes(times_ratio(word[x], f[0], f[1])) | pair_codes(times_ratio(word[x] >> 16, f[2], f[3])) << 16;
+                    }
+                }
+                uint8_t* at = vc + page * pages.v_stride + id / 4 * kPageTokens + r0;
+                if (r0 + 16 <= rows) *reinterpret_cast<uint4*>(at) = make_uint4(word[0], word[1], word[2], word[3]);
+                else
+                    for (int e = 0; r0 + e < rows; ++e) at[e] = (uint8_t)(word[e >> 2] >> (8 * (e & 3)));
+            }
+        }
+        if (t == 0) scales[page * pages.scale_stride + plane * pages.n_kv] = scale;
+        plane_sync(plane);                                                      // warp_most and the staged pages are free again
+    }
+}
+
+size_t move_bytes(int hd, int max_length, int budget) {
+    const size_t max_pages = (max_length + kPageTokens - 1) / kPageTokens;
+    return 2 * (size_t)hd * kVRow + max_pages * kPageTokens * 4 + (size_t)(budget + 63) / 64 * 64 * 4 + max_pages * 12;
+}
+template <int HD>
+int launch_move(const E4M3Pages& pages, const EvictStrides& strides, int* dropped, const int* slots, const int* lengths, int max_length, int budget,
+                int recent, int* kept, int B, int entries, cudaStream_t stream) {
+    const size_t smem = move_bytes(HD, max_length, budget);
+    static size_t configured = 48 * 1024 - 4096;
+    if (smem > configured) {
+        const cudaError_t e = cudaFuncSetAttribute(kv_evict_move_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return (int)e;
+        configured = smem;
+    }
+    kv_evict_move_kernel<HD><<<dim3(pages.n_kv, B, entries), kMoveThreads, smem, stream>>>(pages, strides, dropped, slots, lengths, max_length, budget,
+                                                                                          recent, kept);
+    return launch_status();
+}
+
 template <typename T>
 int launch_store(const StoreInput<T>& in, const E4M3Pages& kv, const int* cu_seqlens, const int* slots, const int* start_pos,
                  int B, int max_q_len, int N, int store, void* q_out, int ldq, cudaStream_t stream) {
@@ -286,7 +593,7 @@ GTG_API int gtg_kv_store_e4m3(int dtype, const void* qkv, int ld, const float* c
 GTG_API int gtg_kv_evict_e4m3(int entries, void* k, long long k_entry, long long k_stride, void* v, long long v_entry, long long v_stride,
                               float* scales, long long scale_entry, long long scale_stride, float* weights, long long weight_entry,
                               long long weight_stride, const int* block_table, int table_stride, int* dropped, int n_kv, int hd, const int* slots,
-                              const int* lengths, int B, int budget, int recent, int* kept, cudaStream_t stream) {
+                              const int* lengths, int B, int max_length, int budget, int recent, int* kept, cudaStream_t stream) {
     if (B <= 0 || entries <= 0) return 0;
     if (budget <= 0 || recent < 0 || recent > budget || n_kv <= 0 || hd <= 0 || !weights || !kept) return kErrBadArgument;
     if (B > 65535 || entries > 65535) return kErrUnsupported;
@@ -295,6 +602,12 @@ GTG_API int gtg_kv_evict_e4m3(int entries, void* k, long long k_entry, long long
     const E4M3Pages pages = {(uint8_t*)k, (uint8_t*)v, k_stride, v_stride, scales, scale_stride, weights, weight_stride, block_table, table_stride,
                              nullptr, n_kv, hd};
     const EvictStrides strides = {k_entry, v_entry, scale_entry, weight_entry};
+    // sequences whose weights fit in shared memory, heads of a multiple of 16 channels; else the general form
+    if (hd % 16 == 0 && hd <= 128 && move_bytes(hd, max_length, budget) <= 200 * 1024) {
+#define GTG_MOVE(HD) case HD: return launch_move<HD>(pages, strides, dropped, slots, lengths, max_length, budget, recent, kept, B, entries, stream);
+        switch (hd) { GTG_MOVE(16) GTG_MOVE(32) GTG_MOVE(48) GTG_MOVE(64) GTG_MOVE(80) GTG_MOVE(96) GTG_MOVE(112) GTG_MOVE(128) }
+#undef GTG_MOVE
+    }
     kv_evict_kernel<<<dim3(n_kv, B, entries), kEvictThreads, smem, stream>>>(pages, strides, dropped, slots, lengths, budget, recent, kept);
     return launch_status();
 }
