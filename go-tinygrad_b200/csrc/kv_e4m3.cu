@@ -556,11 +556,269 @@ int launch_move(const E4M3Pages& pages, const EvictStrides& strides, int* droppe
     return launch_status();
 }
 
+// ---- storing, for heads of a multiple of 16 channels whose rows lie on 16-byte boundaries.  A block of the cache is read once,
+// 16 channels a thread (two runs of 8 that the rotation pairs), kept in registers while the block's largest value is
+// found, and written in pieces of 16 or 8 bytes; values go through shared memory, since their rows are innermost in the cache.
+// Query rows are rotated by blocks of their own, the angles of 16 channels read once for several heads.
+constexpr int kRowsThreads = 256;
+
+__device__ __forceinline__ void load8(const bf16* p, float* x) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { x[2 * e] = __uint_as_float(w[e] << 16); x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+}
+__device__ __forceinline__ void load8(const float* p, float* x) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void store8(bf16* p, const float* x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store8(float* p, const float* x) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+// Unit u of a head: two runs of 8 channels, starting at *a and *b.  Half-split pairs: run u and its partner; else neighbours.
+__device__ __forceinline__ void runs_of(int u, int rot, int interleaved, int* a, int* b) {
+    if (!interleaved && u < rot / 16) { *a = 8 * u; *b = *a + rot / 2; }
+    else { *a = 16 * u; *b = *a + 8; }
+}
+// What turns a unit: for half-split pairs 8 angles, for neighbours 4 and 4; (1, 0) where nothing turns.
+__device__ __forceinline__ void angles_of(int u, int rot, int interleaved, const float2* __restrict__ cs, float2* t) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int i = 8 * u + e;                                                // also of the pair (16 u + 2 e, 16 u + 2 e + 1)
+        t[e] = 2 * i < rot ? cs[i] : make_float2(1.f, 0.f);
+    }
+}
+__device__ __forceinline__ void turn(float& x, float& y, float2 c) {
+    const float a = __fsub_rn(__fmul_rn(x, c.x), __fmul_rn(y, c.y));
+    y = __fadd_rn(__fmul_rn(x, c.y), __fmul_rn(y, c.x));
+    x = a;
+}
+__device__ __forceinline__ void turn_unit(int u, int rot, int interleaved, const float2* t, float* x) {   // x: run a, run b
+    if (interleaved) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (16 * u + 2 * e < rot) turn(x[2 * e], x[2 * e + 1], t[e]);
+    } else if (u < rot / 16) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) turn(x[e], x[8 + e], t[e]);
+    }
+}
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+    return e4m3_code(a) | (uint32_t)e4m3_code(b) << 8 | (uint32_t)e4m3_code(c) << 16 | (uint32_t)e4m3_code(d) << 24;
+}
+// A word's bytes below `n` times a power of two; the others as they are.
+__device__ __forceinline__ uint32_t rescaled_bytes(uint32_t w, int n, float ratio) {
+    if (n <= 0) return w;
+    const uint32_t mask = n >= 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
+    const uint32_t r = pair_codes(times_ratio(w, ratio, ratio)) | pair_codes(times_ratio(w >> 16, ratio, ratio)) << 16;
+    return (r & mask) | (w & ~mask);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kRowsThreads)
+kv_store_rows_kernel(const StoreInput<T> in, const E4M3Pages kv, const int* __restrict__ cu_seqlens, const int* __restrict__ slots,
+                     const int* __restrict__ start_pos, int blocks_per_seq, int blocks_kv, int N, int heads_each, T* __restrict__ q_out, int ldq) {
+    constexpr int UNITS = HD / 16;                                              // of a row
+    constexpr int K_MINE = (64 * UNITS + kRowsThreads - 1) / kRowsThreads;
+    constexpr int V_RUNS = HD / 8, V_MINE = (16 * V_RUNS + kRowsThreads - 1) / kRowsThreads;
+    __shared__ float warp_most[kRowsThreads / 32];
+    __shared__ uint32_t turned[HD * 16];                                        // a value block: [channel][16 words of 4 rows]
+    chain_wait();
+    chain_release();                  // only now: what comes next may read older pages at once (all before this kernel is complete)
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x >= blocks_kv) {
+        // ---- queries: a thread a unit of a token, heads_each heads
+        const int id = ((int)blockIdx.x - blocks_kv) * kRowsThreads + tid;
+        const int groups = (in.n_heads + heads_each - 1) / heads_each;
+        const int u = id % UNITS, rest = id / UNITS, group = rest % groups, token = rest / groups;
+        if (token >= N) return;
+        float2 t[8];
+        angles_of(u, in.rot, in.interleaved, in.cos_sin + (size_t)token * (in.rot >> 1), t);
+        int a, b;
+        runs_of(u, in.rot, in.interleaved, &a, &b);
+        const int h1 = min(in.n_heads, (group + 1) * heads_each);
+#pragma unroll 4
+        for (int h = group * heads_each; h < h1; ++h) {
+            float x[16];
+            const T* row = in.qkv + (size_t)token * in.ld + h * HD;
+            load8(row + a, x);
+            load8(row + b, x + 8);
+            turn_unit(u, in.rot, in.interleaved, t, x);
+            T* to = q_out + (size_t)token * ldq + h * HD;
+            store8(to + a, x);
+            store8(to + b, x + 8);
+        }
+        return;
+    }
+    int id = blockIdx.x;
+    const int j = id % blocks_per_seq; id /= blocks_per_seq;
+    const int plane = id & 1; id >>= 1;
+    const int h = id % kv.n_kv, b = id / kv.n_kv;
+    const int first = cu_seqlens[b], n_new = cu_seqlens[b + 1] - first;
+    if (n_new <= 0) return;
+    const int slot = slots[b];
+    const int start = start_pos[b] - (kv.dropped ? kv.dropped[slot] : 0);
+    const int block = start / kPageTokens + j;
+    const int lo = max(start - block * kPageTokens, 0), hi = min(start + n_new - block * kPageTokens, kPageTokens);
+    if (hi <= lo) return;                                                       // rows [lo, hi) of the block are new
+    const size_t page = kv.block_table[(size_t)slot * kv.table_stride + block];
+    const int token0 = first + block * kPageTokens - start;                     // of row 0
+    const T* column = in.qkv + (in.n_heads + h) * HD + (plane ? in.v_offset : 0);
+    float x[K_MINE > 2 * V_MINE ? K_MINE : 2 * V_MINE][16];                     // keys: a unit each; values: rows 0, 1 and 2, 3 of a run
+    float most = 0.f;
+    if (plane == 0) {
+#pragma unroll
+        for (int m = 0; m < K_MINE; ++m) {
+            const int unit = tid + kRowsThreads * m, r = lo + unit / UNITS, u = unit % UNITS;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[m][e] = 0.f;
+            if (r < hi) {
+                int a, c;
+                runs_of(u, in.rot, in.interleaved, &a, &c);
+                const T* row = column + (size_t)(token0 + r) * in.ld;
+                load8(row + a, x[m]);
+                load8(row + c, x[m] + 8);
+                float2 t[8];
+                angles_of(u, in.rot, in.interleaved, in.cos_sin + (size_t)(token0 + r) * (in.rot >> 1), t);
+                turn_unit(u, in.rot, in.interleaved, t, x[m]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int m = 0; m < V_MINE; ++m) {
+            const int unit = tid + kRowsThreads * m, r0 = unit / V_RUNS * 4, run = unit % V_RUNS;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float* at = x[2 * m + i / 2] + i % 2 * 8;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) at[e] = 0.f;
+                if (r0 + i >= lo && r0 + i < hi) load8(column + (size_t)(token0 + r0 + i) * in.ld + 8 * run, at);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < (K_MINE > 2 * V_MINE ? K_MINE : 2 * V_MINE); ++m)
+        if (m < (plane ? 2 * V_MINE : K_MINE)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) most = fmaxf(most, finite_f32(x[m][e]) ? fabsf(x[m][e]) : 0.f);
+        }
+    most = warp_max(most);
+    if ((tid & 31) == 0) warp_most[tid >> 5] = most;
+    float* scale_at = kv.scales + page * kv.scale_stride + plane * kv.n_kv + h;
+    const float before = lo > 0 ? *scale_at : 0.f;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kRowsThreads / 32; ++w) most = fmaxf(most, warp_most[w]);
+    float scale = e4m3_needed_scale(most);
+    uint8_t* codes = plane ? kv.v + page * kv.v_stride + (size_t)h * kPageTokens * HD : kv.k + page * kv.k_stride + (size_t)h * kPageTokens * HD;
+    if (lo > 0) {
+        if (before >= scale) {
+            scale = before;
+        } else {                                                                // older rows' codes under the larger scale
+            const float ratio = before * pow2_inverse(scale);
+            if (plane == 0) {
+                for (int i = tid; i < lo * UNITS; i += kRowsThreads) {
+                    uint4* at = reinterpret_cast<uint4*>(codes) + i;
+                    const uint4 u = *at;
+                    *at = make_uint4(rescaled_bytes(u.x, 4, ratio), rescaled_bytes(u.y, 4, ratio), rescaled_bytes(u.z, 4, ratio), rescaled_bytes(u.w, 4, ratio));
+                }
+            } else {
+                for (int i = tid; i < 4 * HD; i += kRowsThreads) {
+                    const int n = lo - i % 4 * 16;                              // older rows of this piece
+                    if (n <= 0) continue;
+                    uint4* at = reinterpret_cast<uint4*>(codes) + i;
+                    const uint4 u = *at;
+                    *at = make_uint4(rescaled_bytes(u.x, n, ratio), rescaled_bytes(u.y, n - 4, ratio), rescaled_bytes(u.z, n - 8, ratio),
+                                     rescaled_bytes(u.w, n - 12, ratio));
+                }
+                __syncthreads();                                                // pieces that hold older and new rows are written again
+            }
+        }
+    }
+    const float inverse = pow2_inverse(scale);
+    if (plane == 0) {
+#pragma unroll
+        for (int m = 0; m < K_MINE; ++m) {
+            const int unit = tid + kRowsThreads * m, r = lo + unit / UNITS, u = unit % UNITS;
+            if (r >= hi) continue;
+            int a, c;
+            runs_of(u, in.rot, in.interleaved, &a, &c);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[m][e] *= inverse;
+            *reinterpret_cast<uint2*>(codes + r * HD + a) = make_uint2(codes4(x[m][0], x[m][1], x[m][2], x[m][3]), codes4(x[m][4], x[m][5], x[m][6], x[m][7]));
+            *reinterpret_cast<uint2*>(codes + r * HD + c) = make_uint2(codes4(x[m][8], x[m][9], x[m][10], x[m][11]), codes4(x[m][12], x[m][13], x[m][14], x[m][15]));
+        }
+        if (kv.weights)
+            for (int r = lo + tid; r < hi; r += kRowsThreads) kv.weights[page * kv.weight_stride + h * kPageTokens + r] = 0.f;
+    } else {
+#pragma unroll
+        for (int m = 0; m < V_MINE; ++m) {
+            const int unit = tid + kRowsThreads * m, r4 = unit / V_RUNS, run = unit % V_RUNS;
+            if (r4 >= 16) continue;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)                                         // (the place is turned so that lanes of a run fall into different banks)
+                turned[(8 * run + e) * 16 + (r4 ^ (run & 15))] = codes4(x[2 * m][e] * inverse, x[2 * m][8 + e] * inverse, x[2 * m + 1][e] * inverse, x[2 * m + 1][8 + e] * inverse);
+        }
+        __syncthreads();
+        for (int i = tid; i < 4 * HD; i += kRowsThreads) {
+            const int channel = i / 4, r0 = i % 4 * 16;
+            if (r0 >= hi || r0 + 16 <= lo) continue;
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = turned[channel * 16 + ((i % 4 * 4 + e) ^ ((channel >> 3) & 15))];
+            uint8_t* at = codes + channel * kPageTokens + r0;
+            if (r0 >= lo && r0 + 16 <= hi) {
+                *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (r0 + e >= lo && r0 + e < hi) at[e] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+            }
+        }
+    }
+    if (tid == 0) *scale_at = scale;                                            // (every thread has read it before the first barrier)
+}
+
+template <typename T>
+bool rows_take(const StoreInput<T>& in, const void* q_out, int ldq) {
+    constexpr int per16 = 16 / sizeof(T);
+    return in.hd % 16 == 0 && in.hd <= 128 && (in.interleaved || in.rot % 16 == 0) && (in.cos_sin == nullptr || in.rot > 0) && in.ld % per16 == 0 &&
+           (uintptr_t)in.qkv % 16 == 0 && (!q_out || (ldq % per16 == 0 && (uintptr_t)q_out % 16 == 0));
+}
+template <typename T, int HD>
+int launch_store_rows(const StoreInput<T>& in, const E4M3Pages& kv, const int* cu_seqlens, const int* slots, const int* start_pos, int per_seq,
+                      long long blocks_kv, int N, void* q_out, int ldq, cudaStream_t stream) {
+    // heads a thread turns with the same angles: four (31.5 us at 4,696 tokens of 32 + 16 heads of 128; one: 33.9, eight: 32.9)
+    // once that leaves a thousand threads a multiprocessor
+    const int heads_each = (long long)N * (HD / 16) * in.n_heads >= 4LL * 148 * 1024 ? 4 : 1;
+    const long long threads = q_out ? (long long)N * ((in.n_heads + heads_each - 1) / heads_each) * (HD / 16) : 0;
+    const long long blocks = blocks_kv + (threads + kRowsThreads - 1) / kRowsThreads;
+    if (blocks <= 0) return 0;
+    if (blocks > 0x7fffffffLL || threads > 0x7fffffffLL) return kErrUnsupported;
+    return launch_chained(kv_store_rows_kernel<T, HD>, dim3((unsigned)blocks), dim3(kRowsThreads), 0, stream, in, kv, cu_seqlens, slots, start_pos,
+                          per_seq, (int)blocks_kv, N, heads_each, (T*)q_out, ldq);
+}
+
 template <typename T>
 int launch_store(const StoreInput<T>& in, const E4M3Pages& kv, const int* cu_seqlens, const int* slots, const int* start_pos,
                  int B, int max_q_len, int N, int store, void* q_out, int ldq, cudaStream_t stream) {
     const int per_seq = (max_q_len + kPageTokens - 2) / kPageTokens + 1;
     const long long blocks_kv = store ? (long long)B * kv.n_kv * 2 * per_seq : 0;
+    if (rows_take(in, q_out, ldq) && blocks_kv < 0x7fffffffLL) {
+#define GTG_ROWS(HD) case HD: return launch_store_rows<T, HD>(in, kv, cu_seqlens, slots, start_pos, per_seq, blocks_kv, N, q_out, ldq, stream);
+        switch (in.hd) { GTG_ROWS(16) GTG_ROWS(32) GTG_ROWS(48) GTG_ROWS(64) GTG_ROWS(80) GTG_ROWS(96) GTG_ROWS(112) GTG_ROWS(128) }
+#undef GTG_ROWS
+    }
     const long long blocks = blocks_kv + (q_out ? N : 0);
     if (blocks <= 0) return 0;
     if (blocks > 0x7fffffffLL) return kErrUnsupported;
