@@ -4,8 +4,8 @@
 // One block per (128 query rows, key/value head, sequence).  A query row is a (token, head of the group) pair, heads
 // innermost, so that the heads that share keys share their pages too and a short run of queries still fills a tile.  Per step of BK
 // rows of the cache (two pages for heads of 64 channels, one for 128):
-//   codes -> half   three warps read the step's codes from memory (16 bytes a lane, a step ahead of their use), turn them into
-//                   halves, which is exact, and leave them in shared memory as swizzled tiles: keys [row][channel], values
+//   codes -> half   three warps fetch the step's codes (asynchronous copies, two or three steps ahead), turn them into halves,
+//                   which is exact, and leave them in shared memory as swizzled tiles: keys [row][channel], values
 //                   [channel][row], both K-major as the cache has them;
 //   S  = Q K^T      tcgen05.mma 128 x BK x head size, operands in shared memory, S in tensor memory; queries are scaled by a
 //                   power of two a row to fill half's range, so that rounding bfloat16 to half loses nothing that counts;
@@ -34,9 +34,12 @@ constexpr int kSoftmaxRegs = 168, kOtherRegs = 88;
 template <int HD> struct Shape {
     static constexpr int kPages = HD == 64 ? 2 : 1;      // of a step
     static constexpr int BK = 64 * kPages;
-    static constexpr int kStages = 2;
+    static constexpr int kStages = 2;                    // key tiles; one value tile: it is wanted a softmax later
+    static constexpr int kRaw = HD == 64 ? 3 : 2;        // steps of codes on their way
     static constexpr int kQBytes = BQ * HD * 2, kTileBytes = BK * HD * 2;
-    static constexpr int kOffK = kQBytes, kOffV = kOffK + kStages * kTileBytes, kOffBar = kOffV + kStages * kTileBytes;
+    static constexpr int kOffK = kQBytes, kOffV = kOffK + kStages * kTileBytes, kOffRaw = kOffV + kTileBytes;
+    static constexpr int kRawBytes = BK * HD;            // a step's codes of keys (or of values)
+    static constexpr int kOffBar = kOffRaw + kRaw * 2 * kRawBytes;
     static constexpr int kSmemBytes = kOffBar + 256;
     static constexpr int kColO = BK, kColP = BK + HD;
     static_assert(BK + HD + BK / 2 <= kTmemCols, "tensor memory");
@@ -63,6 +66,15 @@ struct PromptArgs {
 
 __device__ __forceinline__ void store_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 load_shared16(uint32_t at) {
+    uint4 u;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at) : "memory");
+    return u;
+}
+// 16-byte copy global -> shared; `bytes` = 0 fills the destination with zeros.
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 // 16 codes as 16 halves: two chunks of a swizzled row.
 __device__ __forceinline__ void store_halves(uint32_t row_at, int chunk, int swizzle, const uint4& u) {
@@ -93,8 +105,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     const uint32_t q_full = bars, s_full = bars + 8, s_free = bars + 16, p_full = bars + 24, pv_done = bars + 32;
     auto k_full = [&](int s) { return bars + 40u + 8u * s; };
     auto k_free = [&](int s) { return bars + 56u + 8u * s; };
-    auto v_full = [&](int s) { return bars + 72u + 8u * s; };
-    auto v_free = [&](int s) { return bars + 88u + 8u * s; };
+    const uint32_t v_full = bars + 72, v_free = bars + 80;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + S::kOffBar + 128);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kOffBar + 136);
     volatile int* odd_flag = reinterpret_cast<volatile int*>(smem + S::kOffBar + 140);   // a NaN code in a page not all rows see whole
@@ -120,9 +131,9 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
         for (int s = 0; s < S::kStages; ++s) {
             mbar_init(k_full(s), kConvWarps);
             mbar_init(k_free(s), 1);
-            mbar_init(v_full(s), kConvWarps);
-            mbar_init(v_free(s), 1);
         }
+        mbar_init(v_full, kConvWarps);
+        mbar_init(v_free, 1);
         *abort_flag = 0;
         *odd_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::);
@@ -145,53 +156,68 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             // ------------------------------------------------------------ codes to halves
             const int t = threadIdx.x - 5 * 32;
             const int total = start + q_len;                     // rows that exist after this step
-            uint4 k[S::kMine], v[S::kMine];
             auto page_of = [&](int i, int pg) { const int j = j_lo + S::kPages * i + pg; return j <= j_hi ? j : -1; };
-            auto fetch = [&](int i, bool values, uint4* u) {
+            // The codes come by asynchronous copies, kRaw steps ahead, each 16-byte piece to a place that only the lane that will
+            // convert it reads: nothing is waited for but a lane's own copies.  Page numbers are read a step earlier still.
+            int page_k[S::kPages], page_v[S::kPages];            // of the next step to be asked for: page or -1
+            auto look_up = [&](int i, int* page) {
 #pragma unroll
-                for (int m = 0; m < S::kMine; ++m) {
-                    const int id = t + 32 * kConvWarps * m;
-                    u[m] = make_uint4(0, 0, 0, 0);               // a page behind the last: zeros, which no row sees
-                    const int pg = id / (S::kPieces / S::kPages), in = id % (S::kPieces / S::kPages);
-                    const int j = id < S::kPieces ? page_of(i, pg) : -1;
-                    if (j >= 0) {
-                        const size_t page = table[j];
-                        const uint8_t* at = values ? kv.v + page * kv.v_stride : kv.k + page * kv.k_stride;
-                        u[m] = *reinterpret_cast<const uint4*>(at + (size_t)h * kPageTokens * HD + in * 16);
-                    }
+                for (int pg = 0; pg < S::kPages; ++pg) {
+                    const int j = page_of(i, pg);
+                    page[pg] = j >= 0 ? table[j] : -1;
                 }
             };
-            fetch(0, false, k);
-            fetch(0, true, v);
+            auto slot_of = [&](int i, int values, int id) { return base + S::kOffRaw + ((i % S::kRaw) * 2 + values) * S::kRawBytes + id * 16; };
+            auto ask = [&](int i, int values, int* page) {
+                if (i < n_steps) {
+#pragma unroll
+                    for (int m = 0; m < S::kMine; ++m) {
+                        const int id = t + 32 * kConvWarps * m;
+                        if (id < S::kPieces) {
+                            const int pg = id / (S::kPieces / S::kPages), in = id % (S::kPieces / S::kPages), p = S::kPages == 1 || pg == 0 ? page[0] : page[S::kPages - 1];
+                            const uint8_t* at = values ? kv.v + (size_t)max(p, 0) * kv.v_stride : kv.k + (size_t)max(p, 0) * kv.k_stride;
+                            // a page behind the last: zeros, which no row sees
+                            copy_async16(slot_of(i, values, id), at + (size_t)h * kPageTokens * HD + in * 16, p >= 0 ? 16 : 0);
+                        }
+                    }
+                    look_up(i + 1, page);
+                }
+                asm volatile("cp.async.commit_group;\n" ::);
+            };
+            look_up(0, page_k);
+            look_up(0, page_v);
+            for (int i = 0; i < S::kRaw; ++i) { ask(i, 0, page_k); ask(i, 1, page_v); }
             for (int i = 0; i < n_steps; ++i) {
                 const int s = i % S::kStages;
-                const uint32_t turn = (((uint32_t)i / S::kStages) & 1u) ^ 1u;
-                if (!__all_sync(0xffffffffu, mbar_wait<kTest>(k_free(s), turn, abort_flag))) break;
+                asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S::kRaw - 1));
+                if (!__all_sync(0xffffffffu, mbar_wait<kTest>(k_free(s), (((uint32_t)i / S::kStages) & 1u) ^ 1u, abort_flag))) break;
                 const uint32_t kt = base + S::kOffK + s * S::kTileBytes;
 #pragma unroll
                 for (int m = 0; m < S::kMine; ++m) {
                     const int id = t + 32 * kConvWarps * m;
                     if (id < S::kPieces) {
                         const int row = id / (HD / 16), piece = id % (HD / 16);
-                        store_halves(kt + (piece / 4) * (BK * 128) + row * 128, piece % 4 * 2, row & 7, k[m]);
+                        store_halves(kt + (piece / 4) * (BK * 128) + row * 128, piece % 4 * 2, row & 7, load_shared16(slot_of(i, 0, id)));
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 __syncwarp();
                 if (lane == 0 && !Waits<kTest>::kSkipCopies) mbar_arrive(k_full(s));
-                if (i + 1 < n_steps) fetch(i + 1, false, k);
-                if (!__all_sync(0xffffffffu, mbar_wait<kTest>(v_free(s), turn, abort_flag))) break;
-                const uint32_t vt = base + S::kOffV + s * S::kTileBytes;
+                ask(i + S::kRaw, 0, page_k);
+                asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S::kRaw - 1));
+                if (!__all_sync(0xffffffffu, mbar_wait<kTest>(v_free, ((uint32_t)i & 1u) ^ 1u, abort_flag))) break;
+                const uint32_t vt = base + S::kOffV;
 #pragma unroll
                 for (int m = 0; m < S::kMine; ++m) {
                     const int id = t + 32 * kConvWarps * m;
                     if (id < S::kPieces) {
+                        uint4 v = load_shared16(slot_of(i, 1, id));
                         const int pg = id / (HD * 4), channel = id / 4 % HD, piece = id % 4;
                         const int j = page_of(i, pg), at = j * kPageTokens + piece * 16;       // rows at .. at + 15
                         if (j >= 0 && (j * kPageTokens + kPageTokens - 1 > first_at || (a.window > 0 && j * kPageTokens <= last_at - a.window))) {
                             // A page that not every query sees whole.  Rows nobody has written yet become zeros; so do NaN codes, which
                             // P's zeros would not silence: who does see them gets them back at the end.
-                            uint32_t w[4] = {v[m].x, v[m].y, v[m].z, v[m].w};
+                            uint32_t w[4] = {v.x, v.y, v.z, v.w};
                             uint32_t found = 0;
 #pragma unroll
                             for (int c = 0; c < 4; ++c) {
@@ -202,16 +228,17 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                                 w[c] &= ~nan;
                             }
                             if (found) *odd_flag = 1;
-                            v[m] = make_uint4(w[0], w[1], w[2], w[3]);
+                            v = make_uint4(w[0], w[1], w[2], w[3]);
                         }
-                        store_halves(vt + pg * (HD * 128) + channel * 128, piece * 2, channel & 7, v[m]);
+                        store_halves(vt + pg * (HD * 128) + channel * 128, piece * 2, channel & 7, v);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 __syncwarp();
-                if (lane == 0 && !Waits<kTest>::kSkipCopies) mbar_arrive(v_full(s));
-                if (i + 1 < n_steps) fetch(i + 1, true, v);
+                if (lane == 0 && !Waits<kTest>::kSkipCopies) mbar_arrive(v_full);
+                ask(i + S::kRaw, 1, page_v);
             }
+            asm volatile("cp.async.wait_group 0;\n" ::);
         } else if (lane == 0) {
             // ------------------------------------------------------------ products
             const uint32_t idesc_s = f16_idesc(BQ, BK), idesc_pv = f16_idesc(BQ, HD);
@@ -237,17 +264,16 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                     ok = mbar_wait<kTest>(s_free, (uint32_t)i & 1u, abort_flag) && issue_s(i + 1);
                     if (!ok) break;
                 }
-                const int s = i % S::kStages;
-                ok = mbar_wait<kTest>(v_full(s), ((uint32_t)i / S::kStages) & 1u, abort_flag) &&
+                ok = mbar_wait<kTest>(v_full, (uint32_t)i & 1u, abort_flag) &&
                      mbar_wait<kTest>(p_full, (uint32_t)i & 1u, abort_flag);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
 #pragma unroll
                 for (int kk = 0; kk < BK / 16; ++kk) {
-                    const uint64_t dv = umma_desc(base + S::kOffV + s * S::kTileBytes + (kk / 4) * (HD * 128)) + 2 * (kk % 4);
+                    const uint64_t dv = umma_desc(base + S::kOffV + (kk / 4) * (HD * 128)) + 2 * (kk % 4);
                     umma_ts(tmem_o, tmem_p + 8 * kk, dv, idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
                 }
-                umma_commit(v_free(s));
+                umma_commit(v_free);
                 umma_commit(pv_done);
             }
         }
