@@ -2,49 +2,48 @@
 // bfloat16 queries, causal, with an optional window.  (Layout and codes: e4m3.cuh.)
 //
 // One block per (128 query rows, key/value head, sequence).  A query row is a (token, head of the group) pair, heads
-// innermost, so that the heads that share keys share their pages too and a short run of queries still fills a tile.  Per step of BK
-// rows of the cache (two pages for heads of 64 channels, one for 128):
-//   codes -> half   three warps fetch the step's codes (asynchronous copies, two or three steps ahead), turn them into halves,
+// innermost, so that the heads that share keys share their pages too and a short run of queries still fills a tile.  Per page:
+//   codes -> half   four warps fetch the page's codes (asynchronous copies, two or four pages ahead), turn them into halves,
 //                   which is exact, and leave them in shared memory as swizzled tiles: keys [row][channel], values
 //                   [channel][row], both K-major as the cache has them;
-//   S  = Q K^T      tcgen05.mma 128 x BK x head size, operands in shared memory, S in tensor memory; queries are scaled by a
+//   S  = Q K^T      tcgen05.mma 128 x 64 x head size, operands in shared memory, S in tensor memory; queries are scaled by a
 //                   power of two a row to fill half's range, so that rounding bfloat16 to half loses nothing that counts;
-//   P  = softmax    four warps, a thread a row, scores straight from tensor memory; P goes back there as halves;
-//   O += P V        tcgen05.mma 128 x head size x BK, A = P from tensor memory, O stays there.
+//   P  = softmax    eight warps, two threads a row, scores straight from tensor memory; P goes back there as halves;
+//   O += P V        tcgen05.mma 128 x head size x 64, A = P from tensor memory, O stays there.
 // Scales.  A page's key scale multiplies its scores.  Its value scale 2^v cannot multiply O, which adds up over pages, and
 // must not squeeze P's range either: it goes into the exponent.  With x_j = score_j + v_j (in powers of two) and M the running
 // maximum of x, P_j = 2^(x_j - M), O = sum P_j code_j and the sum is l = sum P_j 2^(-v_j): O / l is the result, whatever the
 // scales (as long as two blocks of values that both count are not 2^100 apart).  M is raised only when a step's maximum exceeds it
 // by 2^8; P, times 2^7 besides, then stays below half's largest number.
-// What bounds it: for 128 channels the two products (the conversion's 1.5 operations a pair of codes and its stores run beside
-// them), for 64 the exponentials, one a score at 16 a cycle.  Every wait is bounded (status word as in the products).
+// What bounds it is the softmax's latency: a tile's page takes its warps longer than its products (512 cycles for 128 channels).
+// With four warps, a thread a row, it was 2,400 cycles alone and 3,000 with a second block beside it.  Every wait is bounded
+// (status word as in the products).
 #include "e4m3.cuh"
 #include "tcgen05_attention.cuh"
 
 namespace {
 constexpr int BQ = 128;
-constexpr int kConvWarps = 3;
-constexpr int kThreads = 32 * (5 + kConvWarps);          // softmax 0-3, products 4, conversion 5-7
+constexpr int BK = kPageTokens;                          // rows of the cache a step: a page, which has one scale
+constexpr int kSoftmaxWarps = 8, kConvWarps = 4, kProductWarp = kSoftmaxWarps;
+constexpr int kThreads = 32 * (kSoftmaxWarps + 1 + kConvWarps);
 constexpr int kTmemCols = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaiseBy = 8.0f, kPShift = 7.0f;
-// Registers: the softmax's warps hold a step's scores, the others little; 168 + 88 is twice the 128 a thread is launched with.
-constexpr int kSoftmaxRegs = 168, kOtherRegs = 88;
 
 template <int HD> struct Shape {
-    static constexpr int kPages = HD == 64 ? 2 : 1;      // of a step
-    static constexpr int BK = 64 * kPages;
-    static constexpr int kStages = 2;                    // key tiles; one value tile: it is wanted a softmax later
-    static constexpr int kRaw = HD == 64 ? 3 : 2;        // steps of codes on their way
+    static constexpr int kKeyTiles = 2;
+    static constexpr int kValueTiles = HD == 64 ? 2 : 1; // one is enough where there is no room: values are wanted a softmax later
+    static constexpr int kRaw = HD == 64 ? 4 : 2;        // steps of codes on their way
     static constexpr int kQBytes = BQ * HD * 2, kTileBytes = BK * HD * 2;
-    static constexpr int kOffK = kQBytes, kOffV = kOffK + kStages * kTileBytes, kOffRaw = kOffV + kTileBytes;
+    static constexpr int kOffK = kQBytes, kOffV = kOffK + kKeyTiles * kTileBytes, kOffRaw = kOffV + kValueTiles * kTileBytes;
     static constexpr int kRawBytes = BK * HD;            // a step's codes of keys (or of values)
     static constexpr int kOffBar = kOffRaw + kRaw * 2 * kRawBytes;
-    static constexpr int kSmemBytes = kOffBar + 256;
-    static constexpr int kColO = BK, kColP = BK + HD;
-    static_assert(BK + HD + BK / 2 <= kTmemCols, "tensor memory");
-    static constexpr int kPieces = BK * HD / 16;         // of 16 codes in a step's keys (or values): 512
-    static constexpr int kMine = (kPieces + 32 * kConvWarps - 1) / (32 * kConvWarps);
+    static constexpr int kSmemBytes = kOffBar + 160;
+    static constexpr int kColO = BK, kColP = BK + HD;    // of tensor memory: S, O, two of P
+    static_assert(BK + HD + BK <= kTmemCols, "tensor memory");
+    static constexpr int kPieces = BK * HD / 16;         // of 16 codes in a step's keys (or values)
+    static constexpr int kMine = kPieces / (32 * kConvWarps);
+    static_assert(kPieces % (32 * kConvWarps) == 0, "pieces are dealt evenly");
 };
 
 // kind::f16, half operands, both K-major, float sums.
@@ -72,9 +71,24 @@ __device__ __forceinline__ uint4 load_shared16(uint32_t at) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at) : "memory");
     return u;
 }
-// 16-byte copy global -> shared; `bytes` = 0 fills the destination with zeros.
-__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// Wait for a phase, the warp asleep meanwhile (up to some 10 us at a time): a block of thirteen warps that poll instead spends half
+// of its issue slots on it.  Bounded like mbar_wait.
+template <bool kTest>
+__device__ __forceinline__ bool mbar_sleep(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    for (unsigned i = 0; i < (kTest ? 64u : 1u << 18); ++i) {
+        uint32_t done;
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+                     "selp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity), "r"(10000u) : "memory");
+        if (done) return true;
+        if (*abort_flag) return false;
+    }
+    *abort_flag = 1;
+    atomicExch(&g_status, 1);
+    return false;
+}
+// 16-byte copy global -> shared.
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
 }
 // 16 codes as 16 halves: two chunks of a swizzled row.
 __device__ __forceinline__ void store_halves(uint32_t row_at, int chunk, int swizzle, const uint4& u) {
@@ -82,13 +96,54 @@ __device__ __forceinline__ void store_halves(uint32_t row_at, int chunk, int swi
     store_shared16(row_at + (((chunk + 1) ^ swizzle) << 4), e4m3_pair_f16(u.z), e4m3_pair_f16(u.z >> 16), e4m3_pair_f16(u.w), e4m3_pair_f16(u.w >> 16));
 }
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Two floats at a time.
+__device__ __forceinline__ uint64_t two(float a, float b) { return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a); }
+__device__ __forceinline__ float first_of(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float second_of(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+
+// Products and commits issued by one lane of a warp that runs its loop as a whole: with the loop inside one lane's branch the
+// descriptors do not stay in the warp's uniform registers, and a step's products took some 60 cycles each to issue.
+__device__ __forceinline__ void warp_umma_ss(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void warp_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p, e;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %4, 0;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void warp_umma_commit(uint32_t bar) {
+    asm volatile("{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar) : "memory");
+}
 
 // grid: (kv heads, sequences, tiles of query rows), the longest tiles first.
 template <int HD, bool kTest>
 __global__ void __launch_bounds__(kThreads, 2)
 attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     using S = Shape<HD>;
-    constexpr int BK = S::BK;
     extern __shared__ __align__(1024) unsigned char smem[];
     const int h = blockIdx.x, b = blockIdx.y;
     const int tile = gridDim.z - 1 - blockIdx.z;
@@ -102,10 +157,14 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
         return;
     }
     const uint32_t bars = base + S::kOffBar;
-    const uint32_t q_full = bars, s_full = bars + 8, s_free = bars + 16, p_full = bars + 24, pv_done = bars + 32;
-    auto k_full = [&](int s) { return bars + 40u + 8u * s; };
-    auto k_free = [&](int s) { return bars + 56u + 8u * s; };
-    const uint32_t v_full = bars + 72, v_free = bars + 80;
+    // A step's scores and products have barriers by the step's parity: S of step i also frees its key tile, P V its values and P.
+    const uint32_t q_full = bars, s_free = bars + 8, l_full = bars + 16;
+    auto s_full = [&](int i) { return bars + 32u + 8u * (i & 1); };
+    auto p_full = [&](int i) { return bars + 48u + 8u * (i & 1); };
+    auto pv_done = [&](int i) { return bars + 64u + 8u * (i & 1); };
+    auto k_full = [&](int i) { return bars + 80u + 8u * (i & 1); };
+    auto v_full = [&](int i) { return bars + 96u + 8u * (i & 1); };
+    auto phase = [](int i) { return ((uint32_t)i >> 1) & 1u; };  // of step i's barriers
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + S::kOffBar + 128);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kOffBar + 136);
     volatile int* odd_flag = reinterpret_cast<volatile int*>(smem + S::kOffBar + 140);   // a NaN code in a page not all rows see whole
@@ -119,26 +178,27 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     const int first_at = start + row0 / a.group;                 // cache row of the tile's first query, and of its last
     const int last_at = start + (row0 + rows_here - 1) / a.group;
     const int k_min = a.window > 0 ? max(0, first_at - a.window + 1) : 0;
-    const int j_lo = k_min / kPageTokens, j_hi = last_at / kPageTokens;
-    const int n_steps = (j_hi - j_lo + S::kPages) / S::kPages;
+    const int j_lo = k_min / kPageTokens, n_steps = last_at / kPageTokens - j_lo + 1;
+    auto page_not_whole = [&](int j) {                           // a page that not every query of the tile sees whole
+        return j * kPageTokens + kPageTokens - 1 > first_at || (a.window > 0 && j * kPageTokens <= last_at - a.window);
+    };
 
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 4);
-        mbar_init(s_full, 1);
-        mbar_init(s_free, 4);
-        mbar_init(p_full, 4);
-        mbar_init(pv_done, 1);
-        for (int s = 0; s < S::kStages; ++s) {
+        mbar_init(q_full, kSoftmaxWarps);
+        mbar_init(s_free, kSoftmaxWarps);
+        mbar_init(l_full, kSoftmaxWarps);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(s_full(s), 1);
+            mbar_init(p_full(s), kSoftmaxWarps);
+            mbar_init(pv_done(s), 1);
             mbar_init(k_full(s), kConvWarps);
-            mbar_init(k_free(s), 1);
+            mbar_init(v_full(s), kConvWarps);
         }
-        mbar_init(v_full, kConvWarps);
-        mbar_init(v_free, 1);
         *abort_flag = 0;
         *odd_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::);
     }
-    if (warp == 4) {
+    if (warp == kProductWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n"
                      ::"r"(smem_addr(tmem_holder)), "r"(kTmemCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
@@ -150,151 +210,133 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     chain_wait();                                                // queries and the newest rows come from the kernel before
     chain_release();
 
-    if (warp >= 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
-        if (warp >= 5) {
-            // ------------------------------------------------------------ codes to halves
-            const int t = threadIdx.x - 5 * 32;
-            const int total = start + q_len;                     // rows that exist after this step
-            auto page_of = [&](int i, int pg) { const int j = j_lo + S::kPages * i + pg; return j <= j_hi ? j : -1; };
-            // The codes come by asynchronous copies, kRaw steps ahead, each 16-byte piece to a place that only the lane that will
-            // convert it reads: nothing is waited for but a lane's own copies.  Page numbers are read a step earlier still.
-            int page_k[S::kPages], page_v[S::kPages];            // of the next step to be asked for: page or -1
-            auto look_up = [&](int i, int* page) {
+    if (warp > kProductWarp) {
+        // ------------------------------------------------------------ codes to halves
+        const int t = threadIdx.x - 32 * (kProductWarp + 1);
+        const int total = start + q_len;                         // rows that exist after this step
+        // The codes come by asynchronous copies, kRaw steps ahead, each 16-byte piece to a place that only the lane that will
+        // convert it reads: nothing is waited for but a lane's own copies.  Page numbers are read 32 steps at a time.
+        int pages = 0;                                           // lane l: page of step (asked / 32 * 32 + l)
+        auto slot_of = [&](int i, int values, int m) { return base + S::kOffRaw + ((i % S::kRaw) * 2 + values) * S::kRawBytes + (t + 32 * kConvWarps * m) * 16; };
+        const uint8_t* k_at = kv.k + (size_t)h * kPageTokens * HD + t * 16;
+        const uint8_t* v_at = kv.v + (size_t)h * kPageTokens * HD + t * 16;
+        auto ask = [&](int i, int values) {
+            if (i < n_steps) {
+                if (!values && (i & 31) == 0) pages = i + lane < n_steps ? table[j_lo + i + lane] : 0;
+                const size_t page = __shfl_sync(0xffffffffu, pages, i & 31);
+                const uint8_t* at = values ? v_at + page * kv.v_stride : k_at + page * kv.k_stride;
 #pragma unroll
-                for (int pg = 0; pg < S::kPages; ++pg) {
-                    const int j = page_of(i, pg);
-                    page[pg] = j >= 0 ? table[j] : -1;
-                }
-            };
-            auto slot_of = [&](int i, int values, int id) { return base + S::kOffRaw + ((i % S::kRaw) * 2 + values) * S::kRawBytes + id * 16; };
-            auto ask = [&](int i, int values, int* page) {
-                if (i < n_steps) {
-#pragma unroll
-                    for (int m = 0; m < S::kMine; ++m) {
-                        const int id = t + 32 * kConvWarps * m;
-                        if (id < S::kPieces) {
-                            const int pg = id / (S::kPieces / S::kPages), in = id % (S::kPieces / S::kPages), p = S::kPages == 1 || pg == 0 ? page[0] : page[S::kPages - 1];
-                            const uint8_t* at = values ? kv.v + (size_t)max(p, 0) * kv.v_stride : kv.k + (size_t)max(p, 0) * kv.k_stride;
-                            // a page behind the last: zeros, which no row sees
-                            copy_async16(slot_of(i, values, id), at + (size_t)h * kPageTokens * HD + in * 16, p >= 0 ? 16 : 0);
-                        }
-                    }
-                    look_up(i + 1, page);
-                }
-                asm volatile("cp.async.commit_group;\n" ::);
-            };
-            look_up(0, page_k);
-            look_up(0, page_v);
-            for (int i = 0; i < S::kRaw; ++i) { ask(i, 0, page_k); ask(i, 1, page_v); }
-            for (int i = 0; i < n_steps; ++i) {
-                const int s = i % S::kStages;
-                asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S::kRaw - 1));
-                if (!__all_sync(0xffffffffu, mbar_wait<kTest>(k_free(s), (((uint32_t)i / S::kStages) & 1u) ^ 1u, abort_flag))) break;
-                const uint32_t kt = base + S::kOffK + s * S::kTileBytes;
-#pragma unroll
-                for (int m = 0; m < S::kMine; ++m) {
-                    const int id = t + 32 * kConvWarps * m;
-                    if (id < S::kPieces) {
-                        const int row = id / (HD / 16), piece = id % (HD / 16);
-                        store_halves(kt + (piece / 4) * (BK * 128) + row * 128, piece % 4 * 2, row & 7, load_shared16(slot_of(i, 0, id)));
-                    }
-                }
-                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                __syncwarp();
-                if (lane == 0 && !Waits<kTest>::kSkipCopies) mbar_arrive(k_full(s));
-                ask(i + S::kRaw, 0, page_k);
-                asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S::kRaw - 1));
-                if (!__all_sync(0xffffffffu, mbar_wait<kTest>(v_free, ((uint32_t)i & 1u) ^ 1u, abort_flag))) break;
-                const uint32_t vt = base + S::kOffV;
-#pragma unroll
-                for (int m = 0; m < S::kMine; ++m) {
-                    const int id = t + 32 * kConvWarps * m;
-                    if (id < S::kPieces) {
-                        uint4 v = load_shared16(slot_of(i, 1, id));
-                        const int pg = id / (HD * 4), channel = id / 4 % HD, piece = id % 4;
-                        const int j = page_of(i, pg), at = j * kPageTokens + piece * 16;       // rows at .. at + 15
-                        if (j >= 0 && (j * kPageTokens + kPageTokens - 1 > first_at || (a.window > 0 && j * kPageTokens <= last_at - a.window))) {
-                            // A page that not every query sees whole.  Rows nobody has written yet become zeros; so do NaN codes, which
-                            // P's zeros would not silence: who does see them gets them back at the end.
-                            uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                            uint32_t found = 0;
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                const int there = min(max(total - at - 4 * c, 0), 4);           // rows of this word that exist
-                                w[c] &= there == 4 ? 0xffffffffu : (1u << (8 * there)) - 1u;
-                                const uint32_t nan = nan_codes(w[c]);
-                                found |= nan;
-                                w[c] &= ~nan;
-                            }
-                            if (found) *odd_flag = 1;
-                            v = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                        store_halves(vt + pg * (HD * 128) + channel * 128, piece * 2, channel & 7, v);
-                    }
-                }
-                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                __syncwarp();
-                if (lane == 0 && !Waits<kTest>::kSkipCopies) mbar_arrive(v_full);
-                ask(i + S::kRaw, 1, page_v);
+                for (int m = 0; m < S::kMine; ++m) copy_async16(slot_of(i, values, m), at + 32 * kConvWarps * m * 16);
             }
-            asm volatile("cp.async.wait_group 0;\n" ::);
-        } else if (lane == 0) {
-            // ------------------------------------------------------------ products
-            const uint32_t idesc_s = f16_idesc(BQ, BK), idesc_pv = f16_idesc(BQ, HD);
-            bool ok = mbar_wait<kTest>(q_full, 0, abort_flag);
-            auto issue_s = [&](int i) {
-                const int s = i % S::kStages;
-                if (!mbar_wait<kTest>(k_full(s), ((uint32_t)i / S::kStages) & 1u, abort_flag)) return false;
-                asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-                const uint32_t kbase = base + S::kOffK + s * S::kTileBytes;
+            asm volatile("cp.async.commit_group;\n" ::);
+        };
+        // (keys of step i + kRaw are asked for between values of steps i - 1 + kRaw and i + kRaw: the 32 page numbers of a
+        // stretch serve its keys and its values alike)
+        for (int i = 0; i < S::kRaw; ++i) { ask(i, 0); ask(i, 1); }
+        for (int i = 0; i < n_steps; ++i) {
+            const int s = i % S::kKeyTiles, sv = i % S::kValueTiles;
+            uint4 u[S::kMine];
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S::kRaw - 1) : "memory");
 #pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk) {
-                    const uint64_t dq = umma_desc(base + (kk / 4) * (BQ * 128)) + 2 * (kk % 4);
-                    const uint64_t dk = umma_desc(kbase + (kk / 4) * (BK * 128)) + 2 * (kk % 4);
-                    umma_ss(tmem_s, dq, dk, idesc_s, kk > 0 ? 1u : 0u);
+            for (int m = 0; m < S::kMine; ++m) u[m] = load_shared16(slot_of(i, 0, m));
+            if (i >= 2 && !__all_sync(0xffffffffu, mbar_sleep<kTest>(s_full(i), phase(i - 2), abort_flag))) break;
+            const uint32_t kt = base + S::kOffK + s * S::kTileBytes;
+#pragma unroll
+            for (int m = 0; m < S::kMine; ++m) {
+                const int id = t + 32 * kConvWarps * m, row = id / (HD / 16), piece = id % (HD / 16);
+                store_halves(kt + (piece / 4) * (BK * 128) + row * 128, piece % 4 * 2, row & 7, u[m]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0 && !Waits<kTest>::kSkipCopies) mbar_arrive(k_full(i));
+            ask(i + S::kRaw, 0);
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S::kRaw - 1) : "memory");
+#pragma unroll
+            for (int m = 0; m < S::kMine; ++m) u[m] = load_shared16(slot_of(i, 1, m));
+            const int j = j_lo + i;
+            if (page_not_whole(j)) {
+                // Rows nobody has written yet become zeros; so do NaN codes, which P's zeros would not silence: who does see them
+                // gets them back at the end.
+#pragma unroll
+                for (int m = 0; m < S::kMine; ++m) {
+                    const int at = j * kPageTokens + (t + 32 * kConvWarps * m) % 4 * 16;       // rows at .. at + 15
+                    uint32_t w[4] = {u[m].x, u[m].y, u[m].z, u[m].w};
+                    uint32_t found = 0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int there = min(max(total - at - 4 * c, 0), 4);                   // rows of this word that exist
+                        w[c] &= there == 4 ? 0xffffffffu : (1u << (8 * there)) - 1u;
+                        const uint32_t nan = nan_codes(w[c]);
+                        found |= nan;
+                        w[c] &= ~nan;
+                    }
+                    if (found) *odd_flag = 1;
+                    u[m] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                umma_commit(k_free(s));
-                umma_commit(s_full);
-                return true;
-            };
-            if (ok) ok = issue_s(0);
-            for (int i = 0; i < n_steps && ok; ++i) {
-                if (i + 1 < n_steps) {
-                    ok = mbar_wait<kTest>(s_free, (uint32_t)i & 1u, abort_flag) && issue_s(i + 1);
-                    if (!ok) break;
-                }
-                ok = mbar_wait<kTest>(v_full, (uint32_t)i & 1u, abort_flag) &&
-                     mbar_wait<kTest>(p_full, (uint32_t)i & 1u, abort_flag);
+            }
+            const int before = i - S::kValueTiles;               // whose values lie there
+            if (before >= 0 && !__all_sync(0xffffffffu, mbar_sleep<kTest>(pv_done(before), phase(before), abort_flag))) break;
+            const uint32_t vt = base + S::kOffV + sv * S::kTileBytes;
+#pragma unroll
+            for (int m = 0; m < S::kMine; ++m) {
+                const int id = t + 32 * kConvWarps * m, channel = id / 4, piece = id % 4;
+                store_halves(vt + channel * 128, piece * 2, channel & 7, u[m]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0 && !Waits<kTest>::kSkipCopies) mbar_arrive(v_full(i));
+            ask(i + S::kRaw, 1);
+        }
+        asm volatile("cp.async.wait_group 0;\n" ::);
+    } else if (warp == kProductWarp) {
+        // ------------------------------------------------------------ products
+        constexpr uint32_t idesc_s = f16_idesc(BQ, BK), idesc_pv = f16_idesc(BQ, HD);
+        const uint64_t q_desc = umma_desc(base), k_desc = umma_desc(base + S::kOffK), v_desc = umma_desc(base + S::kOffV);
+        // (a wait's answer is the whole warp's before anything is issued: the elected lane waits for all)
+        auto all_wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_sleep<kTest>(bar, parity, abort_flag)); };
+        auto issue_s = [&](int i) {
+            if (!all_wait(k_full(i), phase(i))) return false;
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
+            const uint64_t dk = k_desc + (uint64_t)(i % S::kKeyTiles * (S::kTileBytes >> 4));
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)
+                warp_umma_ss(tmem_s, q_desc + (kk / 4) * (BQ * 128 >> 4) + 2 * (kk % 4), dk + (kk / 4) * (BK * 128 >> 4) + 2 * (kk % 4), idesc_s, kk > 0 ? 1u : 0u);
+            warp_umma_commit(s_full(i));
+            return true;
+        };
+        bool ok = all_wait(q_full, 0) && issue_s(0);
+        for (int i = 0; i < n_steps && ok; ++i) {
+            if (i + 1 < n_steps) {
+                ok = all_wait(s_free, (uint32_t)i & 1u) && issue_s(i + 1);
                 if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-#pragma unroll
-                for (int kk = 0; kk < BK / 16; ++kk) {
-                    const uint64_t dv = umma_desc(base + S::kOffV + (kk / 4) * (HD * 128)) + 2 * (kk % 4);
-                    umma_ts(tmem_o, tmem_p + 8 * kk, dv, idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
-                }
-                umma_commit(v_free);
-                umma_commit(pv_done);
             }
+            ok = all_wait(v_full(i), phase(i)) && all_wait(p_full(i), phase(i));
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
+            const uint64_t dv = v_desc + (uint64_t)(i % S::kValueTiles * (S::kTileBytes >> 4));
+            const uint32_t p_at = tmem_p + 32 * (i & 1);
+#pragma unroll
+            for (int kk = 0; kk < BK / 16; ++kk) warp_umma_ts(tmem_o, p_at + 8 * kk, dv + 2 * kk, idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
+            warp_umma_commit(pv_done(i));
         }
     } else {
-        // ------------------------------------------------------------ softmax and output: a thread a query row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
+        // ------------------------------------------------------------ softmax and output: two threads a query row, 32 columns each.
+        // Both find the maximum of the whole row (its scores are cheap to read, a second thread's answer is not), so neither
+        // waits for the other before the end.
         const unsigned full = 0xffffffffu;
-        const int r = warp * 32 + lane;
+        const int half = warp >> 2, r = (warp & 3) * 32 + lane;
         const bool real = r < rows_here;
         const int token = (row0 + (real ? r : 0)) / a.group, head = h * a.group + (row0 + (real ? r : 0)) % a.group;
         const int pos = start + token;                            // the query's own cache row
-        const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
         float factor;                                             // a raw score times this and the page's key scale: powers of two
         {
             const bf16* src = a.q + (size_t)(q_begin + token) * a.ldq + (size_t)head * HD;
-            uint4 u[HD / 8];
             float most = 0.f;
 #pragma unroll
             for (int c = 0; c < HD / 8; ++c) {
-                u[c] = real ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
-                const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+                const uint4 u = real ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float lo = fabsf(__uint_as_float(w[e] << 16)), hi = fabsf(__uint_as_float(w[e] & 0xffff0000u));
@@ -307,8 +349,9 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             const float f = __uint_as_float((uint32_t)(127 + up) << 23) * (a.scale < 0.f ? -1.f : 1.f);
             factor = fmaxf(fabsf(a.scale) * kLog2e * __uint_as_float((uint32_t)(127 - up) << 23), 1e-37f);
 #pragma unroll
-            for (int c = 0; c < HD / 8; ++c) {
-                const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+            for (int c = half * (HD / 16); c < (half + 1) * (HD / 16); ++c) {
+                const uint4 u = real ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
                 uint32_t o[4];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
@@ -321,64 +364,52 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
         }
-        // scales of the step's pages, read a step ahead
-        float k_next[S::kPages], v_next[S::kPages];
-        auto fetch_scales = [&](int i) {
-#pragma unroll
-            for (int pg = 0; pg < S::kPages; ++pg) {
-                const int j = j_lo + S::kPages * i + pg;
-                const float* at = kv.scales + (size_t)table[j <= j_hi ? j : j_hi] * kv.scale_stride + h;
-                k_next[pg] = at[0];
-                v_next[pg] = at[kv.n_kv];
-            }
-        };
-        fetch_scales(0);
+        // scales, 32 steps at a time: lane l has those of step (i / 32 * 32 + l)
+        float k_scales = 0.f, v_scales = 1.f;
         float m_run = -INFINITY, l_run = 0.f;
-        uint32_t sv[BK];
+        uint32_t sv[32];
         bool ok = true;
         for (int i = 0; i < n_steps; ++i) {
-            const int key0 = (j_lo + S::kPages * i) * kPageTokens;
-            float sl[S::kPages], add[S::kPages], back[S::kPages];
-#pragma unroll
-            for (int pg = 0; pg < S::kPages; ++pg) {
-                sl[pg] = factor * k_next[pg];
-                add[pg] = (float)((int)(__float_as_uint(v_next[pg]) >> 23) - 127);   // log2 of the value scale
-                back[pg] = pow2_inverse(v_next[pg]);
+            const int key0 = (j_lo + i) * kPageTokens;
+            if ((i & 31) == 0 && i + lane < n_steps) {
+                const float* at = kv.scales + (size_t)table[j_lo + i + lane] * kv.scale_stride + h;
+                k_scales = at[0];
+                v_scales = at[kv.n_kv];
             }
-            if (i + 1 < n_steps) fetch_scales(i + 1);
-            ok = __all_sync(full, mbar_wait<kTest>(s_full, (uint32_t)i & 1u, abort_flag));
+            const float sl = factor * __shfl_sync(full, k_scales, i & 31);
+            const float v_scale = __shfl_sync(full, v_scales, i & 31);
+            const float add = (float)((int)(__float_as_uint(v_scale) >> 23) - 127);             // log2 of the value scale
+            ok = __all_sync(full, mbar_sleep<kTest>(s_full(i), phase(i), abort_flag));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-#pragma unroll
-            for (int c = 0; c < BK / 32; ++c) tmem_ld32(tmem_s + lane_off + 32 * c, sv + 32 * c);
+            uint32_t other[32];
+            tmem_ld32(tmem_s + lane_off + 32 * half, sv);
+            tmem_ld32(tmem_s + lane_off + 32 * (half ^ 1), other);
             asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
             __syncwarp();
-            if (lane == 0) mbar_arrive(s_free);
-            const bool all_visible = key0 + BK - 1 <= pos && (a.window <= 0 || key0 > pos - a.window);
-            if (!all_visible) {
+            if (lane == 0) mbar_arrive(s_free);                  // the scores are in registers: the tile takes the next step's
+            if (!(key0 + BK - 1 <= pos && (a.window <= 0 || key0 > pos - a.window))) {
+                const int hi = pos - key0, lo = a.window > 0 ? pos - a.window - key0 : -1;       // columns lo + 1 .. hi are seen
 #pragma unroll
-                for (int c = 0; c < BK; ++c) {
-                    const int key = key0 + c;
-                    if (key > pos || (a.window > 0 && key <= pos - a.window)) sv[c] = __float_as_uint(-INFINITY);
+                for (int c = 0; c < 32; ++c) {
+                    const int mine = 32 * half + c, its = 32 * (half ^ 1) + c;
+                    if (mine > hi || mine <= lo) sv[c] = __float_as_uint(-INFINITY);
+                    if (its > hi || its <= lo) other[c] = __float_as_uint(-INFINITY);
                 }
             }
-            float m_step = -INFINITY;
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int pg = 0; pg < S::kPages; ++pg) {
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int c = 0; c < 32; c += 4)
 #pragma unroll
-                for (int c = 0; c < 64; c += 4)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(sv[64 * pg + c + e]));
-                m_step = fmaxf(m_step, fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), sl[pg], add[pg]));
-            }
+                for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sv[c + e]), __uint_as_float(other[c + e]));
+            const float m_step = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), sl, add);
             if (i == 0) {
                 m_run = m_step;
             } else {
                 const bool raise = m_step > m_run + kRaiseBy;    // also: the first visible row of a query
                 if (__any_sync(full, raise)) {
-                    ok = __all_sync(full, mbar_wait<kTest>(pv_done, (uint32_t)(i - 1) & 1u, abort_flag));
+                    ok = __all_sync(full, mbar_sleep<kTest>(pv_done(i - 1), phase(i - 1), abort_flag));
                     if (!ok) break;
                     float corr = 1.0f;
                     if (raise) {
@@ -389,7 +420,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
                     uint32_t ov[8];
 #pragma unroll 1
-                    for (int part = 0; part < HD / 8; ++part) {
+                    for (int part = half * (HD / 16); part < (half + 1) * (HD / 16); ++part) {   // its half of the row of O
                         tmem_ld8(tmem_o + lane_off + 8 * part, ov);
                         asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
@@ -398,54 +429,60 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                     }
                 }
             }
-            const float m_use = (m_run == -INFINITY ? 0.f : m_run) - kPShift;
+            const float shift = add - (m_run == -INFINITY ? 0.f : m_run) + kPShift;
+            const uint64_t sl2 = two(sl, sl), shift2 = two(shift, shift);
+            uint64_t sums[2] = {0, 0};
 #pragma unroll
-            for (int pg = 0; pg < S::kPages; ++pg) {
-                const float shift = add[pg] - m_use;
-                float l0 = 0.f, l1 = 0.f;
+            for (int c = 0; c < 32; c += 8) {                     // scores c .. c + 7 become words c / 2 .. c / 2 + 3
+                uint64_t x[4];
+                float p[8];
 #pragma unroll
-                for (int c = 32 * pg; c < 32 * pg + 32; c += 4) {    // scores 2c .. 2c + 7 become words c .. c + 3
-                    float p[8];
+                for (int e = 0; e < 4; ++e) x[e] = fma2(two(__uint_as_float(sv[c + 2 * e]), __uint_as_float(sv[c + 2 * e + 1])), sl2, shift2);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = fmaf(__uint_as_float(sv[2 * c + e]), sl[pg], shift);
+                for (int e = 0; e < 4; ++e) { p[2 * e] = exp2_in_order(first_of(x[e])); p[2 * e + 1] = exp2_in_order(second_of(x[e])); }
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = exp2_in_order(p[e]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        l0 += p[2 * e];
-                        l1 += p[2 * e + 1];
-                        const __half2 hh = __floats2half2_rn(p[2 * e], p[2 * e + 1]);
-                        sv[c + e] = *reinterpret_cast<const uint32_t*>(&hh);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    sums[e & 1] = add2(sums[e & 1], two(p[2 * e], p[2 * e + 1]));
+                    const __half2 hh = __floats2half2_rn(p[2 * e], p[2 * e + 1]);
+                    sv[c / 2 + e] = *reinterpret_cast<const uint32_t*>(&hh);
                 }
-                l_run = fmaf(l0 + l1, back[pg], l_run);
             }
-            if (i > 0) {
-                ok = __all_sync(full, mbar_wait<kTest>(pv_done, (uint32_t)(i - 1) & 1u, abort_flag));
+            sums[0] = add2(sums[0], sums[1]);
+            l_run = fmaf(first_of(sums[0]) + second_of(sums[0]), pow2_inverse(v_scale), l_run);
+            if (i > 1) {                                          // the P of two steps ago has been read
+                ok = __all_sync(full, mbar_sleep<kTest>(pv_done(i), phase(i - 2), abort_flag));
                 if (!ok) break;
             }
-#pragma unroll
-            for (int c = 0; c < BK / 64; ++c) tmem_st32(tmem_p + lane_off + 32 * c, sv + 32 * c);
+            tmem_st16(tmem_p + 32 * (i & 1) + lane_off + 16 * half, sv);
             asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
+            if (lane == 0) mbar_arrive(p_full(i));
         }
-        if (ok) ok = __all_sync(full, mbar_wait<kTest>(pv_done, (uint32_t)(n_steps - 1) & 1u, abort_flag));
+        // ---- the row's sum, of both threads; each writes its half of the channels
+        if (ok) ok = __all_sync(full, mbar_sleep<kTest>(pv_done(n_steps - 1), phase(n_steps - 1), abort_flag));
+        float* ls = reinterpret_cast<float*>(smem + S::kOffRaw);  // (all codes have been read: the last product is done)
+        if (ok) {
+            ls[half * BQ + r] = l_run;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(l_full);
+            ok = __all_sync(full, mbar_sleep<kTest>(l_full, 0, abort_flag));
+        }
         if (ok) {
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-            const float inv = 1.0f / l_run;
-            if (a.stats && real) a.stats[(size_t)(q_begin + token) * a.n_heads + head] = make_float2((m_run == -INFINITY ? 0.f : m_run) - kPShift, l_run);
+            const float l_row = ls[r] + ls[BQ + r], inv = 1.0f / l_row;
+            if (a.stats && real && half == 0)
+                a.stats[(size_t)(q_begin + token) * a.n_heads + head] = make_float2((m_run == -INFINITY ? 0.f : m_run) - kPShift, l_row);
             bf16* dst = a.out + (size_t)(q_begin + token) * a.ldo + (size_t)head * HD;
             const bool odd = *odd_flag != 0;
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
+            for (int c = half * (HD / 64); c < (half + 1) * (HD / 64); ++c) {
                 tmem_ld32(tmem_o + lane_off + 32 * c, sv);
                 asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
                 if (odd && real) {
                     // NaN codes of rows that this query sees, in pages where they were taken out
-                    for (int j = j_lo; j <= j_hi; ++j) {
-                        if (!(j * kPageTokens + kPageTokens - 1 > first_at || (a.window > 0 && j * kPageTokens <= last_at - a.window))) continue;
+                    for (int j = j_lo; j < j_lo + n_steps; ++j) {
+                        if (!page_not_whole(j)) continue;
                         const uint8_t* vp = kv.v + (size_t)table[j] * kv.v_stride + ((size_t)h * HD + 32 * c) * kPageTokens;
                         const int lo = a.window > 0 ? max(0, pos - a.window + 1 - j * kPageTokens) : 0, hi = min(pos - j * kPageTokens, kPageTokens - 1);
                         for (int tt = lo; tt <= hi; ++tt)
@@ -471,7 +508,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
     __syncthreads();
-    if (warp == 4) {
+    if (warp == kProductWarp) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_s), "r"(kTmemCols));
     }
@@ -578,7 +615,7 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                 const Span sp = span_of(kt);
                 for (int i = 0; i < sp.per_head * a.group; ++i, ++n) {
                     const int s = n % S::kStages;
-                    ok = mbar_wait<kTest>(q_free(s), (((uint32_t)n / S::kStages) & 1u) ^ 1u, abort_flag);
+                    ok = mbar_sleep<kTest>(q_free(s), (((uint32_t)n / S::kStages) & 1u) ^ 1u, abort_flag);
                     if (!ok) break;
                     mbar_expect_tx(q_full(s), S::kTileBytes);
                     for (int hh = 0; hh < HD / 64; ++hh)
@@ -594,11 +631,11 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
             for (int kt = blockIdx.x, turn = 0; kt * 128 < start + q_len && ok; kt += gridDim.x) {
                 const Span sp = span_of(kt);
                 if (sp.per_head == 0) continue;                  // (rows that no query sees: no role takes a turn for them)
-                ok = mbar_wait<kTest>(k_full, (uint32_t)turn++ & 1u, abort_flag);
+                ok = mbar_sleep<kTest>(k_full, (uint32_t)turn++ & 1u, abort_flag);
                 for (int i = 0; i < sp.per_head * a.group && ok; ++i, ++n) {
                     const int s = n % S::kStages, buf = n & 1;
-                    ok = mbar_wait<kTest>(q_full(s), ((uint32_t)n / S::kStages) & 1u, abort_flag) &&
-                         mbar_wait<kTest>(s_free(buf), (((uint32_t)n >> 1) & 1u) ^ 1u, abort_flag);
+                    ok = mbar_sleep<kTest>(q_full(s), ((uint32_t)n / S::kStages) & 1u, abort_flag) &&
+                         mbar_sleep<kTest>(s_free(buf), (((uint32_t)n >> 1) & 1u) ^ 1u, abort_flag);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
                     const uint32_t qbase = base + S::kOffQ + s * S::kTileBytes;
@@ -660,8 +697,8 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(y_full(buf));
                 mine = statistic(i + 1);
-                ok = __all_sync(full, mbar_wait<kTest>(y_full(buf), ((uint32_t)n >> 1) & 1u, abort_flag) &&
-                                          mbar_wait<kTest>(s_full(buf), ((uint32_t)n >> 1) & 1u, abort_flag));
+                ok = __all_sync(full, mbar_sleep<kTest>(y_full(buf), ((uint32_t)n >> 1) & 1u, abort_flag) &&
+                                          mbar_sleep<kTest>(s_full(buf), ((uint32_t)n >> 1) & 1u, abort_flag));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
                 const int t0 = sp.t_lo + i % sp.per_head * 128;
