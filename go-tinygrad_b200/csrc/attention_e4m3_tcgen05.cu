@@ -20,30 +20,30 @@
 // (status word as in the products).
 #include "e4m3.cuh"
 #include "tcgen05_attention.cuh"
+#include <type_traits>
 
 namespace {
-constexpr int BQ = 128;
+constexpr int BQ = 128;                                  // query rows of a tile; a block has two
 constexpr int BK = kPageTokens;                          // rows of the cache a step: a page, which has one scale
-constexpr int kSoftmaxWarps = 8, kConvWarps = 4, kProductWarp = kSoftmaxWarps;
-constexpr int kThreads = 32 * (kSoftmaxWarps + 1 + kConvWarps);
-constexpr int kTmemCols = 256;
+// Warps: 0-3 and 4-7 the tiles' softmax; 8, 9 convert keys, 10, 11 values; 12, 13 issue the tiles' scores, 14, 15 their
+// P V (sixteen: 128 registers).  A warp's waits stand behind the products it has issued, so one warp that issued all of them
+// saw every answer hundreds of cycles late: 3,600 cycles a page where the softmax takes 1,900.
+constexpr int kKeyWarps = 2, kValueWarps = 2, kScoreWarp = 12, kOutputWarp = 14;
+constexpr int kThreads = 512;
+constexpr int kTmemCols = 512, kTileCols = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaiseBy = 8.0f, kPShift = 7.0f;
 
 template <int HD> struct Shape {
-    static constexpr int kKeyTiles = 2;
-    static constexpr int kValueTiles = HD == 64 ? 2 : 1; // one is enough where there is no room: values are wanted a softmax later
-    static constexpr int kRaw = HD == 64 ? 4 : 2;        // steps of codes on their way
+    static constexpr int kRaw = HD == 64 ? 6 : 4;        // steps of codes on their way
     static constexpr int kQBytes = BQ * HD * 2, kTileBytes = BK * HD * 2;
-    static constexpr int kOffK = kQBytes, kOffV = kOffK + kKeyTiles * kTileBytes, kOffRaw = kOffV + kValueTiles * kTileBytes;
+    static constexpr int kOffK = 2 * kQBytes, kOffV = kOffK + 2 * kTileBytes, kOffRaw = kOffV + 2 * kTileBytes;
     static constexpr int kRawBytes = BK * HD;            // a step's codes of keys (or of values)
     static constexpr int kOffBar = kOffRaw + kRaw * 2 * kRawBytes;
-    static constexpr int kSmemBytes = kOffBar + 160;
-    static constexpr int kColO = BK, kColP = BK + HD;    // of tensor memory: S, O, two of P
-    static_assert(BK + HD + BK <= kTmemCols, "tensor memory");
+    static constexpr int kSmemBytes = kOffBar + 256;
+    static constexpr int kColO = BK, kColP = BK + HD;    // of a tile's tensor memory: S, O, two of P
+    static_assert(BK + HD + BK <= kTileCols, "tensor memory");
     static constexpr int kPieces = BK * HD / 16;         // of 16 codes in a step's keys (or values)
-    static constexpr int kMine = kPieces / (32 * kConvWarps);
-    static_assert(kPieces % (32 * kConvWarps) == 0, "pieces are dealt evenly");
 };
 
 // kind::f16, half operands, both K-major, float sums.
@@ -139,66 +139,72 @@ __device__ __forceinline__ void warp_umma_commit(uint32_t bar) {
                  "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar) : "memory");
 }
 
-// grid: (kv heads, sequences, tiles of query rows), the longest tiles first.
+// grid: (kv heads, sequences, pairs of tiles of query rows), the longest first.
 template <int HD, bool kTest>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 1)
 attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     using S = Shape<HD>;
     extern __shared__ __align__(1024) unsigned char smem[];
     const int h = blockIdx.x, b = blockIdx.y;
-    const int tile = gridDim.z - 1 - blockIdx.z;
+    const int row_begin = (gridDim.z - 1 - blockIdx.z) * 2 * BQ;
     const int q_begin = a.cu_seqlens[b];
     const int q_len = a.cu_seqlens[b + 1] - q_begin;
     const int n_rows = q_len * a.group;
-    if (tile * BQ >= n_rows) return;                             // before any barrier or tensor memory
+    if (row_begin >= n_rows) return;                             // before any barrier or tensor memory
     const uint32_t base = smem_addr(smem);
     if (base & 1023u) {
         if (threadIdx.x == 0) atomicExch(&g_status, 2);
         return;
     }
     const uint32_t bars = base + S::kOffBar;
-    // A step's scores and products have barriers by the step's parity: S of step i also frees its key tile, P V its values and P.
-    const uint32_t q_full = bars, s_free = bars + 8, l_full = bars + 16;
-    auto s_full = [&](int i) { return bars + 32u + 8u * (i & 1); };
-    auto p_full = [&](int i) { return bars + 48u + 8u * (i & 1); };
-    auto pv_done = [&](int i) { return bars + 64u + 8u * (i & 1); };
-    auto k_full = [&](int i) { return bars + 80u + 8u * (i & 1); };
-    auto v_full = [&](int i) { return bars + 96u + 8u * (i & 1); };
-    auto phase = [](int i) { return ((uint32_t)i >> 1) & 1u; };  // of step i's barriers
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + S::kOffBar + 128);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kOffBar + 136);
-    volatile int* odd_flag = reinterpret_cast<volatile int*>(smem + S::kOffBar + 140);   // a NaN code in a page not all rows see whole
+    // by tile: queries there, scores read; by tile and the step's parity: scores there, P there, P V done; by parity: key and
+    // value tiles there and free
+    auto q_full = [&](int t) { return bars + 8u * t; };
+    auto s_free = [&](int t) { return bars + 16u + 8u * t; };
+    auto s_full = [&](int t) { return bars + 32u + 8u * t; };
+    auto p_full = [&](int t, int i) { return bars + 48u + 16u * t + 8u * (i & 1); };
+    auto pv_done = [&](int t, int i) { return bars + 80u + 16u * t + 8u * (i & 1); };
+    auto k_full = [&](int i) { return bars + 112u + 8u * (i & 1); };
+    auto k_free = [&](int i) { return bars + 128u + 8u * (i & 1); };
+    auto v_full = [&](int i) { return bars + 144u + 8u * (i & 1); };
+    auto v_free = [&](int i) { return bars + 160u + 8u * (i & 1); };
+    auto phase = [](int i) { return ((uint32_t)i >> 1) & 1u; };  // of step i's barriers that go by parity
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + S::kOffBar + 192);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kOffBar + 200);
+    volatile int* odd_flag = reinterpret_cast<volatile int*>(smem + S::kOffBar + 204);   // a NaN code in a page not all rows see whole
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int slot = a.slots[b];
     const int start = a.start_pos[b] - (kv.dropped ? kv.dropped[slot] : 0);
     const int* table = kv.block_table + (size_t)slot * kv.table_stride;
-    const int row0 = tile * BQ;
-    const int rows_here = min(BQ, n_rows - row0);
-    const int first_at = start + row0 / a.group;                 // cache row of the tile's first query, and of its last
-    const int last_at = start + (row0 + rows_here - 1) / a.group;
-    const int k_min = a.window > 0 ? max(0, first_at - a.window + 1) : 0;
-    const int j_lo = k_min / kPageTokens, n_steps = last_at / kPageTokens - j_lo + 1;
-    auto page_not_whole = [&](int j) {                           // a page that not every query of the tile sees whole
+    const int n_tiles = n_rows - row_begin > BQ ? 2 : 1;
+    const int first_at = start + row_begin / a.group;            // cache row of the block's first query, and of its last
+    const int last_at = start + (min(row_begin + 2 * BQ, n_rows) - 1) / a.group;
+    const int j_lo = (a.window > 0 ? max(0, first_at - a.window + 1) : 0) / kPageTokens;
+    const int steps_last = last_at / kPageTokens - j_lo + 1;     // of the last tile; an earlier one may see less
+    const int steps_first = n_tiles == 2 ? (start + (row_begin + BQ - 1) / a.group) / kPageTokens - j_lo + 1 : steps_last;
+    auto page_not_whole = [&](int j) {                           // a page that not every query of the block sees whole
         return j * kPageTokens + kPageTokens - 1 > first_at || (a.window > 0 && j * kPageTokens <= last_at - a.window);
     };
 
     if (threadIdx.x == 0) {
-        mbar_init(q_full, kSoftmaxWarps);
-        mbar_init(s_free, kSoftmaxWarps);
-        mbar_init(l_full, kSoftmaxWarps);
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(s_full(s), 1);
-            mbar_init(p_full(s), kSoftmaxWarps);
-            mbar_init(pv_done(s), 1);
-            mbar_init(k_full(s), kConvWarps);
-            mbar_init(v_full(s), kConvWarps);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(q_full(t), 4);
+            mbar_init(s_free(t), 4);
+            mbar_init(s_full(t), 1);
+            for (int i = 0; i < 2; ++i) { mbar_init(p_full(t, i), 4); mbar_init(pv_done(t, i), 1); }
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(k_full(i), kKeyWarps);
+            mbar_init(k_free(i), n_tiles);
+            mbar_init(v_full(i), kValueWarps);
+            mbar_init(v_free(i), n_tiles);
         }
         *abort_flag = 0;
         *odd_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::);
     }
-    if (warp == kProductWarp) {
+    if (warp == kScoreWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n"
                      ::"r"(smem_addr(tmem_holder)), "r"(kTmemCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
@@ -206,60 +212,47 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-    const uint32_t tmem_s = *tmem_holder, tmem_o = tmem_s + S::kColO, tmem_p = tmem_s + S::kColP;
+    const uint32_t tmem = *tmem_holder;
     chain_wait();                                                // queries and the newest rows come from the kernel before
     chain_release();
+    // (a wait's answer is the whole warp's before anything is issued: an elected lane waits for all)
+    auto all_wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_sleep<kTest>(bar, parity, abort_flag)); };
 
-    if (warp > kProductWarp) {
-        // ------------------------------------------------------------ codes to halves
-        const int t = threadIdx.x - 32 * (kProductWarp + 1);
+    // ---- codes to halves: two warps the keys, two the values
+    auto convert = [&](auto of_values, const int t) {
+        constexpr bool values = decltype(of_values)::value;
+        constexpr int threads = 32 * (values ? kValueWarps : kKeyWarps), mine = (S::kPieces + threads - 1) / threads;
         const int total = start + q_len;                         // rows that exist after this step
         // The codes come by asynchronous copies, kRaw steps ahead, each 16-byte piece to a place that only the lane that will
         // convert it reads: nothing is waited for but a lane's own copies.  Page numbers are read 32 steps at a time.
         int pages = 0;                                           // lane l: page of step (asked / 32 * 32 + l)
-        auto slot_of = [&](int i, int values, int m) { return base + S::kOffRaw + ((i % S::kRaw) * 2 + values) * S::kRawBytes + (t + 32 * kConvWarps * m) * 16; };
-        const uint8_t* k_at = kv.k + (size_t)h * kPageTokens * HD + t * 16;
-        const uint8_t* v_at = kv.v + (size_t)h * kPageTokens * HD + t * 16;
-        auto ask = [&](int i, int values) {
-            if (i < n_steps) {
-                if (!values && (i & 31) == 0) pages = i + lane < n_steps ? table[j_lo + i + lane] : 0;
-                const size_t page = __shfl_sync(0xffffffffu, pages, i & 31);
-                const uint8_t* at = values ? v_at + page * kv.v_stride : k_at + page * kv.k_stride;
+        auto slot_of = [&](int i, int id) { return base + S::kOffRaw + ((i % S::kRaw) * 2 + values) * S::kRawBytes + id * 16; };
+        const uint8_t* source = (values ? kv.v : kv.k) + (size_t)h * kPageTokens * HD + t * 16;
+        const long long stride = values ? kv.v_stride : kv.k_stride;
+        auto ask = [&](int i) {
+            if (i < steps_last) {
+                if ((i & 31) == 0) pages = i + lane < steps_last ? table[j_lo + i + lane] : 0;
+                const uint8_t* at = source + (size_t)__shfl_sync(0xffffffffu, pages, i & 31) * stride;
 #pragma unroll
-                for (int m = 0; m < S::kMine; ++m) copy_async16(slot_of(i, values, m), at + 32 * kConvWarps * m * 16);
+                for (int m = 0; m < mine; ++m)
+                    if (t + threads * m < S::kPieces) copy_async16(slot_of(i, t + threads * m), at + threads * m * 16);
             }
             asm volatile("cp.async.commit_group;\n" ::);
         };
-        // (keys of step i + kRaw are asked for between values of steps i - 1 + kRaw and i + kRaw: the 32 page numbers of a
-        // stretch serve its keys and its values alike)
-        for (int i = 0; i < S::kRaw; ++i) { ask(i, 0); ask(i, 1); }
-        for (int i = 0; i < n_steps; ++i) {
-            const int s = i % S::kKeyTiles, sv = i % S::kValueTiles;
-            uint4 u[S::kMine];
-            asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S::kRaw - 1) : "memory");
+        for (int i = 0; i < S::kRaw; ++i) ask(i);
+        for (int i = 0; i < steps_last; ++i) {
+            uint4 u[mine];
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(S::kRaw - 1) : "memory");
 #pragma unroll
-            for (int m = 0; m < S::kMine; ++m) u[m] = load_shared16(slot_of(i, 0, m));
-            if (i >= 2 && !__all_sync(0xffffffffu, mbar_sleep<kTest>(s_full(i), phase(i - 2), abort_flag))) break;
-            const uint32_t kt = base + S::kOffK + s * S::kTileBytes;
-#pragma unroll
-            for (int m = 0; m < S::kMine; ++m) {
-                const int id = t + 32 * kConvWarps * m, row = id / (HD / 16), piece = id % (HD / 16);
-                store_halves(kt + (piece / 4) * (BK * 128) + row * 128, piece % 4 * 2, row & 7, u[m]);
-            }
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            __syncwarp();
-            if (lane == 0 && !Waits<kTest>::kSkipCopies) mbar_arrive(k_full(i));
-            ask(i + S::kRaw, 0);
-            asm volatile("cp.async.wait_group %0;\n" ::"n"(2 * S::kRaw - 1) : "memory");
-#pragma unroll
-            for (int m = 0; m < S::kMine; ++m) u[m] = load_shared16(slot_of(i, 1, m));
+            for (int m = 0; m < mine; ++m)
+                if (t + threads * m < S::kPieces) u[m] = load_shared16(slot_of(i, t + threads * m));
             const int j = j_lo + i;
-            if (page_not_whole(j)) {
+            if (values && page_not_whole(j)) {
                 // Rows nobody has written yet become zeros; so do NaN codes, which P's zeros would not silence: who does see them
                 // gets them back at the end.
 #pragma unroll
-                for (int m = 0; m < S::kMine; ++m) {
-                    const int at = j * kPageTokens + (t + 32 * kConvWarps * m) % 4 * 16;       // rows at .. at + 15
+                for (int m = 0; m < mine; ++m) {
+                    const int at = j * kPageTokens + (t + threads * m) % 4 * 16;                // rows at .. at + 15
                     uint32_t w[4] = {u[m].x, u[m].y, u[m].z, u[m].w};
                     uint32_t found = 0;
 #pragma unroll
@@ -270,73 +263,98 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                         found |= nan;
                         w[c] &= ~nan;
                     }
-                    if (found) *odd_flag = 1;
+                    if (found && t + threads * m < S::kPieces) *odd_flag = 1;
                     u[m] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
-            const int before = i - S::kValueTiles;               // whose values lie there
-            if (before >= 0 && !__all_sync(0xffffffffu, mbar_sleep<kTest>(pv_done(before), phase(before), abort_flag))) break;
-            const uint32_t vt = base + S::kOffV + sv * S::kTileBytes;
+            if (i >= 2 && !all_wait(values ? v_free(i) : k_free(i), phase(i - 2))) break;
+            const uint32_t tile = base + (values ? S::kOffV : S::kOffK) + (i & 1) * S::kTileBytes;
 #pragma unroll
-            for (int m = 0; m < S::kMine; ++m) {
-                const int id = t + 32 * kConvWarps * m, channel = id / 4, piece = id % 4;
-                store_halves(vt + channel * 128, piece * 2, channel & 7, u[m]);
+            for (int m = 0; m < mine; ++m) {
+                const int id = t + threads * m;
+                if (id >= S::kPieces) continue;
+                if (values) store_halves(tile + id / 4 * 128, id % 4 * 2, id / 4 & 7, u[m]);
+                else store_halves(tile + id % (HD / 16) / 4 * (BK * 128) + id / (HD / 16) * 128, id % 4 * 2, id / (HD / 16) & 7, u[m]);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
-            if (lane == 0 && !Waits<kTest>::kSkipCopies) mbar_arrive(v_full(i));
-            ask(i + S::kRaw, 1);
+            if (lane == 0 && !Waits<kTest>::kSkipCopies) mbar_arrive(values ? v_full(i) : k_full(i));
+            ask(i + S::kRaw);
         }
         asm volatile("cp.async.wait_group 0;\n" ::);
-    } else if (warp == kProductWarp) {
-        // ------------------------------------------------------------ products
-        constexpr uint32_t idesc_s = f16_idesc(BQ, BK), idesc_pv = f16_idesc(BQ, HD);
-        const uint64_t q_desc = umma_desc(base), k_desc = umma_desc(base + S::kOffK), v_desc = umma_desc(base + S::kOffV);
-        // (a wait's answer is the whole warp's before anything is issued: the elected lane waits for all)
-        auto all_wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_sleep<kTest>(bar, parity, abort_flag)); };
-        auto issue_s = [&](int i) {
-            if (!all_wait(k_full(i), phase(i))) return false;
-            asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-            const uint64_t dk = k_desc + (uint64_t)(i % S::kKeyTiles * (S::kTileBytes >> 4));
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk)
-                warp_umma_ss(tmem_s, q_desc + (kk / 4) * (BQ * 128 >> 4) + 2 * (kk % 4), dk + (kk / 4) * (BK * 128 >> 4) + 2 * (kk % 4), idesc_s, kk > 0 ? 1u : 0u);
-            warp_umma_commit(s_full(i));
-            return true;
-        };
-        bool ok = all_wait(q_full, 0) && issue_s(0);
-        for (int i = 0; i < n_steps && ok; ++i) {
-            if (i + 1 < n_steps) {
-                ok = all_wait(s_free, (uint32_t)i & 1u) && issue_s(i + 1);
+    };
+    if (warp >= 8 + kKeyWarps && warp < kScoreWarp) {
+        convert(std::true_type(), (int)threadIdx.x - 32 * (8 + kKeyWarps));
+    } else if (warp >= 8 && warp < kScoreWarp) {
+        convert(std::false_type(), (int)threadIdx.x - 32 * 8);
+    } else if (warp >= kScoreWarp) {
+        // ------------------------------------------------------------ products: a warp a tile for the scores, another for P V.
+        // A tile that sees fewer pages than the block's last one lets the rest of its tiles' places go as they come.
+        const int t = (warp - kScoreWarp) & 1;
+        const int n_steps = t == n_tiles - 1 ? steps_last : steps_first;
+        if (t >= n_tiles) {
+        } else if (warp < kOutputWarp) {
+            constexpr uint32_t idesc = f16_idesc(BQ, BK);
+            const uint64_t dq = umma_desc(base + t * S::kQBytes), k_desc = umma_desc(base + S::kOffK);
+            bool ok = all_wait(q_full(t), 0);
+            for (int i = 0; i < steps_last && ok; ++i) {
+                ok = all_wait(k_full(i), phase(i));
                 if (!ok) break;
-            }
-            ok = all_wait(v_full(i), phase(i)) && all_wait(p_full(i), phase(i));
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-            const uint64_t dv = v_desc + (uint64_t)(i % S::kValueTiles * (S::kTileBytes >> 4));
-            const uint32_t p_at = tmem_p + 32 * (i & 1);
+                if (i >= n_steps) {
+                    if (lane == 0) mbar_arrive(k_free(i));
+                    continue;
+                }
+                if (i > 0) ok = all_wait(s_free(t), (uint32_t)(i - 1) & 1u);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
+                const uint64_t dk = k_desc + (uint64_t)((i & 1) * (S::kTileBytes >> 4));
 #pragma unroll
-            for (int kk = 0; kk < BK / 16; ++kk) warp_umma_ts(tmem_o, p_at + 8 * kk, dv + 2 * kk, idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
-            warp_umma_commit(pv_done(i));
+                for (int kk = 0; kk < HD / 16; ++kk)
+                    warp_umma_ss(tmem + t * kTileCols, dq + (kk / 4) * (BQ * 128 >> 4) + 2 * (kk % 4), dk + (kk / 4) * (BK * 128 >> 4) + 2 * (kk % 4), idesc,
+                                 kk > 0 ? 1u : 0u);
+                warp_umma_commit(s_full(t));
+                warp_umma_commit(k_free(i));
+            }
+        } else {
+            constexpr uint32_t idesc = f16_idesc(BQ, HD);
+            const uint64_t v_desc = umma_desc(base + S::kOffV);
+            bool ok = true;
+            for (int i = 0; i < steps_last && ok; ++i) {
+                ok = all_wait(v_full(i), phase(i));
+                if (!ok) break;
+                if (i >= n_steps) {
+                    if (lane == 0) mbar_arrive(v_free(i));
+                    continue;
+                }
+                ok = all_wait(p_full(t, i), phase(i));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
+                const uint64_t dv = v_desc + (uint64_t)((i & 1) * (S::kTileBytes >> 4));
+                const uint32_t p_at = tmem + t * kTileCols + S::kColP + 32 * (i & 1);
+#pragma unroll
+                for (int kk = 0; kk < BK / 16; ++kk) warp_umma_ts(tmem + t * kTileCols + S::kColO, p_at + 8 * kk, dv + 2 * kk, idesc, (i > 0 || kk > 0) ? 1u : 0u);
+                warp_umma_commit(pv_done(t, i));
+                warp_umma_commit(v_free(i));
+            }
         }
-    } else {
-        // ------------------------------------------------------------ softmax and output: two threads a query row, 32 columns each.
-        // Both find the maximum of the whole row (its scores are cheap to read, a second thread's answer is not), so neither
-        // waits for the other before the end.
+    } else if (warp / 4 < n_tiles) {
+        // ------------------------------------------------------------ softmax and output: a thread a query row
         const unsigned full = 0xffffffffu;
-        const int half = warp >> 2, r = (warp & 3) * 32 + lane;
-        const bool real = r < rows_here;
+        const int tt = warp >> 2, r = (warp & 3) * 32 + lane;
+        const int row0 = row_begin + tt * BQ, n_steps = tt == n_tiles - 1 ? steps_last : steps_first;
+        const bool real = row0 + r < n_rows;
         const int token = (row0 + (real ? r : 0)) / a.group, head = h * a.group + (row0 + (real ? r : 0)) % a.group;
         const int pos = start + token;                            // the query's own cache row
-        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tile_at = tmem + tt * kTileCols + ((uint32_t)((warp & 3) * 32) << 16);
         float factor;                                             // a raw score times this and the page's key scale: powers of two
         {
             const bf16* src = a.q + (size_t)(q_begin + token) * a.ldq + (size_t)head * HD;
+            uint4 u[HD / 8];
             float most = 0.f;
 #pragma unroll
             for (int c = 0; c < HD / 8; ++c) {
-                const uint4 u = real ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                u[c] = real ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+                const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float lo = fabsf(__uint_as_float(w[e] << 16)), hi = fabsf(__uint_as_float(w[e] & 0xffff0000u));
@@ -349,25 +367,24 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             const float f = __uint_as_float((uint32_t)(127 + up) << 23) * (a.scale < 0.f ? -1.f : 1.f);
             factor = fmaxf(fabsf(a.scale) * kLog2e * __uint_as_float((uint32_t)(127 - up) << 23), 1e-37f);
 #pragma unroll
-            for (int c = half * (HD / 16); c < (half + 1) * (HD / 16); ++c) {
-                const uint4 u = real ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            for (int c = 0; c < HD / 8; ++c) {
+                const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
                 uint32_t o[4];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     const __half2 hh = __floats2half2_rn(__uint_as_float(w[x] << 16) * f, __uint_as_float(w[x] & 0xffff0000u) * f);
                     o[x] = *reinterpret_cast<const uint32_t*>(&hh);
                 }
-                store_shared16(base + (c / 8) * (BQ * 128) + r * 128 + (((c % 8) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
+                store_shared16(base + tt * S::kQBytes + (c / 8) * (BQ * 128) + r * 128 + (((c % 8) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
+            if (lane == 0) mbar_arrive(q_full(tt));
         }
         // scales, 32 steps at a time: lane l has those of step (i / 32 * 32 + l)
         float k_scales = 0.f, v_scales = 1.f;
         float m_run = -INFINITY, l_run = 0.f;
-        uint32_t sv[32];
+        uint32_t sv[BK];
         bool ok = true;
         for (int i = 0; i < n_steps; ++i) {
             const int key0 = (j_lo + i) * kPageTokens;
@@ -379,37 +396,37 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             const float sl = factor * __shfl_sync(full, k_scales, i & 31);
             const float v_scale = __shfl_sync(full, v_scales, i & 31);
             const float add = (float)((int)(__float_as_uint(v_scale) >> 23) - 127);             // log2 of the value scale
-            ok = __all_sync(full, mbar_sleep<kTest>(s_full(i), phase(i), abort_flag));
+            ok = all_wait(s_full(tt), (uint32_t)i & 1u);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-            uint32_t other[32];
-            tmem_ld32(tmem_s + lane_off + 32 * half, sv);
-            tmem_ld32(tmem_s + lane_off + 32 * (half ^ 1), other);
+            tmem_ld32(tile_at, sv);
+            tmem_ld32(tile_at + 32, sv + 32);
             asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
             __syncwarp();
-            if (lane == 0) mbar_arrive(s_free);                  // the scores are in registers: the tile takes the next step's
+            if (lane == 0) mbar_arrive(s_free(tt));              // the scores are in registers: the tile takes the next step's
             if (!(key0 + BK - 1 <= pos && (a.window <= 0 || key0 > pos - a.window))) {
                 const int hi = pos - key0, lo = a.window > 0 ? pos - a.window - key0 : -1;       // columns lo + 1 .. hi are seen
 #pragma unroll
-                for (int c = 0; c < 32; ++c) {
-                    const int mine = 32 * half + c, its = 32 * (half ^ 1) + c;
-                    if (mine > hi || mine <= lo) sv[c] = __float_as_uint(-INFINITY);
-                    if (its > hi || its <= lo) other[c] = __float_as_uint(-INFINITY);
-                }
+                for (int c = 0; c < BK; ++c)
+                    if (c > hi || c <= lo) sv[c] = __float_as_uint(-INFINITY);
             }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float mx[8];
 #pragma unroll
-            for (int c = 0; c < 32; c += 4)
+            for (int e = 0; e < 8; ++e) mx[e] = max3(__uint_as_float(sv[e]), __uint_as_float(sv[8 + e]), __uint_as_float(sv[16 + e]));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sv[c + e]), __uint_as_float(other[c + e]));
-            const float m_step = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), sl, add);
+            for (int c = 24; c < 56; c += 16)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx[e] = max3(mx[e], __uint_as_float(sv[c + e]), __uint_as_float(sv[c + 8 + e]));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sv[56 + e]), __uint_as_float(sv[60 + e]));
+            const float m_step = fmaf(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])), sl, add);
             if (i == 0) {
                 m_run = m_step;
             } else {
                 const bool raise = m_step > m_run + kRaiseBy;    // also: the first visible row of a query
                 if (__any_sync(full, raise)) {
-                    ok = __all_sync(full, mbar_sleep<kTest>(pv_done(i - 1), phase(i - 1), abort_flag));
+                    ok = all_wait(pv_done(tt, i - 1), phase(i - 1));
                     if (!ok) break;
                     float corr = 1.0f;
                     if (raise) {
@@ -420,20 +437,20 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
                     uint32_t ov[8];
 #pragma unroll 1
-                    for (int part = half * (HD / 16); part < (half + 1) * (HD / 16); ++part) {   // its half of the row of O
-                        tmem_ld8(tmem_o + lane_off + 8 * part, ov);
+                    for (int part = 0; part < HD / 8; ++part) {
+                        tmem_ld8(tile_at + S::kColO + 8 * part, ov);
                         asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
                         for (int d = 0; d < 8; ++d) ov[d] = __float_as_uint(__uint_as_float(ov[d]) * corr);
-                        tmem_st8(tmem_o + lane_off + 8 * part, ov);
+                        tmem_st8(tile_at + S::kColO + 8 * part, ov);
                     }
                 }
             }
             const float shift = add - (m_run == -INFINITY ? 0.f : m_run) + kPShift;
             const uint64_t sl2 = two(sl, sl), shift2 = two(shift, shift);
-            uint64_t sums[2] = {0, 0};
+            uint64_t sums[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < 32; c += 8) {                     // scores c .. c + 7 become words c / 2 .. c / 2 + 3
+            for (int c = 0; c < BK; c += 8) {                     // scores c .. c + 7 become words c / 2 .. c / 2 + 3
                 uint64_t x[4];
                 float p[8];
 #pragma unroll
@@ -442,42 +459,33 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                 for (int e = 0; e < 4; ++e) { p[2 * e] = exp2_in_order(first_of(x[e])); p[2 * e + 1] = exp2_in_order(second_of(x[e])); }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    sums[e & 1] = add2(sums[e & 1], two(p[2 * e], p[2 * e + 1]));
+                    sums[e] = add2(sums[e], two(p[2 * e], p[2 * e + 1]));
                     const __half2 hh = __floats2half2_rn(p[2 * e], p[2 * e + 1]);
                     sv[c / 2 + e] = *reinterpret_cast<const uint32_t*>(&hh);
                 }
             }
-            sums[0] = add2(sums[0], sums[1]);
+            sums[0] = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
             l_run = fmaf(first_of(sums[0]) + second_of(sums[0]), pow2_inverse(v_scale), l_run);
             if (i > 1) {                                          // the P of two steps ago has been read
-                ok = __all_sync(full, mbar_sleep<kTest>(pv_done(i), phase(i - 2), abort_flag));
+                ok = all_wait(pv_done(tt, i), phase(i - 2));
                 if (!ok) break;
             }
-            tmem_st16(tmem_p + 32 * (i & 1) + lane_off + 16 * half, sv);
+            tmem_st32(tile_at + S::kColP + 32 * (i & 1), sv);
             asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full(i));
+            if (lane == 0) mbar_arrive(p_full(tt, i));
         }
-        // ---- the row's sum, of both threads; each writes its half of the channels
-        if (ok) ok = __all_sync(full, mbar_sleep<kTest>(pv_done(n_steps - 1), phase(n_steps - 1), abort_flag));
-        float* ls = reinterpret_cast<float*>(smem + S::kOffRaw);  // (all codes have been read: the last product is done)
-        if (ok) {
-            ls[half * BQ + r] = l_run;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(l_full);
-            ok = __all_sync(full, mbar_sleep<kTest>(l_full, 0, abort_flag));
-        }
+        if (ok) ok = all_wait(pv_done(tt, n_steps - 1), phase(n_steps - 1));
         if (ok) {
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-            const float l_row = ls[r] + ls[BQ + r], inv = 1.0f / l_row;
-            if (a.stats && real && half == 0)
-                a.stats[(size_t)(q_begin + token) * a.n_heads + head] = make_float2((m_run == -INFINITY ? 0.f : m_run) - kPShift, l_row);
+            const float inv = 1.0f / l_run;
+            if (a.stats && real) a.stats[(size_t)(q_begin + token) * a.n_heads + head] = make_float2((m_run == -INFINITY ? 0.f : m_run) - kPShift, l_run);
             bf16* dst = a.out + (size_t)(q_begin + token) * a.ldo + (size_t)head * HD;
             const bool odd = *odd_flag != 0;
 #pragma unroll 1
-            for (int c = half * (HD / 64); c < (half + 1) * (HD / 64); ++c) {
-                tmem_ld32(tmem_o + lane_off + 32 * c, sv);
+            for (int c = 0; c < HD / 32; ++c) {
+                tmem_ld32(tile_at + S::kColO + 32 * c, sv);
                 asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
                 if (odd && real) {
                     // NaN codes of rows that this query sees, in pages where they were taken out
@@ -485,10 +493,10 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                         if (!page_not_whole(j)) continue;
                         const uint8_t* vp = kv.v + (size_t)table[j] * kv.v_stride + ((size_t)h * HD + 32 * c) * kPageTokens;
                         const int lo = a.window > 0 ? max(0, pos - a.window + 1 - j * kPageTokens) : 0, hi = min(pos - j * kPageTokens, kPageTokens - 1);
-                        for (int tt = lo; tt <= hi; ++tt)
+                        for (int row = lo; row <= hi; ++row)
 #pragma unroll
                             for (int d = 0; d < 32; ++d)
-                                if ((vp[d * kPageTokens + tt] & 0x7f) == 0x7f) sv[d] = 0x7fc00000u;
+                                if ((vp[d * kPageTokens + row] & 0x7f) == 0x7f) sv[d] = 0x7fc00000u;
                     }
                 }
                 if (real) {
@@ -508,9 +516,9 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
     __syncthreads();
-    if (warp == kProductWarp) {
+    if (warp == kScoreWarp) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem_s), "r"(kTmemCols));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols));
     }
 }
 
@@ -523,7 +531,7 @@ int launch(const PromptArgs& a, const E4M3Pages& kv, int B, int max_q_len, cudaS
         configured = true;
     }
     const long long rows = (long long)max_q_len * a.group;
-    return launch_chained(attention_e4m3_prompt_kernel<HD, kTest>, dim3(kv.n_kv, B, (unsigned)((rows + BQ - 1) / BQ)), dim3(kThreads),
+    return launch_chained(attention_e4m3_prompt_kernel<HD, kTest>, dim3(kv.n_kv, B, (unsigned)((rows + 2 * BQ - 1) / (2 * BQ))), dim3(kThreads),
                           (size_t)Shape<HD>::kSmemBytes, stream, a, kv);
 }
 // ============================================================== gathered weights of prompts and chunks
@@ -535,6 +543,7 @@ int launch(const PromptArgs& a, const E4M3Pages& kv, int B, int max_q_len, cudaS
 //   sums   four warps, S from tensor memory, 1 / l folded into the exponent: one multiply-add, one exponential and one add a
 //          score.  The exponentials bound it (16 a cycle).
 // Nothing is shared between blocks, so a weight does not depend on what else runs.
+constexpr int kWeightCols = 256;
 constexpr int kWeightThreads = 192;                      // sums 0-3, copies 4, products 5
 template <int HD> struct WeightShape {
     static constexpr int kStages = HD == 64 ? 3 : 2;
@@ -588,7 +597,7 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
     }
     if (warp == 5) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n"
-                     ::"r"(smem_addr(tmem_holder)), "r"(kTmemCols));
+                     ::"r"(smem_addr(tmem_holder)), "r"(kWeightCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
@@ -737,7 +746,7 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
     __syncthreads();
     if (warp == 5) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kWeightCols));
     }
 }
 
