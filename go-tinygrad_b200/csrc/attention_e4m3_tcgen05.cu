@@ -32,7 +32,7 @@ constexpr int kKeyWarps = 2, kValueWarps = 2, kScoreWarp = 12, kOutputWarp = 14;
 constexpr int kThreads = 512;
 constexpr int kTmemCols = 512, kTileCols = 256;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRaiseBy = 8.0f, kPShift = 7.0f;
+constexpr float kPShift = 7.0f, kMostSum = 32768.0f;
 
 template <int HD> struct Shape {
     static constexpr int kRaw = HD == 64 ? 6 : 4;        // steps of codes on their way
@@ -79,6 +79,21 @@ __device__ __forceinline__ bool mbar_sleep(uint32_t bar, uint32_t parity, volati
         uint32_t done;
         asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
                      "selp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity), "r"(10000u) : "memory");
+        if (done) return true;
+        if (*abort_flag) return false;
+    }
+    *abort_flag = 1;
+    atomicExch(&g_status, 1);
+    return false;
+}
+// Two phases at once: their answers are asked for side by side.
+template <bool kTest>
+__device__ __forceinline__ bool mbar_sleep_both(uint32_t bar, uint32_t parity, uint32_t other, uint32_t other_parity, volatile int* abort_flag) {
+    for (unsigned i = 0; i < (kTest ? 64u : 1u << 18); ++i) {
+        uint32_t done;
+        asm volatile("{\n.reg .pred p, q;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %5;\n"
+                     "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4, %5;\nand.pred p, p, q;\n"
+                     "selp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity), "r"(other), "r"(other_parity), "r"(10000u) : "memory");
         if (done) return true;
         if (*abort_flag) return false;
     }
@@ -396,7 +411,9 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             const float sl = factor * __shfl_sync(full, k_scales, i & 31);
             const float v_scale = __shfl_sync(full, v_scales, i & 31);
             const float add = (float)((int)(__float_as_uint(v_scale) >> 23) - 127);             // log2 of the value scale
-            ok = all_wait(s_full(tt), (uint32_t)i & 1u);
+            // the step's scores; and the P of two steps ago has been read
+            ok = i < 2 ? all_wait(s_full(tt), (uint32_t)i & 1u)
+                       : (bool)__all_sync(full, mbar_sleep_both<kTest>(s_full(tt), (uint32_t)i & 1u, pv_done(tt, i), phase(i - 2), abort_flag));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
             tmem_ld32(tile_at, sv);
@@ -411,33 +428,55 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                 for (int c = 0; c < BK; ++c)
                     if (c > hi || c <= lo) sv[c] = __float_as_uint(-INFINITY);
             }
-            float mx[8];
+            // P against the maximum so far, without looking for the step's own: if none of the 64 exceeds 2^15 no sum of
+            // them does that half could not hold.  Only where the sum does -- and for a row that has seen nothing yet -- is
+            // the maximum found and the step done again.
+            uint32_t pw[BK / 2];
+            uint64_t sum;
+            auto exponentials = [&]() {
+                const float shift = add - (m_run == -INFINITY ? 0.f : m_run) + kPShift;
+                const uint64_t sl2 = two(sl, sl), shift2 = two(shift, shift);
+                uint64_t sums[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mx[e] = max3(__uint_as_float(sv[e]), __uint_as_float(sv[8 + e]), __uint_as_float(sv[16 + e]));
+                for (int c = 0; c < BK; c += 8) {
+                    uint64_t x[4];
+                    float p[8];
 #pragma unroll
-            for (int c = 24; c < 56; c += 16)
+                    for (int e = 0; e < 4; ++e) x[e] = fma2(two(__uint_as_float(sv[c + 2 * e]), __uint_as_float(sv[c + 2 * e + 1])), sl2, shift2);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) mx[e] = max3(mx[e], __uint_as_float(sv[c + e]), __uint_as_float(sv[c + 8 + e]));
+                    for (int e = 0; e < 4; ++e) { p[2 * e] = exp2_in_order(first_of(x[e])); p[2 * e + 1] = exp2_in_order(second_of(x[e])); }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sv[56 + e]), __uint_as_float(sv[60 + e]));
-            const float m_step = fmaf(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])), sl, add);
-            if (i == 0) {
-                m_run = m_step;
-            } else {
-                const bool raise = m_step > m_run + kRaiseBy;    // also: the first visible row of a query
-                if (__any_sync(full, raise)) {
+                    for (int e = 0; e < 4; ++e) {
+                        sums[e] = add2(sums[e], two(p[2 * e], p[2 * e + 1]));
+                        const __half2 hh = __floats2half2_rn(p[2 * e], p[2 * e + 1]);
+                        pw[c / 2 + e] = *reinterpret_cast<const uint32_t*>(&hh);
+                    }
+                }
+                sum = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
+            };
+            const bool fresh = __any_sync(full, m_run == -INFINITY);
+            if (!fresh) exponentials();
+            if (fresh || __any_sync(full, first_of(sum) + second_of(sum) > kMostSum)) {
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < BK; c += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sv[c + e]), __uint_as_float(sv[c + 4 + e]));
+                const float m_step = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), sl, add);
+                const bool raise = m_step > m_run;
+                float corr = 1.0f;
+                if (raise) {
+                    corr = fast_exp2(m_run - m_step);             // 0 for a row that has seen nothing
+                    m_run = m_step;
+                    l_run *= corr;
+                }
+                if (i > 0) {                                      // O may only be touched between products
                     ok = all_wait(pv_done(tt, i - 1), phase(i - 1));
                     if (!ok) break;
-                    float corr = 1.0f;
-                    if (raise) {
-                        corr = fast_exp2(m_run - m_step);
-                        m_run = m_step;
-                        l_run *= corr;
-                    }
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-                    uint32_t ov[8];
 #pragma unroll 1
                     for (int part = 0; part < HD / 8; ++part) {
+                        uint32_t ov[8];
                         tmem_ld8(tile_at + S::kColO + 8 * part, ov);
                         asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
@@ -445,32 +484,10 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                         tmem_st8(tile_at + S::kColO + 8 * part, ov);
                     }
                 }
+                exponentials();
             }
-            const float shift = add - (m_run == -INFINITY ? 0.f : m_run) + kPShift;
-            const uint64_t sl2 = two(sl, sl), shift2 = two(shift, shift);
-            uint64_t sums[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int c = 0; c < BK; c += 8) {                     // scores c .. c + 7 become words c / 2 .. c / 2 + 3
-                uint64_t x[4];
-                float p[8];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = fma2(two(__uint_as_float(sv[c + 2 * e]), __uint_as_float(sv[c + 2 * e + 1])), sl2, shift2);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { p[2 * e] = exp2_in_order(first_of(x[e])); p[2 * e + 1] = exp2_in_order(second_of(x[e])); }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    sums[e] = add2(sums[e], two(p[2 * e], p[2 * e + 1]));
-                    const __half2 hh = __floats2half2_rn(p[2 * e], p[2 * e + 1]);
-                    sv[c / 2 + e] = *reinterpret_cast<const uint32_t*>(&hh);
-                }
-            }
-            sums[0] = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
-            l_run = fmaf(first_of(sums[0]) + second_of(sums[0]), pow2_inverse(v_scale), l_run);
-            if (i > 1) {                                          // the P of two steps ago has been read
-                ok = all_wait(pv_done(tt, i), phase(i - 2));
-                if (!ok) break;
-            }
-            tmem_st32(tile_at + S::kColP + 32 * (i & 1), sv);
+            l_run = fmaf(first_of(sum) + second_of(sum), pow2_inverse(v_scale), l_run);
+            tmem_st32(tile_at + S::kColP + 32 * (i & 1), pw);
             asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
             __syncwarp();
