@@ -553,13 +553,15 @@ int launch(const PromptArgs& a, const E4M3Pages& kv, int B, int max_q_len, cudaS
 }
 // ============================================================== gathered weights of prompts and chunks
 // weight_j += sum over the queries that see row j, of all heads of the group, of 2^(score - x) / l, x and l the query's
-// statistics that the attention left.  The products again, the other way round: one block per (128 rows of the cache, key/value
+// statistics that the attention left.  The products again, the other way round: one block per (128 rows of the cache, query
 // head, sequence), the rows as the tile's rows, so that a thread owns a row and its sum:
 //   K      converted once to bfloat16 (exact) into shared memory, S = K Q^T by tcgen05.mma 128 x 128 x head size;
 //   Q      128 tokens of one head at a time by tensor copies through a ring, as they are (bfloat16);
 //   sums   four warps, S from tensor memory, 1 / l folded into the exponent: one multiply-add, one exponential and one add a
 //          score.  The exponentials bound it (16 a cycle).
-// Nothing is shared between blocks, so a weight does not depend on what else runs.
+// A block a head of the group leaves its sums beside the others', and a second kernel adds them in the heads' order (a block for
+// all heads: one block's 48 tiles were the time of all, 95 us of 147 for prompts of 200 to 1,500 tokens).  So a weight does
+// not depend on what else runs.
 constexpr int kWeightCols = 256;
 constexpr int kWeightThreads = 192;                      // sums 0-3, copies 4, products 5
 template <int HD> struct WeightShape {
@@ -578,12 +580,14 @@ __device__ __forceinline__ void bf16_of_codes(uint32_t w, uint32_t& lo, uint32_t
     hi = *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// parts: [sequence][query head][part_rows]; rows behind part_rows (a sequence that has outgrown the plan) are done for all heads
+// by the block of the group's first.
 template <int HD, bool kTest>
 __global__ void __launch_bounds__(kWeightThreads, 2)
-e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs a, const E4M3Pages kv) {
+e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs a, const E4M3Pages kv, float* __restrict__ parts, int part_rows) {
     using S = WeightShape<HD>;
     extern __shared__ __align__(1024) unsigned char smem[];
-    const int h = blockIdx.y, b = blockIdx.z;
+    const int h = blockIdx.y / a.group, g0 = blockIdx.y % a.group, b = blockIdx.z;
     const int q_begin = a.cu_seqlens[b];
     const int q_len = a.cu_seqlens[b + 1] - q_begin;
     const int slot = a.slots[b];
@@ -624,13 +628,14 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
     chain_wait();
     chain_release();
 
-    // the tokens that see any of rows 128 kt .. 128 kt + 127: [t_lo, t_hi), cut into tiles for each head of the group
-    struct Span { int t_lo, t_hi, per_head; };
+    // the tokens that see any of rows 128 kt .. 128 kt + 127: [t_lo, t_hi), cut into tiles for each of this block's heads
+    struct Span { int t_lo, t_hi, per_head, heads; };
     auto span_of = [&](int kt) {
         Span s;
+        s.heads = kt * 128 < part_rows ? 1 : g0 == 0 ? a.group : 0;
         s.t_lo = max(0, kt * 128 - start);
         s.t_hi = a.window > 0 ? min((long long)q_len, (long long)kt * 128 + 127 + a.window - start) : q_len;
-        s.per_head = s.t_hi > s.t_lo ? (s.t_hi - s.t_lo + 127) / 128 : 0;
+        s.per_head = s.t_hi > s.t_lo && s.heads > 0 ? (s.t_hi - s.t_lo + 127) / 128 : 0;
         return s;
     };
     int n = 0;                                                   // tiles so far, of all turns
@@ -639,13 +644,13 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
             bool ok = true;
             for (int kt = blockIdx.x; kt * 128 < start + q_len && ok; kt += gridDim.x) {
                 const Span sp = span_of(kt);
-                for (int i = 0; i < sp.per_head * a.group; ++i, ++n) {
+                for (int i = 0; i < sp.per_head * sp.heads; ++i, ++n) {
                     const int s = n % S::kStages;
                     ok = mbar_sleep<kTest>(q_free(s), (((uint32_t)n / S::kStages) & 1u) ^ 1u, abort_flag);
                     if (!ok) break;
                     mbar_expect_tx(q_full(s), S::kTileBytes);
                     for (int hh = 0; hh < HD / 64; ++hh)
-                        tma_load_2d<kTest>(base + S::kOffQ + s * S::kTileBytes + hh * (128 * 128), &map_q, (h * a.group + i / sp.per_head) * HD + 64 * hh,
+                        tma_load_2d<kTest>(base + S::kOffQ + s * S::kTileBytes + hh * (128 * 128), &map_q, (h * a.group + g0 + i / sp.per_head) * HD + 64 * hh,
                                            q_begin + sp.t_lo + i % sp.per_head * 128, q_full(s));
                 }
             }
@@ -658,7 +663,7 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                 const Span sp = span_of(kt);
                 if (sp.per_head == 0) continue;                  // (rows that no query sees: no role takes a turn for them)
                 ok = mbar_sleep<kTest>(k_full, (uint32_t)turn++ & 1u, abort_flag);
-                for (int i = 0; i < sp.per_head * a.group && ok; ++i, ++n) {
+                for (int i = 0; i < sp.per_head * sp.heads && ok; ++i, ++n) {
                     const int s = n % S::kStages, buf = n & 1;
                     ok = mbar_sleep<kTest>(q_full(s), ((uint32_t)n / S::kStages) & 1u, abort_flag) &&
                          mbar_sleep<kTest>(s_free(buf), (((uint32_t)n >> 1) & 1u) ^ 1u, abort_flag);
@@ -684,10 +689,14 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
         bool ok = true;
         for (int kt = blockIdx.x; kt * 128 < start + q_len && ok; kt += gridDim.x) {
             const Span sp = span_of(kt);
-            const int tiles = sp.per_head * a.group;
-            if (tiles == 0) continue;
+            const int tiles = sp.per_head * sp.heads;
             const int row = kt * 128 + r;
-            const bool there = row < start + q_len;
+            const bool there = row < start + q_len, in_parts = kt * 128 < part_rows;
+            float* part = parts + ((size_t)b * a.n_heads + blockIdx.y) * part_rows + row;
+            if (tiles == 0) {
+                if (in_parts) *part = 0.f;
+                continue;
+            }
             // ---- the tile's keys (all products of the turn before are complete: this warp has seen the last one's barrier)
 #pragma unroll
             for (int m = 0; m < HD / 16; ++m) {
@@ -713,7 +722,7 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
             auto statistic = [&](int i) {                        // of tile i's column r: what takes a score to its probability's exponent
                 const int token = sp.t_lo + i % sp.per_head * 128 + r;
                 if (i >= tiles || token >= sp.t_hi) return 0.f;
-                const float2 st = a.stats[(size_t)(q_begin + token) * a.n_heads + h * a.group + i / sp.per_head];
+                const float2 st = a.stats[(size_t)(q_begin + token) * a.n_heads + h * a.group + g0 + i / sp.per_head];
                 return -(st.x + log2f(st.y));
             };
             float mine = statistic(0), total = 0.f;
@@ -756,7 +765,8 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                 if (lane == 0) mbar_arrive(s_free(buf));
                 total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
-            if (ok && there) kv.weights[page * kv.weight_stride + (size_t)h * kPageTokens + row % kPageTokens] += total;
+            if (ok && in_parts) *part = total;
+            else if (ok && there) kv.weights[page * kv.weight_stride + (size_t)h * kPageTokens + row % kPageTokens] += total;
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
@@ -767,16 +777,34 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
     }
 }
 
+// The heads' parts added up, in the heads' order.
+__global__ void __launch_bounds__(256)
+e4m3_weights_sum_kernel(const PromptArgs a, const E4M3Pages kv, const float* __restrict__ parts, int part_rows) {
+    chain_release();
+    chain_wait();
+    const int row = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y, b = blockIdx.z;
+    const int slot = a.slots[b], q_len = a.cu_seqlens[b + 1] - a.cu_seqlens[b];
+    const int start = a.start_pos[b] - (kv.dropped ? kv.dropped[slot] : 0);
+    if (q_len <= 0 || row >= part_rows || row >= start + q_len) return;
+    float sum = 0.f;
+    for (int g = 0; g < a.group; ++g) sum += parts[((size_t)b * a.n_heads + h * a.group + g) * part_rows + row];
+    const size_t page = kv.block_table[(size_t)slot * kv.table_stride + row / kPageTokens];
+    kv.weights[page * kv.weight_stride + (size_t)h * kPageTokens + row % kPageTokens] += sum;
+}
+
 template <int HD, bool kTest>
-int launch_weights(const PromptArgs& a, const E4M3Pages& kv, const CUtensorMap& map_q, int B, int max_kv_len, cudaStream_t stream) {
+int launch_weights(const PromptArgs& a, const E4M3Pages& kv, const CUtensorMap& map_q, int B, int max_kv_len, float* parts, cudaStream_t stream) {
     static bool configured = false;
     if (!configured) {
         const cudaError_t e = cudaFuncSetAttribute(e4m3_weights_kernel<HD, kTest>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightShape<HD>::kSmemBytes);
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
-    return launch_chained(e4m3_weights_kernel<HD, kTest>, dim3((max_kv_len + 127) / 128, kv.n_kv, B), dim3(kWeightThreads),
-                          (size_t)WeightShape<HD>::kSmemBytes, stream, map_q, a, kv);
+    const int part_rows = (max_kv_len + 127) / 128 * 128;
+    const int st = launch_chained(e4m3_weights_kernel<HD, kTest>, dim3(part_rows / 128, a.n_heads, B), dim3(kWeightThreads),
+                                  (size_t)WeightShape<HD>::kSmemBytes, stream, map_q, a, kv, parts, part_rows);
+    if (st != 0) return st;
+    return launch_chained(e4m3_weights_sum_kernel, dim3((part_rows + 255) / 256, kv.n_kv, B), dim3(256), 0, stream, a, kv, (const float*)parts, part_rows);
 }
 }  // namespace
 
@@ -787,15 +815,15 @@ GTG_API int gtg_attention_e4m3_tcgen05_status() {
 }
 
 // Heads of 64 or 128 channels, bfloat16 rows of q and out on 16-byte boundaries.  weights (or null) gather what the rows get;
-// stats: float2 [N][n_heads] of scratch for that.
+// scratch for that: 2 N n_heads floats and n_heads B times max_kv_len rounded up to 128.
 GTG_API int gtg_attention_e4m3_tcgen05(const void* q, int ldq, void* out, int ldo, void* k, long long k_stride, void* v, long long v_stride,
                                        float* scales, long long scale_stride, float* weights, long long weight_stride, const int* block_table,
                                        int table_stride, const int* dropped, const int* cu_seqlens, const int* slots, const int* start_pos, int B,
-                                       int max_q_len, int max_kv_len, int N, int n_heads, int n_kv, int hd, float scale, int window, float* stats,
+                                       int max_q_len, int max_kv_len, int N, int n_heads, int n_kv, int hd, float scale, int window, float* scratch,
                                        cudaStream_t stream) {
     if (B <= 0 || max_q_len <= 0 || N <= 0) return 0;
-    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || window < 0 || max_kv_len <= 0 || (weights && !stats)) return kErrBadArgument;
-    if (n_kv > 65535) return kErrUnsupported;
+    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || window < 0 || max_kv_len <= 0 || (weights && !scratch)) return kErrBadArgument;
+    if (n_heads > 65535) return kErrUnsupported;
     if ((hd != 64 && hd != 128) || ldq % 8 || ldo % 8 || (uintptr_t)q % 16 || (uintptr_t)out % 16) return kErrUnsupported;
     if (B > 65535 || ((long long)max_q_len * (n_heads / n_kv) + BQ - 1) / BQ > 65535) return kErrUnsupported;
     const E4M3Pages kv = {(uint8_t*)k, (uint8_t*)v, k_stride, v_stride, scales, scale_stride, weights, weight_stride, block_table, table_stride, dropped, n_kv, hd};
@@ -803,7 +831,8 @@ GTG_API int gtg_attention_e4m3_tcgen05(const void* q, int ldq, void* out, int ld
     a.q = (const bf16*)q; a.ldq = ldq; a.out = (bf16*)out; a.ldo = ldo;
     a.cu_seqlens = cu_seqlens; a.slots = slots; a.start_pos = start_pos;
     a.n_heads = n_heads; a.group = n_heads / n_kv; a.scale = scale; a.window = window;
-    a.stats = weights ? (float2*)stats : nullptr;
+    a.stats = weights ? (float2*)scratch : nullptr;
+    float* parts = scratch + (weights ? 2 * (size_t)N * n_heads : 0);
     const bool test = g_test_waits;
     const int st = hd == 64 ? (test ? launch<64, true>(a, kv, B, max_q_len, stream) : launch<64, false>(a, kv, B, max_q_len, stream))
                             : (test ? launch<128, true>(a, kv, B, max_q_len, stream) : launch<128, false>(a, kv, B, max_q_len, stream));
@@ -811,8 +840,8 @@ GTG_API int gtg_attention_e4m3_tcgen05(const void* q, int ldq, void* out, int ld
     CUtensorMap map_q;
     const int mt = make_map(&map_q, q, N, n_heads * hd, ldq, 128);
     if (mt != 0) return mt;
-    return hd == 64 ? (test ? launch_weights<64, true>(a, kv, map_q, B, max_kv_len, stream) : launch_weights<64, false>(a, kv, map_q, B, max_kv_len, stream))
-                    : (test ? launch_weights<128, true>(a, kv, map_q, B, max_kv_len, stream) : launch_weights<128, false>(a, kv, map_q, B, max_kv_len, stream));
+    return hd == 64 ? (test ? launch_weights<64, true>(a, kv, map_q, B, max_kv_len, parts, stream) : launch_weights<64, false>(a, kv, map_q, B, max_kv_len, parts, stream))
+                    : (test ? launch_weights<128, true>(a, kv, map_q, B, max_kv_len, parts, stream) : launch_weights<128, false>(a, kv, map_q, B, max_kv_len, parts, stream));
 }
 
 // For the test of the give-up path: while set, launches take the kTest form, in which the conversion's warps never say that a

@@ -1767,12 +1767,19 @@ def _e4m3_prompt_form(dt: int, max_q_len: int, n_heads: int, n_kv: int, hd: int)
     return dt == 1 and (hd == 64 or hd == 128) and max_q_len * (n_heads // n_kv) > E4M3_FEW_QUERIES
 
 
+def _e4m3_prompt_scratch(n_seqs: int, n_tokens: int, n_heads: int, kv, max_kv_len: int) -> int:
+    """Statistics a query, and the weights of each head's block, which are added up in the heads' order."""
+    if kv.weights is None:
+        return 0
+    return n_heads * (2 * n_tokens + n_seqs * ((max_kv_len + 127) // 128 * 128))
+
+
 def attention_e4m3_scratch_floats(dtype: torch.dtype, n_seqs: int, n_tokens: int, max_q_len: int, n_heads: int, kv, max_kv_len: int,
                                   total_kv_len: int = 0, window: Optional[int] = None) -> int:
     """Floats of scratch `attention_e4m3` needs for the same arguments (0: none)."""
     window = kv.window if window is None else window
     if _e4m3_prompt_form(0 if dtype == torch.float32 else 1, max_q_len, n_heads, kv.n_kv_heads, kv.head_dim):
-        return 2 * n_tokens * n_heads if kv.weights is not None else 0
+        return _e4m3_prompt_scratch(n_seqs, n_tokens, n_heads, kv, int(max_kv_len))
     return int(_fn("gtg_attention_e4m3_scratch_floats")(0 if dtype == torch.float32 else 1, n_seqs, n_tokens, int(max_q_len), n_heads, kv.n_kv_heads,
                                                         kv.head_dim, int(max_kv_len), int(total_kv_len), int(window or 0),
                                                         1 if kv.weights is not None else 0))
@@ -1808,7 +1815,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
         return
     prompt = _e4m3_prompt_form(dt, max_q_len, n_heads, kv.n_kv_heads, hd)
     if prompt:
-        need = 2 * N * n_heads if kv.weights is not None else 0
+        need = _e4m3_prompt_scratch(B, N, n_heads, kv, int(max_kv_len))
     else:
         need = int(_fn("gtg_attention_e4m3_scratch_floats")(dt, B, N, int(max_q_len), n_heads, kv.n_kv_heads, hd, int(max_kv_len), int(total_kv_len),
                                                             int(window or 0), 1 if kv.weights is not None else 0))
