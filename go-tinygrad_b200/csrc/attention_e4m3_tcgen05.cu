@@ -35,11 +35,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPShift = 7.0f, kMostSum = 32768.0f;
 
 template <int HD> struct Shape {
-    static constexpr int kRaw = HD == 64 ? 6 : 4;        // steps of codes on their way
     static constexpr int kQBytes = BQ * HD * 2, kTileBytes = BK * HD * 2;
-    static constexpr int kOffK = 2 * kQBytes, kOffV = kOffK + 2 * kTileBytes, kOffRaw = kOffV + 2 * kTileBytes;
-    static constexpr int kRawBytes = BK * HD;            // a step's codes of keys (or of values)
-    static constexpr int kOffBar = kOffRaw + kRaw * 2 * kRawBytes;
+    static constexpr int kOffK = 2 * kQBytes, kOffV = kOffK + 2 * kTileBytes, kOffBar = kOffV + 2 * kTileBytes;
     static constexpr int kSmemBytes = kOffBar + 256;
     static constexpr int kColO = BK, kColP = BK + HD;    // of a tile's tensor memory: S, O, two of P
     static_assert(BK + HD + BK <= kTileCols, "tensor memory");
@@ -65,11 +62,6 @@ struct PromptArgs {
 
 __device__ __forceinline__ void store_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-__device__ __forceinline__ uint4 load_shared16(uint32_t at) {
-    uint4 u;
-    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at) : "memory");
-    return u;
 }
 // Wait for a phase, the warp asleep meanwhile (up to some 10 us at a time): a block of thirteen warps that poll instead spends half
 // of its issue slots on it.  Bounded like mbar_wait.
@@ -101,14 +93,14 @@ __device__ __forceinline__ bool mbar_sleep_both(uint32_t bar, uint32_t parity, u
     atomicExch(&g_status, 1);
     return false;
 }
-// 16-byte copy global -> shared.
-__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
-}
-// 16 codes as 16 halves: two chunks of a swizzled row.
-__device__ __forceinline__ void store_halves(uint32_t row_at, int chunk, int swizzle, const uint4& u) {
-    store_shared16(row_at + ((chunk ^ swizzle) << 4), e4m3_pair_f16(u.x), e4m3_pair_f16(u.x >> 16), e4m3_pair_f16(u.y), e4m3_pair_f16(u.y >> 16));
-    store_shared16(row_at + (((chunk + 1) ^ swizzle) << 4), e4m3_pair_f16(u.z), e4m3_pair_f16(u.z >> 16), e4m3_pair_f16(u.w), e4m3_pair_f16(u.w >> 16));
+// 16 codes as 16 halves: two chunks of a swizzled row, the second first where `turned` is odd (lanes whose tiles' blocks share
+// banks then store to different ones).
+__device__ __forceinline__ void store_halves(uint32_t row_at, int chunk, int swizzle, const uint4& u, int turned = 0) {
+    const uint32_t a[4] = {e4m3_pair_f16(u.x), e4m3_pair_f16(u.x >> 16), e4m3_pair_f16(u.y), e4m3_pair_f16(u.y >> 16)};
+    const uint32_t b[4] = {e4m3_pair_f16(u.z), e4m3_pair_f16(u.z >> 16), e4m3_pair_f16(u.w), e4m3_pair_f16(u.w >> 16)};
+    const uint32_t first = row_at + (((chunk + turned) ^ swizzle) << 4), second = row_at + (((chunk + 1 - turned) ^ swizzle) << 4);
+    store_shared16(first, turned ? b[0] : a[0], turned ? b[1] : a[1], turned ? b[2] : a[2], turned ? b[3] : a[3]);
+    store_shared16(second, turned ? a[0] : b[0], turned ? a[1] : b[1], turned ? a[2] : b[2], turned ? a[3] : b[3]);
 }
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -238,29 +230,21 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
         constexpr bool values = decltype(of_values)::value;
         constexpr int threads = 32 * (values ? kValueWarps : kKeyWarps), mine = (S::kPieces + threads - 1) / threads;
         const int total = start + q_len;                         // rows that exist after this step
-        // The codes come by asynchronous copies, kRaw steps ahead, each 16-byte piece to a place that only the lane that will
-        // convert it reads: nothing is waited for but a lane's own copies.  Page numbers are read 32 steps at a time.
-        int pages = 0;                                           // lane l: page of step (asked / 32 * 32 + l)
-        auto slot_of = [&](int i, int id) { return base + S::kOffRaw + ((i % S::kRaw) * 2 + values) * S::kRawBytes + id * 16; };
+        // The codes come straight to registers, a step ahead of their use (through shared memory, several steps ahead, they
+        // cost it the traffic that the products want).  Page numbers are read 32 steps at a time.
+        int pages = 0;                                           // lane l: page of step (fetched / 32 * 32 + l)
         const uint8_t* source = (values ? kv.v : kv.k) + (size_t)h * kPageTokens * HD + t * 16;
         const long long stride = values ? kv.v_stride : kv.k_stride;
-        auto ask = [&](int i) {
-            if (i < steps_last) {
-                if ((i & 31) == 0) pages = i + lane < steps_last ? table[j_lo + i + lane] : 0;
-                const uint8_t* at = source + (size_t)__shfl_sync(0xffffffffu, pages, i & 31) * stride;
-#pragma unroll
-                for (int m = 0; m < mine; ++m)
-                    if (t + threads * m < S::kPieces) copy_async16(slot_of(i, t + threads * m), at + threads * m * 16);
-            }
-            asm volatile("cp.async.commit_group;\n" ::);
-        };
-        for (int i = 0; i < S::kRaw; ++i) ask(i);
-        for (int i = 0; i < steps_last; ++i) {
-            uint4 u[mine];
-            asm volatile("cp.async.wait_group %0;\n" ::"n"(S::kRaw - 1) : "memory");
+        uint4 u[mine];
+        auto fetch = [&](int i) {
+            if ((i & 31) == 0) pages = i + lane < steps_last ? table[j_lo + i + lane] : 0;
+            const uint8_t* at = source + (size_t)__shfl_sync(0xffffffffu, pages, i & 31) * stride;
 #pragma unroll
             for (int m = 0; m < mine; ++m)
-                if (t + threads * m < S::kPieces) u[m] = load_shared16(slot_of(i, t + threads * m));
+                if (t + threads * m < S::kPieces) u[m] = *reinterpret_cast<const uint4*>(at + threads * m * 16);
+        };
+        fetch(0);
+        for (int i = 0; i < steps_last; ++i) {
             const int j = j_lo + i;
             if (values && page_not_whole(j)) {
                 // Rows nobody has written yet become zeros; so do NaN codes, which P's zeros would not silence: who does see them
@@ -289,14 +273,13 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                 const int id = t + threads * m;
                 if (id >= S::kPieces) continue;
                 if (values) store_halves(tile + id / 4 * 128, id % 4 * 2, id / 4 & 7, u[m]);
-                else store_halves(tile + id % (HD / 16) / 4 * (BK * 128) + id / (HD / 16) * 128, id % 4 * 2, id / (HD / 16) & 7, u[m]);
+                else store_halves(tile + id % (HD / 16) / 4 * (BK * 128) + id / (HD / 16) * 128, id % 4 * 2, id / (HD / 16) & 7, u[m], id % (HD / 16) / 4);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
             if (lane == 0 && !Waits<kTest>::kSkipCopies) mbar_arrive(values ? v_full(i) : k_full(i));
-            ask(i + S::kRaw);
+            if (i + 1 < steps_last) fetch(i + 1);
         }
-        asm volatile("cp.async.wait_group 0;\n" ::);
     };
     if (warp >= 8 + kKeyWarps && warp < kScoreWarp) {
         convert(std::true_type(), (int)threadIdx.x - 32 * (8 + kKeyWarps));
