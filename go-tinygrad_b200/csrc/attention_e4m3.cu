@@ -185,7 +185,7 @@ int launch_row_weights(const void* q, int ldq, const E4M3Pages& kv, const int* c
     const size_t smem = ((size_t)kPageTokens * (kv.hd + 1) + 8 * (size_t)kv.hd) * sizeof(float);
     cudaError_t e = cudaFuncSetAttribute(row_weights_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    return launch_chained(row_weights_kernel<T>, dim3((max_kv_len + kPageTokens - 1) / kPageTokens, kv.n_kv, B), dim3(kRowThreads), smem, stream,
+    return launch_behind(row_weights_kernel<T>, dim3((max_kv_len + kPageTokens - 1) / kPageTokens, kv.n_kv, B), dim3(kRowThreads), smem, stream,
                           (const T*)q, ldq, kv, cu_seqlens, slots, start_pos, n_heads, scale, window, stats);
 }
 

@@ -104,7 +104,8 @@ struct FewArgs {
     int window;
     int columns;                 // max_q_len * group: queries of the longest run
     int tiles;                   // of 4 NT queries in them
-    int workers;                 // warps that share the pages
+    int workers;                 // warps that share the pages: all but the last block's
+    long long* line;             // [B + 1]: pages a worker takes, then where on the line each sequence begins
     float* part_o;               // [worker + unit][4 NT][HD]
     float* part_ml;              // [worker + unit][4 NT][2]
     float* scores;               // [b][kv head][column][score_pages][64] or null
@@ -127,25 +128,53 @@ __device__ __forceinline__ FewSpan few_span(const FewArgs& a, const E4M3Pages& k
 }
 // All pages of all units -- a unit is a (sequence, kv head, tile of queries) -- lie on one line: sequence by sequence, unit by
 // unit, page by page.  Every worker takes an equal stretch of it, so all finish together whatever the lengths are, and
-// whatever a plan was made for.  Called by whole warps: pages per worker, and where on the line sequence `b` begins.
-struct FewLine {
-    long long per, begin;
-};
-__device__ __forceinline__ FewLine few_line(const FewArgs& a, const E4M3Pages& kv, int units, int b) {
+// whatever a plan was made for.  Called by whole warps: `from` on the line -> the sequence it falls into and how far behind the
+// sequence's begin; -1 behind the line's end.  Sequences are looked at 32 at a time, the first 128 of them once.
+constexpr int kSeenOnce = 4;
+struct FewPlace { long long per, from, offset; int b; };
+// (WRITE: also keep the line for the joining kernel.  Behind chain_wait, for a call before this one may still read its own.)
+template <bool WRITE>
+__device__ __forceinline__ FewPlace few_place(const FewArgs& a, const E4M3Pages& kv, int units, int worker) {
     const int lane = threadIdx.x & 31;
-    long long total = 0, begin = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-        const int mine = b0 + lane;
-        const int pages = mine < a.B ? few_span(a, kv, mine).pages() : 0;
-        const int before = mine < b ? pages : 0;
-        total += __reduce_add_sync(0xffffffffu, pages);
-        begin += __reduce_add_sync(0xffffffffu, before);
-    }
-    FewLine line;
+    int pages[kSeenOnce];
+    long long total = 0;
+    auto pages_of = [&](int b) { return b < a.B ? few_span(a, kv, b).pages() : 0; };
+#pragma unroll
+    for (int x = 0; x < kSeenOnce; ++x) pages[x] = 32 * x < a.B ? pages_of(32 * x + lane) : 0;
+#pragma unroll
+    for (int x = 0; x < kSeenOnce; ++x) total += __reduce_add_sync(0xffffffffu, pages[x]);
+    for (int b0 = 32 * kSeenOnce; b0 < a.B; b0 += 32) total += __reduce_add_sync(0xffffffffu, pages_of(b0 + lane));
+    FewPlace p;
     // (a stretch is at least two pages: below that, joining costs more than it saves)
-    line.per = max(2LL, (total * units + a.workers - 1) / a.workers);
-    line.begin = begin * units;
-    return line;
+    p.per = max(2LL, (total * units + a.workers - 1) / a.workers);
+    p.from = worker * p.per;
+    p.b = -1;
+    p.offset = 0;
+    if (WRITE && lane == 0) a.line[0] = p.per;
+    long long at = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        int mine = 0;
+#pragma unroll
+        for (int x = 0; x < kSeenOnce; ++x)
+            if (b0 == 32 * x) mine = pages[x];
+        if (b0 >= 32 * kSeenOnce) mine = pages_of(b0 + lane);
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        if (WRITE && b0 + lane < a.B) a.line[1 + b0 + lane] = at + (long long)(incl - mine) * units;
+        const unsigned past = __ballot_sync(0xffffffffu, at + (long long)incl * units > p.from);
+        if (past && p.b < 0) {
+            const int who = __ffs(past) - 1;
+            p.b = b0 + who;
+            p.offset = p.from - (at + (long long)__shfl_sync(0xffffffffu, incl - mine, who) * units);
+            if (!WRITE) break;
+        }
+        at += (long long)__shfl_sync(0xffffffffu, incl, 31) * units;
+    }
+    return p;
 }
 
 // A warp a worker; NT tiles of four queries a unit.
@@ -162,36 +191,16 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
     const uint32_t ring = smem_u32(smem) + warp * F::STAGES * 2 * F::HALF_BYTES;
     const unsigned char* ring_at = smem + warp * F::STAGES * 2 * F::HALF_BYTES;
 
-    // ---- this worker's stretch of the line: its first page's sequence, unit and page
-    int b = 0, in_b = 0;                                                        // in_b: unit within the sequence
-    long long left, offset = 0;                                                 // pages still to do; from the sequence's begin
-    {
-        const FewLine line = few_line(a, kv, units, 0);
-        const long long from = (long long)worker * line.per;
-        left = line.per;
-        long long at = 0;
-        int found = -1;
-        for (int b0 = 0; b0 < a.B && found < 0; b0 += 32) {
-            const int mine = b0 + lane;
-            const int pages = mine < a.B ? few_span(a, kv, mine).pages() : 0;
-            int incl = pages;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += up;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, at + (long long)incl * units > from);
-            if (past) {
-                const int who = __ffs(past) - 1;
-                const int before = __shfl_sync(0xffffffffu, incl - pages, who);
-                found = b0 + who;
-                offset = from - (at + (long long)before * units);
-            }
-            at += (long long)__shfl_sync(0xffffffffu, incl, 31) * units;
-        }
-        if (found < 0) return;
-        b = found;
+    // ---- this worker's stretch of the line
+    if (worker >= a.workers) {                                                  // the block behind the workers
+        chain_wait();
+        if (worker == a.workers) few_place<true>(a, kv, units, worker);
+        return;
     }
+    const FewPlace place = few_place<false>(a, kv, units, worker);
+    if (place.b < 0) return;
+    int b = place.b, in_b = 0;                                                  // in_b: unit within the sequence
+    long long left = place.per, offset = place.offset;                          // pages still to do; from the sequence's begin
     bool waited = false;
     while (left > 0) {
         const FewSpan span = few_span(a, kv, b);
@@ -528,10 +537,10 @@ few_join_kernel(const FewArgs a, const E4M3Pages kv, int join_blocks) {
     const int n_columns = span.n_new * a.group, n_pages = span.pages();
     if (n_columns <= 0) return;
     const int units = kv.n_kv * a.tiles;
-    const FewLine line = few_line(a, kv, units, b);
+    const long long per = a.line[0], begin = a.line[1 + b];
     // the workers that share tile t of this head: first and last
-    auto first_worker = [&](int t) { return (line.begin + (long long)(h * a.tiles + t) * n_pages) / line.per; };
-    auto last_worker = [&](int t) { return (line.begin + (long long)(h * a.tiles + t + 1) * n_pages - 1) / line.per; };
+    auto first_worker = [&](int t) { return (begin + (long long)(h * a.tiles + t) * n_pages) / per; };
+    auto last_worker = [&](int t) { return (begin + (long long)(h * a.tiles + t + 1) * n_pages - 1) / per; };
     auto part_of = [&](long long worker, int c) { return ((size_t)worker + (size_t)b * units + h * a.tiles + c / (4 * NT)) * 4 * NT + c % (4 * NT); };
     for (int c = tid >> 5; c < n_columns; c += kJoinThreads / 32) {             // a warp a query: its maximum and sum over the parts
         const long long w0 = first_worker(c / (4 * NT)), w1 = last_worker(c / (4 * NT));
@@ -599,8 +608,8 @@ int few_tiles(int columns) { return columns <= 4 ? 1 : columns <= 8 ? 2 : 4; }
 // How many warps run at once, and the scratch they need.
 struct FewPlan {
     int columns, nt, tiles, workers, score_pages;
-    long long part_o, part_ml, scores;                                          // floats, each a multiple of 4
-    long long floats() const { return part_o + part_ml + scores; }
+    long long line, part_o, part_ml, scores;                                    // floats, each a multiple of 4
+    long long floats() const { return line + part_o + part_ml + scores; }
 };
 
 // Warps of this kernel that the current device runs at once (asked once a device).
@@ -617,7 +626,7 @@ int few_workers() {
             (void)cudaGetLastError();
             return kFewWarps;
         }
-        cached[dev] = blocks * sms * kFewWarps;
+        cached[dev] = (blocks * sms - 1) * kFewWarps;                           // one block keeps the line
     }
     return cached[dev];
 }
@@ -631,6 +640,7 @@ FewPlan few_plan_for(int B, int max_q_len, int n_heads, int n_kv, int max_kv_len
     plan.workers = plan.nt == 4 ? few_workers<HD, 4>() : plan.nt == 2 ? few_workers<HD, 2>() : few_workers<HD, 1>();
     plan.score_pages = weigh ? (max_kv_len + kPageTokens - 1) / kPageTokens : 0;
     const long long parts = ((long long)plan.workers + (long long)B * n_kv * plan.tiles) * 4 * plan.nt;
+    plan.line = ((long long)B + 2) / 2 * 4;
     plan.part_o = parts * HD;
     plan.part_ml = parts * 2;
     plan.scores = (long long)B * n_kv * plan.columns * plan.score_pages * kPageTokens;
@@ -639,12 +649,12 @@ FewPlan few_plan_for(int B, int max_q_len, int n_heads, int n_kv, int max_kv_len
 
 template <int HD, int NT>
 int launch_few_tiles(const FewArgs& a, const E4M3Pages& kv, cudaStream_t stream) {
-    const int st = launch_chained(few_queries_kernel<HD, NT>, dim3((a.workers + kFewWarps - 1) / kFewWarps), dim3(kFewThreads), Few<HD>::RING,
+    const int st = launch_chained(few_queries_kernel<HD, NT>, dim3(a.workers / kFewWarps + 1), dim3(kFewThreads), Few<HD>::RING,
                                   stream, a, kv);
     if (st != 0) return st;
     const int join = (a.columns * HD + kJoinThreads - 1) / kJoinThreads;
     const int pages = a.score_pages ? (a.score_pages * kPageTokens + kJoinThreads - 1) / kJoinThreads : 0;
-    return launch_chained(few_join_kernel<HD, NT>, dim3(join + pages, kv.n_kv, a.B), dim3(kJoinThreads), 0, stream, a, kv, join);
+    return launch_behind(few_join_kernel<HD, NT>, dim3(join + pages, kv.n_kv, a.B), dim3(kJoinThreads), 0, stream, a, kv, join);
 }
 
 template <int HD>
@@ -653,9 +663,10 @@ int launch_few(FewArgs a, const E4M3Pages& kv, const FewPlan& plan, float* scrat
     a.tiles = plan.tiles;
     a.workers = plan.workers;
     a.score_pages = plan.score_pages;
-    a.part_o = scratch;
-    a.part_ml = scratch + plan.part_o;
-    a.scores = plan.scores ? scratch + plan.part_o + plan.part_ml : nullptr;
+    a.line = (long long*)scratch;
+    a.part_o = scratch + plan.line;
+    a.part_ml = a.part_o + plan.part_o;
+    a.scores = plan.scores ? a.part_ml + plan.part_ml : nullptr;
     return plan.nt == 4 ? launch_few_tiles<HD, 4>(a, kv, stream)
          : plan.nt == 2 ? launch_few_tiles<HD, 2>(a, kv, stream) : launch_few_tiles<HD, 1>(a, kv, stream);
 }

@@ -122,13 +122,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n"
-                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-                 : "memory");
-}
-
 // Products and commits issued by one lane of a warp that runs its loop as a whole: with the loop inside one lane's branch the
 // descriptors do not stay in the warp's uniform registers, and a step's products took some 60 cycles each to issue.
 __device__ __forceinline__ void warp_umma_ss(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -391,9 +384,6 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                 k_scales = at[0];
                 v_scales = at[kv.n_kv];
             }
-            const float sl = factor * __shfl_sync(full, k_scales, i & 31);
-            const float v_scale = __shfl_sync(full, v_scales, i & 31);
-            const float add = (float)((int)(__float_as_uint(v_scale) >> 23) - 127);             // log2 of the value scale
             // the step's scores; and the P of two steps ago has been read
             ok = i < 2 ? all_wait(s_full(tt), (uint32_t)i & 1u)
                        : (bool)__all_sync(full, mbar_sleep_both<kTest>(s_full(tt), (uint32_t)i & 1u, pv_done(tt, i), phase(i - 2), abort_flag));
@@ -401,6 +391,9 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
             tmem_ld32(tile_at, sv);
             tmem_ld32(tile_at + 32, sv + 32);
+            const float sl = factor * __shfl_sync(full, k_scales, i & 31);
+            const float v_scale = __shfl_sync(full, v_scales, i & 31);
+            const float add = (float)((int)(__float_as_uint(v_scale) >> 23) - 127);             // log2 of the value scale
             asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
             __syncwarp();
@@ -784,10 +777,10 @@ int launch_weights(const PromptArgs& a, const E4M3Pages& kv, const CUtensorMap& 
         configured = true;
     }
     const int part_rows = (max_kv_len + 127) / 128 * 128;
-    const int st = launch_chained(e4m3_weights_kernel<HD, kTest>, dim3(part_rows / 128, a.n_heads, B), dim3(kWeightThreads),
+    const int st = launch_behind(e4m3_weights_kernel<HD, kTest>, dim3(part_rows / 128, a.n_heads, B), dim3(kWeightThreads),
                                   (size_t)WeightShape<HD>::kSmemBytes, stream, map_q, a, kv, parts, part_rows);
     if (st != 0) return st;
-    return launch_chained(e4m3_weights_sum_kernel, dim3((part_rows + 255) / 256, kv.n_kv, B), dim3(256), 0, stream, a, kv, (const float*)parts, part_rows);
+    return launch_behind(e4m3_weights_sum_kernel, dim3((part_rows + 255) / 256, kv.n_kv, B), dim3(256), 0, stream, a, kv, (const float*)parts, part_rows);
 }
 }  // namespace
 

@@ -32,6 +32,17 @@ struct E4M3Pages {
 
 constexpr int kLeastExponent = -126;
 
+// A kernel that only goes on with what the launch before it (of the same call) has left: it may begin while that one drains,
+// whether the caller chains its kernels or not, and waits for it itself (chain_wait).
+template <typename... Params, typename... Args>
+static inline int launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+    const int chained = g_chained_launch;
+    g_chained_launch = 1;
+    const int st = launch_chained(kernel, grid, block, smem, stream, args...);
+    g_chained_launch = chained;
+    return st;
+}
+
 __device__ __forceinline__ bool finite_f32(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 // The least power of two 2^k, k >= -126, with most <= 448 * 2^k, for finite most >= 0: 448 = 1.75 * 2^8, so k is the
