@@ -522,52 +522,85 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
     if (!waited) chain_wait();
 }
 
-// Joins the parts (blocks x < join_blocks: queries of one (sequence, kv head)) and, where weights are gathered, adds to
-// them (the other blocks, four pages at a time).
+// Joins the parts (blocks x < join_blocks: some queries of one (sequence, kv head)) and, where weights are gathered, adds to
+// them (the other blocks, four pages at a time).  Both are a few short reads that wait for one another, so the parts of a
+// query are spread over all threads that its channels leave.
 constexpr int kJoinThreads = 256;
+
+template <int HD> struct Join {
+    static constexpr int LANES = HD / 4;                                        // threads of a query's channels
+    static constexpr int ROWS = kJoinThreads / LANES;
+    __host__ __device__ static int share(int columns) { return columns >= ROWS ? 1 : ROWS / columns; }    // rows that share a query's parts
+    __host__ __device__ static int columns_each(int columns) { return ROWS / share(columns); }
+};
 
 template <int HD, int NT>
 __global__ void __launch_bounds__(kJoinThreads)
 few_join_kernel(const FewArgs a, const E4M3Pages kv, int join_blocks) {
+    using J = Join<HD>;
     chain_release();
     chain_wait();
     __shared__ float top[kFewColumns], inverse[kFewColumns];
+    __shared__ int first_worker[kFewColumns / (4 * NT)], last_worker[kFewColumns / (4 * NT)];             // that share a tile's pages
+    __shared__ float4 sums[J::ROWS * J::LANES];
     const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
+    const long long per = a.line[0], begin = a.line[1 + b];
     const FewSpan span = few_span(a, kv, b);
     const int n_columns = span.n_new * a.group, n_pages = span.pages();
-    if (n_columns <= 0) return;
+    const bool joins = (int)blockIdx.x < join_blocks;
+    const int share = J::share(a.columns), c_begin = joins ? blockIdx.x * J::columns_each(a.columns) : 0;
+    const int c_end = joins ? min(n_columns, c_begin + J::columns_each(a.columns)) : n_columns;
+    if (c_begin >= c_end) return;
     const int units = kv.n_kv * a.tiles;
-    const long long per = a.line[0], begin = a.line[1 + b];
-    // the workers that share tile t of this head: first and last
-    auto first_worker = [&](int t) { return (begin + (long long)(h * a.tiles + t) * n_pages) / per; };
-    auto last_worker = [&](int t) { return (begin + (long long)(h * a.tiles + t + 1) * n_pages - 1) / per; };
-    auto part_of = [&](long long worker, int c) { return ((size_t)worker + (size_t)b * units + h * a.tiles + c / (4 * NT)) * 4 * NT + c % (4 * NT); };
-    for (int c = tid >> 5; c < n_columns; c += kJoinThreads / 32) {             // a warp a query: its maximum and sum over the parts
-        const long long w0 = first_worker(c / (4 * NT)), w1 = last_worker(c / (4 * NT));
+    if (tid < a.tiles) {
+        const long long at = begin + (long long)(h * a.tiles + tid) * n_pages;
+        first_worker[tid] = (int)(at / per);
+        last_worker[tid] = (int)((at + n_pages - 1) / per);
+    }
+    __syncthreads();
+    auto part_of = [&](int worker, int c) { return ((size_t)worker + (size_t)b * units + h * a.tiles + c / (4 * NT)) * 4 * NT + c % (4 * NT); };
+    for (int c = c_begin + (tid >> 5); c < c_end; c += kJoinThreads / 32) {     // a warp a query: its maximum and sum over the parts
+        const int w0 = first_worker[c / (4 * NT)], w1 = last_worker[c / (4 * NT)];
         if (w0 == w1 && !a.scores) continue;                                    // it is not in parts
         float M = -INFINITY, L = 0.f;
-        for (long long w = w0 + (tid & 31); w <= w1; w += 32) M = fmaxf(M, a.part_ml[part_of(w, c) * 2]);
-        M = warp_max(M);
-        const float use = M == -INFINITY ? 0.f : M;
-        for (long long w = w0 + (tid & 31); w <= w1; w += 32) {
-            const float* ml = a.part_ml + part_of(w, c) * 2;
-            L += exp2_fast(ml[0] - use) * ml[1];
+        for (int w = w0 + (tid & 31); w <= w1; w += 32) {
+            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + part_of(w, c) * 2);
+            const float now = fmaxf(M, ml.x);
+            L = L * exp2_fast(M - (now == -INFINITY ? 0.f : now)) + exp2_fast(ml.x - (now == -INFINITY ? 0.f : now)) * ml.y;
+            M = now;
         }
-        L = warp_sum(L);
+        const float all = warp_max(M), use = all == -INFINITY ? 0.f : all;
+        L = warp_sum(exp2_fast(M - use) * L);
         if ((tid & 31) == 0) { top[c] = use; inverse[c] = 1.0f / L; }
     }
     __syncthreads();
-    if ((int)blockIdx.x < join_blocks) {
-        for (int idx = blockIdx.x * kJoinThreads + tid; idx < n_columns * HD; idx += join_blocks * kJoinThreads) {
-            const int c = idx / HD, d = idx % HD;
-            const long long w0 = first_worker(c / (4 * NT)), w1 = last_worker(c / (4 * NT));
-            if (w0 == w1) continue;
-            float acc = 0.f;
-            for (long long w = w0; w <= w1; ++w) {
+    if (joins) {
+        const int row = tid / J::LANES, d = tid % J::LANES * 4, c = c_begin + row / share;
+        const bool mine = row < J::ROWS && c < c_end;
+        const int w0 = mine ? first_worker[c / (4 * NT)] : 0, w1 = mine ? last_worker[c / (4 * NT)] : 0;
+        if (w0 < w1) {
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int w = w0 + row % share; w <= w1; w += share) {
                 const size_t at = part_of(w, c);
-                acc += exp2_fast(a.part_ml[at * 2] - top[c]) * a.part_o[at * HD + d];
+                const float4 o = *reinterpret_cast<const float4*>(a.part_o + at * HD + d);
+                const float f = exp2_fast(a.part_ml[at * 2] - top[c]);
+                acc.x = fmaf(f, o.x, acc.x); acc.y = fmaf(f, o.y, acc.y); acc.z = fmaf(f, o.z, acc.z); acc.w = fmaf(f, o.w, acc.w);
             }
-            a.out[(size_t)(span.first + c / a.group) * a.ldo + (size_t)(h * a.group + c % a.group) * HD + d] = __float2bfloat16_rn(acc * inverse[c]);
+            sums[tid] = acc;
+        }
+        __syncthreads();
+        if (w0 < w1 && row % share == 0) {
+            float4 acc = sums[tid];
+            for (int i = 1; i < share; ++i) {
+                const float4 o = sums[tid + i * J::LANES];
+                acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
+            }
+            bf16* out = a.out + (size_t)(span.first + c / a.group) * a.ldo + (size_t)(h * a.group + c % a.group) * HD + d;
+            out[0] = __float2bfloat16_rn(acc.x * inverse[c]);
+            out[1] = __float2bfloat16_rn(acc.y * inverse[c]);
+            out[2] = __float2bfloat16_rn(acc.z * inverse[c]);
+            out[3] = __float2bfloat16_rn(acc.w * inverse[c]);
         }
         return;
     }
@@ -652,7 +685,7 @@ int launch_few_tiles(const FewArgs& a, const E4M3Pages& kv, cudaStream_t stream)
     const int st = launch_chained(few_queries_kernel<HD, NT>, dim3(a.workers / kFewWarps + 1), dim3(kFewThreads), Few<HD>::RING,
                                   stream, a, kv);
     if (st != 0) return st;
-    const int join = (a.columns * HD + kJoinThreads - 1) / kJoinThreads;
+    const int join = (a.columns + Join<HD>::columns_each(a.columns) - 1) / Join<HD>::columns_each(a.columns);
     const int pages = a.score_pages ? (a.score_pages * kPageTokens + kJoinThreads - 1) / kJoinThreads : 0;
     return launch_behind(few_join_kernel<HD, NT>, dim3(join + pages, kv.n_kv, a.B), dim3(kJoinThreads), 0, stream, a, kv, join);
 }
