@@ -7,6 +7,8 @@
 //   few_queries:      bfloat16, heads of up to 128 channels in steps of 16, few queries a sequence (attention_e4m3_few.cuh);
 //   attention_rows:   any head size and type, one block per (token, query head); scores, softmax and sums in float.
 //   row_weights:      the weights, once every row's maximum and sum are known: a block per (cache page, head, sequence).
+#include <algorithm>
+
 #include "attention_e4m3_few.cuh"
 
 namespace {
@@ -211,9 +213,10 @@ GTG_API long long gtg_attention_e4m3_scratch_floats(int dtype, int B, int N, int
                                                     long long total_kv_len, int window, int weigh) {
     (void)total_kv_len; (void)window;
     if (B <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || max_q_len <= 0 || max_kv_len <= 0) return 0;
+    const long long rows = weigh ? 2LL * N * n_heads : 0;
     if (few_takes(dtype, max_q_len, n_heads, n_kv, hd))
-        return few_plan(B, max_q_len, n_heads, n_kv, hd, max_kv_len, weigh).floats();
-    return weigh ? 2LL * N * n_heads : 0;
+        return std::max(few_plan(B, max_q_len, n_heads, n_kv, hd, max_kv_len, weigh).floats(), rows);
+    return rows;
 }
 
 // dtype: of q and out (0 float, 1 bfloat16).  max_kv_len: rows of the longest sequence after this step; total_kv_len: of all
@@ -228,11 +231,11 @@ GTG_API int gtg_attention_e4m3(int dtype, const void* q, int ldq, void* out, int
     if (hd > kMaxChannels || B > 65535 || n_heads > 65535) return kErrUnsupported;
     const E4M3Pages kv = {(uint8_t*)k, (uint8_t*)v, k_stride, v_stride, scales, scale_stride, weights, weight_stride, block_table, table_stride,
                           dropped, n_kv, hd};
-    if (few_takes(dtype, max_q_len, n_heads, n_kv, hd)) {
+    if (few_takes(dtype, max_q_len, n_heads, n_kv, hd) && few_counts(B, max_q_len, n_heads, n_kv, table_stride)) {
         const FewPlan plan = few_plan(B, max_q_len, n_heads, n_kv, hd, max_kv_len, weights != nullptr);
         if (plan.floats() && !scratch) return kErrBadArgument;
         FewArgs a = {};
-        a.q = (const bf16*)q; a.ldq = ldq; a.out = (bf16*)out; a.ldo = ldo;
+        a.q = (const bf16*)q; a.ldq = ldq; a.wide = (uintptr_t)q % 16 == 0 && ldq % 8 == 0; a.chained = g_chained_launch; a.out = (bf16*)out; a.ldo = ldo;
         a.cu_seqlens = cu_seqlens; a.slots = slots; a.start_pos = start_pos;
         a.B = B; a.n_heads = n_heads; a.group = n_heads / n_kv; a.scale = scale; a.window = window;
 #define GTG_FEW(HD) case HD: return launch_few<HD>(a, kv, plan, scratch, stream);

@@ -37,7 +37,20 @@ constexpr float kLog2e = 1.4426950408889634f;
 #define GTG_FEW_STAGES 2
 #endif
 constexpr int kFewWarps = GTG_FEW_WARPS, kFewThreads = 32 * kFewWarps;
+#ifndef GTG_FEW_BLOCKS
+#define GTG_FEW_BLOCKS 6
+#endif
+#ifndef GTG_FEW_BLOCKS64
+#define GTG_FEW_BLOCKS64 6
+#endif
+#ifndef GTG_FEW_COST
+#define GTG_FEW_COST 2
+#endif
+#ifndef GTG_FEW_LEAST
+#define GTG_FEW_LEAST 2
+#endif
 constexpr int kFewColumns = 32;          // queries a key/value head that these kernels take
+constexpr int kStepRows = 32;            // cache rows a warp takes at a time: half a page
 constexpr float kPShift = 8.0f;          // probabilities are held times 2^8
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -45,7 +58,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
-// D += A(16 x 32, row) B(32 x 8, col): e4m3 operands, float sums.
+// D = A(16 x 32, row) B(32 x 8, col) (+ D): e4m3 operands, float sums.
+__device__ __forceinline__ void mma_e4m3_16832_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_e4m3_16832(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -70,14 +89,14 @@ __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src));
 }
 
-// Cache row within its page of row r (0..15) of score tile j: the rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a tile are four
+// Cache row within its step of row r (0..15) of score tile j: the rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a tile are four
 // neighbouring rows, those of the word that lane t has of a row of V^T.
-__device__ __forceinline__ int tile_row(int j, int r) { return ((r & 7) >> 1) * 16 + 4 * j + (r & 1) + (r >> 3) * 2; }
+__device__ __forceinline__ int tile_row(int j, int r) { return ((r & 7) >> 1) * 8 + 4 * j + (r & 1) + (r >> 3) * 2; }
 // A transposed word holds the codes of the rows 2 t, 2 t + 8, 2 t + 1, 2 t + 9.
 __device__ __forceinline__ uint32_t in_row_order(uint32_t w) { return __byte_perm(w, 0, 0x3120); }
-// Where a page's row stands among a query's 64 kept scores: a lane's eight side by side.
+// Where a row stands among the kept scores of a query and step: a lane's four side by side.
 __device__ __forceinline__ int score_place(int row) {
-    return (((row >> 4) * 2 + (row & 1)) << 3) + ((row >> 2) & 3) * 2 + ((row >> 1) & 1);
+    return (((row >> 3) * 2 + (row & 1)) << 2) + ((row >> 2) & 1) * 2 + ((row >> 1) & 1);
 }
 
 template <int HD> struct Few {
@@ -86,14 +105,17 @@ template <int HD> struct Few {
     static constexpr int WORDS = HD / 16;                                      // of a key row a lane has
     static constexpr int STEPS = (WORDS + 1) / 2;                              // of 32 channels
     static constexpr int TILES = HD / 16;                                      // of 16 channels
-    static constexpr int HALF_BYTES = 64 * HD;                                 // a page's keys (or values) of one head
+    static constexpr int PAGE_BYTES = kPageTokens * HD;                        // a page's keys (or values) of one head
+    static constexpr int HALF_BYTES = kStepRows * HD;                          // a step's
+    // rows of 128 bytes: where two neighbours would share banks, the odd ones lie with their halves exchanged
+    static constexpr int SWAP = HD == 128 ? 1 : 0;
     static constexpr int STAGES = GTG_FEW_STAGES;
     static constexpr int RING = kFewWarps * STAGES * 2 * HALF_BYTES;
 };
 
 struct FewArgs {
     const bf16* q;
-    int ldq;
+    int ldq, wide, chained;      // wide: rows of q begin on 16 bytes; chained: the kernel before this one may still run
     bf16* out;
     int ldo;
     const int* cu_seqlens;
@@ -104,82 +126,94 @@ struct FewArgs {
     int window;
     int columns;                 // max_q_len * group: queries of the longest run
     int tiles;                   // of 4 NT queries in them
-    int workers;                 // warps that share the pages: all but the last block's
-    long long* line;             // [B + 1]: pages a worker takes, then where on the line each sequence begins
+    int workers;                 // warps that share the line
     float* part_o;               // [worker + unit][4 NT][HD]
     float* part_ml;              // [worker + unit][4 NT][2]
     float* scores;               // [b][kv head][column][score_pages][64] or null
     int score_pages;
 };
 
-// The rows of sequence b that a step's queries see, in pages.
-struct FewSpan {
-    int first, n_new, start, p_first, p_last;
-    __device__ __forceinline__ int pages() const { return n_new > 0 ? p_last - p_first + 1 : 0; }
+// The rows of a sequence that its queries see, in steps, and where they lie on the line of all.
+struct FewSeq {
+    int begin, first, n_new, start, p_first, p_last, slot;
+    __device__ __forceinline__ int steps() const { return n_new > 0 ? p_last - p_first + 1 : 0; }
 };
-__device__ __forceinline__ FewSpan few_span(const FewArgs& a, const E4M3Pages& kv, int b) {
-    FewSpan s;
+__device__ __forceinline__ FewSeq few_seq(const FewArgs& a, const E4M3Pages& kv, int b) {
+    FewSeq s;
+    s.begin = 0;
     s.first = a.cu_seqlens[b];
     s.n_new = a.cu_seqlens[b + 1] - s.first;
-    s.start = a.start_pos[b] - (kv.dropped ? kv.dropped[a.slots[b]] : 0);
-    s.p_first = (a.window > 0 ? max(0, s.start - a.window + 1) : 0) / kPageTokens;
-    s.p_last = (s.start + s.n_new - 1) / kPageTokens;
+    s.slot = a.slots[b];
+    s.start = a.start_pos[b] - (kv.dropped ? kv.dropped[s.slot] : 0);
+    s.p_first = (a.window > 0 ? max(0, s.start - a.window + 1) : 0) / kStepRows;
+    s.p_last = (s.start + s.n_new - 1) / kStepRows;
     return s;
 }
-// All pages of all units -- a unit is a (sequence, kv head, tile of queries) -- lie on one line: sequence by sequence, unit by
-// unit, page by page.  Every worker takes an equal stretch of it, so all finish together whatever the lengths are, and
-// whatever a plan was made for.  Called by whole warps: `from` on the line -> the sequence it falls into and how far behind the
-// sequence's begin; -1 behind the line's end.  Sequences are looked at 32 at a time, the first 128 of them once.
-constexpr int kSeenOnce = 4;
-struct FewPlace { long long per, from, offset; int b; };
-// (WRITE: also keep the line for the joining kernel.  Behind chain_wait, for a call before this one may still read its own.)
-template <bool WRITE>
-__device__ __forceinline__ FewPlace few_place(const FewArgs& a, const E4M3Pages& kv, int units, int worker) {
+// All steps of all units -- a unit is a (sequence, kv head, tile of queries) -- lie on one line: sequence by sequence, unit by
+// unit, step by step.  Every worker takes an equal stretch of it, so all finish together whatever the lengths are, and
+// whatever a plan was made for.  A unit's begin costs a worker queries, a page number and a result: kUnitCost empty steps
+// before its first stand for that.  Called by whole warps, which look at 32 sequences at a time, at the first 64 once:
+// the steps a worker takes, where worker's stretch begins, and the sequence that this (BY_WORKER) falls into, b = -1 behind
+// the line's end; or sequence `which`.
+constexpr int kSeenOnce = 2, kUnitCost = GTG_FEW_COST;
+__device__ __forceinline__ int on_line(int steps) { return steps > 0 ? steps + kUnitCost : 0; }
+struct FewPlace { int per, from, b; FewSeq seq; };
+template <bool BY_WORKER>
+__device__ __forceinline__ FewPlace few_place(const FewArgs& a, const E4M3Pages& kv, int units, int which) {
     const int lane = threadIdx.x & 31;
-    int pages[kSeenOnce];
-    long long total = 0;
-    auto pages_of = [&](int b) { return b < a.B ? few_span(a, kv, b).pages() : 0; };
+    FewSeq seen[kSeenOnce];
+    auto at = [&](int b) {                                                      // (no branch: the reads of several do not wait for each other)
+        FewSeq s = few_seq(a, kv, min(b, a.B - 1));
+        if (b >= a.B) s.n_new = 0;
+        return s;
+    };
+    int total = 0;
 #pragma unroll
-    for (int x = 0; x < kSeenOnce; ++x) pages[x] = 32 * x < a.B ? pages_of(32 * x + lane) : 0;
+    for (int x = 0; x < kSeenOnce; ++x) seen[x] = at(32 * x + lane);
 #pragma unroll
-    for (int x = 0; x < kSeenOnce; ++x) total += __reduce_add_sync(0xffffffffu, pages[x]);
-    for (int b0 = 32 * kSeenOnce; b0 < a.B; b0 += 32) total += __reduce_add_sync(0xffffffffu, pages_of(b0 + lane));
+    for (int x = 0; x < kSeenOnce; ++x) total += __reduce_add_sync(0xffffffffu, on_line(seen[x].steps()));
+    for (int b0 = 32 * kSeenOnce; b0 < a.B; b0 += 32) total += __reduce_add_sync(0xffffffffu, on_line(at(b0 + lane).steps()));
     FewPlace p;
-    // (a stretch is at least two pages: below that, joining costs more than it saves)
-    p.per = max(2LL, (total * units + a.workers - 1) / a.workers);
-    p.from = worker * p.per;
+    // (shorter stretches would cost more in joining than they save)
+    p.per = max(GTG_FEW_LEAST, (int)(((unsigned)total * units + a.workers - 1) / a.workers));
+    p.from = BY_WORKER ? which * p.per : 0;
     p.b = -1;
-    p.offset = 0;
-    if (WRITE && lane == 0) a.line[0] = p.per;
-    long long at = 0;
+    int begin = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
-        int mine = 0;
+        FewSeq s = seen[0];
 #pragma unroll
-        for (int x = 0; x < kSeenOnce; ++x)
-            if (b0 == 32 * x) mine = pages[x];
-        if (b0 >= 32 * kSeenOnce) mine = pages_of(b0 + lane);
+        for (int x = 1; x < kSeenOnce; ++x)
+            if (b0 == 32 * x) s = seen[x];
+        if (b0 >= 32 * kSeenOnce) s = at(b0 + lane);
+        const int mine = on_line(s.steps());
         int incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int up = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += up;
         }
-        if (WRITE && b0 + lane < a.B) a.line[1 + b0 + lane] = at + (long long)(incl - mine) * units;
-        const unsigned past = __ballot_sync(0xffffffffu, at + (long long)incl * units > p.from);
-        if (past && p.b < 0) {
+        s.begin = begin + (incl - mine) * units;
+        const unsigned past = __ballot_sync(0xffffffffu, BY_WORKER ? begin + incl * units > p.from : b0 + lane == which);
+        if (past) {
             const int who = __ffs(past) - 1;
             p.b = b0 + who;
-            p.offset = p.from - (at + (long long)__shfl_sync(0xffffffffu, incl - mine, who) * units);
-            if (!WRITE) break;
+            p.seq.begin = __shfl_sync(0xffffffffu, s.begin, who);
+            p.seq.first = __shfl_sync(0xffffffffu, s.first, who);
+            p.seq.n_new = __shfl_sync(0xffffffffu, s.n_new, who);
+            p.seq.start = __shfl_sync(0xffffffffu, s.start, who);
+            p.seq.p_first = __shfl_sync(0xffffffffu, s.p_first, who);
+            p.seq.p_last = __shfl_sync(0xffffffffu, s.p_last, who);
+            p.seq.slot = __shfl_sync(0xffffffffu, s.slot, who);
+            break;
         }
-        at += (long long)__shfl_sync(0xffffffffu, incl, 31) * units;
+        begin += __shfl_sync(0xffffffffu, incl, 31) * units;
     }
     return p;
 }
 
 // A warp a worker; NT tiles of four queries a unit.
 template <int HD, int NT>
-__global__ void __launch_bounds__(kFewThreads)
+__global__ void __launch_bounds__(kFewThreads, NT == 4 ? 4 : HD <= 64 ? GTG_FEW_BLOCKS64 : GTG_FEW_BLOCKS)
 few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
     using F = Few<HD>;
     constexpr int W = F::WORDS;
@@ -192,117 +226,139 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
     const unsigned char* ring_at = smem + warp * F::STAGES * 2 * F::HALF_BYTES;
 
     // ---- this worker's stretch of the line
-    if (worker >= a.workers) {                                                  // the block behind the workers
+    const FewPlace place = few_place<true>(a, kv, units, worker);
+    if (place.b < 0) {
         chain_wait();
-        if (worker == a.workers) few_place<true>(a, kv, units, worker);
         return;
     }
-    const FewPlace place = few_place<false>(a, kv, units, worker);
-    if (place.b < 0) return;
-    int b = place.b, in_b = 0;                                                  // in_b: unit within the sequence
-    long long left = place.per, offset = place.offset;                          // pages still to do; from the sequence's begin
+    FewSeq span = place.seq;
+    int b = place.b, left = place.per, offset = place.from - span.begin;        // steps still to do; from the sequence's begin
     bool waited = false;
     while (left > 0) {
-        const FewSpan span = few_span(a, kv, b);
-        const int n_pages = span.pages();
-        if (n_pages == 0) {
-            if (++b == a.B) break;
-            offset = 0;
-            continue;
-        }
-        in_b = (int)(offset / n_pages);
+        const int n_steps = span.steps(), n_line = on_line(n_steps);
+        const int in_b = n_steps > 0 ? offset / n_line : units;                 // unit within the sequence
         if (in_b >= units) {
             if (++b == a.B) break;
+            span = few_seq(a, kv, b);
             offset = 0;
             continue;
         }
-        const int skip = (int)(offset - (long long)in_b * n_pages);
-        const int n_mine = (int)min(left, (long long)(n_pages - skip));
-        left -= n_mine;
-        offset += n_mine;
+        const int from = offset - in_b * n_line, mine = min(left, n_line - from);
+        left -= mine;
+        offset += mine;
+        const int skip = max(from - kUnitCost, 0), n_mine = max(from + mine - kUnitCost, 0) - skip;
+        if (n_mine == 0) continue;
         const int h = in_b / a.tiles, c0 = in_b % a.tiles * 4 * NT;
         const int n_columns = span.n_new * a.group;
         if (c0 >= n_columns) continue;                                          // a shorter run of queries than the longest
         const int p_begin = span.p_first + skip;
-        const int* table = kv.block_table + (size_t)a.slots[b] * kv.table_stride;
-        const uint8_t* kh = kv.k + (size_t)h * F::HALF_BYTES + lane * 16;
-        const uint8_t* vh = kv.v + (size_t)h * F::HALF_BYTES + lane * 16;
+        const int* table = kv.block_table + (size_t)span.slot * kv.table_stride;
+        const uint8_t* kh = kv.k + (size_t)h * F::PAGE_BYTES + lane * 16;
+        const uint8_t* vh = kv.v + (size_t)h * F::PAGE_BYTES + lane / 2 * kPageTokens + lane % 2 * 16;
 
-        int ahead_pages = 0;                                                    // lane i: page (ahead / 32 * 32 + i) of the stretch
+        int ahead_pages = lane < n_mine ? table[(p_begin + lane) / 2] : 0;      // lane i: page of step (ahead / 32 * 32 + i) of the stretch
         auto load = [&](int i) {
-            if ((i & 31) == 0) ahead_pages = i + lane < n_mine ? table[p_begin + i + lane] : 0;
+            if (i > 0 && (i & 31) == 0) ahead_pages = i + lane < n_mine ? table[(p_begin + i + lane) / 2] : 0;
             const size_t page = __shfl_sync(0xffffffffu, ahead_pages, i & 31);
+            const int odd = (p_begin + i) & 1;
             const uint32_t dst = ring + (i % F::STAGES) * 2 * F::HALF_BYTES + lane * 16;
-            const uint8_t* ks = kh + page * kv.k_stride;
-            const uint8_t* vs = vh + page * kv.v_stride;
+            const uint8_t* ks = kh + page * kv.k_stride + odd * F::HALF_BYTES;
+            const uint8_t* vs = vh + page * kv.v_stride + odd * kStepRows;
 #pragma unroll
-            for (int c = 0; c < F::HALF_BYTES; c += 512) {
-                copy_async16(dst + c, ks + c);
-                copy_async16(dst + F::HALF_BYTES + c, vs + c);
+            for (int c = 0; c < HD / 16; ++c) {
+                copy_async16((F::SWAP ? dst ^ (lane << 3 & 64) : dst) + c * 512, ks + c * 512);           // bit 3 of the lane: the row's parity
+                copy_async16(dst + F::HALF_BYTES + c * 512, vs + c * 16 * kPageTokens);
             }
         };
-        // Pages before the newest were complete before the kernel that stores this step's rows began (it lets its successor
-        // begin only after its own wait), so their copies may start while it runs; the pages that take new rows may not.
-        const int p_new = waited ? 0x7fffffff : span.start / kPageTokens;
         int ahead = 0;
         __syncwarp();                                                           // the stretch before has been read
-#pragma unroll
-        for (int s = 0; s < F::STAGES - 1; ++s) {
-            if (ahead == s && s < n_mine && p_begin + s < p_new) load(ahead++);
-        }
         if (!waited) {
+            // Pages before the newest were complete before the kernel that stores this step's rows began (it lets its successor
+            // begin only after its own wait), so their copies may start while it runs; the pages that take new rows may not.
+            if (a.chained) {
+#pragma unroll
+                for (int s = 0; s < F::STAGES - 1; ++s)
+                    if (ahead == s && s < n_mine && p_begin + s < span.start / kPageTokens * 2) load(ahead++);
+            }
             chain_wait();
             waited = true;
+        }
+        // ---- queries: column g of a tile is query g / 2, its high codes (even g) or its low ones
+        uint32_t qf[NT][2 * F::STEPS];
+        float factor[NT];                                                           // of query t4: what a score is multiplied with
+        int seen_to[NT];                                                            // the last row query t4 sees; -1: no such query
+        uint32_t x[NT][HD / 8];                                                     // two channels each
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int c = c0 + nt * 4 + (g >> 1);
+            const bool real = c < n_columns;
+            const bf16* src = a.q + (size_t)(span.first + (real ? c / a.group : 0)) * a.ldq + (size_t)(h * a.group + (real ? c % a.group : 0)) * HD +
+                              t4 * F::PIECE;
+#pragma unroll
+            for (int pc = 0; pc < F::PIECES; ++pc) {
+                uint32_t* to = x[nt] + pc * F::PIECE / 2;
+                const bf16* from = src + pc * 4 * F::PIECE;
+                if (a.wide) {
+                    if constexpr (F::PIECE == 4) {
+                        const uint2 u = *reinterpret_cast<const uint2*>(from);
+                        to[0] = u.x; to[1] = u.y;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < F::PIECE / 8; ++i) {
+                            const uint4 u = reinterpret_cast<const uint4*>(from)[i];
+                            to[4 * i] = u.x; to[4 * i + 1] = u.y; to[4 * i + 2] = u.z; to[4 * i + 3] = u.w;
+                        }
+                    }
+                } else {
+                    const uint16_t* each = reinterpret_cast<const uint16_t*>(from);
+#pragma unroll
+                    for (int i = 0; i < F::PIECE / 2; ++i) to[i] = each[2 * i] | (uint32_t)each[2 * i + 1] << 16;
+                }
+            }
+            if (!real) {
+#pragma unroll
+                for (int i = 0; i < HD / 8; ++i) x[nt][i] = 0;
+            }
         }
 #pragma unroll
         for (int s = 0; s < F::STAGES - 1; ++s) {
             if (ahead == s && s < n_mine) load(ahead++);
             cp_async_commit();
         }
-
-        // ---- queries: column g of a tile is query g / 2, its high codes (even g) or its low ones
-        uint32_t qf[NT][2 * F::STEPS];
-        float factor[NT];                                                           // of query t4: what a score is multiplied with
-        int seen_to[NT];                                                            // the last row query t4 sees; -1: no such query
+        float k_scales = 0.f, v_scales = 0.f;                                       // lane i: of step (i / 32 * 32 + i) of the stretch
+        auto load_scales = [&](int pages) {
+            const float* s = kv.scales + (size_t)pages * kv.scale_stride + h;
+            k_scales = s[0];
+            v_scales = s[kv.n_kv];
+        };
+        if (lane < n_mine) load_scales(ahead_pages);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int c = c0 + nt * 4 + (g >> 1);
-            const bool real = c < n_columns;
-            const bf16* src = a.q + (size_t)(span.first + (real ? c / a.group : 0)) * a.ldq + (size_t)(h * a.group + (real ? c % a.group : 0)) * HD;
-            float x[W][4];
-            float most = 0.f;
+            uint32_t most = 0;                                                      // the largest magnitude, as bits
 #pragma unroll
-            for (int s = 0; s < W; ++s) {
-                const int d = s / (F::PIECE / 4) * 4 * F::PIECE + t4 * F::PIECE + s % (F::PIECE / 4) * 4;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[s][e] = real ? __bfloat162float(src[d + e]) : 0.f;
-                    most = fmaxf(most, finite_f32(x[s][e]) ? fabsf(x[s][e]) : 0.f);
-                }
-            }
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            for (int i = 0; i < HD / 8; ++i) most = __vmaxu2(most, x[nt][i] & 0x7fff7fffu);
+            most = max(most & 0xffffu, most >> 16);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
             // the largest channel comes to lie in [128, 256)
-            const int e = (int)(__float_as_uint(most) >> 23);
-            const int up = e == 0 ? 0 : min(max(7 - (e - 127), -100), 100);
+            const int e = (int)(most >> 7), up = e == 0 ? 0 : min(max(7 - (e - 127), -100), 100);
             const float f = __uint_as_float((uint32_t)(127 + up) << 23);
             const float back = a.scale * kLog2e * __uint_as_float((uint32_t)(127 - up) << 23);
             factor[nt] = __shfl_sync(0xffffffffu, back, 8 * t4);
             const int cq = c0 + nt * 4 + t4;
             seen_to[nt] = cq < n_columns ? span.start + cq / a.group : -1;
+            const bool whole = e < 255;                                             // else the scores are NaN, whatever its other channels are
+            uint32_t pair[HD / 8];
 #pragma unroll
-            for (int s = 0; s < 2 * F::STEPS; ++s) {
-                uint32_t word = 0;
-                if (s < W) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float y = x[s < W ? s : 0][i] * f;
-                        const uint8_t hi = e4m3_code(y);
-                        word |= (uint32_t)((g & 1) && finite_f32(y) ? e4m3_code((y - e4m3_value(hi)) * 16.f) : hi) << (8 * i);
-                    }
-                }
-                qf[nt][s] = word;
+            for (int i = 0; i < HD / 8; ++i) {                                      // (8 bits in a half's 11: exact down to 2^-22 of the largest)
+                const __half2 y = __floats2half2_rn(__uint_as_float(x[nt][i] << 16) * f, __uint_as_float(x[nt][i] & 0xffff0000u) * f);
+                const uint32_t hi = codes_of_f16(y);
+                const uint32_t lo = codes_of_f16(__hmul2(__hsub2(y, f16_of_codes(hi)), __floats2half2_rn(16.f, 16.f)));
+                pair[i] = !whole ? 0x7f7fu : g & 1 ? lo : hi;
             }
+#pragma unroll
+            for (int s = 0; s < W; ++s) qf[nt][s] = pair[2 * s] | pair[2 * s + 1] << 16;
+            if (W & 1) qf[nt][2 * F::STEPS - 1] = 0;
         }
         const int least_to = span.start + c0 / a.group;
         const int most_to = span.start + min(n_columns - 1, c0 + 4 * NT - 1) / a.group;
@@ -315,14 +371,9 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
             for (int i = 0; i < F::TILES; ++i) o[i][nt][0] = o[i][nt][1] = 0.f;
         }
 
-        float k_scales = 0.f, v_scales = 0.f;                                       // lane i: of page (i / 32 * 32 + i) of the stretch
         for (int i = 0; i < n_mine; ++i) {
             const int p = p_begin + i;
-            if ((i & 31) == 0 && i + lane < n_mine) {
-                const float* s = kv.scales + (size_t)table[p + lane] * kv.scale_stride + h;
-                k_scales = s[0];
-                v_scales = s[kv.n_kv];
-            }
+            if (i > 0 && (i & 31) == 0 && i + lane < n_mine) load_scales(table[(p + lane) / 2]);
             const float k_scale = __shfl_sync(0xffffffffu, k_scales, i & 31), v_scale = __shfl_sync(0xffffffffu, v_scales, i & 31);
             cp_async_wait<F::STAGES - 2>();
             __syncwarp();                                                           // page i is there, page i - 1 has been read
@@ -330,17 +381,17 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
             if (ahead < n_mine) load(ahead++);                                      // where page i - 1 was
             cp_async_commit();
             // (queries that do not exist are zeros and see what they like)
-            const bool all_seen = p * kPageTokens + kPageTokens - 1 <= least_to && (a.window <= 0 || p * kPageTokens > most_to - a.window);
-            // ---- scores of the page's 64 rows: of query t4, rows g and g + 8 of each tile
-            float s[4][NT][2];
+            const bool all_seen = p * kStepRows + kStepRows - 1 <= least_to && (a.window <= 0 || p * kStepRows > most_to - a.window);
+            // ---- scores of the step's 32 rows: of query t4, rows g and g + 8 of each tile
+            float s[2][NT][2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
                 uint32_t w[2][2 * F::STEPS];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
 #pragma unroll
                     for (int pc = 0; pc < F::PIECES; ++pc) {
-                        const unsigned char* at = stage + tile_row(j, g + 8 * r) * HD + pc * 4 * F::PIECE + t4 * F::PIECE;
+                        const unsigned char* at = stage + tile_row(j, g + 8 * r) * HD + (F::SWAP ? pc ^ (g & 1) : pc) * 4 * F::PIECE + t4 * F::PIECE;
                         if constexpr (F::PIECE == 16) {
                             const uint4 u = *reinterpret_cast<const uint4*>(at);
                             w[r][4 * pc] = u.x; w[r][4 * pc + 1] = u.y; w[r][4 * pc + 2] = u.z; w[r][4 * pc + 3] = u.w;
@@ -355,9 +406,10 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    float c[4];
+                    mma_e4m3_16832_first(c, w[0][0], w[1][0], w[0][1], w[1][1], qf[nt][0], qf[nt][1]);
 #pragma unroll
-                    for (int k = 0; k < F::STEPS; ++k)
+                    for (int k = 1; k < F::STEPS; ++k)
                         mma_e4m3_16832(c, w[0][2 * k], w[1][2 * k], w[0][2 * k + 1], w[1][2 * k + 1], qf[nt][2 * k], qf[nt][2 * k + 1]);
                     const float f = factor[nt] * k_scale;
                     s[j][nt][0] = fmaf(c[1], 0.0625f, c[0]) * f;
@@ -369,33 +421,32 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
                 for (int nt = 0; nt < NT; ++nt) {
                     const int to = seen_to[nt], from = a.window > 0 ? to - a.window : -1;              // rows from + 1 .. to
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int j = 0; j < 2; ++j)
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            const int row = p * kPageTokens + tile_row(j, g + 8 * r);
+                            const int row = p * kStepRows + tile_row(j, g + 8 * r);
                             if (row > to || row <= from) s[j][nt][r] = -INFINITY;
                         }
                 }
             }
-            if (a.scores && p < a.score_pages) {
+            if (a.scores && p < 2 * a.score_pages) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const int c = c0 + nt * 4 + t4;
                     if (c < n_columns) {
-                        float4* at = reinterpret_cast<float4*>(a.scores + ((((size_t)b * kv.n_kv + h) * a.columns + c) * a.score_pages + p) * kPageTokens + g * 8);
-                        at[0] = make_float4(s[0][nt][0], s[0][nt][1], s[1][nt][0], s[1][nt][1]);
-                        at[1] = make_float4(s[2][nt][0], s[2][nt][1], s[3][nt][0], s[3][nt][1]);
+                        float* at = a.scores + (((size_t)b * kv.n_kv + h) * a.columns + c) * a.score_pages * kPageTokens + (size_t)p * kStepRows + g * 4;
+                        *reinterpret_cast<float4*>(at) = make_float4(s[0][nt][0], s[0][nt][1], s[1][nt][0], s[1][nt][1]);
                     }
                 }
             }
             // ---- running maximum and sum; probabilities' codes as the second product's right operand: columns (query, p1 | p2)
-            //      in pf[0], (query, p3 | nothing) in pf[1]
+            //      in pf, and in ph the p3 of two tiles (of one, and nothing)
+            constexpr int NH = (NT + 1) / 2;
             float corr[NT];
-            uint32_t pf[2][4][NT];
+            uint32_t pf[2][NT], ph[2][NH];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float mx = fmaxf(fmaxf(fmaxf(s[0][nt][0], s[0][nt][1]), fmaxf(s[1][nt][0], s[1][nt][1])),
-                                 fmaxf(fmaxf(s[2][nt][0], s[2][nt][1]), fmaxf(s[3][nt][0], s[3][nt][1])));
+                float mx = fmaxf(fmaxf(s[0][nt][0], s[0][nt][1]), fmaxf(s[1][nt][0], s[1][nt][1]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -405,7 +456,7 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
                 m[nt] = now;
                 float sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < 2; ++j) {
                     const float p0 = exp2_fast(s[j][nt][0] - use + kPShift), p1 = exp2_fast(s[j][nt][1] - use + kPShift);
                     sum += p0 + p1;
                     const __half2 sixteen = __floats2half2_rn(16.f, 16.f);
@@ -414,20 +465,22 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
                     rest = __hmul2(__hsub2(rest, f16_of_codes(c1)), sixteen);
                     const uint32_t c2 = codes_of_f16(rest);
                     rest = __hmul2(__hsub2(rest, f16_of_codes(c2)), sixteen);
-                    pf[0][j][nt] = in_row_order(transpose_8x8(c1 | c2 << 16));
-                    pf[1][j][nt] = in_row_order(transpose_8x8(codes_of_f16(rest)));
+                    const uint32_t c3 = codes_of_f16(rest);
+                    pf[j][nt] = in_row_order(transpose_8x8(c1 | c2 << 16));
+                    ph[j][nt / 2] = nt & 1 ? ph[j][nt / 2] | c3 << 16 : c3;
+                    if ((nt & 1) || nt == NT - 1) ph[j][nt / 2] = in_row_order(transpose_8x8(ph[j][nt / 2]));
                 }
                 l[nt] = l[nt] * corr[nt] + sum;
             }
             // ---- O^T += V^T P^T, 16 channels at a time
-            bool odd = false;                                                       // a NaN code in a page that not every query sees whole
+            bool odd = false;                                                       // a NaN code in a step that not every query sees whole
 #pragma unroll
             for (int ct = 0; ct < F::TILES; ++ct) {
-                uint32_t w[2][4];
+                uint32_t w[2][2];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(stage + F::HALF_BYTES + (16 * ct + 8 * r + g) * kPageTokens + t4 * 16);
-                    w[r][0] = u.x; w[r][1] = u.y; w[r][2] = u.z; w[r][3] = u.w;
+                    const uint2 u = *reinterpret_cast<const uint2*>(stage + F::HALF_BYTES + (16 * ct + 8 * r + g) * kStepRows + t4 * 8);
+                    w[r][0] = u.x; w[r][1] = u.y;
                 }
                 if (!all_seen) {
                     // A row that a query does not see has probability 0 there; its values may still be the NaN code, which
@@ -435,56 +488,54 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
+                        for (int j = 0; j < 2; ++j) {
                             const uint32_t nan = __vcmpeq4(w[r][j] & 0x7f7f7f7fu, 0x7f7f7f7fu);
                             odd |= nan != 0;
                             w[r][j] &= ~nan;
                         }
                 }
+                float u[NH][4];
+#pragma unroll
+                for (int nh = 0; nh < NH; ++nh) mma_e4m3_16832_first(u[nh], w[0][0], w[1][0], w[0][1], w[1][1], ph[0][nh], ph[1][nh]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float t[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        mma_e4m3_16832(t, w[0][2 * k], w[1][2 * k], w[0][2 * k + 1], w[1][2 * k + 1], pf[0][2 * k][nt], pf[0][2 * k + 1][nt]);
-                        mma_e4m3_16832(u, w[0][2 * k], w[1][2 * k], w[0][2 * k + 1], w[1][2 * k + 1], pf[1][2 * k][nt], pf[1][2 * k + 1][nt]);
-                    }
+                    float t[4];
+                    mma_e4m3_16832_first(t, w[0][0], w[1][0], w[0][1], w[1][1], pf[0][nt], pf[1][nt]);
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
-                        o[ct][nt][r] = fmaf(o[ct][nt][r], corr[nt], fmaf(u[2 * r], 0.00390625f, fmaf(t[2 * r + 1], 0.0625f, t[2 * r])) * v_scale);
+                        o[ct][nt][r] = fmaf(o[ct][nt][r], corr[nt],
+                                            fmaf(u[nt / 2][2 * r + (nt & 1)], 0.00390625f, fmaf(t[2 * r + 1], 0.0625f, t[2 * r])) * v_scale);
                 }
             }
             if (__any_sync(0xffffffffu, odd)) {
                 // how many NaN codes of rows it sees a query meets in each channel: ones (code 0x38) for the codes, ones for the rows seen
-                uint32_t seen[4][NT];
+                uint32_t seen[2][NT];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < 2; ++j) {
                         uint32_t pair = 0;
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            const int to = seen_to[nt], row = p * kPageTokens + tile_row(j, g + 8 * r);
+                            const int to = seen_to[nt], row = p * kStepRows + tile_row(j, g + 8 * r);
                             if (row <= to && (a.window <= 0 || row > to - a.window)) pair |= 0x38u << (8 * r);
                         }
                         seen[j][nt] = in_row_order(transpose_8x8(pair));
                     }
 #pragma unroll
                 for (int ct = 0; ct < F::TILES; ++ct) {
-                    uint32_t w[2][4];
+                    uint32_t w[2][2];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const uint4 u = *reinterpret_cast<const uint4*>(stage + F::HALF_BYTES + (16 * ct + 8 * r + g) * kPageTokens + t4 * 16);
-                        w[r][0] = u.x; w[r][1] = u.y; w[r][2] = u.z; w[r][3] = u.w;
+                        const uint2 u = *reinterpret_cast<const uint2*>(stage + F::HALF_BYTES + (16 * ct + 8 * r + g) * kStepRows + t4 * 8);
+                        w[r][0] = u.x; w[r][1] = u.y;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) w[r][j] = __vcmpeq4(w[r][j] & 0x7f7f7f7fu, 0x7f7f7f7fu) & 0x38383838u;
+                        for (int j = 0; j < 2; ++j) w[r][j] = __vcmpeq4(w[r][j] & 0x7f7f7f7fu, 0x7f7f7f7fu) & 0x38383838u;
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            mma_e4m3_16832(t, w[0][2 * k], w[1][2 * k], w[0][2 * k + 1], w[1][2 * k + 1], seen[2 * k][nt], seen[2 * k + 1][nt]);
+                        float t[4];
+                        mma_e4m3_16832_first(t, w[0][0], w[1][0], w[0][1], w[1][1], seen[0][nt], seen[1][nt]);
                         if (t[0] > 0.f) o[ct][nt][0] = __uint_as_float(0x7fc00000u);
                         if (t[2] > 0.f) o[ct][nt][1] = __uint_as_float(0x7fc00000u);
                     }
@@ -494,7 +545,7 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
         cp_async_wait<0>();
 
         // ---- the whole of its pages: the unit's result; else a part of it, for the joining kernel
-        const bool whole = n_mine == n_pages;
+        const bool whole = n_mine == n_steps;
         const size_t part = ((size_t)worker + (size_t)b * units + in_b) * 4 * NT;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -539,80 +590,89 @@ __global__ void __launch_bounds__(kJoinThreads)
 few_join_kernel(const FewArgs a, const E4M3Pages kv, int join_blocks) {
     using J = Join<HD>;
     chain_release();
-    chain_wait();
-    __shared__ float top[kFewColumns], inverse[kFewColumns];
-    __shared__ int first_worker[kFewColumns / (4 * NT)], last_worker[kFewColumns / (4 * NT)];             // that share a tile's pages
-    __shared__ float4 sums[J::ROWS * J::LANES];
     const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
-    const long long per = a.line[0], begin = a.line[1 + b];
-    const FewSpan span = few_span(a, kv, b);
-    const int n_columns = span.n_new * a.group, n_pages = span.pages();
-    const bool joins = (int)blockIdx.x < join_blocks;
-    const int share = J::share(a.columns), c_begin = joins ? blockIdx.x * J::columns_each(a.columns) : 0;
-    const int c_end = joins ? min(n_columns, c_begin + J::columns_each(a.columns)) : n_columns;
-    if (c_begin >= c_end) return;
-    const int units = kv.n_kv * a.tiles;
-    if (tid < a.tiles) {
-        const long long at = begin + (long long)(h * a.tiles + tid) * n_pages;
-        first_worker[tid] = (int)(at / per);
-        last_worker[tid] = (int)((at + n_pages - 1) / per);
+    const FewPlace place = few_place<false>(a, kv, kv.n_kv * a.tiles, b);       // (of what the kernel before this one only reads, too)
+    const FewSeq span = place.seq;
+    const int per = place.per, n_columns = span.n_new * a.group, n_line = on_line(span.steps());
+    chain_wait();
+    if (n_columns <= 0) return;
+    const size_t unit = (size_t)(b * kv.n_kv + h) * a.tiles;
+    auto part_of = [&](int worker, int c) { return ((size_t)worker + unit + c / (4 * NT)) * 4 * NT + c % (4 * NT); };
+    // the workers that share the steps of query c: first and last
+    auto first_worker = [&](int c) { return (span.begin + (h * a.tiles + c / (4 * NT)) * n_line + kUnitCost) / per; };
+    auto last_worker = [&](int c) { return (span.begin + (h * a.tiles + c / (4 * NT) + 1) * n_line - 1) / per; };
+    // a running maximum and sum, and another part's: what each of the two is multiplied with
+    auto join = [](float& M, float m, float& mine, float& theirs) {
+        const float now = fmaxf(M, m), use = now == -INFINITY ? 0.f : now;
+        mine = exp2_fast(M - use);
+        theirs = exp2_fast(m - use);
+        M = now;
+    };
+    if ((int)blockIdx.x < join_blocks) {
+        __shared__ float4 sums[J::ROWS * J::LANES];
+        __shared__ float2 stats[J::ROWS];
+        const int share = J::share(a.columns), row = tid / J::LANES, d = tid % J::LANES * 4;
+        const int c = blockIdx.x * J::columns_each(a.columns) + row / share;
+        const bool mine = row / share < J::columns_each(a.columns) && c < n_columns;
+        const int w0 = mine ? first_worker(c) : 0, w1 = mine ? last_worker(c) : 0;                        // w0 == w1: it is not in parts
+        if (w0 < w1) {
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float M = -INFINITY, L = 0.f, f, g;
+#pragma unroll 4
+            for (int w = w0 + row % share; w <= w1; w += share) {
+                const size_t at = part_of(w, c);
+                const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+                const float4 o = *reinterpret_cast<const float4*>(a.part_o + at * HD + d);
+                join(M, ml.x, f, g);
+                L = fmaf(g, ml.y, L * f);
+                acc.x = fmaf(g, o.x, acc.x * f); acc.y = fmaf(g, o.y, acc.y * f); acc.z = fmaf(g, o.z, acc.z * f); acc.w = fmaf(g, o.w, acc.w * f);
+            }
+            sums[tid] = acc;
+            if (d == 0) stats[row] = make_float2(M, L);
+        }
+        __syncthreads();
+        if (w0 < w1 && row % share == 0) {
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float M = -INFINITY, L = 0.f, f, g;
+            for (int i = 0; i < share; ++i) {
+                const float4 o = sums[tid + i * J::LANES];
+                const float2 ml = stats[row + i];
+                join(M, ml.x, f, g);
+                L = fmaf(g, ml.y, L * f);
+                acc.x = fmaf(g, o.x, acc.x * f); acc.y = fmaf(g, o.y, acc.y * f); acc.z = fmaf(g, o.z, acc.z * f); acc.w = fmaf(g, o.w, acc.w * f);
+            }
+            const float inverse = 1.0f / L;
+            bf16* out = a.out + (size_t)(span.first + c / a.group) * a.ldo + (size_t)(h * a.group + c % a.group) * HD + d;
+            out[0] = __float2bfloat16_rn(acc.x * inverse);
+            out[1] = __float2bfloat16_rn(acc.y * inverse);
+            out[2] = __float2bfloat16_rn(acc.z * inverse);
+            out[3] = __float2bfloat16_rn(acc.w * inverse);
+        }
+        return;
     }
-    __syncthreads();
-    auto part_of = [&](int worker, int c) { return ((size_t)worker + (size_t)b * units + h * a.tiles + c / (4 * NT)) * 4 * NT + c % (4 * NT); };
-    for (int c = c_begin + (tid >> 5); c < c_end; c += kJoinThreads / 32) {     // a warp a query: its maximum and sum over the parts
-        const int w0 = first_worker[c / (4 * NT)], w1 = last_worker[c / (4 * NT)];
-        if (w0 == w1 && !a.scores) continue;                                    // it is not in parts
-        float M = -INFINITY, L = 0.f;
+    __shared__ float top[kFewColumns], inverse[kFewColumns];
+    for (int c = tid >> 5; c < n_columns; c += kJoinThreads / 32) {             // a warp a query: its maximum and sum over the parts
+        const int w0 = first_worker(c), w1 = last_worker(c);
+        float M = -INFINITY, L = 0.f, f, g;
         for (int w = w0 + (tid & 31); w <= w1; w += 32) {
             const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + part_of(w, c) * 2);
-            const float now = fmaxf(M, ml.x);
-            L = L * exp2_fast(M - (now == -INFINITY ? 0.f : now)) + exp2_fast(ml.x - (now == -INFINITY ? 0.f : now)) * ml.y;
-            M = now;
+            join(M, ml.x, f, g);
+            L = fmaf(g, ml.y, L * f);
         }
         const float all = warp_max(M), use = all == -INFINITY ? 0.f : all;
         L = warp_sum(exp2_fast(M - use) * L);
         if ((tid & 31) == 0) { top[c] = use; inverse[c] = 1.0f / L; }
     }
     __syncthreads();
-    if (joins) {
-        const int row = tid / J::LANES, d = tid % J::LANES * 4, c = c_begin + row / share;
-        const bool mine = row < J::ROWS && c < c_end;
-        const int w0 = mine ? first_worker[c / (4 * NT)] : 0, w1 = mine ? last_worker[c / (4 * NT)] : 0;
-        if (w0 < w1) {
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (int w = w0 + row % share; w <= w1; w += share) {
-                const size_t at = part_of(w, c);
-                const float4 o = *reinterpret_cast<const float4*>(a.part_o + at * HD + d);
-                const float f = exp2_fast(a.part_ml[at * 2] - top[c]);
-                acc.x = fmaf(f, o.x, acc.x); acc.y = fmaf(f, o.y, acc.y); acc.z = fmaf(f, o.z, acc.z); acc.w = fmaf(f, o.w, acc.w);
-            }
-            sums[tid] = acc;
-        }
-        __syncthreads();
-        if (w0 < w1 && row % share == 0) {
-            float4 acc = sums[tid];
-            for (int i = 1; i < share; ++i) {
-                const float4 o = sums[tid + i * J::LANES];
-                acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
-            }
-            bf16* out = a.out + (size_t)(span.first + c / a.group) * a.ldo + (size_t)(h * a.group + c % a.group) * HD + d;
-            out[0] = __float2bfloat16_rn(acc.x * inverse[c]);
-            out[1] = __float2bfloat16_rn(acc.y * inverse[c]);
-            out[2] = __float2bfloat16_rn(acc.z * inverse[c]);
-            out[3] = __float2bfloat16_rn(acc.w * inverse[c]);
-        }
-        return;
-    }
-    const int* table = kv.block_table + (size_t)a.slots[b] * kv.table_stride;
+    const int* table = kv.block_table + (size_t)span.slot * kv.table_stride;
     const int stride = ((int)gridDim.x - join_blocks) * (kJoinThreads / kPageTokens);
-    for (int p = span.p_first + ((int)blockIdx.x - join_blocks) * (kJoinThreads / kPageTokens) + tid / kPageTokens; p <= span.p_last; p += stride) {
+    for (int p = span.p_first / 2 + ((int)blockIdx.x - join_blocks) * (kJoinThreads / kPageTokens) + tid / kPageTokens; p <= span.p_last / 2; p += stride) {
         const int t = tid % kPageTokens, row = p * kPageTokens + t;
-        if (row >= span.start + span.n_new) continue;
+        if (row < span.p_first * kStepRows || row >= span.start + span.n_new) continue;                   // seen by no query
         const size_t page = table[p];
         float sum = 0.f;
         if (p < a.score_pages) {
-            const float* at = a.scores + (((size_t)b * kv.n_kv + h) * a.columns * a.score_pages + p) * kPageTokens + score_place(t);
+            const float* at = a.scores + (((size_t)b * kv.n_kv + h) * a.columns * a.score_pages + p) * kPageTokens + t / kStepRows * kStepRows + score_place(t % kStepRows);
             for (int c = 0; c < n_columns; ++c)
                 sum += exp2_fast(at[(size_t)c * a.score_pages * kPageTokens] - top[c] + kPShift) * inverse[c];
         } else {                                                                // a sequence that has outgrown the plan: score the row again
@@ -637,12 +697,17 @@ bool few_takes(int dtype, int max_q_len, int n_heads, int n_kv, int hd) {
 
 // Tiles of four queries a unit has.
 int few_tiles(int columns) { return columns <= 4 ? 1 : columns <= 8 ? 2 : 4; }
+// The line is counted in 32 bits: no table of this width holds more steps than that.
+bool few_counts(int B, int max_q_len, int n_heads, int n_kv, int table_width) {
+    const int columns = max_q_len * (n_heads / n_kv), each = 4 * few_tiles(columns);
+    return (double)B * n_kv * ((columns + each - 1) / each) * ((double)table_width * (kPageTokens / kStepRows) + 1 + kUnitCost) < 1 << 30;
+}
 
 // How many warps run at once, and the scratch they need.
 struct FewPlan {
     int columns, nt, tiles, workers, score_pages;
-    long long line, part_o, part_ml, scores;                                    // floats, each a multiple of 4
-    long long floats() const { return line + part_o + part_ml + scores; }
+    long long part_o, part_ml, scores;                                          // floats, each a multiple of 4
+    long long floats() const { return part_o + part_ml + scores; }
 };
 
 // Warps of this kernel that the current device runs at once (asked once a device).
@@ -659,7 +724,7 @@ int few_workers() {
             (void)cudaGetLastError();
             return kFewWarps;
         }
-        cached[dev] = (blocks * sms - 1) * kFewWarps;                           // one block keeps the line
+        cached[dev] = blocks * sms * kFewWarps;
     }
     return cached[dev];
 }
@@ -673,7 +738,6 @@ FewPlan few_plan_for(int B, int max_q_len, int n_heads, int n_kv, int max_kv_len
     plan.workers = plan.nt == 4 ? few_workers<HD, 4>() : plan.nt == 2 ? few_workers<HD, 2>() : few_workers<HD, 1>();
     plan.score_pages = weigh ? (max_kv_len + kPageTokens - 1) / kPageTokens : 0;
     const long long parts = ((long long)plan.workers + (long long)B * n_kv * plan.tiles) * 4 * plan.nt;
-    plan.line = ((long long)B + 2) / 2 * 4;
     plan.part_o = parts * HD;
     plan.part_ml = parts * 2;
     plan.scores = (long long)B * n_kv * plan.columns * plan.score_pages * kPageTokens;
@@ -682,7 +746,7 @@ FewPlan few_plan_for(int B, int max_q_len, int n_heads, int n_kv, int max_kv_len
 
 template <int HD, int NT>
 int launch_few_tiles(const FewArgs& a, const E4M3Pages& kv, cudaStream_t stream) {
-    const int st = launch_chained(few_queries_kernel<HD, NT>, dim3(a.workers / kFewWarps + 1), dim3(kFewThreads), Few<HD>::RING,
+    const int st = launch_chained(few_queries_kernel<HD, NT>, dim3(a.workers / kFewWarps), dim3(kFewThreads), Few<HD>::RING,
                                   stream, a, kv);
     if (st != 0) return st;
     const int join = (a.columns + Join<HD>::columns_each(a.columns) - 1) / Join<HD>::columns_each(a.columns);
@@ -696,8 +760,7 @@ int launch_few(FewArgs a, const E4M3Pages& kv, const FewPlan& plan, float* scrat
     a.tiles = plan.tiles;
     a.workers = plan.workers;
     a.score_pages = plan.score_pages;
-    a.line = (long long*)scratch;
-    a.part_o = scratch + plan.line;
+    a.part_o = scratch;
     a.part_ml = a.part_o + plan.part_o;
     a.scores = plan.scores ? a.part_ml + plan.part_ml : nullptr;
     return plan.nt == 4 ? launch_few_tiles<HD, 4>(a, kv, stream)
