@@ -7,8 +7,6 @@
 //   few_queries:      bfloat16, heads of up to 128 channels in steps of 16, few queries a sequence (attention_e4m3_few.cuh);
 //   attention_rows:   any head size and type, one block per (token, query head); scores, softmax and sums in float.
 //   row_weights:      the weights, once every row's maximum and sum are known: a block per (cache page, head, sequence).
-#include <algorithm>
-
 #include "attention_e4m3_few.cuh"
 
 namespace {

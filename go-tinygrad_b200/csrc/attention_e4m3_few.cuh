@@ -5,50 +5,38 @@
 // from memory to the tensor cores as they are, once, and everything else is arranged around the order in which they lie.
 //
 //   * Both products multiply codes with codes: the cache's rows (or, in the second, its channels) are the M = 16 rows of an
-//     e4m3 product, S^T = K Q^T and O^T = V^T P^T, and nothing of the cache is converted.  (A first form turned every pair of
-//     codes into halves: 835 instructions a warp and page of 64 x 64, more than half of them for that, and 64 us where this one
-//     takes the time given below.)
+//     e4m3 product, S^T = K Q^T and O^T = V^T P^T, and nothing of the cache is converted.  (A form that turned every pair of
+//     codes into halves spent more than half of its instructions on that.)
 //   * The other operand is split into codes that add up to it, each with columns of its own.  A bfloat16 query has 8 significant
 //     bits, two codes of 4: q 2^a = hi + lo / 16, exact down to 2^-13 of the row's largest channel and off by at most 2^-21 of
 //     it below.  A probability, times 2^8 and rounded to half (11 bits, half a step 2^-11), is three codes:
 //     p1 + p2 / 16 + p3 / 256.  The products of codes are exact and are summed in float, so no other rounding enters.
 //   * A lane's operand fragment of 16 rows x 32 channels is four words of four codes of two rows.  Which channel is which k
 //     index of the product is free as long as keys and queries agree, so a lane takes 16 neighbouring channels of its row
-//     (one 16-byte piece: the fragments of two k steps), and the same of V^T, whose rows are channels and whose 64 columns are the
-//     page's rows.  The rows of the score tiles are dealt so that the scores come out where the second product wants them
+//     (one 16-byte piece: the fragments of two k steps), and 8 of V^T, whose rows are channels and whose columns are the cache's
+//     rows.  The rows of the score tiles are dealt so that the scores come out where the second product wants them
 //     (tile_row); one 8 x 8 transpose of 16-bit pairs then makes four probabilities' codes the word of a fragment.
 //   * Scores, maxima, sums and outputs are float.  The scales of a page's block multiply a score and a page's output sums
 //     once: an exact product.
-//   * Every warp copies whole pages ahead of itself into places of its own in shared memory (cp.async, whole lines in
-//     order: with every lane fetching just the pieces it multiplies, half lines in the tiles' order, the same kernel was
-//     slower), so that no warp waits for another; the warps of a block take turns with the pages, blocks share a
-//     sequence's pages (split), and a second kernel joins the parts -- and, where weights are gathered, turns the scores, kept
-//     in float, into probabilities now that every query's maximum and sum are known.
+//   * A warp works by itself: it copies half pages (32 rows of keys and of values) ahead of itself into places of its own in
+//     shared memory (cp.async) and has its own running maximum and sum.  Half pages, because 10 to 12 warps an SM then find
+//     room: with whole pages six did, and each waited for itself (64 sequences of 130 to 2,300 rows, 8 kv heads of 128: 57.9 us
+//     where this form took 52.4 before the steps below).  All warps share the pages of all sequences evenly (few_place).
+//   * What is left beside the reading is each warp's begin -- where its stretch lies, page numbers, queries, each a wait
+//     for memory -- and the joining kernel, whose waits are the same and which therefore finds its place while the first one
+//     still runs, reads all parts of a query at once and, where weights are gathered, turns the scores, kept in float, into
+//     probabilities now that every query's maximum and sum are known.
+// Measured on a B200, both kernels: 8 sequences of 8,192 rows, 32 heads of 64: 52.0 us for 268 MB of codes (5.2 TB/s; a plain
+// copy moves 6.5); the ragged batch above: 37.5 us for 165 MB; 8 of 4,000 with weights, 8 kv heads of 64: 16.5 us for 33 MB; one
+// of 2,251, 32 heads of 64: 8.9 us, all of it waits.
 #pragma once
 #include "mma_helpers.cuh"
 #include "e4m3.cuh"
+#include <algorithm>
 
 namespace {
 constexpr float kLog2e = 1.4426950408889634f;
-#ifndef GTG_FEW_WARPS
-#define GTG_FEW_WARPS 2
-#endif
-#ifndef GTG_FEW_STAGES
-#define GTG_FEW_STAGES 2
-#endif
-constexpr int kFewWarps = GTG_FEW_WARPS, kFewThreads = 32 * kFewWarps;
-#ifndef GTG_FEW_BLOCKS
-#define GTG_FEW_BLOCKS 6
-#endif
-#ifndef GTG_FEW_BLOCKS64
-#define GTG_FEW_BLOCKS64 6
-#endif
-#ifndef GTG_FEW_COST
-#define GTG_FEW_COST 2
-#endif
-#ifndef GTG_FEW_LEAST
-#define GTG_FEW_LEAST 2
-#endif
+constexpr int kFewWarps = 2, kFewThreads = 32 * kFewWarps;
 constexpr int kFewColumns = 32;          // queries a key/value head that these kernels take
 constexpr int kStepRows = 32;            // cache rows a warp takes at a time: half a page
 constexpr float kPShift = 8.0f;          // probabilities are held times 2^8
@@ -109,7 +97,7 @@ template <int HD> struct Few {
     static constexpr int HALF_BYTES = kStepRows * HD;                          // a step's
     // rows of 128 bytes: where two neighbours would share banks, the odd ones lie with their halves exchanged
     static constexpr int SWAP = HD == 128 ? 1 : 0;
-    static constexpr int STAGES = GTG_FEW_STAGES;
+    static constexpr int STAGES = 2;                                           // three: one sequence of 2,251 rows 8.9 -> 9.3 us
     static constexpr int RING = kFewWarps * STAGES * 2 * HALF_BYTES;
 };
 
@@ -152,10 +140,11 @@ __device__ __forceinline__ FewSeq few_seq(const FewArgs& a, const E4M3Pages& kv,
 // All steps of all units -- a unit is a (sequence, kv head, tile of queries) -- lie on one line: sequence by sequence, unit by
 // unit, step by step.  Every worker takes an equal stretch of it, so all finish together whatever the lengths are, and
 // whatever a plan was made for.  A unit's begin costs a worker queries, a page number and a result: kUnitCost empty steps
-// before its first stand for that.  Called by whole warps, which look at 32 sequences at a time, at the first 64 once:
+// before its first stand for that (none: 43.5 us where
+// two take 39.2, 64 sequences of 130 to 2,300 rows, 8 kv heads of 128).  Called by whole warps, which look at 32 sequences at a time, at the first 64 once:
 // the steps a worker takes, where worker's stretch begins, and the sequence that this (BY_WORKER) falls into, b = -1 behind
 // the line's end; or sequence `which`.
-constexpr int kSeenOnce = 2, kUnitCost = GTG_FEW_COST;
+constexpr int kSeenOnce = 2, kUnitCost = 2, kLeastSteps = 2;
 __device__ __forceinline__ int on_line(int steps) { return steps > 0 ? steps + kUnitCost : 0; }
 struct FewPlace { int per, from, b; FewSeq seq; };
 template <bool BY_WORKER>
@@ -175,7 +164,7 @@ __device__ __forceinline__ FewPlace few_place(const FewArgs& a, const E4M3Pages&
     for (int b0 = 32 * kSeenOnce; b0 < a.B; b0 += 32) total += __reduce_add_sync(0xffffffffu, on_line(at(b0 + lane).steps()));
     FewPlace p;
     // (shorter stretches would cost more in joining than they save)
-    p.per = max(GTG_FEW_LEAST, (int)(((unsigned)total * units + a.workers - 1) / a.workers));
+    p.per = max(kLeastSteps, (int)(((unsigned)total * units + a.workers - 1) / a.workers));
     p.from = BY_WORKER ? which * p.per : 0;
     p.b = -1;
     int begin = 0;
@@ -213,7 +202,7 @@ __device__ __forceinline__ FewPlace few_place(const FewArgs& a, const E4M3Pages&
 
 // A warp a worker; NT tiles of four queries a unit.
 template <int HD, int NT>
-__global__ void __launch_bounds__(kFewThreads, NT == 4 ? 4 : HD <= 64 ? GTG_FEW_BLOCKS64 : GTG_FEW_BLOCKS)
+__global__ void __launch_bounds__(kFewThreads, NT == 4 || (NT == 2 && HD > 80) ? 4 : HD <= 64 ? 6 : 5)
 few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
     using F = Few<HD>;
     constexpr int W = F::WORDS;
@@ -576,7 +565,7 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
 // Joins the parts (blocks x < join_blocks: some queries of one (sequence, kv head)) and, where weights are gathered, adds to
 // them (the other blocks, four pages at a time).  Both are a few short reads that wait for one another, so the parts of a
 // query are spread over all threads that its channels leave.
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinBlocks = 4;                             // blocks an SM
 
 template <int HD> struct Join {
     static constexpr int LANES = HD / 4;                                        // threads of a query's channels
@@ -586,7 +575,7 @@ template <int HD> struct Join {
 };
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(kJoinThreads, kJoinBlocks)
 few_join_kernel(const FewArgs a, const E4M3Pages kv, int join_blocks) {
     using J = Join<HD>;
     chain_release();
@@ -618,14 +607,28 @@ few_join_kernel(const FewArgs a, const E4M3Pages kv, int join_blocks) {
         if (w0 < w1) {
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
             float M = -INFINITY, L = 0.f, f, g;
-#pragma unroll 4
-            for (int w = w0 + row % share; w <= w1; w += share) {
-                const size_t at = part_of(w, c);
-                const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-                const float4 o = *reinterpret_cast<const float4*>(a.part_o + at * HD + d);
-                join(M, ml.x, f, g);
-                L = fmaf(g, ml.y, L * f);
-                acc.x = fmaf(g, o.x, acc.x * f); acc.y = fmaf(g, o.y, acc.y * f); acc.z = fmaf(g, o.z, acc.z * f); acc.w = fmaf(g, o.w, acc.w * f);
+            constexpr int kAtOnce = 4;                                              // reads in flight
+            for (int w = w0 + row % share; w <= w1; w += kAtOnce * share) {
+                float2 ml[kAtOnce];
+                float4 o[kAtOnce];
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const bool there = w + i * share <= w1;
+                    const size_t at = part_of(there ? w + i * share : w, c);
+                    ml[i] = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+                    o[i] = *reinterpret_cast<const float4*>(a.part_o + at * HD + d);
+                    if (!there) {
+                        ml[i] = make_float2(-INFINITY, 0.f);
+                        o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    join(M, ml[i].x, f, g);
+                    L = fmaf(g, ml[i].y, L * f);
+                    acc.x = fmaf(g, o[i].x, acc.x * f); acc.y = fmaf(g, o[i].y, acc.y * f);
+                    acc.z = fmaf(g, o[i].z, acc.z * f); acc.w = fmaf(g, o[i].w, acc.w * f);
+                }
             }
             sums[tid] = acc;
             if (d == 0) stats[row] = make_float2(M, L);
@@ -633,13 +636,15 @@ few_join_kernel(const FewArgs a, const E4M3Pages kv, int join_blocks) {
         __syncthreads();
         if (w0 < w1 && row % share == 0) {
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            float M = -INFINITY, L = 0.f, f, g;
+            float M = -INFINITY, L = 0.f;
+            for (int i = 0; i < share; ++i) M = fmaxf(M, stats[row + i].x);
+            const float use = M == -INFINITY ? 0.f : M;
+#pragma unroll 4
             for (int i = 0; i < share; ++i) {
                 const float4 o = sums[tid + i * J::LANES];
-                const float2 ml = stats[row + i];
-                join(M, ml.x, f, g);
-                L = fmaf(g, ml.y, L * f);
-                acc.x = fmaf(g, o.x, acc.x * f); acc.y = fmaf(g, o.y, acc.y * f); acc.z = fmaf(g, o.z, acc.z * f); acc.w = fmaf(g, o.w, acc.w * f);
+                const float f = exp2_fast(stats[row + i].x - use);
+                L = fmaf(f, stats[row + i].y, L);
+                acc.x = fmaf(f, o.x, acc.x); acc.y = fmaf(f, o.y, acc.y); acc.z = fmaf(f, o.z, acc.z); acc.w = fmaf(f, o.w, acc.w);
             }
             const float inverse = 1.0f / L;
             bf16* out = a.out + (size_t)(span.first + c / a.group) * a.ldo + (size_t)(h * a.group + c % a.group) * HD + d;
@@ -750,7 +755,9 @@ int launch_few_tiles(const FewArgs& a, const E4M3Pages& kv, cudaStream_t stream)
                                   stream, a, kv);
     if (st != 0) return st;
     const int join = (a.columns + Join<HD>::columns_each(a.columns) - 1) / Join<HD>::columns_each(a.columns);
-    const int pages = a.score_pages ? (a.score_pages * kPageTokens + kJoinThreads - 1) / kJoinThreads : 0;
+    // no more blocks than run at once: each begins with the same few reads, and a second turn would wait for them again
+    const int pages = a.score_pages ? std::max(1, std::min((a.score_pages * kPageTokens + kJoinThreads - 1) / kJoinThreads,
+                                                           kJoinBlocks * 148 / (kv.n_kv * a.B) - join)) : 0;
     return launch_behind(few_join_kernel<HD, NT>, dim3(join + pages, kv.n_kv, a.B), dim3(kJoinThreads), 0, stream, a, kv, join);
 }
 
