@@ -2,6 +2,7 @@
 //
 //   kv_store:  rotates a step's queries and keys and stores its keys and values, block by block;
 //   kv_evict:  keeps a sequence's newest rows and the heaviest of the others, in place.
+#include "mma_helpers.cuh"
 #include "e4m3.cuh"
 
 namespace {
@@ -252,17 +253,19 @@ kv_evict_kernel(const E4M3Pages pages, const EvictStrides strides, int* __restri
 // ---- the same for heads of a multiple of 16 channels, with the sequence's weights, pages and scales in shared memory.
 // Choosing: the weights are read once; the need-th largest is found eight bits a pass (equal digits of a warp counted by one
 // lane, the digit found by one warp), then every warp places a stretch of the rows by itself, after one exchange of counts.
-// Moving: eight warps move the keys and eight the values, tile by tile of 64 rows from the first that changes, the next
-// tile's codes on their way while one is worked on (what a tile overwrites no later one reads).  A value tile is gathered byte by
-// byte from its source pages' rows in shared memory, since the rows of the cache are innermost there.
+// Moving: eight warps move the keys and eight the values, tile by tile of 64 rows from the first that changes, the next codes on
+// their way while a tile is worked on (what a tile overwrites no later one reads).  The rows of the values are innermost, so
+// a value tile is gathered out of whole pages in shared memory, each copied there once: a thread has the same four rows of
+// the tile in HD / 16 channels, and a word of four codes comes out of the four words that hold them by three byte permutations.
 constexpr int kMoveThreads = 512, kMoveWarps = kMoveThreads / 32, kPlaneThreads = kMoveThreads / 2;
-constexpr int kVRow = 80;                  // bytes between channels of a staged value page: 16-byte pieces of 8 channels in 8 places
+constexpr int kStaged = 4;                 // value pages in shared memory: two that a tile is gathered from, two on their way
 template <int HD> struct Move {
     static constexpr int MINE = (4 * HD + kPlaneThreads - 1) / kPlaneThreads;    // 16-byte pieces of a page a thread has
-    static constexpr int V_BYTES = 2 * HD * kVRow;
+    static constexpr int V_PAGE = HD * kPageTokens;
+    static constexpr int V_BYTES = kStaged * V_PAGE;
 };
 
-__device__ __forceinline__ void plane_sync(int plane) { asm volatile("bar.sync %0, %1;\n" ::"r"(1 + plane), "n"(kPlaneThreads) : "memory"); }
+template <int PLANE> __device__ __forceinline__ void plane_sync() { asm volatile("bar.sync %0, %1;\n" ::"n"(1 + PLANE), "n"(kPlaneThreads) : "memory"); }
 
 // 16 codes times a power of two each word's pair shares: x[e] is codes 2 e, 2 e + 1, r[e] the factors (in half: clamped to what
 // half holds, beyond which codes are all zero, or all become zero).
@@ -276,23 +279,20 @@ __device__ __forceinline__ uint32_t pair_codes(__half2 x) {
     asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;\n" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&x)));
     return r;
 }
-// The largest |code| of a word that is not NaN, as a float.
-__device__ __forceinline__ float largest_code(uint32_t w) {
-    w &= 0x7f7f7f7fu;
-    w &= ~__vcmpeq4(w, 0x7f7f7f7fu);
-    const uint32_t a = __vmaxu4(w, w >> 16);
-    return e4m3_value((uint8_t)max(a & 0xffu, (a >> 8) & 0xffu));
-}
+// Each byte's |code| + 1, or 0 for NaN: the even bytes of a word and the odd ones, as 16-bit numbers that maxima are taken of.
+__device__ __forceinline__ uint32_t even_sizes(uint32_t w) { return ((w & 0x007f007fu) + 0x00010001u) & 0x007f007fu; }
+__device__ __forceinline__ uint32_t odd_sizes(uint32_t w) { return even_sizes(w >> 8); }
+__device__ __forceinline__ float size_value(uint32_t size) { return e4m3_value((uint8_t)(max(size, 1u) - 1u)); }
 
 template <int HD>
-__global__ void __launch_bounds__(kMoveThreads)
+__global__ void __launch_bounds__(kMoveThreads, 2)
 kv_evict_move_kernel(const E4M3Pages pages, const EvictStrides strides, int* __restrict__ dropped, const int* __restrict__ slots,
                      const int* __restrict__ lengths, int max_length, int budget, int recent, int* __restrict__ kept_out) {
     using M = Move<HD>;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int histogram[256];
     __shared__ int greater[kMoveWarps], equal[kMoveWarps];
-    __shared__ float warp_most[kMoveWarps];
+    __shared__ float warp_most[2 * kMoveWarps];
     __shared__ int choice[2], first_gone;
     const int h = blockIdx.x, b = blockIdx.y, entry = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int length = lengths[b], slot = slots[b];
@@ -303,7 +303,7 @@ kv_evict_move_kernel(const E4M3Pages pages, const EvictStrides strides, int* __r
     }
     if (h == 0 && entry == 0 && tid == 0 && dropped) dropped[slot] += length - budget;
     const int max_pages = (max_length + kPageTokens - 1) / kPageTokens, n_pages = (length + kPageTokens - 1) / kPageTokens;
-    unsigned char* staged = smem;                                               // two value pages
+    unsigned char* staged = smem;                                               // value pages
     float* w = reinterpret_cast<float*>(smem + M::V_BYTES);                     // [max_pages * 64]
     int* kept = reinterpret_cast<int*>(w + max_pages * kPageTokens);            // [budget rounded up to 64]
     int* page_id = kept + (budget + 63) / 64 * 64;                              // [max_pages]
@@ -410,136 +410,158 @@ kv_evict_move_kernel(const E4M3Pages pages, const EvictStrides strides, int* __r
     // ---- tiles to the front
     const int plane = tid / kPlaneThreads, t = tid % kPlaneThreads;
     const float* old_scale = page_scale + plane * max_pages;
-    uint4 ahead[2][M::MINE];
+    uint4 ahead[M::MINE];                                                       // of the next key tile
     auto rows_of = [&](int to) { return min(kPageTokens, budget - to * kPageTokens); };
-    // keys: the tile's rows; values: two pages from source page `p` on
-    auto fetch = [&](int to, int p) {
-#pragma unroll
-        for (int m = 0; m < M::MINE; ++m) {
-            const int id = t + kPlaneThreads * m;
-            if (plane == 0) {
-                const int r = id / (HD / 16);
-                if (r < rows_of(to)) {
-                    const int src = kept[to * kPageTokens + r];
-                    ahead[0][m] = *reinterpret_cast<const uint4*>(kc + (size_t)page_id[src / kPageTokens] * pages.k_stride + src % kPageTokens * HD + id % (HD / 16) * 16);
-                }
-            } else if (id < 4 * HD) {
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    if (p + x < n_pages) ahead[x][m] = *reinterpret_cast<const uint4*>(vc + (size_t)page_id[p + x] * pages.v_stride + id * 16);
-            }
-        }
-    };
-    auto first_page = [&](int to) { return kept[to * kPageTokens] / kPageTokens; };
-    auto block_most = [&](float most) {
+    // the largest of a tile's values, in all threads of a plane; tiles take turns with two places
+    auto block_most = [&](float most, int to, auto sync) {
         most = warp_max(most);
-        if (lane == 0) warp_most[warp] = most;
-        plane_sync(plane);
+        float* at = warp_most + (to & 1) * kMoveWarps + plane * (kMoveWarps / 2);
+        if (lane == 0) at[warp % (kMoveWarps / 2)] = most;
+        sync();
         most = 0.f;
 #pragma unroll
-        for (int x = 0; x < kMoveWarps / 2; ++x) most = fmaxf(most, warp_most[plane * (kMoveWarps / 2) + x]);
+        for (int x = 0; x < kMoveWarps / 2; ++x) most = fmaxf(most, at[x]);
         return most;
     };
-    if (first_tile < tiles) fetch(first_tile, first_page(first_tile));
-    for (int to = first_tile; to < tiles; ++to) {
-        const int rows = rows_of(to);
-        const int* source = kept + to * kPageTokens;
-        uint4 mine[M::MINE];
-        float most = 0.f;
-        if (plane == 0) {
+    if (plane == 0) {
+        auto fetch = [&](int to) {
+#pragma unroll
+            for (int m = 0; m < M::MINE; ++m) {
+                const int id = t + kPlaneThreads * m, r = id / (HD / 16);
+                if (r < rows_of(to)) {
+                    const int src = kept[to * kPageTokens + r];
+                    ahead[m] = *reinterpret_cast<const uint4*>(kc + (size_t)page_id[src / kPageTokens] * pages.k_stride + src % kPageTokens * HD + id % (HD / 16) * 16);
+                }
+            }
+        };
+        if (first_tile < tiles) fetch(first_tile);
+        for (int to = first_tile; to < tiles; ++to) {
+            const int rows = rows_of(to);
+            const int* source = kept + to * kPageTokens;
+            uint4 mine[M::MINE];
+            float was[M::MINE], most = 0.f;
 #pragma unroll
             for (int m = 0; m < M::MINE; ++m) {
                 const int r = (t + kPlaneThreads * m) / (HD / 16);
-                mine[m] = ahead[0][m];
+                mine[m] = ahead[m];
                 if (r < rows) {
-                    const float c = fmaxf(fmaxf(largest_code(mine[m].x), largest_code(mine[m].y)), fmaxf(largest_code(mine[m].z), largest_code(mine[m].w)));
-                    most = fmaxf(most, c * old_scale[source[r] / kPageTokens]);
+                    was[m] = old_scale[source[r] / kPageTokens];
+                    const uint32_t even = __vmaxu2(__vmaxu2(even_sizes(mine[m].x), even_sizes(mine[m].y)), __vmaxu2(even_sizes(mine[m].z), even_sizes(mine[m].w)));
+                    const uint32_t odd = __vmaxu2(__vmaxu2(odd_sizes(mine[m].x), odd_sizes(mine[m].y)), __vmaxu2(odd_sizes(mine[m].z), odd_sizes(mine[m].w)));
+                    const uint32_t both = __vmaxu2(even, odd);
+                    most = fmaxf(most, size_value(max(both & 0xffffu, both >> 16)) * was[m]);
                 }
             }
-        } else {
-            const int last = source[rows - 1] / kPageTokens;
-            int p = source[0] / kPageTokens;
+            const float scale = e4m3_needed_scale(block_most(most, to, plane_sync<0>)), inverse = pow2_inverse(scale);
+            if (to + 1 < tiles) fetch(to + 1);
+            uint8_t* at = kc + (size_t)page_id[to] * pages.k_stride;
 #pragma unroll
-            for (int m = 0; m < M::MINE; ++m) mine[m] = make_uint4(0, 0, 0, 0);
-            for (;; p += 2) {
-                plane_sync(plane);                                              // the pages before have been read
-#pragma unroll
-                for (int m = 0; m < M::MINE; ++m) {
-                    const int id = t + kPlaneThreads * m;
-                    if (id < 4 * HD) {
-                        *reinterpret_cast<uint4*>(staged + id / 4 * kVRow + id % 4 * 16) = ahead[0][m];
-                        *reinterpret_cast<uint4*>(staged + (HD + id / 4) * kVRow + id % 4 * 16) = ahead[1][m];
-                    }
-                }
-                plane_sync(plane);
-                if (p + 2 <= last) fetch(to, p + 2);
-#pragma unroll
-                for (int m = 0; m < M::MINE; ++m) {
-                    const int id = t + kPlaneThreads * m;                       // channel id / 4, rows 16 (id % 4) ..
-                    if (id >= 4 * HD) continue;
-                    uint32_t word[4] = {mine[m].x, mine[m].y, mine[m].z, mine[m].w};
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int r = id % 4 * 16 + e;
-                        if (r >= rows) continue;
-                        const int src = source[r], x = src / kPageTokens - p;
-                        if (x < 0 || x > 1) continue;
-                        const uint32_t c = staged[(x * HD + id / 4) * kVRow + src % kPageTokens];
-                        word[e >> 2] |= c << (8 * (e & 3));
-                        const uint32_t size = c & 0x7fu;
-                        most = fmaxf(most, e4m3_value((uint8_t)(size == 0x7fu ? 0u : size)) * old_scale[p + x]);
-                    }
-                    mine[m] = make_uint4(word[0], word[1], word[2], word[3]);
-                }
-                if (p + 2 > last) break;
-            }
-        }
-        const float scale = e4m3_needed_scale(block_most(most)), inverse = pow2_inverse(scale);
-        if (to + 1 < tiles) fetch(to + 1, first_page(to + 1));
-        const size_t page = page_id[to];
-#pragma unroll
-        for (int m = 0; m < M::MINE; ++m) {
-            const int id = t + kPlaneThreads * m;
-            uint32_t word[4] = {mine[m].x, mine[m].y, mine[m].z, mine[m].w};
-            if (plane == 0) {
-                const int r = id / (HD / 16);
-                if (r >= rows) continue;
-                const float ratio = old_scale[source[r] / kPageTokens] * inverse;
+            for (int m = 0; m < M::MINE; ++m) {
+                const int id = t + kPlaneThreads * m;
+                if (id / (HD / 16) >= rows) continue;
+                uint32_t word[4] = {mine[m].x, mine[m].y, mine[m].z, mine[m].w};
+                const float ratio = was[m] * inverse;
                 if (ratio != 1.f) {
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
                         word[x] = pair_codes(times_ratio(word[x], ratio, ratio)) | pair_codes(times_ratio(word[x] >> 16, ratio, ratio)) << 16;
                 }
-                *reinterpret_cast<uint4*>(kc + page * pages.k_stride + r * HD + id % (HD / 16) * 16) = make_uint4(word[0], word[1], word[2], word[3]);
-            } else if (id < 4 * HD) {
-                const int r0 = id % 4 * 16;
-                if (r0 >= rows) continue;
-                const float first = old_scale[source[r0] / kPageTokens] * inverse, last = old_scale[source[min(r0 + 15, rows - 1)] / kPageTokens] * inverse;
-                // (a piece whose rows come from two pages or fewer has the scales of its first and last row)
-                const bool two = source[min(r0 + 15, rows - 1)] / kPageTokens - source[r0] / kPageTokens <= 1;
-                if (!(two && first == 1.f && last == 1.f)) {
+                *reinterpret_cast<uint4*>(at + id * 16) = make_uint4(word[0], word[1], word[2], word[3]);
+            }
+            if (t == 0) scales[(size_t)page_id[to] * pages.scale_stride] = scale;
+        }
+        return;
+    }
+    if (first_tile >= tiles) return;
+    constexpr int CHANNELS = HD / 16;                                           // of a thread: t / 16 + 16 i
+    const int r0 = t % 16 * 4;                                                  // its rows of a tile: r0 .. r0 + 3
+    const int last_page = kept[budget - 1] / kPageTokens;
+    int issued = kept[first_tile * kPageTokens] / kPageTokens, there = issued;  // pages below: on their way; there for all threads
+    auto issue = [&]() {
+        const uint8_t* from = vc + (size_t)page_id[issued] * pages.v_stride;
+        const uint32_t to = smem_u32(staged) + issued % kStaged * M::V_PAGE;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        float f[4];
+        for (int m = 0; m < M::MINE; ++m) {
+            const int id = t + kPlaneThreads * m;
+            if (id < 4 * HD) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to + id * 16), "l"(from + id * 16));
+        }
+        cp_async_commit();
+        ++issued;
+    };
+    for (int to = first_tile; to < tiles; ++to) {
+        const int rows = rows_of(to);
+        int src[4];
+        float was[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) f[e] = old_scale[source[min(r0 + 4 * x + e, rows - 1)] / kPageTokens] * inverse;
-                        word[x] = pair_codes(times_ratio(word[x], f[0], f[1])) | pair_codes(times_ratio(word[x] >> 16, f[2], f[3])) << 16;
-                    }
+        for (int e = 0; e < 4; ++e) {
+            src[e] = r0 + e < rows ? kept[to * kPageTokens + r0 + e] : -1;
+            was[e] = old_scale[max(src[e], 0) / kPageTokens];
+        }
+        uint32_t word[CHANNELS] = {}, even = 0, odd = 0;
+        const int page_end = kept[to * kPageTokens + rows - 1] / kPageTokens;
+        for (int p = kept[to * kPageTokens] / kPageTokens; p <= page_end; p += 2) {
+            // pages p and p + 1.  Those before have been read by all when a barrier has passed since: this one, or the last
+            // tile's; so pages up to p + 3 may take their places.
+            const int need = min(p + 1, page_end);
+            if (need >= there) {
+                if (issued < p) {                                               // pages between of which no row stays
+                    cp_async_wait<0>();                                         // (a copy under way could land on one's that takes its place)
+                    issued = p;
                 }
-                uint8_t* at = vc + page * pages.v_stride + id / 4 * kPageTokens + r0;
-                if (r0 + 16 <= rows) *reinterpret_cast<uint4*>(at) = make_uint4(word[0], word[1], word[2], word[3]);
-                else
-                    for (int e = 0; r0 + e < rows; ++e) at[e] = (uint8_t)(word[e >> 2] >> (8 * (e & 3)));
+                while (issued <= need) issue();
+                if (issued - 1 - need >= 2) cp_async_wait<2>();
+                else if (issued - 1 - need == 1) cp_async_wait<1>();
+                else cp_async_wait<0>();
+                plane_sync<1>();
+                there = need + 1;
+            }
+            while (issued <= min(p + 3, last_page)) issue();
+            uint32_t offset[4], mask = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int x = src[e] / kPageTokens;
+                const bool here = src[e] >= 0 && x >= p && x <= p + 1;
+                offset[e] = here ? x % kStaged * M::V_PAGE + src[e] % kPageTokens / 4 * 4 : 0;
+                mask |= here ? 0xffu << (8 * e) : 0u;
+            }
+            const uint32_t low = (src[0] & 3) | (4 + (src[1] & 3)) << 4, high = (src[2] & 3) | (4 + (src[3] & 3)) << 4;
+#pragma unroll
+            for (int i = 0; i < CHANNELS; ++i) {
+                const unsigned char* at = staged + (t / 16 + 16 * i) * kPageTokens;
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = *reinterpret_cast<const uint32_t*>(at + offset[e]);
+                word[i] |= __byte_perm(__byte_perm(w[0], w[1], low), __byte_perm(w[2], w[3], high), 0x5410) & mask;
             }
         }
-        if (t == 0) scales[page * pages.scale_stride + plane * pages.n_kv] = scale;
-        plane_sync(plane);                                                      // warp_most and the staged pages are free again
+#pragma unroll
+        for (int i = 0; i < CHANNELS; ++i) {
+            even = __vmaxu2(even, even_sizes(word[i]));
+            odd = __vmaxu2(odd, odd_sizes(word[i]));
+        }
+        const float most = fmaxf(fmaxf(size_value(even & 0xffffu) * was[0], size_value(odd & 0xffffu) * was[1]),
+                                 fmaxf(size_value(even >> 16) * was[2], size_value(odd >> 16) * was[3]));
+        const float scale = e4m3_needed_scale(block_most(most, to, plane_sync<1>)), inverse = pow2_inverse(scale);
+        const bool same = was[0] == scale && was[1] == scale && was[2] == scale && was[3] == scale;
+        uint8_t* at = vc + (size_t)page_id[to] * pages.v_stride + r0;
+#pragma unroll
+        for (int i = 0; i < CHANNELS; ++i) {
+            if (!same)
+                word[i] = pair_codes(times_ratio(word[i], was[0] * inverse, was[1] * inverse)) |
+                          pair_codes(times_ratio(word[i] >> 16, was[2] * inverse, was[3] * inverse)) << 16;
+            uint8_t* row = at + (t / 16 + 16 * i) * kPageTokens;
+            if (r0 + 4 <= rows) *reinterpret_cast<uint32_t*>(row) = word[i];
+            else
+                for (int e = 0; r0 + e < rows; ++e) row[e] = (uint8_t)(word[i] >> (8 * e));
+        }
+        if (t == 0) scales[(size_t)page_id[to] * pages.scale_stride + pages.n_kv] = scale;
     }
+    cp_async_wait<0>();
 }
 
 size_t move_bytes(int hd, int max_length, int budget) {
     const size_t max_pages = (max_length + kPageTokens - 1) / kPageTokens;
-    return 2 * (size_t)hd * kVRow + max_pages * kPageTokens * 4 + (size_t)(budget + 63) / 64 * 64 * 4 + max_pages * 12;
+    return kStaged * (size_t)hd * kPageTokens + max_pages * kPageTokens * 4 + (size_t)(budget + 63) / 64 * 64 * 4 + max_pages * 12;
 }
 template <int HD>
 int launch_move(const E4M3Pages& pages, const EvictStrides& strides, int* dropped, const int* slots, const int* lengths, int max_length, int budget,
