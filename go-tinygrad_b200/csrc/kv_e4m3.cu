@@ -253,11 +253,14 @@ kv_evict_kernel(const E4M3Pages pages, const EvictStrides strides, int* __restri
 // ---- the same for heads of a multiple of 16 channels, with the sequence's weights, pages and scales in shared memory.
 // Choosing: the weights are read once; the need-th largest is found eight bits a pass (equal digits of a warp counted by one
 // lane, the digit found by one warp), then every warp places a stretch of the rows by itself, after one exchange of counts.
-// Moving: eight warps move the keys and eight the values, tile by tile of 64 rows from the first that changes, the next codes on
+// Moving: four warps move the keys and four the values, tile by tile of 64 rows from the first that changes, the next codes on
 // their way while a tile is worked on (what a tile overwrites no later one reads).  The rows of the values are innermost, so
 // a value tile is gathered out of whole pages in shared memory, each copied there once: a thread has the same four rows of
-// the tile in HD / 16 channels, and a word of four codes comes out of the four words that hold them by three byte permutations.
-constexpr int kMoveThreads = 512, kMoveWarps = kMoveThreads / 32, kPlaneThreads = kMoveThreads / 2;
+// the tile in several channels, and a word of four codes comes out of the four words that hold them by three byte permutations.
+// What bounds it is instructions: 24 entries x 3 sequences of 2,000 rows x 32 heads of 64 take 337 us on a B200, their 875 MB
+// would take 136.  Eight warps, each with twice the channels that sixteen have, because much of a tile's work is the same for
+// all its channels (sixteen: 440 us; eight cost 2 us of 17 where there are fewer blocks than multiprocessors).
+constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32, kPlaneThreads = kMoveThreads / 2;
 constexpr int kStaged = 4;                 // value pages in shared memory: two that a tile is gathered from, two on their way
 template <int HD> struct Move {
     static constexpr int MINE = (4 * HD + kPlaneThreads - 1) / kPlaneThreads;    // 16-byte pieces of a page a thread has
@@ -285,7 +288,7 @@ __device__ __forceinline__ uint32_t odd_sizes(uint32_t w) { return even_sizes(w 
 __device__ __forceinline__ float size_value(uint32_t size) { return e4m3_value((uint8_t)(max(size, 1u) - 1u)); }
 
 template <int HD>
-__global__ void __launch_bounds__(kMoveThreads, 2)
+__global__ void __launch_bounds__(kMoveThreads, 1024 / kMoveThreads)
 kv_evict_move_kernel(const E4M3Pages pages, const EvictStrides strides, int* __restrict__ dropped, const int* __restrict__ slots,
                      const int* __restrict__ lengths, int max_length, int budget, int recent, int* __restrict__ kept_out) {
     using M = Move<HD>;
@@ -473,7 +476,7 @@ kv_evict_move_kernel(const E4M3Pages pages, const EvictStrides strides, int* __r
         return;
     }
     if (first_tile >= tiles) return;
-    constexpr int CHANNELS = HD / 16;                                           // of a thread: t / 16 + 16 i
+    constexpr int APART = kPlaneThreads / 16, CHANNELS = HD / APART;            // channels of a thread: t / 16 + APART i
     const int r0 = t % 16 * 4;                                                  // its rows of a tile: r0 .. r0 + 3
     const int last_page = kept[budget - 1] / kPageTokens;
     int issued = kept[first_tile * kPageTokens] / kPageTokens, there = issued;  // pages below: on their way; there for all threads
@@ -527,7 +530,7 @@ kv_evict_move_kernel(const E4M3Pages pages, const EvictStrides strides, int* __r
             const uint32_t low = (src[0] & 3) | (4 + (src[1] & 3)) << 4, high = (src[2] & 3) | (4 + (src[3] & 3)) << 4;
 #pragma unroll
             for (int i = 0; i < CHANNELS; ++i) {
-                const unsigned char* at = staged + (t / 16 + 16 * i) * kPageTokens;
+                const unsigned char* at = staged + (t / 16 + APART * i) * kPageTokens;
                 uint32_t w[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[e] = *reinterpret_cast<const uint32_t*>(at + offset[e]);
@@ -549,7 +552,7 @@ kv_evict_move_kernel(const E4M3Pages pages, const EvictStrides strides, int* __r
             if (!same)
                 word[i] = pair_codes(times_ratio(word[i], was[0] * inverse, was[1] * inverse)) |
                           pair_codes(times_ratio(word[i] >> 16, was[2] * inverse, was[3] * inverse)) << 16;
-            uint8_t* row = at + (t / 16 + 16 * i) * kPageTokens;
+            uint8_t* row = at + (t / 16 + APART * i) * kPageTokens;
             if (r0 + 4 <= rows) *reinterpret_cast<uint32_t*>(row) = word[i];
             else
                 for (int e = 0; r0 + e < rows; ++e) row[e] = (uint8_t)(word[i] >> (8 * e));
