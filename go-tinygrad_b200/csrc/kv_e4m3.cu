@@ -585,6 +585,9 @@ int launch_move(const E4M3Pages& pages, const EvictStrides& strides, int* droppe
 // 16 channels a thread (two runs of 8 that the rotation pairs), kept in registers while the block's largest value is
 // found, and written in pieces of 16 or 8 bytes; values go through shared memory, since their rows are innermost in the cache.
 // Query rows are rotated by blocks of their own, the angles of 16 channels read once for several heads.
+// What bounds it: its reads wait for memory, in 32 warps a multiprocessor (four blocks: 26.6 us where three take 29.6 and five 28.3, the
+// prompts named below; their bytes take 16.8), and turning and rounding take half of all issue slots, so codes are made two at
+// a time and only a thread that has met a number that is not finite looks at each.
 constexpr int kRowsThreads = 256;
 
 __device__ __forceinline__ void load8(const bf16* p, float* x) {
@@ -638,7 +641,14 @@ __device__ __forceinline__ void turn_unit(int u, int rot, int interleaved, const
         for (int e = 0; e < 8; ++e) turn(x[e], x[8 + e], t[e]);
     }
 }
-__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+// Four codes; odd: of numbers that may not be finite.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, bool odd) {
+    if (!odd) {
+        unsigned short lo, hi;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(lo) : "f"(b), "f"(a));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(hi) : "f"(d), "f"(c));
+        return lo | (uint32_t)hi << 16;
+    }
     return e4m3_code(a) | (uint32_t)e4m3_code(b) << 8 | (uint32_t)e4m3_code(c) << 16 | (uint32_t)e4m3_code(d) << 24;
 }
 // A word's bytes below `n` times a power of two; the others as they are.
@@ -650,7 +660,7 @@ __device__ __forceinline__ uint32_t rescaled_bytes(uint32_t w, int n, float rati
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kRowsThreads)
+__global__ void __launch_bounds__(kRowsThreads, 4)
 kv_store_rows_kernel(const StoreInput<T> in, const E4M3Pages kv, const int* __restrict__ cu_seqlens, const int* __restrict__ slots,
                      const int* __restrict__ start_pos, int blocks_per_seq, int blocks_kv, int N, int heads_each, T* __restrict__ q_out, int ldq) {
     constexpr int UNITS = HD / 16;                                              // of a row
@@ -700,7 +710,6 @@ kv_store_rows_kernel(const StoreInput<T> in, const E4M3Pages kv, const int* __re
     const int token0 = first + block * kPageTokens - start;                     // of row 0
     const T* column = in.qkv + (in.n_heads + h) * HD + (plane ? in.v_offset : 0);
     float x[K_MINE > 2 * V_MINE ? K_MINE : 2 * V_MINE][16];                     // keys: a unit each; values: rows 0, 1 and 2, 3 of a run
-    float most = 0.f;
     if (plane == 0) {
 #pragma unroll
         for (int m = 0; m < K_MINE; ++m) {
@@ -731,12 +740,25 @@ kv_store_rows_kernel(const StoreInput<T> in, const E4M3Pages kv, const int* __re
             }
         }
     }
+    constexpr int MINE = K_MINE > 2 * V_MINE ? K_MINE : 2 * V_MINE;
+    uint32_t top = 0;                                                           // the largest magnitude's bits: from 0x7f800000 on not finite
 #pragma unroll
-    for (int m = 0; m < (K_MINE > 2 * V_MINE ? K_MINE : 2 * V_MINE); ++m)
+    for (int m = 0; m < MINE; ++m)
         if (m < (plane ? 2 * V_MINE : K_MINE)) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) most = fmaxf(most, finite_f32(x[m][e]) ? fabsf(x[m][e]) : 0.f);
+            for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[m][e]) & 0x7fffffffu);
         }
+    const bool odd = top >= 0x7f800000u;
+    float most = __uint_as_float(top);
+    if (odd) {
+        most = 0.f;
+#pragma unroll
+        for (int m = 0; m < MINE; ++m)
+            if (m < (plane ? 2 * V_MINE : K_MINE)) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) most = fmaxf(most, finite_f32(x[m][e]) ? fabsf(x[m][e]) : 0.f);
+            }
+    }
     most = warp_max(most);
     if ((tid & 31) == 0) warp_most[tid >> 5] = most;
     float* scale_at = kv.scales + page * kv.scale_stride + plane * kv.n_kv + h;
@@ -780,8 +802,8 @@ kv_store_rows_kernel(const StoreInput<T> in, const E4M3Pages kv, const int* __re
             runs_of(u, in.rot, in.interleaved, &a, &c);
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[m][e] *= inverse;
-            *reinterpret_cast<uint2*>(codes + r * HD + a) = make_uint2(codes4(x[m][0], x[m][1], x[m][2], x[m][3]), codes4(x[m][4], x[m][5], x[m][6], x[m][7]));
-            *reinterpret_cast<uint2*>(codes + r * HD + c) = make_uint2(codes4(x[m][8], x[m][9], x[m][10], x[m][11]), codes4(x[m][12], x[m][13], x[m][14], x[m][15]));
+            *reinterpret_cast<uint2*>(codes + r * HD + a) = make_uint2(codes4(x[m][0], x[m][1], x[m][2], x[m][3], odd), codes4(x[m][4], x[m][5], x[m][6], x[m][7], odd));
+            *reinterpret_cast<uint2*>(codes + r * HD + c) = make_uint2(codes4(x[m][8], x[m][9], x[m][10], x[m][11], odd), codes4(x[m][12], x[m][13], x[m][14], x[m][15], odd));
         }
         if (kv.weights)
             for (int r = lo + tid; r < hi; r += kRowsThreads) kv.weights[page * kv.weight_stride + h * kPageTokens + r] = 0.f;
@@ -792,7 +814,7 @@ kv_store_rows_kernel(const StoreInput<T> in, const E4M3Pages kv, const int* __re
             if (r4 >= 16) continue;
 #pragma unroll
             for (int e = 0; e < 8; ++e)                                         // (the place is turned so that lanes of a run fall into different banks)
-                turned[(8 * run + e) * 16 + (r4 ^ (run & 15))] = codes4(x[2 * m][e] * inverse, x[2 * m][8 + e] * inverse, x[2 * m + 1][e] * inverse, x[2 * m + 1][8 + e] * inverse);
+                turned[(8 * run + e) * 16 + (r4 ^ (run & 15))] = codes4(x[2 * m][e] * inverse, x[2 * m][8 + e] * inverse, x[2 * m + 1][e] * inverse, x[2 * m + 1][8 + e] * inverse, odd);
         }
         __syncthreads();
         for (int i = tid; i < 4 * HD; i += kRowsThreads) {
@@ -823,7 +845,7 @@ bool rows_take(const StoreInput<T>& in, const void* q_out, int ldq) {
 template <typename T, int HD>
 int launch_store_rows(const StoreInput<T>& in, const E4M3Pages& kv, const int* cu_seqlens, const int* slots, const int* start_pos, int per_seq,
                       long long blocks_kv, int N, void* q_out, int ldq, cudaStream_t stream) {
-    // heads a thread turns with the same angles: four (31.5 us at 4,696 tokens of 32 + 16 heads of 128; one: 33.9, eight: 32.9)
+    // heads a thread turns with the same angles: four (26.6 us at 4,696 tokens of 32 + 16 heads of 128; one: 27.9, eight: 26.6)
     // once that leaves a thousand threads a multiprocessor
     const int heads_each = (long long)N * (HD / 16) * in.n_heads >= 4LL * 148 * 1024 ? 4 : 1;
     const long long threads = q_out ? (long long)N * ((in.n_heads + heads_each - 1) / heads_each) * (HD / 16) : 0;

@@ -8,6 +8,7 @@ is no other route for the same work (no library attention, no CPU path).
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 from ctypes import c_double, c_float, c_int, c_longlong, c_ulonglong, c_void_p
 from dataclasses import dataclass
@@ -1774,15 +1775,22 @@ def _e4m3_prompt_scratch(n_seqs: int, n_tokens: int, n_heads: int, kv, max_kv_le
     return n_heads * (2 * n_tokens + n_seqs * ((max_kv_len + 127) // 128 * 128))
 
 
+@functools.lru_cache(maxsize=1024)
+def _e4m3_few_scratch(device: int, dt: int, n_seqs: int, n_tokens: int, max_q_len: int, n_heads: int, n_kv: int, hd: int, max_kv_len: int,
+                      total_kv_len: int, window: int, weigh: int) -> int:
+    """Floats for these sizes on the current device, number `device` (-1: none): a call of the library that says so is not made twice."""
+    return int(_fn("gtg_attention_e4m3_scratch_floats")(dt, n_seqs, n_tokens, max_q_len, n_heads, n_kv, hd, max_kv_len, total_kv_len, window, weigh))
+
+
 def attention_e4m3_scratch_floats(dtype: torch.dtype, n_seqs: int, n_tokens: int, max_q_len: int, n_heads: int, kv, max_kv_len: int,
                                   total_kv_len: int = 0, window: Optional[int] = None) -> int:
     """Floats of scratch `attention_e4m3` needs for the same arguments (0: none)."""
     window = kv.window if window is None else window
     if _e4m3_prompt_form(0 if dtype == torch.float32 else 1, max_q_len, n_heads, kv.n_kv_heads, kv.head_dim):
         return _e4m3_prompt_scratch(n_seqs, n_tokens, n_heads, kv, int(max_kv_len))
-    return int(_fn("gtg_attention_e4m3_scratch_floats")(0 if dtype == torch.float32 else 1, n_seqs, n_tokens, int(max_q_len), n_heads, kv.n_kv_heads,
-                                                        kv.head_dim, int(max_kv_len), int(total_kv_len), int(window or 0),
-                                                        1 if kv.weights is not None else 0))
+    device = kv.k.device.index
+    return _e4m3_few_scratch(-1 if device is None else device, 0 if dtype == torch.float32 else 1, n_seqs, n_tokens, int(max_q_len), n_heads,
+                             kv.n_kv_heads, kv.head_dim, int(max_kv_len), int(total_kv_len), int(window or 0), 1 if kv.weights is not None else 0)
 
 
 def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Tensor, slots: torch.Tensor, start_pos: torch.Tensor, max_q_len: int,
@@ -1817,8 +1825,8 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
     if prompt:
         need = _e4m3_prompt_scratch(B, N, n_heads, kv, int(max_kv_len))
     else:
-        need = int(_fn("gtg_attention_e4m3_scratch_floats")(dt, B, N, int(max_q_len), n_heads, kv.n_kv_heads, hd, int(max_kv_len), int(total_kv_len),
-                                                            int(window or 0), 1 if kv.weights is not None else 0))
+        need = _e4m3_few_scratch(q.device.index, dt, B, N, int(max_q_len), n_heads, kv.n_kv_heads, hd, int(max_kv_len), int(total_kv_len),
+                                 int(window or 0), 1 if kv.weights is not None else 0)
     if need:
         if scratch is None:
             scratch = torch.empty(need, dtype=torch.float32, device=q.device)
