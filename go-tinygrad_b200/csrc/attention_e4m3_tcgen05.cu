@@ -1,23 +1,26 @@
 // Attention of prompts and chunks over the 8-bit cache on the fifth-generation tensor cores: heads of 64 or 128 channels,
 // bfloat16 queries, causal, with an optional window.  (Layout and codes: e4m3.cuh.)
 //
-// One block per (128 query rows, key/value head, sequence).  A query row is a (token, head of the group) pair, heads
+// One block per (two tiles of 128 query rows, key/value head, sequence).  A query row is a (token, head of the group) pair, heads
 // innermost, so that the heads that share keys share their pages too and a short run of queries still fills a tile.  Per page:
-//   codes -> half   four warps fetch the page's codes (asynchronous copies, two or four pages ahead), turn them into halves,
-//                   which is exact, and leave them in shared memory as swizzled tiles: keys [row][channel], values
-//                   [channel][row], both K-major as the cache has them;
+//   codes -> half   four warps read the page's codes, a page ahead, turn them into halves, which is exact, and leave them in
+//                   shared memory as swizzled tiles: keys [row][channel], values [channel][row], both K-major as the cache has them;
 //   S  = Q K^T      tcgen05.mma 128 x 64 x head size, operands in shared memory, S in tensor memory; queries are scaled by a
 //                   power of two a row to fill half's range, so that rounding bfloat16 to half loses nothing that counts;
-//   P  = softmax    eight warps, two threads a row, scores straight from tensor memory; P goes back there as halves;
+//   P  = softmax    four warps a tile, a thread a row, scores straight from tensor memory; P goes back there as halves;
 //   O += P V        tcgen05.mma 128 x head size x 64, A = P from tensor memory, O stays there.
 // Scales.  A page's key scale multiplies its scores.  Its value scale 2^v cannot multiply O, which adds up over pages, and
 // must not squeeze P's range either: it goes into the exponent.  With x_j = score_j + v_j (in powers of two) and M the running
-// maximum of x, P_j = 2^(x_j - M), O = sum P_j code_j and the sum is l = sum P_j 2^(-v_j): O / l is the result, whatever the
-// scales (as long as two blocks of values that both count are not 2^100 apart).  M is raised only when a step's maximum exceeds it
-// by 2^8; P, times 2^7 besides, then stays below half's largest number.
-// What bounds it is the softmax's latency: a tile's page takes its warps longer than its products (512 cycles for 128 channels).
-// With four warps, a thread a row, it was 2,400 cycles alone and 3,000 with a second block beside it.  Every wait is bounded
-// (status word as in the products).
+// maximum of x, P_j = 2^(x_j - M) and O = sum P_j code_j.  The sum is l = sum P_j 2^(w - v_j) = sum 2^(score_j - M + w), w the
+// largest v of the block's pages, and O 2^w / l the result.  Where v_j is so far below w that P_j could be 0 while its probability is
+// not (a block of zeros among others, for one), v_j counts as w - 96 and the codes are made smaller for it.
+// M is raised only when a step's sum of P exceeds 2^15, so P, times 2^7 besides, stays below half's largest number.
+// What bounds it is the softmax: its exponentials alone are 1,024 cycles of the 2,500 that a step of both tiles takes, its wait for
+// scores 400 to 540, their products 800.  Measured on a B200: 2,048 tokens, 32 heads of 64: 56 us; 512 tokens behind 7,680,
+// 2 sequences, 8 kv heads of 128 under 32: 165 us, 0.83 of what the same kernel for a bfloat16 cache takes in the second case and
+// 1.2 of it in the first, where the blocks' begins count.  Steps on the way there, in the second case: 128 rows a block, two threads
+// a row 257; issuing from warps of their own 180; codes straight to registers instead of through shared memory 177; two
+// threads a row again, with 24 warps, 195.  Every wait is bounded (status word as in the products).
 #include "e4m3.cuh"
 #include "tcgen05_attention.cuh"
 #include <type_traits>
@@ -33,6 +36,7 @@ constexpr int kThreads = 512;
 constexpr int kTmemCols = 512, kTileCols = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPShift = 7.0f, kMostSum = 32768.0f;
+constexpr int kMostApart = 96;                           // powers of two that a block's value scales span at most
 
 template <int HD> struct Shape {
     static constexpr int kQBytes = BQ * HD * 2, kTileBytes = BK * HD * 2;
@@ -101,6 +105,16 @@ __device__ __forceinline__ void store_halves(uint32_t row_at, int chunk, int swi
     const uint32_t first = row_at + (((chunk + turned) ^ swizzle) << 4), second = row_at + (((chunk + 1 - turned) ^ swizzle) << 4);
     store_shared16(first, turned ? b[0] : a[0], turned ? b[1] : a[1], turned ? b[2] : a[2], turned ? b[3] : a[3]);
     store_shared16(second, turned ? a[0] : b[0], turned ? a[1] : b[1], turned ? a[2] : b[2], turned ? a[3] : b[3]);
+}
+// Sixteen codes times a power of two below 1, rounded to codes.  (Next to a block 2^96 times larger, what is lost is little.)
+__device__ __forceinline__ uint32_t smaller_codes(uint32_t w, float ratio) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r |= (uint32_t)e4m3_code(e4m3_value((uint8_t)(w >> (8 * e))) * ratio) << (8 * e);
+    return r;
+}
+__device__ __noinline__ uint4 smaller_codes(uint4 u, float ratio) {
+    return make_uint4(smaller_codes(u.x, ratio), smaller_codes(u.y, ratio), smaller_codes(u.z, ratio), smaller_codes(u.w, ratio));
 }
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -218,6 +232,17 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     // (a wait's answer is the whole warp's before anything is issued: an elected lane waits for all)
     auto all_wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_sleep<kTest>(bar, parity, abort_flag)); };
 
+    // 2^(w - kMostApart), w the largest value scale's logarithm among the block's pages: smaller ones are raised to it.  (A warp's
+    // answer; the scales are powers of two from 2^-126 on.)
+    auto least_value_scale = [&]() {
+        uint32_t top = 0;
+#pragma unroll 4
+        for (int i = lane; i < steps_last; i += 32)
+            top = max(top, __float_as_uint(kv.scales[(size_t)table[j_lo + i] * kv.scale_stride + kv.n_kv + h]));
+        top = __reduce_max_sync(0xffffffffu, top);
+        return __uint_as_float(max(top, (uint32_t)(kMostApart + 1) << 23) - ((uint32_t)kMostApart << 23));
+    };
+
     // ---- codes to halves: two warps the keys, two the values
     auto convert = [&](auto of_values, const int t) {
         constexpr bool values = decltype(of_values)::value;
@@ -229,6 +254,8 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
         const uint8_t* source = (values ? kv.v : kv.k) + (size_t)h * kPageTokens * HD + t * 16;
         const long long stride = values ? kv.v_stride : kv.k_stride;
         uint4 u[mine];
+        const float v_least = values ? least_value_scale() : 0.f;
+        float v_scales = 1.f;                                    // lane l: of step (i / 32 * 32 + l)
         auto fetch = [&](int i) {
             if ((i & 31) == 0) pages = i + lane < steps_last ? table[j_lo + i + lane] : 0;
             const uint8_t* at = source + (size_t)__shfl_sync(0xffffffffu, pages, i & 31) * stride;
@@ -257,6 +284,14 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                     }
                     if (found && t + threads * m < S::kPieces) *odd_flag = 1;
                     u[m] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            if (values) {
+                if ((i & 31) == 0 && i + lane < steps_last) v_scales = kv.scales[(size_t)table[j + lane] * kv.scale_stride + kv.n_kv + h];
+                const float v_scale = __shfl_sync(0xffffffffu, v_scales, i & 31);
+                if (v_scale < v_least) {                         // counted as larger than they are: the codes make up for it
+#pragma unroll
+                    for (int m = 0; m < mine; ++m) u[m] = smaller_codes(u[m], v_scale * pow2_inverse(v_least));
                 }
             }
             if (i >= 2 && !all_wait(values ? v_free(i) : k_free(i), phase(i - 2))) break;
@@ -372,6 +407,8 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full(tt));
         }
+        const float v_least = least_value_scale();
+        const uint32_t top_bits = __float_as_uint(v_least) + ((uint32_t)(kMostApart + 127) << 23);             // 1 / s = top_bits - bits of s, times 2^w
         // scales, 32 steps at a time: lane l has those of step (i / 32 * 32 + l)
         float k_scales = 0.f, v_scales = 1.f;
         float m_run = -INFINITY, l_run = 0.f;
@@ -382,7 +419,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             if ((i & 31) == 0 && i + lane < n_steps) {
                 const float* at = kv.scales + (size_t)table[j_lo + i + lane] * kv.scale_stride + h;
                 k_scales = at[0];
-                v_scales = at[kv.n_kv];
+                v_scales = fmaxf(at[kv.n_kv], v_least);
             }
             // the step's scores; and the P of two steps ago has been read
             ok = i < 2 ? all_wait(s_full(tt), (uint32_t)i & 1u)
@@ -391,7 +428,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
             tmem_ld32(tile_at, sv);
             tmem_ld32(tile_at + 32, sv + 32);
-            const float sl = factor * __shfl_sync(full, k_scales, i & 31);
+            const float sl = fmaxf(factor * __shfl_sync(full, k_scales, i & 31), 1e-37f);       // (not 0, which would make NaN of masked scores)
             const float v_scale = __shfl_sync(full, v_scales, i & 31);
             const float add = (float)((int)(__float_as_uint(v_scale) >> 23) - 127);             // log2 of the value scale
             asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
@@ -462,7 +499,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                 }
                 exponentials();
             }
-            l_run = fmaf(first_of(sum) + second_of(sum), pow2_inverse(v_scale), l_run);
+            l_run = fmaf(first_of(sum) + second_of(sum), __uint_as_float(top_bits - __float_as_uint(v_scale)), l_run);
             tmem_st32(tile_at + S::kColP + 32 * (i & 1), pw);
             asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
@@ -472,8 +509,8 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
         if (ok) ok = all_wait(pv_done(tt, n_steps - 1), phase(n_steps - 1));
         if (ok) {
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
-            const float inv = 1.0f / l_run;
-            if (a.stats && real) a.stats[(size_t)(q_begin + token) * a.n_heads + head] = make_float2((m_run == -INFINITY ? 0.f : m_run) - kPShift, l_run);
+            const float inv = 1.0f / l_run, unit = __uint_as_float(__float_as_uint(v_least) + ((uint32_t)kMostApart << 23));    // 2^w
+            if (a.stats && real) a.stats[(size_t)(q_begin + token) * a.n_heads + head] = make_float2(m_run == -INFINITY ? 0.f : m_run - (float)((int)(__float_as_uint(unit) >> 23) - 127) - kPShift, l_run);
             bf16* dst = a.out + (size_t)(q_begin + token) * a.ldo + (size_t)head * HD;
             const bool odd = *odd_flag != 0;
 #pragma unroll 1
@@ -498,7 +535,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                         uint32_t o4[4];
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            const __nv_bfloat162 hh = __floats2bfloat162_rn(__uint_as_float(sv[8 * piece + 2 * x]) * inv, __uint_as_float(sv[8 * piece + 2 * x + 1]) * inv);
+                            const __nv_bfloat162 hh = __floats2bfloat162_rn(__uint_as_float(sv[8 * piece + 2 * x]) * inv * unit, __uint_as_float(sv[8 * piece + 2 * x + 1]) * inv * unit);
                             o4[x] = *reinterpret_cast<const uint32_t*>(&hh);
                         }
                         *reinterpret_cast<uint4*>(dst + 32 * c + 8 * piece) = make_uint4(o4[0], o4[1], o4[2], o4[3]);

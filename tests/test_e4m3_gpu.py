@@ -377,6 +377,39 @@ def test_scales_far_apart(dtype, hd, new):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128, 48])
+@pytest.mark.parametrize("new", [1, 70, 330])
+@pytest.mark.parametrize("small", [0.0, 2.0 ** -90])
+@pytest.mark.parametrize("order", [(0, 1, 1, 0, 1, 0), (1, 0, 0, 1, 0, 1)])
+def test_blocks_of_zeros_have_their_share_of_the_probability(dtype, hd, new, small, order):
+    """Blocks of values that are zero, or next to it, among others, with keys of their own or zero too: their scales are as small
+    as scales get, their probabilities are not.  Bound: attention_case's, each channel's sizes summed."""
+    n, heads = 64 * len(order), 2
+    p = Pages([n], 1, hd, seed=21, weights=True)
+    rng = np.random.default_rng(22)
+    k, v = p.rows[0][0]
+    k.codes, k.scales, v.codes, v.scales = np.zeros((0, hd)), [], np.zeros((0, hd)), []
+    keys = rng.standard_normal((n, hd))
+    keys[64:128] = 0.0
+    k.append(keys)
+    v.append(rng.standard_normal((n, hd)) * np.repeat([1.0 if x else small for x in order], 64)[:, None])
+    p.write(0)
+    q = torch.from_numpy(rng.standard_normal((new, heads * hd))).to(dtype).to(DEV)
+    out = torch.empty_like(q)
+    ops.attention_e4m3(q, out, p.view(), cut([new]), ints(p.slots), ints([n - new]), new, heads, hd ** -0.5, max_kv_len=n, total_kv_len=n)
+    qs = q.double().cpu().numpy().reshape(new, heads, hd)
+    want, gathered = plain.attend(qs, k.values(), v.values(), n - new, hd ** -0.5)
+    size, _ = plain.attend(qs, k.values(), np.abs(v.values()), n - new, hd ** -0.5)
+    rel = 2 * (hd + 4) * 2.0 ** -23 * (np.abs(qs).reshape(-1, hd) @ np.abs(k.values()).T).max() * hd ** -0.5 + 2.0 ** -21 + n * 2.0 ** -24
+    bound = size * (2 * rel + (2.0 ** -11 if dtype == BF16 else 0.0)) + np.abs(want) * HALF_STEP[dtype] * (1 + 2.0 ** -7) + 1e-30
+    got = out.double().cpu().numpy().reshape(want.shape)
+    assert (np.abs(got - want) <= bound).all(), (np.abs(got - want) / bound).max()
+    total = p.gathered[0][0] + gathered
+    bound = gathered * (2 * rel + new * heads * 2.0 ** -24) + total * 2.0 ** -23 + 1e-30
+    assert (np.abs(p.read_weights(0, 0, n) - total) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("new", [1, 40])
 def test_what_is_not_finite_stays_with_who_sees_it(dtype, new):
     """A NaN key spoils the queries that see its row, of its own head alone; NaN behind the window spoils nobody."""
