@@ -149,8 +149,9 @@ def _check_e4m3(k, v, scales, block_table, weights, dropped, lead: int) -> None:
             raise ValueError(f"the {name} of a page must start on a 16-byte boundary")
         if t is weights and (t.data_ptr() % 16 or any(st % 4 for st in t.stride()[:lead])):
             raise ValueError("the weights of a page must start on a 16-byte boundary")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.device != k.device:
-        raise ValueError("the block table must be int32 [slots, pages of a sequence] on the keys' device")
+    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 or block_table.stride(0) < block_table.shape[1]
+            or block_table.device != k.device):
+        raise ValueError("the block table must be int32 [slots, pages of a sequence], row by row, on the keys' device")
     if dropped is not None and (dropped.dtype != torch.int32 or not dropped.is_contiguous() or dropped.numel() != block_table.shape[0]
                                 or dropped.device != k.device):
         raise ValueError("dropped must be contiguous int32 [slots] on the keys' device")

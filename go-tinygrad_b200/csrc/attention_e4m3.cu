@@ -39,7 +39,7 @@ attention_rows_kernel(const T* __restrict__ q, int ldq, T* __restrict__ out, int
     const int* table = kv.block_table + (size_t)slot * kv.table_stride;
     const int row = start_pos[b] - (kv.dropped ? kv.dropped[slot] : 0) + token - cu_seqlens[b];
     const int first = window > 0 ? max(0, row - window + 1) : 0;
-    for (int d = tid; d < hd; d += kRowThreads) qs[d] = to_f32(q[(size_t)token * ldq + head * hd + d]) * scale;
+    for (int d = tid; d < hd; d += kRowThreads) qs[d] = to_f32(q[(size_t)token * ldq + head * hd + d]) * kDown * scale;
     __syncthreads();
     float m = -INFINITY, l = 0.f;
     float o[kMaxChannels / 32];
@@ -69,7 +69,7 @@ attention_rows_kernel(const T* __restrict__ q, int ldq, T* __restrict__ out, int
                 for (int d = 0; d < hd; ++d) s = fmaf(qs[d], e4m3_value(kr[d]), s);
             }
         }
-        s = seen ? s * k_scale : -INFINITY;
+        s = seen ? s * k_scale * kUp : -INFINITY;
         const float m_new = fmaxf(m, warp_max(s));
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
         const float p = seen ? expf(s - m_use) : 0.f, corr = expf(m - m_use);
@@ -148,7 +148,7 @@ row_weights_kernel(const T* __restrict__ q, int ldq, const E4M3Pages kv, const i
         const uint8_t* kr = kv.k + page * kv.k_stride + (size_t)h * kPageTokens * hd;
         __syncthreads();
         for (int i = tid; i < kPageTokens * hd; i += kRowThreads) ks[i / hd * ld + i % hd] = e4m3_value(kr[i]);
-        const float k_scale = kv.scales[page * kv.scale_stride + h] * kLog2e;
+        const float k_scale = kv.scales[page * kv.scale_stride + h];
         const int row = block * kPageTokens + t;
         const int from = max(0, block * kPageTokens - start);                   // queries before that one see none of these rows
         const int pairs = (n_new - from) * group;
@@ -158,7 +158,7 @@ row_weights_kernel(const T* __restrict__ q, int ldq, const E4M3Pages kv, const i
             const int here = min(kAtOnce, pairs - p0);
             for (int i = tid; i < here * hd; i += kRowThreads) {
                 const int pair = p0 + i / hd;
-                qs[i] = to_f32(q[(size_t)(first + from + pair / group) * ldq + (h * group + pair % group) * hd + i % hd]) * scale;
+                qs[i] = to_f32(q[(size_t)(first + from + pair / group) * ldq + (h * group + pair % group) * hd + i % hd]) * kDown * scale;
             }
             if (tid < here) st[tid] = stats[(size_t)(first + from + (p0 + tid) / group) * n_heads + h * group + (p0 + tid) % group];
             __syncthreads();
@@ -167,7 +167,7 @@ row_weights_kernel(const T* __restrict__ q, int ldq, const E4M3Pages kv, const i
                 if (row > at || (window > 0 && row <= at - window)) continue;
                 float s = 0.f;
                 for (int d = 0; d < hd; ++d) s = fmaf(qs[i * hd + d], ks[t * ld + d], s);
-                sum += exp2f(fmaf(s, k_scale, -st[i].x)) / st[i].y;
+                sum += exp2f(min_or_nan(fmaf(s * k_scale, kUp * kLog2e, -st[i].x), 0.f)) / st[i].y;
             }
         }
         if (part) half_sum[t] = sum;

@@ -36,6 +36,9 @@
 
 namespace {
 constexpr float kLog2e = 1.4426950408889634f;
+// Where a query's channels are multiplied with codes in float: kept smaller, so that the products of the largest ones do not
+// leave float's range before the key scale is in.
+constexpr float kUp = 4294967296.0f, kDown = 1.0f / kUp;
 constexpr int kFewWarps = 2, kFewThreads = 32 * kFewWarps;
 constexpr int kFewColumns = 32;          // queries a key/value head that these kernels take
 constexpr int kStepRows = 32;            // cache rows a warp takes at a time: half a page
@@ -238,7 +241,7 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
         const int skip = max(from - kUnitCost, 0), n_mine = max(from + mine - kUnitCost, 0) - skip;
         if (n_mine == 0) continue;
         const int h = in_b / a.tiles, c0 = in_b % a.tiles * 4 * NT;
-        const int n_columns = span.n_new * a.group;
+        const int n_columns = min(span.n_new * a.group, a.columns);
         if (c0 >= n_columns) continue;                                          // a shorter run of queries than the longest
         const int p_begin = span.p_first + skip;
         const int* table = kv.block_table + (size_t)span.slot * kv.table_stride;
@@ -330,7 +333,7 @@ few_queries_kernel(const FewArgs a, const E4M3Pages kv) {
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
             // the largest channel comes to lie in [128, 256)
-            const int e = (int)(most >> 7), up = e == 0 ? 0 : min(max(7 - (e - 127), -100), 100);
+            const int e = (int)(most >> 7), up = e == 0 ? 0 : min(7 - (e - 127), 100);
             const float f = __uint_as_float((uint32_t)(127 + up) << 23);
             const float back = a.scale * kLog2e * __uint_as_float((uint32_t)(127 - up) << 23);
             factor[nt] = __shfl_sync(0xffffffffu, back, 8 * t4);
@@ -582,7 +585,7 @@ few_join_kernel(const FewArgs a, const E4M3Pages kv, int join_blocks) {
     const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
     const FewPlace place = few_place<false>(a, kv, kv.n_kv * a.tiles, b);       // (of what the kernel before this one only reads, too)
     const FewSeq span = place.seq;
-    const int per = place.per, n_columns = span.n_new * a.group, n_line = on_line(span.steps());
+    const int per = place.per, n_columns = min(span.n_new * a.group, a.columns), n_line = on_line(span.steps());
     chain_wait();
     if (n_columns <= 0) return;
     const size_t unit = (size_t)(b * kv.n_kv + h) * a.tiles;
@@ -678,8 +681,10 @@ few_join_kernel(const FewArgs a, const E4M3Pages kv, int join_blocks) {
         float sum = 0.f;
         if (p < a.score_pages) {
             const float* at = a.scores + (((size_t)b * kv.n_kv + h) * a.columns * a.score_pages + p) * kPageTokens + t / kStepRows * kStepRows + score_place(t % kStepRows);
-            for (int c = 0; c < n_columns; ++c)
-                sum += exp2_fast(at[(size_t)c * a.score_pages * kPageTokens] - top[c] + kPShift) * inverse[c];
+            for (int c = 0; c < n_columns; ++c) {
+                const float s = at[(size_t)c * a.score_pages * kPageTokens];
+                sum += s == -INFINITY ? 0.f : exp2_fast(s - top[c] + kPShift) * inverse[c];               // (not seen: not NaN either)
+            }
         } else {                                                                // a sequence that has outgrown the plan: score the row again
             const uint8_t* kr = kv.k + page * kv.k_stride + ((size_t)h * kPageTokens + t) * HD;
             const float k_scale = kv.scales[page * kv.scale_stride + h] * a.scale * kLog2e;
@@ -688,8 +693,8 @@ few_join_kernel(const FewArgs a, const E4M3Pages kv, int join_blocks) {
                 if (row > to || (a.window > 0 && row <= to - a.window)) continue;
                 const bf16* qr = a.q + (size_t)(span.first + c / a.group) * a.ldq + (size_t)(h * a.group + c % a.group) * HD;
                 float s = 0.f;
-                for (int d = 0; d < HD; ++d) s = fmaf(__bfloat162float(qr[d]), e4m3_value(kr[d]), s);
-                sum += exp2_fast(s * k_scale - top[c] + kPShift) * inverse[c];
+                for (int d = 0; d < HD; ++d) s = fmaf(__bfloat162float(qr[d]) * kDown, e4m3_value(kr[d]), s);
+                sum += exp2_fast(s * k_scale * kUp - top[c] + kPShift) * inverse[c];
             }
         }
         kv.weights[page * kv.weight_stride + h * kPageTokens + t] += sum;

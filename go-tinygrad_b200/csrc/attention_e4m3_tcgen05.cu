@@ -389,7 +389,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             }
             // the largest channel comes to lie in [2^14, 2^15); a negative scale turns the queries round
             const int e = (int)(__float_as_uint(most) >> 23);
-            const int up = e == 0 ? 0 : min(max(14 - (e - 127), -100), 100);
+            const int up = e == 0 ? 0 : min(14 - (e - 127), 100);
             const float f = __uint_as_float((uint32_t)(127 + up) << 23) * (a.scale < 0.f ? -1.f : 1.f);
             factor = fmaxf(fabsf(a.scale) * kLog2e * __uint_as_float((uint32_t)(127 - up) << 23), 1e-37f);
 #pragma unroll
@@ -446,9 +446,8 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             // the maximum found and the step done again.
             uint32_t pw[BK / 2];
             uint64_t sum;
-            auto exponentials = [&]() {
-                const float shift = add - (m_run == -INFINITY ? 0.f : m_run) + kPShift;
-                const uint64_t sl2 = two(sl, sl), shift2 = two(shift, shift);
+            auto exponentials = [&](float mult, float shift) {
+                const uint64_t sl2 = two(mult, mult), shift2 = two(shift, shift);
                 uint64_t sums[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int c = 0; c < BK; c += 8) {
@@ -468,7 +467,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                 sum = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
             };
             const bool fresh = __any_sync(full, m_run == -INFINITY);
-            if (!fresh) exponentials();
+            if (!fresh) exponentials(sl, add - m_run + kPShift);
             if (fresh || __any_sync(full, first_of(sum) + second_of(sum) > kMostSum)) {
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -497,7 +496,16 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                         tmem_st8(tile_at + S::kColO + 8 * part, ov);
                     }
                 }
-                exponentials();
+                const float m_use = m_run == -INFINITY ? 0.f : m_run;
+                float mult = sl, shift = add - m_use + kPShift;
+                if (__any_sync(full, fabsf(m_use) > 4194304.0f)) {
+                    // M's own rounding is a quarter and more here: take it from scores rounded as it was, which leaves 0 for its row
+#pragma unroll
+                    for (int c = 0; c < BK; ++c) sv[c] = __float_as_uint(fmaf(__uint_as_float(sv[c]), sl, add) - m_use);
+                    mult = 1.0f;
+                    shift = kPShift;
+                }
+                exponentials(mult, shift);
             }
             l_run = fmaf(first_of(sum) + second_of(sum), __uint_as_float(top_bits - __float_as_uint(v_scale)), l_run);
             tmem_st32(tile_at + S::kColP + 32 * (i & 1), pw);
@@ -768,7 +776,8 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                         const float ys[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            const float p = fast_exp2(fmaf(__uint_as_float(sv[e + x]), f, ys[x]));
+                            // (no probability is above 1: the bound is for scores so large that their roundings are powers of two)
+                            const float p = fast_exp2(min_or_nan(fmaf(__uint_as_float(sv[e + x]), f, ys[x]), 0.f));
                             sum[x] += whole || (c + e + x >= lo && c + e + x < hi) ? p : 0.f;
                         }
                     }

@@ -45,6 +45,12 @@ static inline int launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block
 
 __device__ __forceinline__ bool finite_f32(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // The least power of two 2^k, k >= -126, with most <= 448 * 2^k, for finite most >= 0: 448 = 1.75 * 2^8, so k is the
 // exponent less 8, one more where the mantissa exceeds 1.75.
 __device__ __forceinline__ float e4m3_needed_scale(float most) {

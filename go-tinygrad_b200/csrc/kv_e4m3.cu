@@ -143,7 +143,7 @@ struct EvictStrides { long long k, v, scales, weights; };
 
 __global__ void __launch_bounds__(kEvictThreads)
 kv_evict_kernel(const E4M3Pages pages, const EvictStrides strides, int* __restrict__ dropped, const int* __restrict__ slots,
-                const int* __restrict__ lengths, int budget, int recent, int* __restrict__ kept_out) {
+                const int* __restrict__ lengths, int max_length, int budget, int recent, int* __restrict__ kept_out) {
     extern __shared__ uint8_t tile[];                                           // 64 rows x hd codes
     __shared__ int histogram[256];
     __shared__ int warp_sums[kEvictThreads / 32];
@@ -152,8 +152,8 @@ kv_evict_kernel(const E4M3Pages pages, const EvictStrides strides, int* __restri
     const int h = blockIdx.x, b = blockIdx.y, entry = blockIdx.z, tid = threadIdx.x;
     const int length = lengths[b], slot = slots[b], hd = pages.hd;
     int* kept = kept_out + (((size_t)entry * gridDim.y + b) * pages.n_kv + h) * budget;
-    if (length <= budget) {
-        for (int i = tid; i < budget; i += kEvictThreads) kept[i] = i < length ? i : -1;
+    if (length <= budget || length > max_length) {
+        for (int i = tid; i < budget; i += kEvictThreads) kept[i] = i < length && length <= budget ? i : -1;
         return;
     }
     if (h == 0 && entry == 0 && tid == 0 && dropped) dropped[slot] += length - budget;
@@ -913,6 +913,6 @@ GTG_API int gtg_kv_evict_e4m3(int entries, void* k, long long k_entry, long long
         switch (hd) { GTG_MOVE(16) GTG_MOVE(32) GTG_MOVE(48) GTG_MOVE(64) GTG_MOVE(80) GTG_MOVE(96) GTG_MOVE(112) GTG_MOVE(128) }
 #undef GTG_MOVE
     }
-    kv_evict_kernel<<<dim3(n_kv, B, entries), kEvictThreads, smem, stream>>>(pages, strides, dropped, slots, lengths, budget, recent, kept);
+    kv_evict_kernel<<<dim3(n_kv, B, entries), kEvictThreads, smem, stream>>>(pages, strides, dropped, slots, lengths, max_length, budget, recent, kept);
     return launch_status();
 }

@@ -1703,8 +1703,18 @@ def _need_e4m3(kv, what: str, q, slots, start_pos, cu_seqlens) -> None:
     device = kv.k.device
     if slots.device != device or start_pos.device != device or cu_seqlens.device != device or q.device != device:
         raise KernelError(f"{what}: the step's tensors must be on the cache's device")
+    _need_current(device, what)
+
+
+def _need_current(device: torch.device, what: str) -> None:
     if device.type == "cuda" and device.index != torch.cuda.current_device():
         raise KernelError(f"{what}: the cache is on {device}, which is not the current device")
+
+
+def _need_gpu(device: torch.device, what: str) -> None:
+    """Last before a launch, so that everything else is checked without a GPU too."""
+    if device.type != "cuda":
+        raise KernelError(f"{what}: the cache is on {device}, which is no CUDA device")
 
 
 def _check_access_e4m3(what: str, kv, slots, start_pos, cu_seqlens) -> None:
@@ -1752,8 +1762,12 @@ def kv_store_e4m3(qkv: torch.Tensor, cos_sin: Optional[torch.Tensor], n_heads: i
         _rows2d(q_out, "kv_store_e4m3: q_out")
         if q_out.dtype != qkv.dtype or tuple(q_out.shape) != (N, n_heads * hd):
             raise KernelError("kv_store_e4m3: q_out must be [N, n_heads * head_dim] of qkv's dtype")
+    for t in (cos_sin, q_out):
+        if t is not None and t.device != qkv.device:
+            raise KernelError("kv_store_e4m3: cos_sin and q_out must be on the cache's device")
     if n_kv_store:
         _check_access_e4m3("kv_store_e4m3", kv, slots, start_pos, cu_seqlens)
+    _need_gpu(qkv.device, "kv_store_e4m3")
     _check(_fn("gtg_kv_store_e4m3")(dt, qkv.data_ptr(), qkv.stride(0), _ptr(cos_sin), n_heads, kv.n_kv_heads, hd, rot, ROTARY_PAIRINGS[pairing],
                                     1 if values_from_keys else 0, 1 if n_kv_store else 0, *kv.address(), cu_seqlens.data_ptr(), slots.data_ptr(),
                                     start_pos.data_ptr(), slots.numel(), int(max_q_len), N, _ptr(q_out), q_out.stride(0) if q_out is not None else 0,
@@ -1810,6 +1824,8 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
     dt, hd, N = _dt(q), kv.head_dim, q.shape[0]
     if out.dtype != q.dtype or q.shape[1] != n_heads * hd or out.shape[1] != n_heads * hd or out.shape[0] < N:
         raise KernelError("attention_e4m3: q and out must be [N, n_heads * head_dim] of one dtype")
+    if out.device != q.device:
+        raise KernelError("attention_e4m3: out must be on the cache's device")
     if n_heads <= 0 or n_heads % kv.n_kv_heads:
         raise KernelError(f"attention_e4m3: {n_heads} query heads cannot share {kv.n_kv_heads} key/value heads")
     if N and (max_q_len < 1 or max_kv_len < 1):
@@ -1821,6 +1837,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
     _check_access_e4m3("attention_e4m3", kv, slots, start_pos, cu_seqlens)
     if N == 0 or B == 0:
         return
+    _need_gpu(q.device, "attention_e4m3")
     prompt = _e4m3_prompt_form(dt, max_q_len, n_heads, kv.n_kv_heads, hd)
     if prompt:
         need = _e4m3_prompt_scratch(B, N, n_heads, kv, int(max_kv_len))
@@ -1830,8 +1847,9 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
     if need:
         if scratch is None:
             scratch = torch.empty(need, dtype=torch.float32, device=q.device)
-        elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need or scratch.data_ptr() % 16:
-            raise KernelError(f"attention_e4m3: scratch needs {need} contiguous floats on a 16-byte boundary")
+        elif (scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need or scratch.data_ptr() % 16
+              or scratch.device != q.device):
+            raise KernelError(f"attention_e4m3: scratch needs {need} contiguous floats on a 16-byte boundary of the cache's device")
     if prompt and not (q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16):
         _check(_fn("gtg_attention_e4m3_tcgen05")(q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *kv.address(), cu_seqlens.data_ptr(),
                                                  slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), N, n_heads, kv.n_kv_heads,
@@ -1849,12 +1867,13 @@ def kv_evict_e4m3(storage, slots: torch.Tensor, lengths: torch.Tensor, max_lengt
     `recent` newest and of the others the budget - recent of largest gathered weight (the lower row on a tie), in their order, at
     rows 0..budget-1.  Blocks all of whose rows stay in place are left as they were; any other gets the least scale that holds
     its rows, and their codes are rounded to it (which changes only codes that need the smallest steps).  A sequence of at
-    most `budget` rows is left alone.  storage.dropped[slot], where given, grows by the rows cut.  Returns `kept` (int32
+    most `budget` rows is left alone, and so is one of more than `max_length` (its `kept` is -1).  storage.dropped[slot], where given, grows by the rows cut.  Returns `kept` (int32
     [entries, n, n_kv_heads, budget], made if None): the former row of each row kept, -1 behind a shorter sequence's last.
     A slot must not appear twice."""
     _need(getattr(storage, "format", None) == "e4m3" and storage.k.dim() == 5, "kv_evict_e4m3: needs the storage of an e4m3 cache")
     _need(storage.weights is not None, "kv_evict_e4m3: this cache gathers no attention weights")
     n, device = slots.numel(), storage.k.device
+    _need_current(device, "kv_evict_e4m3")
     for t in (slots, lengths):
         _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n and t.device == device,
               "kv_evict_e4m3: slots and lengths must be contiguous int32 of one size on the cache's device")
@@ -1868,6 +1887,7 @@ def kv_evict_e4m3(storage, slots: torch.Tensor, lengths: torch.Tensor, max_lengt
               "kv_evict_e4m3: kept must be contiguous int32 [entries, n, n_kv_heads, budget]")
     if n == 0:
         return kept
+    _need_gpu(device, "kv_evict_e4m3")
     k, v, s, w = storage.k, storage.v, storage.scales, storage.weights
     if _checked:
         start = (lengths - 1).clamp(min=0)

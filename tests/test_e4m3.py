@@ -187,6 +187,7 @@ def view(pages=4, heads=2, dim=16, slots=3, weights=True, **swap):
     (dict(k=torch.zeros(4, 2, 16, 64).to(torch.float8_e4m3fn).transpose(2, 3)), "in one piece"),
     (dict(k=torch.zeros(4 * 2 * 64 * 16 + 8).to(torch.float8_e4m3fn)[8:].view(4, 2, 64, 16)), "16-byte boundary"),
     (dict(block_table=torch.zeros(3, 4, dtype=torch.int64)), "block table"),
+    (dict(block_table=torch.zeros(1, 4, dtype=torch.int32).expand(3, 4)), "row by row"),
     (dict(dropped=torch.zeros(2, dtype=torch.int32)), "dropped"),
 ])
 def test_a_view_refuses(swap, what):

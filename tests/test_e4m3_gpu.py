@@ -377,6 +377,33 @@ def test_scales_far_apart(dtype, hd, new):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("new", [1, 70])
+def test_queries_as_large_as_their_type_holds(dtype, new):
+    """Scores of 2^80 and more: each query sees one row, and its result is that row's values, codes that bfloat16 holds."""
+    n, hd = 200, 64
+    p = Pages([n], 1, hd, seed=41, weights=True)
+    rng = np.random.default_rng(42)
+    k, v = p.rows[0][0]
+    k.codes, k.scales, v.codes, v.scales = np.zeros((0, hd)), [], np.zeros((0, hd)), []
+    k.append(rng.standard_normal((n, hd)) * 2.0 ** -40)
+    v.append(rng.standard_normal((n, hd)))
+    p.write(0)
+    q = torch.from_numpy(rng.uniform(-1, 1, (new, hd)) * 2.0 ** 127.9).to(dtype).to(DEV)
+    out = torch.empty_like(q)
+    ops.attention_e4m3(q, out, p.view(), cut([new]), ints(p.slots), ints([n - new]), new, 1, hd ** -0.5, max_kv_len=n)
+    scores = q.double().cpu().numpy() @ k.values().T
+    sizes = np.abs(q.double().cpu().numpy()) @ np.abs(k.values()).T
+    for i in range(new):
+        row = scores[i, : n - new + i + 1]
+        best = int(row.argmax())
+        # which row wins is beyond what rounding a sum of hd products can change
+        assert np.delete(row, best).max() < row[best] - 2 * (hd + 4) * 2.0 ** -23 * sizes[i].max()
+        assert np.array_equal(out[i].double().cpu().numpy(), v.values()[best]), i
+    added = p.read_weights(0, 0, n) - p.gathered[0][0]
+    assert np.isfinite(added).all() and added.min() >= -1e-6 and added.max() <= new * (1 + 2.0 ** -20)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("hd", [64, 128, 48])
 @pytest.mark.parametrize("new", [1, 70, 330])
 @pytest.mark.parametrize("small", [0.0, 2.0 ** -90])
@@ -423,6 +450,23 @@ def test_what_is_not_finite_stays_with_who_sees_it(dtype, new):
     assert bad[0, :, 2:].all() and not bad[0, :, :2].any() and not bad[1].any()
     ops.attention_e4m3(q, out, p.view(), cut([new, new]), ints(p.slots), ints([200 - new, 100 - new]), new, 4, 0.125, max_kv_len=200, window=50)
     assert not out.isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 48])
+@pytest.mark.parametrize("new", [2, 70])
+def test_a_query_that_is_not_a_number_shows_in_the_weights(dtype, hd, new):
+    """Those of all rows it sees, under its own key/value head; its result is NaN, its neighbours' are not."""
+    p = Pages([200], 2, hd, seed=14, weights=True)
+    q = torch.randn(new, 4 * hd, device=DEV).to(dtype)
+    q[new // 2 - 1, 2 * hd + 3] = math.nan                 # head 2, of the second group
+    out = torch.empty_like(q)
+    ops.attention_e4m3(q, out, p.view(), cut([new]), ints(p.slots), ints([200 - new]), new, 4, hd ** -0.5, max_kv_len=200)
+    bad = out.isnan().reshape(new, 4, hd)
+    assert bad[new // 2 - 1, 2].all() and bad.sum() == hd
+    seen = 200 - new + new // 2 - 1
+    w = p.read_weights(0, 1, 200)
+    assert np.isnan(w[: seen + 1]).all() and np.isfinite(w[seen + 1:]).all() and np.isfinite(p.read_weights(0, 0, 200)).all()
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -555,6 +599,12 @@ def test_other_streams_and_devices_are_checked():
     q = torch.randn(1, 64, device=DEV)
     with pytest.raises(KernelError, match="cache's device"):
         ops.attention_e4m3(q.cpu(), torch.empty(1, 64), p.view(), cut([1]), ints(p.slots), ints([69]), 1, 1, 0.125, max_kv_len=70)
+    with pytest.raises(KernelError, match="cache's device"):
+        ops.attention_e4m3(q, torch.empty(1, 64), p.view(), cut([1]), ints(p.slots), ints([69]), 1, 1, 0.125, max_kv_len=70)
+    with pytest.raises(KernelError, match="cache's device"):
+        ops.kv_store_e4m3(torch.zeros(1, 192, device=DEV), None, 1, 1, p.view(), cut([1]), ints(p.slots), ints([70]), 1, torch.empty(1, 64))
+    with pytest.raises(KernelError, match="cache's device"):
+        ops.kv_store_e4m3(torch.zeros(1, 192, device=DEV), torch.zeros(1, 32, 2), 1, 1, p.view(), cut([1]), ints(p.slots), ints([70]), 1, q)
     scratch = torch.empty(1, device=DEV)
     p = Pages([70], 1, 64, seed=16, weights=True)
     need = ops.attention_e4m3_scratch_floats(F32, 1, 1, 1, 1, p.view(), 70)
@@ -654,6 +704,18 @@ def test_evict(lengths, budget, recent, n_kv, hd):
     lambda rng, n: np.arange(n, dtype=np.float32)], ids=["zeros", "tiny", "near", "infinite", "rising"])
 def test_evict_by_weights_of_all_kinds(weights_of):
     evict_case([700, 130], 129, 30, 2, 64, entries=1, weights_of=weights_of)
+
+
+@pytest.mark.parametrize("hd", [64, 20])
+def test_evict_leaves_sequences_longer_than_it_was_told_of(hd):
+    p = Pages([300, 200], 2, hd, seed=31, weights=True, dropped=[0, 0])
+    s = E4M3Storage(p.k[None], p.v[None], p.scales[None], p.table, weights=p.weights[None], dropped=p.dropped)
+    before = [t.clone() for t in (p.k.view(torch.uint8), p.v.view(torch.uint8), p.scales, p.weights)]
+    kept = ops.kv_evict_e4m3(s, ints(p.slots), ints([300, 200]), 250, 130, 10)
+    assert (kept[0, 0] == -1).all() and (kept[0, 1] >= 0).all() and p.dropped[p.slots[0]] == 0 and p.dropped[p.slots[1]] == 70
+    pages = torch.tensor(p.pages[0], device=DEV)
+    for was, now in zip(before, (p.k.view(torch.uint8), p.v.view(torch.uint8), p.scales, p.weights)):
+        assert torch.equal(was[pages], now[pages])
 
 
 def test_evict_keeps_the_code_of_nan():
