@@ -1816,8 +1816,8 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
     a query sees the rows at and before its own, the last `window` of them where a window is given (default: the view's).
     `max_kv_len`: rows of the longest sequence after this step; `total_kv_len`: of all (0: not known).  Both decide only how the work
     is cut: a sequence that has outgrown them is still computed right.  Where the view gathers weights, every row's grows by the
-    sum of its probabilities over the step's queries and the heads that share it.  Rows of q and out behind the last sequence
-    are left alone.  `scratch`: float32, at least `attention_e4m3_scratch_floats` (None: taken from the allocator)."""
+    sum of its probabilities over the step's queries and the heads that share it (no two of the step's sequences may share a page
+    then).  Rows of q and out behind the last sequence are left alone.  `scratch`: float32, at least `attention_e4m3_scratch_floats` (None: taken from the allocator)."""
     _rows2d(q, "attention_e4m3: q")
     _rows2d(out, "attention_e4m3: out")
     _need_e4m3(kv, "attention_e4m3", q, slots, start_pos, cu_seqlens)

@@ -437,6 +437,17 @@ def test_blocks_of_zeros_have_their_share_of_the_probability(dtype, hd, new, sma
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("longest", [1, 3, 40])
+def test_many_sequences_some_without_new_tokens(dtype, longest):
+    rng = np.random.default_rng(51)
+    new = [int(x) for x in rng.integers(0, longest + 1, 150)]
+    new[:3], new[-1] = [0, 0, longest], 0
+    held = [int(m + x) for m, x in zip(new, rng.integers(0, 200, 150))]
+    worst, worst_w = attention_case(dtype, held, new, 4, 2, 64, weights=True, dropped=[int(x) for x in rng.integers(0, 9, 150)])
+    assert worst <= 1 and worst_w <= 1, (worst, worst_w)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("new", [1, 40])
 def test_what_is_not_finite_stays_with_who_sees_it(dtype, new):
     """A NaN key spoils the queries that see its row, of its own head alone; NaN behind the window spoils nobody."""
@@ -568,6 +579,40 @@ def test_rows_of_any_stride(hd, new):
         assert (wide_out[:, :pad] == 0).all()
     # two results that are each within half a step (2^-8) and the products' rounding of the same value
     assert ((outs[0] - outs[1]).abs() <= outs[0].abs() * 2.0 ** -7 + 2.0 ** -9).all() and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("new", [1, 100])
+def test_pages_further_than_32_bits_count(dtype, new):
+    """The same sequence in a small cache and at the end of one of 4.4 GB: attention, a step's store and an eviction agree bit by bit."""
+    n_kv, hd, held, total = 32, 128, 300, 8400
+    p = Pages([held], n_kv, hd, seed=61, weights=True, dropped=[0], room=128)
+    raw = torch.zeros(total, 2, n_kv * 64 * hd, dtype=torch.uint8, device=DEV)
+    k, v = (raw[:, i].view(torch.float8_e4m3fn) for i in (0, 1))
+    k, v = k.unflatten(1, (n_kv, 64, hd)), v.unflatten(1, (n_kv, hd, 64))
+    scales, weights = torch.ones(total, 2, n_kv, device=DEV), torch.zeros(total, n_kv, 64, device=DEV)
+    here, there = torch.tensor(p.pages[0], device=DEV), torch.arange(total - len(p.pages[0]), total, device=DEV)
+
+    def parts(view):
+        return [view.k.view(torch.uint8), view.v.view(torch.uint8), view.scales, view.weights]
+    small = p.view()
+    table = torch.zeros_like(p.table)
+    table[p.slots[0], : len(p.pages[0])] = there.int()
+    big = E4M3KVView(k, v, scales, table, weights=weights, dropped=torch.zeros_like(p.dropped))
+    for a, b in zip(parts(small), parts(big)):
+        b[there] = a[here]
+    q = torch.randn(new, n_kv * hd, device=DEV).to(dtype)
+    qkv = torch.randn(70, 3 * n_kv * hd, device=DEV).to(dtype)
+    outs = []
+    for view in (small, big):
+        out, stored = torch.empty_like(q), torch.empty(70, n_kv * hd, dtype=dtype, device=DEV)
+        ops.attention_e4m3(q, out, view, cut([new]), ints(p.slots), ints([held - new]), new, n_kv, hd ** -0.5, max_kv_len=held)
+        ops.kv_store_e4m3(qkv, None, n_kv, n_kv, view, cut([70]), ints(p.slots), ints([held]), 70, stored)
+        s = E4M3Storage(view.k[None], view.v[None], view.scales[None], view.block_table, weights=view.weights[None], dropped=view.dropped)
+        kept = ops.kv_evict_e4m3(s, ints(p.slots), ints([held + 70]), held + 70, 200, 50)
+        outs.append((out, stored, kept))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert all(torch.equal(a[here], b[there]) for a, b in zip(parts(small), parts(big)))
 
 
 @pytest.mark.parametrize("hd", [64, 128])
