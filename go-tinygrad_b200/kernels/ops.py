@@ -262,8 +262,8 @@ def _need(cond: bool, msg: str) -> None:
 
 
 def _rows2d(t: torch.Tensor, name: str) -> None:
-    _need(t.dim() == 2 and t.stride(1) == 1, f"{name} must be 2-D with a unit inner stride, "
-                                             f"got shape {tuple(t.shape)} strides {t.stride()}")
+    if t.dim() != 2 or t.stride(1) != 1:                   # (the message costs more than the check)
+        raise KernelError(f"{name} must be 2-D with a unit inner stride, got shape {tuple(t.shape)} strides {t.stride()}")
 
 
 # ------------------------------------------------- the debug pass over cache addresses
@@ -1693,28 +1693,31 @@ E4M3_MAX_CHANNELS = 256       # of a head
 
 def _need_e4m3(kv, what: str, q, slots, start_pos, cu_seqlens) -> None:
     """What both kernels ask of an `E4M3KVView` and a step's index tensors."""
-    _need(getattr(kv, "format", None) == "e4m3", f"{what}: needs a view of an e4m3 cache")
-    for t in (slots, start_pos, cu_seqlens):
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise KernelError(f"{what}: slots, start_pos and cu_seqlens must be contiguous int32")
+    if getattr(kv, "format", None) != "e4m3":
+        raise KernelError(f"{what}: needs a view of an e4m3 cache")
+    int32 = torch.int32
+    if (slots.dtype is not int32 or start_pos.dtype is not int32 or cu_seqlens.dtype is not int32
+            or not (slots.is_contiguous() and start_pos.is_contiguous() and cu_seqlens.is_contiguous())):
+        raise KernelError(f"{what}: slots, start_pos and cu_seqlens must be contiguous int32")
     n = slots.numel()
     if start_pos.numel() != n or cu_seqlens.numel() != n + 1:
         raise KernelError(f"{what}: {n} slots need {n} start positions and {n + 1} cumulative lengths")
-    device = kv.k.device
-    if slots.device != device or start_pos.device != device or cu_seqlens.device != device or q.device != device:
+    device = kv.k.get_device()
+    if slots.get_device() != device or start_pos.get_device() != device or cu_seqlens.get_device() != device or q.get_device() != device:
         raise KernelError(f"{what}: the step's tensors must be on the cache's device")
     _need_current(device, what)
 
 
-def _need_current(device: torch.device, what: str) -> None:
-    if device.type == "cuda" and device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: the cache is on {device}, which is not the current device")
+def _need_current(device: int, what: str) -> None:
+    """`device`: a tensor's `get_device()`, -1 for the host's memory."""
+    if device >= 0 and device != torch.cuda.current_device():
+        raise KernelError(f"{what}: the cache is on device {device}, which is not the current one")
 
 
-def _need_gpu(device: torch.device, what: str) -> None:
+def _need_gpu(t: torch.Tensor, what: str) -> None:
     """Last before a launch, so that everything else is checked without a GPU too."""
-    if device.type != "cuda":
-        raise KernelError(f"{what}: the cache is on {device}, which is no CUDA device")
+    if t.get_device() < 0:
+        raise KernelError(f"{what}: the cache is on {t.device}, which is no CUDA device")
 
 
 def _check_access_e4m3(what: str, kv, slots, start_pos, cu_seqlens) -> None:
@@ -1763,11 +1766,11 @@ def kv_store_e4m3(qkv: torch.Tensor, cos_sin: Optional[torch.Tensor], n_heads: i
         if q_out.dtype != qkv.dtype or tuple(q_out.shape) != (N, n_heads * hd):
             raise KernelError("kv_store_e4m3: q_out must be [N, n_heads * head_dim] of qkv's dtype")
     for t in (cos_sin, q_out):
-        if t is not None and t.device != qkv.device:
+        if t is not None and t.get_device() != qkv.get_device():
             raise KernelError("kv_store_e4m3: cos_sin and q_out must be on the cache's device")
     if n_kv_store:
         _check_access_e4m3("kv_store_e4m3", kv, slots, start_pos, cu_seqlens)
-    _need_gpu(qkv.device, "kv_store_e4m3")
+    _need_gpu(qkv, "kv_store_e4m3")
     _check(_fn("gtg_kv_store_e4m3")(dt, qkv.data_ptr(), qkv.stride(0), _ptr(cos_sin), n_heads, kv.n_kv_heads, hd, rot, ROTARY_PAIRINGS[pairing],
                                     1 if values_from_keys else 0, 1 if n_kv_store else 0, *kv.address(), cu_seqlens.data_ptr(), slots.data_ptr(),
                                     start_pos.data_ptr(), slots.numel(), int(max_q_len), N, _ptr(q_out), q_out.stride(0) if q_out is not None else 0,
@@ -1802,8 +1805,7 @@ def attention_e4m3_scratch_floats(dtype: torch.dtype, n_seqs: int, n_tokens: int
     window = kv.window if window is None else window
     if _e4m3_prompt_form(0 if dtype == torch.float32 else 1, max_q_len, n_heads, kv.n_kv_heads, kv.head_dim):
         return _e4m3_prompt_scratch(n_seqs, n_tokens, n_heads, kv, int(max_kv_len))
-    device = kv.k.device.index
-    return _e4m3_few_scratch(-1 if device is None else device, 0 if dtype == torch.float32 else 1, n_seqs, n_tokens, int(max_q_len), n_heads,
+    return _e4m3_few_scratch(kv.k.get_device(), 0 if dtype == torch.float32 else 1, n_seqs, n_tokens, int(max_q_len), n_heads,
                              kv.n_kv_heads, kv.head_dim, int(max_kv_len), int(total_kv_len), int(window or 0), 1 if kv.weights is not None else 0)
 
 
@@ -1824,7 +1826,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
     dt, hd, N = _dt(q), kv.head_dim, q.shape[0]
     if out.dtype != q.dtype or q.shape[1] != n_heads * hd or out.shape[1] != n_heads * hd or out.shape[0] < N:
         raise KernelError("attention_e4m3: q and out must be [N, n_heads * head_dim] of one dtype")
-    if out.device != q.device:
+    if out.get_device() != q.get_device():
         raise KernelError("attention_e4m3: out must be on the cache's device")
     if n_heads <= 0 or n_heads % kv.n_kv_heads:
         raise KernelError(f"attention_e4m3: {n_heads} query heads cannot share {kv.n_kv_heads} key/value heads")
@@ -1837,16 +1839,16 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
     _check_access_e4m3("attention_e4m3", kv, slots, start_pos, cu_seqlens)
     if N == 0 or B == 0:
         return
-    _need_gpu(q.device, "attention_e4m3")
+    _need_gpu(q, "attention_e4m3")
     prompt = _e4m3_prompt_form(dt, max_q_len, n_heads, kv.n_kv_heads, hd)
     if prompt:
         need = _e4m3_prompt_scratch(B, N, n_heads, kv, int(max_kv_len))
     else:
-        need = _e4m3_few_scratch(q.device.index, dt, B, N, int(max_q_len), n_heads, kv.n_kv_heads, hd, int(max_kv_len), int(total_kv_len),
+        need = _e4m3_few_scratch(q.get_device(), dt, B, N, int(max_q_len), n_heads, kv.n_kv_heads, hd, int(max_kv_len), int(total_kv_len),
                                  int(window or 0), 1 if kv.weights is not None else 0)
     if need:
         if scratch is None:
-            scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+            scratch = q.new_empty(need, dtype=torch.float32)
         elif (scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need or scratch.data_ptr() % 16
               or scratch.device != q.device):
             raise KernelError(f"attention_e4m3: scratch needs {need} contiguous floats on a 16-byte boundary of the cache's device")
@@ -1873,12 +1875,14 @@ def kv_evict_e4m3(storage, slots: torch.Tensor, lengths: torch.Tensor, max_lengt
     _need(getattr(storage, "format", None) == "e4m3" and storage.k.dim() == 5, "kv_evict_e4m3: needs the storage of an e4m3 cache")
     _need(storage.weights is not None, "kv_evict_e4m3: this cache gathers no attention weights")
     n, device = slots.numel(), storage.k.device
-    _need_current(device, "kv_evict_e4m3")
+    _need_current(storage.k.get_device(), "kv_evict_e4m3")
     for t in (slots, lengths):
         _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() == n and t.device == device,
               "kv_evict_e4m3: slots and lengths must be contiguous int32 of one size on the cache's device")
-    _need(budget >= 1 and 0 <= recent <= budget, f"kv_evict_e4m3: budget {budget} must be positive and recent {recent} between 0 and it")
-    _need(0 <= max_length <= storage.block_table.shape[1] * PAGE_TOKENS, f"kv_evict_e4m3: the block table holds no {max_length} rows of a sequence")
+    if budget < 1 or not 0 <= recent <= budget:
+        raise KernelError(f"kv_evict_e4m3: budget {budget} must be positive and recent {recent} between 0 and it")
+    if not 0 <= max_length <= storage.block_table.shape[1] * PAGE_TOKENS:
+        raise KernelError(f"kv_evict_e4m3: the block table holds no {max_length} rows of a sequence")
     E, KV = storage.k.shape[0], storage.n_kv_heads
     if kept is None:
         kept = torch.empty(E, n, KV, budget, dtype=torch.int32, device=device)
@@ -1887,7 +1891,7 @@ def kv_evict_e4m3(storage, slots: torch.Tensor, lengths: torch.Tensor, max_lengt
               "kv_evict_e4m3: kept must be contiguous int32 [entries, n, n_kv_heads, budget]")
     if n == 0:
         return kept
-    _need_gpu(device, "kv_evict_e4m3")
+    _need_gpu(storage.k, "kv_evict_e4m3")
     k, v, s, w = storage.k, storage.v, storage.scales, storage.weights
     if _checked:
         start = (lengths - 1).clamp(min=0)
