@@ -38,6 +38,7 @@ layer's cache are in model/kv_staging.go:11-54.
 """
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence, Tuple, Union
 
@@ -157,6 +158,14 @@ def _check_e4m3(k, v, scales, block_table, weights, dropped, lead: int) -> None:
         raise ValueError("dropped must be contiguous int32 [slots] on the keys' device")
 
 
+class _E4M3Pages(ctypes.Structure):
+    """The same in C (csrc/e4m3.cuh)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_stride", ctypes.c_longlong), ("v_stride", ctypes.c_longlong),
+                ("scales", ctypes.c_void_p), ("scale_stride", ctypes.c_longlong), ("weights", ctypes.c_void_p), ("weight_stride", ctypes.c_longlong),
+                ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int), ("dropped", ctypes.c_void_p), ("n_kv", ctypes.c_int),
+                ("hd", ctypes.c_int)]
+
+
 class E4M3KVView:
     """What a kernel needs to address one run's keys and values in an e4m3 cache: k [page, head, 64, channel] and v
     [page, head, channel, 64] (float8_e4m3fn), scales [page, 2, head] (float32 powers of two), the block table, and for a cache
@@ -171,12 +180,14 @@ class E4M3KVView:
         self.n_kv_heads, self.head_dim = k.shape[1], k.shape[3]
         self.value_dim = self.head_dim
         self.page_stride, self.table_stride = k.stride(0), block_table.stride(0)
-        self._address = (k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), scales.data_ptr(), scales.stride(0),
-                         weights.data_ptr() if weights is not None else None, weights.stride(0) if weights is not None else 0,
-                         block_table.data_ptr(), block_table.stride(0), dropped.data_ptr() if dropped is not None else None)
+        self._pages = _E4M3Pages(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), scales.data_ptr(), scales.stride(0),
+                                 weights.data_ptr() if weights is not None else None, weights.stride(0) if weights is not None else 0,
+                                 block_table.data_ptr(), block_table.stride(0), dropped.data_ptr() if dropped is not None else None,
+                                 self.n_kv_heads, self.head_dim)
+        self._address = ctypes.addressof(self._pages)
 
-    def address(self):
-        """Pointers and strides as the kernels take them."""
+    def address(self) -> int:
+        """Where the pointers and strides lie as the kernels take them."""
         return self._address
 
 

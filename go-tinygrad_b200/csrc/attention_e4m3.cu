@@ -219,17 +219,16 @@ GTG_API long long gtg_attention_e4m3_scratch_floats(int dtype, int B, int N, int
 
 // dtype: of q and out (0 float, 1 bfloat16).  max_kv_len: rows of the longest sequence after this step; total_kv_len: of all
 // (0: not known); they decide how the work is cut and how many blocks look for weights.
-GTG_API int gtg_attention_e4m3(int dtype, const void* q, int ldq, void* out, int ldo, void* k, long long k_stride, void* v, long long v_stride,
-                               float* scales, long long scale_stride, float* weights, long long weight_stride, const int* block_table,
-                               int table_stride, const int* dropped, const int* cu_seqlens, const int* slots, const int* start_pos, int B,
-                               int max_q_len, int max_kv_len, long long total_kv_len, int N, int n_heads, int n_kv, int hd, float scale,
-                               int window, float* scratch, cudaStream_t stream) {
+GTG_API int gtg_attention_e4m3(int dtype, const void* q, int ldq, void* out, int ldo, const E4M3Pages* pages, const int* cu_seqlens,
+                               const int* slots, const int* start_pos, int B, int max_q_len, int max_kv_len, long long total_kv_len, int N,
+                               int n_heads, float scale, int window, float* scratch, cudaStream_t stream) {
     if (B <= 0 || N <= 0 || max_q_len <= 0) return 0;
+    const E4M3Pages kv = *pages;
+    const int n_kv = kv.n_kv, hd = kv.hd;
+    float* weights = kv.weights;
     if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || hd <= 0 || max_kv_len <= 0 || window < 0) return kErrBadArgument;
     if (hd > kMaxChannels || B > 65535 || n_heads > 65535) return kErrUnsupported;
-    const E4M3Pages kv = {(uint8_t*)k, (uint8_t*)v, k_stride, v_stride, scales, scale_stride, weights, weight_stride, block_table, table_stride,
-                          dropped, n_kv, hd};
-    if (few_takes(dtype, max_q_len, n_heads, n_kv, hd) && few_counts(B, max_q_len, n_heads, n_kv, table_stride)) {
+    if (few_takes(dtype, max_q_len, n_heads, n_kv, hd) && few_counts(B, max_q_len, n_heads, n_kv, kv.table_stride)) {
         const FewPlan plan = few_plan(B, max_q_len, n_heads, n_kv, hd, max_kv_len, weights != nullptr);
         if (plan.floats() && !scratch) return kErrBadArgument;
         FewArgs a = {};

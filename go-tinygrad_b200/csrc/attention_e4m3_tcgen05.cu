@@ -838,17 +838,17 @@ GTG_API int gtg_attention_e4m3_tcgen05_status() {
 
 // Heads of 64 or 128 channels, bfloat16 rows of q and out on 16-byte boundaries.  weights (or null) gather what the rows get;
 // scratch for that: 2 N n_heads floats and n_heads B times max_kv_len rounded up to 128.
-GTG_API int gtg_attention_e4m3_tcgen05(const void* q, int ldq, void* out, int ldo, void* k, long long k_stride, void* v, long long v_stride,
-                                       float* scales, long long scale_stride, float* weights, long long weight_stride, const int* block_table,
-                                       int table_stride, const int* dropped, const int* cu_seqlens, const int* slots, const int* start_pos, int B,
-                                       int max_q_len, int max_kv_len, int N, int n_heads, int n_kv, int hd, float scale, int window, float* scratch,
-                                       cudaStream_t stream) {
+GTG_API int gtg_attention_e4m3_tcgen05(const void* q, int ldq, void* out, int ldo, const E4M3Pages* pages, const int* cu_seqlens,
+                                       const int* slots, const int* start_pos, int B, int max_q_len, int max_kv_len, int N, int n_heads,
+                                       float scale, int window, float* scratch, cudaStream_t stream) {
     if (B <= 0 || max_q_len <= 0 || N <= 0) return 0;
+    const E4M3Pages kv = *pages;
+    const int n_kv = kv.n_kv, hd = kv.hd;
+    float* weights = kv.weights;
     if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || window < 0 || max_kv_len <= 0 || (weights && !scratch)) return kErrBadArgument;
     if (n_heads > 65535) return kErrUnsupported;
     if ((hd != 64 && hd != 128) || ldq % 8 || ldo % 8 || (uintptr_t)q % 16 || (uintptr_t)out % 16) return kErrUnsupported;
     if (B > 65535 || ((long long)max_q_len * (n_heads / n_kv) + BQ - 1) / BQ > 65535) return kErrUnsupported;
-    const E4M3Pages kv = {(uint8_t*)k, (uint8_t*)v, k_stride, v_stride, scales, scale_stride, weights, weight_stride, block_table, table_stride, dropped, n_kv, hd};
     PromptArgs a = {};
     a.q = (const bf16*)q; a.ldq = ldq; a.out = (bf16*)out; a.ldo = ldo;
     a.cu_seqlens = cu_seqlens; a.slots = slots; a.start_pos = start_pos;

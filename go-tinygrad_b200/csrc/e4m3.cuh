@@ -15,7 +15,8 @@
 // values: v + p v_stride + (h hd + d) 64 + t -- rows innermost, since the second product of attention contracts over them
 // and an 8-bit operand has no transposed load.  scales[p scale_stride + plane n_kv + h] (plane 0 keys, 1 values).
 // weights (or null): [p weight_stride + h 64 + t], the attention weight a row has gathered.  dropped (or null): by slot, how
-// many rows of its sequence have been evicted: position p of the sequence is row p - dropped.
+// many rows of its sequence have been evicted: position p of the sequence is row p - dropped.  A view of the cache holds one, and the
+// C entries copy it.
 struct E4M3Pages {
     uint8_t* k;
     uint8_t* v;

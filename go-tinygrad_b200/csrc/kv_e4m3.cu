@@ -876,15 +876,13 @@ int launch_store(const StoreInput<T>& in, const E4M3Pages& kv, const int* cu_seq
 
 // qkv: [N][ld] of the compute type (dtype 0 float, 1 bfloat16): n_heads query heads, n_kv key heads and, unless values_from_keys,
 // n_kv value heads.  cos_sin: float [N][rot/2][2] or null.  store 0: queries only (another run's cache is read).
-GTG_API int gtg_kv_store_e4m3(int dtype, const void* qkv, int ld, const float* cos_sin, int n_heads, int n_kv, int hd, int rot, int interleaved,
-                              int values_from_keys, int store, void* k, long long k_stride, void* v, long long v_stride, float* scales,
-                              long long scale_stride, float* weights, long long weight_stride, const int* block_table, int table_stride,
-                              const int* dropped, const int* cu_seqlens, const int* slots, const int* start_pos, int B, int max_q_len, int N,
-                              void* q_out, int ldq, cudaStream_t stream) {
+GTG_API int gtg_kv_store_e4m3(int dtype, const void* qkv, int ld, const float* cos_sin, int n_heads, int rot, int interleaved,
+                              int values_from_keys, int store, const E4M3Pages* pages, const int* cu_seqlens, const int* slots,
+                              const int* start_pos, int B, int max_q_len, int N, void* q_out, int ldq, cudaStream_t stream) {
     if (B <= 0 || N <= 0 || max_q_len <= 0) return 0;
+    const E4M3Pages kv = *pages;
+    const int n_kv = kv.n_kv, hd = kv.hd;
     if (n_heads < 0 || n_kv < 0 || hd <= 0 || rot < 0 || rot % 2 || rot > hd) return kErrBadArgument;
-    const E4M3Pages kv = {(uint8_t*)k, (uint8_t*)v, k_stride, v_stride, scales, scale_stride, weights, weight_stride, block_table, table_stride,
-                          dropped, n_kv, hd};
     const int v_offset = values_from_keys ? 0 : n_kv * hd;
     if (dtype == 0) {
         const StoreInput<float> in = {(const float*)qkv, ld, (const float2*)cos_sin, n_heads, n_kv, hd, rot, interleaved, v_offset};

@@ -134,14 +134,11 @@ _SIGNATURES = {
     "gtg_attention_tcgen05_status": ("attention_tcgen05", []),
     "gtg_attention_prefill_tcgen05": ("attention_tcgen05", [_P, _I, _I, _P, _I, _P, _P, _L, _I, _P, _I, _P, _P, _P,
                                                             _I, _I, _I, _I, _I, _F, _I, _I, _P, _F, _I, _P, _P]),
-    "gtg_kv_store_e4m3": ("kv_e4m3", [_I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P,
-                                      _I, _I, _I, _P, _I, _P]),
+    "gtg_kv_store_e4m3": ("kv_e4m3", [_I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P, _I, _P]),
     "gtg_kv_evict_e4m3": ("kv_e4m3", [_I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _P, _P]),
     "gtg_attention_e4m3_scratch_floats": ("attention_e4m3", [_I, _I, _I, _I, _I, _I, _I, _I, _L, _I, _I]),
-    "gtg_attention_e4m3": ("attention_e4m3", [_I, _P, _I, _P, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P,
-                                              _I, _I, _I, _L, _I, _I, _I, _I, _F, _I, _P, _P]),
-    "gtg_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", [_P, _I, _P, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P, _I, _P, _P, _P, _P,
-                                                              _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P]),
+    "gtg_attention_e4m3": ("attention_e4m3", [_I, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _L, _I, _I, _F, _I, _P, _P]),
+    "gtg_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", [_P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _P, _P]),
     "gtg_attention_e4m3_tcgen05_status": ("attention_e4m3_tcgen05", []),
     "gtg_attention_e4m3_tcgen05_test_hooks": ("attention_e4m3_tcgen05", [_I]),
     "gtg_argmax": ("sampling", [_P, _I, _I, _I, _P, _P]),
@@ -1771,8 +1768,8 @@ def kv_store_e4m3(qkv: torch.Tensor, cos_sin: Optional[torch.Tensor], n_heads: i
     if n_kv_store:
         _check_access_e4m3("kv_store_e4m3", kv, slots, start_pos, cu_seqlens)
     _need_gpu(qkv, "kv_store_e4m3")
-    _check(_fn("gtg_kv_store_e4m3")(dt, qkv.data_ptr(), qkv.stride(0), _ptr(cos_sin), n_heads, kv.n_kv_heads, hd, rot, ROTARY_PAIRINGS[pairing],
-                                    1 if values_from_keys else 0, 1 if n_kv_store else 0, *kv.address(), cu_seqlens.data_ptr(), slots.data_ptr(),
+    _check(_fn("gtg_kv_store_e4m3")(dt, qkv.data_ptr(), qkv.stride(0), _ptr(cos_sin), n_heads, rot, ROTARY_PAIRINGS[pairing],
+                                    1 if values_from_keys else 0, 1 if n_kv_store else 0, kv.address(), cu_seqlens.data_ptr(), slots.data_ptr(),
                                     start_pos.data_ptr(), slots.numel(), int(max_q_len), N, _ptr(q_out), q_out.stride(0) if q_out is not None else 0,
                                     _stream()), "kv_store_e4m3")
 
@@ -1853,13 +1850,13 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
               or scratch.device != q.device):
             raise KernelError(f"attention_e4m3: scratch needs {need} contiguous floats on a 16-byte boundary of the cache's device")
     if prompt and not (q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16):
-        _check(_fn("gtg_attention_e4m3_tcgen05")(q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *kv.address(), cu_seqlens.data_ptr(),
-                                                 slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), N, n_heads, kv.n_kv_heads,
-                                                 hd, float(scale), int(window or 0), scratch.data_ptr() if need else None, _stream()), "attention_e4m3")
+        _check(_fn("gtg_attention_e4m3_tcgen05")(q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv.address(), cu_seqlens.data_ptr(),
+                                                 slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), N, n_heads, float(scale),
+                                                 int(window or 0), scratch.data_ptr() if need else None, _stream()), "attention_e4m3")
         return
-    _check(_fn("gtg_attention_e4m3")(dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), *kv.address(), cu_seqlens.data_ptr(),
+    _check(_fn("gtg_attention_e4m3")(dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv.address(), cu_seqlens.data_ptr(),
                                      slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), int(total_kv_len), N, n_heads,
-                                     kv.n_kv_heads, hd, float(scale), int(window or 0), _ptr(scratch) if need else None, _stream()), "attention_e4m3")
+                                     float(scale), int(window or 0), _ptr(scratch) if need else None, _stream()), "attention_e4m3")
 
 
 def kv_evict_e4m3(storage, slots: torch.Tensor, lengths: torch.Tensor, max_length: int, budget: int, recent: int,
