@@ -165,6 +165,15 @@ class _E4M3Pages(ctypes.Structure):
                 ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int), ("dropped", ctypes.c_void_p), ("n_kv", ctypes.c_int),
                 ("hd", ctypes.c_int)]
 
+    @classmethod
+    def of(cls, k, v, scales, block_table, weights, dropped):
+        """Of tensors as `E4M3KVView` has them, or `E4M3Storage`: of its entry 0."""
+        at = k.dim() - 4                                     # the axis of pages
+        return cls(k.data_ptr(), v.data_ptr(), k.stride(at), v.stride(at), scales.data_ptr(), scales.stride(at),
+                   weights.data_ptr() if weights is not None else None, weights.stride(at) if weights is not None else 0,
+                   block_table.data_ptr(), block_table.stride(0), dropped.data_ptr() if dropped is not None else None,
+                   k.shape[at + 1], k.shape[at + 3])
+
 
 class E4M3KVView:
     """What a kernel needs to address one run's keys and values in an e4m3 cache: k [page, head, 64, channel] and v
@@ -180,10 +189,7 @@ class E4M3KVView:
         self.n_kv_heads, self.head_dim = k.shape[1], k.shape[3]
         self.value_dim = self.head_dim
         self.page_stride, self.table_stride = k.stride(0), block_table.stride(0)
-        self._pages = _E4M3Pages(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), scales.data_ptr(), scales.stride(0),
-                                 weights.data_ptr() if weights is not None else None, weights.stride(0) if weights is not None else 0,
-                                 block_table.data_ptr(), block_table.stride(0), dropped.data_ptr() if dropped is not None else None,
-                                 self.n_kv_heads, self.head_dim)
+        self._pages = _E4M3Pages.of(k, v, scales, block_table, weights, dropped)
         self._address = ctypes.addressof(self._pages)
 
     def address(self) -> int:
@@ -200,6 +206,14 @@ class E4M3Storage:
         self.k, self.v, self.scales, self.weights = k, v, scales, weights
         self.block_table, self.dropped, self.window = block_table, dropped, window
         self.n_kv_heads, self.head_dim = k.shape[2], k.shape[4]
+        self._pages = _E4M3Pages.of(k, v, scales, block_table, weights, dropped)
+        self._address = ctypes.addressof(self._pages)
+        # how far entries are apart: keys, values, scales, weights
+        self.entry_strides = (k.stride(0), v.stride(0), scales.stride(0), weights.stride(0) if weights is not None else 0)
+
+    def address(self) -> int:
+        """Where entry 0's pointers and strides lie as the kernels take them."""
+        return self._address
 
     def entry(self, i: int) -> E4M3KVView:
         return E4M3KVView(self.k[i], self.v[i], self.scales[i], self.block_table, self.window,

@@ -893,17 +893,18 @@ GTG_API int gtg_kv_store_e4m3(int dtype, const void* qkv, int ld, const float* c
 }
 
 // lengths[b]: rows that the sequence in slots[b] holds.  kept: [entries][B][n_kv][budget].
-GTG_API int gtg_kv_evict_e4m3(int entries, void* k, long long k_entry, long long k_stride, void* v, long long v_entry, long long v_stride,
-                              float* scales, long long scale_entry, long long scale_stride, float* weights, long long weight_entry,
-                              long long weight_stride, const int* block_table, int table_stride, int* dropped, int n_kv, int hd, const int* slots,
-                              const int* lengths, int B, int max_length, int budget, int recent, int* kept, cudaStream_t stream) {
+GTG_API int gtg_kv_evict_e4m3(int entries, const E4M3Pages* first, long long k_entry, long long v_entry, long long scale_entry,
+                              long long weight_entry, const int* slots, const int* lengths, int B, int max_length, int budget, int recent,
+                              int* kept, cudaStream_t stream) {
     if (B <= 0 || entries <= 0) return 0;
-    if (budget <= 0 || recent < 0 || recent > budget || n_kv <= 0 || hd <= 0 || !weights || !kept) return kErrBadArgument;
+    E4M3Pages pages = *first;                                                   // of entry 0
+    int* dropped = const_cast<int*>(pages.dropped);
+    pages.dropped = nullptr;
+    const int n_kv = pages.n_kv, hd = pages.hd;
+    if (budget <= 0 || recent < 0 || recent > budget || n_kv <= 0 || hd <= 0 || !pages.weights || !kept) return kErrBadArgument;
     if (B > 65535 || entries > 65535) return kErrUnsupported;
     const size_t smem = (size_t)kPageTokens * hd;
     if (smem > 40 * 1024) return kErrUnsupported;
-    const E4M3Pages pages = {(uint8_t*)k, (uint8_t*)v, k_stride, v_stride, scales, scale_stride, weights, weight_stride, block_table, table_stride,
-                             nullptr, n_kv, hd};
     const EvictStrides strides = {k_entry, v_entry, scale_entry, weight_entry};
     // sequences whose weights fit in shared memory, heads of a multiple of 16 channels; else the general form
     if (hd % 16 == 0 && hd <= 128 && move_bytes(hd, max_length, budget) <= 200 * 1024) {

@@ -135,7 +135,7 @@ _SIGNATURES = {
     "gtg_attention_prefill_tcgen05": ("attention_tcgen05", [_P, _I, _I, _P, _I, _P, _P, _L, _I, _P, _I, _P, _P, _P,
                                                             _I, _I, _I, _I, _I, _F, _I, _I, _P, _F, _I, _P, _P]),
     "gtg_kv_store_e4m3": ("kv_e4m3", [_I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P, _I, _P]),
-    "gtg_kv_evict_e4m3": ("kv_e4m3", [_I, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _P, _P]),
+    "gtg_kv_evict_e4m3": ("kv_e4m3", [_I, _P, _L, _L, _L, _L, _P, _P, _I, _I, _I, _I, _P, _P]),
     "gtg_attention_e4m3_scratch_floats": ("attention_e4m3", [_I, _I, _I, _I, _I, _I, _I, _I, _L, _I, _I]),
     "gtg_attention_e4m3": ("attention_e4m3", [_I, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _L, _I, _I, _F, _I, _P, _P]),
     "gtg_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", [_P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _P, _P]),
@@ -1889,14 +1889,11 @@ def kv_evict_e4m3(storage, slots: torch.Tensor, lengths: torch.Tensor, max_lengt
     if n == 0:
         return kept
     _need_gpu(storage.k, "kv_evict_e4m3")
-    k, v, s, w = storage.k, storage.v, storage.scales, storage.weights
     if _checked:
         start = (lengths - 1).clamp(min=0)
         _check_access("kv_evict_e4m3", 2, storage.entry(0), slots, start_pos=start, cu_seqlens=torch.arange(n + 1, dtype=torch.int32, device=device))
-    _check(_fn("gtg_kv_evict_e4m3")(E, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), s.data_ptr(), s.stride(0),
-                                    s.stride(1), w.data_ptr(), w.stride(0), w.stride(1), storage.block_table.data_ptr(), storage.block_table.stride(0),
-                                    _ptr(storage.dropped), KV, storage.head_dim, slots.data_ptr(), lengths.data_ptr(), n, int(max_length), int(budget), int(recent),
-                                    kept.data_ptr(), _stream()), "kv_evict_e4m3")
+    _check(_fn("gtg_kv_evict_e4m3")(E, storage.address(), *storage.entry_strides, slots.data_ptr(), lengths.data_ptr(), n, int(max_length), int(budget),
+                                    int(recent), kept.data_ptr(), _stream()), "kv_evict_e4m3")
     return kept
 
 
