@@ -1,4 +1,4 @@
-// Attention of prompts and chunks over the 8-bit cache on the fifth-generation tensor cores: heads of 64 or 128 channels,
+// Attention of prompts and chunks over the 8-bit cache on the fifth-generation tensor cores: heads of up to 128 channels in steps of 16,
 // bfloat16 queries, causal, with an optional window.  (Layout and codes: e4m3.cuh.)
 //
 // One block per (two tiles of 128 query rows, key/value head, sequence).  A query row is a (token, head of the group) pair, heads
@@ -38,13 +38,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPShift = 7.0f, kMostSum = 32768.0f;
 constexpr int kMostApart = 96;                           // powers of two that a block's value scales span at most
 
+// HD: 64 or 128, what a tile has room for; heads of fewer channels (kExact false; multiples of 16) fill a part of it, and the products
+// take no more than that part.
 template <int HD> struct Shape {
     static constexpr int kQBytes = BQ * HD * 2, kTileBytes = BK * HD * 2;
     static constexpr int kOffK = 2 * kQBytes, kOffV = kOffK + 2 * kTileBytes, kOffBar = kOffV + 2 * kTileBytes;
     static constexpr int kSmemBytes = kOffBar + 256;
     static constexpr int kColO = BK, kColP = BK + HD;    // of a tile's tensor memory: S, O, two of P
     static_assert(BK + HD + BK <= kTileCols, "tensor memory");
-    static constexpr int kPieces = BK * HD / 16;         // of 16 codes in a step's keys (or values)
 };
 
 // kind::f16, half operands, both K-major, float sums.
@@ -154,12 +155,12 @@ __device__ __forceinline__ void warp_umma_commit(uint32_t bar) {
 }
 
 // grid: (kv heads, sequences, pairs of tiles of query rows), the longest first.
-template <int HD, bool kTest>
+template <int HD, bool kExact, bool kTest>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     using S = Shape<HD>;
     extern __shared__ __align__(1024) unsigned char smem[];
-    const int h = blockIdx.x, b = blockIdx.y;
+    const int h = blockIdx.x, b = blockIdx.y, hd = kExact ? HD : kv.hd;
     const int row_begin = (gridDim.z - 1 - blockIdx.z) * 2 * BQ;
     const int q_begin = a.cu_seqlens[b];
     const int q_len = a.cu_seqlens[b + 1] - q_begin;
@@ -246,12 +247,13 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     // ---- codes to halves: two warps the keys, two the values
     auto convert = [&](auto of_values, const int t) {
         constexpr bool values = decltype(of_values)::value;
-        constexpr int threads = 32 * (values ? kValueWarps : kKeyWarps), mine = (S::kPieces + threads - 1) / threads;
+        constexpr int threads = 32 * (values ? kValueWarps : kKeyWarps), mine = (BK * HD / 16 + threads - 1) / threads;
+        const int pieces = BK * hd / 16, row_pieces = hd / 16;   // of 16 codes in a step's keys (or values), in a key
         const int total = start + q_len;                         // rows that exist after this step
         // The codes come straight to registers, a step ahead of their use (through shared memory, several steps ahead, they
         // cost it the traffic that the products want).  Page numbers are read 32 steps at a time.
         int pages = 0;                                           // lane l: page of step (fetched / 32 * 32 + l)
-        const uint8_t* source = (values ? kv.v : kv.k) + (size_t)h * kPageTokens * HD + t * 16;
+        const uint8_t* source = (values ? kv.v : kv.k) + (size_t)h * kPageTokens * hd + t * 16;
         const long long stride = values ? kv.v_stride : kv.k_stride;
         uint4 u[mine];
         const float v_least = values ? least_value_scale() : 0.f;
@@ -261,7 +263,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             const uint8_t* at = source + (size_t)__shfl_sync(0xffffffffu, pages, i & 31) * stride;
 #pragma unroll
             for (int m = 0; m < mine; ++m)
-                if (t + threads * m < S::kPieces) u[m] = *reinterpret_cast<const uint4*>(at + threads * m * 16);
+                if (t + threads * m < pieces) u[m] = *reinterpret_cast<const uint4*>(at + threads * m * 16);
         };
         fetch(0);
         for (int i = 0; i < steps_last; ++i) {
@@ -282,7 +284,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                         found |= nan;
                         w[c] &= ~nan;
                     }
-                    if (found && t + threads * m < S::kPieces) *odd_flag = 1;
+                    if (found && t + threads * m < pieces) *odd_flag = 1;
                     u[m] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
@@ -299,9 +301,12 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
 #pragma unroll
             for (int m = 0; m < mine; ++m) {
                 const int id = t + threads * m;
-                if (id >= S::kPieces) continue;
+                if (id >= pieces) continue;
                 if (values) store_halves(tile + id / 4 * 128, id % 4 * 2, id / 4 & 7, u[m]);
-                else store_halves(tile + id % (HD / 16) / 4 * (BK * 128) + id / (HD / 16) * 128, id % 4 * 2, id / (HD / 16) & 7, u[m], id % (HD / 16) / 4);
+                else {
+                    const int row = id / row_pieces, piece = id - row * row_pieces;
+                    store_halves(tile + piece / 4 * (BK * 128) + row * 128, piece % 4 * 2, row & 7, u[m], piece / 4);
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
@@ -336,13 +341,13 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                 const uint64_t dk = k_desc + (uint64_t)((i & 1) * (S::kTileBytes >> 4));
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk)
-                    warp_umma_ss(tmem + t * kTileCols, dq + (kk / 4) * (BQ * 128 >> 4) + 2 * (kk % 4), dk + (kk / 4) * (BK * 128 >> 4) + 2 * (kk % 4), idesc,
+                    if (kExact || kk < hd / 16) warp_umma_ss(tmem + t * kTileCols, dq + (kk / 4) * (BQ * 128 >> 4) + 2 * (kk % 4), dk + (kk / 4) * (BK * 128 >> 4) + 2 * (kk % 4), idesc,
                                  kk > 0 ? 1u : 0u);
                 warp_umma_commit(s_full(t));
                 warp_umma_commit(k_free(i));
             }
         } else {
-            constexpr uint32_t idesc = f16_idesc(BQ, HD);
+            const uint32_t idesc = f16_idesc(BQ, hd);
             const uint64_t v_desc = umma_desc(base + S::kOffV);
             bool ok = true;
             for (int i = 0; i < steps_last && ok; ++i) {
@@ -374,12 +379,12 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
         const uint32_t tile_at = tmem + tt * kTileCols + ((uint32_t)((warp & 3) * 32) << 16);
         float factor;                                             // a raw score times this and the page's key scale: powers of two
         {
-            const bf16* src = a.q + (size_t)(q_begin + token) * a.ldq + (size_t)head * HD;
+            const bf16* src = a.q + (size_t)(q_begin + token) * a.ldq + (size_t)head * hd;
             uint4 u[HD / 8];
             float most = 0.f;
 #pragma unroll
             for (int c = 0; c < HD / 8; ++c) {
-                u[c] = real ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+                u[c] = real && (kExact || 8 * c < hd) ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0, 0, 0, 0);
                 const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -487,7 +492,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
 #pragma unroll 1
-                    for (int part = 0; part < HD / 8; ++part) {
+                    for (int part = 0; part < hd / 8; ++part) {
                         uint32_t ov[8];
                         tmem_ld8(tile_at + S::kColO + 8 * part, ov);
                         asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
@@ -519,27 +524,28 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
             const float inv = 1.0f / l_run, unit = __uint_as_float(__float_as_uint(v_least) + ((uint32_t)kMostApart << 23));    // 2^w
             if (a.stats && real) a.stats[(size_t)(q_begin + token) * a.n_heads + head] = make_float2(m_run == -INFINITY ? 0.f : m_run - (float)((int)(__float_as_uint(unit) >> 23) - 127) - kPShift, l_run);
-            bf16* dst = a.out + (size_t)(q_begin + token) * a.ldo + (size_t)head * HD;
+            bf16* dst = a.out + (size_t)(q_begin + token) * a.ldo + (size_t)head * hd;
             const bool odd = *odd_flag != 0;
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
+            for (int c = 0; 32 * c < hd; ++c) {
                 tmem_ld32(tile_at + S::kColO + 32 * c, sv);
                 asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
                 if (odd && real) {
                     // NaN codes of rows that this query sees, in pages where they were taken out
                     for (int j = j_lo; j < j_lo + n_steps; ++j) {
                         if (!page_not_whole(j)) continue;
-                        const uint8_t* vp = kv.v + (size_t)table[j] * kv.v_stride + ((size_t)h * HD + 32 * c) * kPageTokens;
+                        const uint8_t* vp = kv.v + (size_t)table[j] * kv.v_stride + ((size_t)h * hd + 32 * c) * kPageTokens;
                         const int lo = a.window > 0 ? max(0, pos - a.window + 1 - j * kPageTokens) : 0, hi = min(pos - j * kPageTokens, kPageTokens - 1);
                         for (int row = lo; row <= hi; ++row)
 #pragma unroll
                             for (int d = 0; d < 32; ++d)
-                                if ((vp[d * kPageTokens + row] & 0x7f) == 0x7f) sv[d] = 0x7fc00000u;
+                                if ((kExact || 32 * c + d < hd) && (vp[d * kPageTokens + row] & 0x7f) == 0x7f) sv[d] = 0x7fc00000u;
                     }
                 }
                 if (real) {
 #pragma unroll
                     for (int piece = 0; piece < 4; ++piece) {
+                        if (!kExact && 32 * c + 8 * piece >= hd) break;
                         uint32_t o4[4];
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
@@ -560,16 +566,16 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     }
 }
 
-template <int HD, bool kTest>
+template <int HD, bool kExact, bool kTest>
 int launch(const PromptArgs& a, const E4M3Pages& kv, int B, int max_q_len, cudaStream_t stream) {
     static bool configured = false;
     if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(attention_e4m3_prompt_kernel<HD, kTest>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::kSmemBytes);
+        const cudaError_t e = cudaFuncSetAttribute(attention_e4m3_prompt_kernel<HD, kExact, kTest>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::kSmemBytes);
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
     const long long rows = (long long)max_q_len * a.group;
-    return launch_chained(attention_e4m3_prompt_kernel<HD, kTest>, dim3(kv.n_kv, B, (unsigned)((rows + 2 * BQ - 1) / (2 * BQ))), dim3(kThreads),
+    return launch_chained(attention_e4m3_prompt_kernel<HD, kExact, kTest>, dim3(kv.n_kv, B, (unsigned)((rows + 2 * BQ - 1) / (2 * BQ))), dim3(kThreads),
                           (size_t)Shape<HD>::kSmemBytes, stream, a, kv);
 }
 // ============================================================== gathered weights of prompts and chunks
@@ -603,12 +609,12 @@ __device__ __forceinline__ void bf16_of_codes(uint32_t w, uint32_t& lo, uint32_t
 
 // parts: [sequence][query head][part_rows]; rows behind part_rows (a sequence that has outgrown the plan) are done for all heads
 // by the block of the group's first.
-template <int HD, bool kTest>
+template <int HD, bool kExact, bool kTest>
 __global__ void __launch_bounds__(kWeightThreads, 2)
 e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs a, const E4M3Pages kv, float* __restrict__ parts, int part_rows) {
     using S = WeightShape<HD>;
     extern __shared__ __align__(1024) unsigned char smem[];
-    const int h = blockIdx.y / a.group, g0 = blockIdx.y % a.group, b = blockIdx.z;
+    const int h = blockIdx.y / a.group, g0 = blockIdx.y % a.group, b = blockIdx.z, hd = kExact ? HD : kv.hd;
     const int q_begin = a.cu_seqlens[b];
     const int q_len = a.cu_seqlens[b + 1] - q_begin;
     const int slot = a.slots[b];
@@ -671,7 +677,7 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                     if (!ok) break;
                     mbar_expect_tx(q_full(s), S::kTileBytes);
                     for (int hh = 0; hh < HD / 64; ++hh)
-                        tma_load_2d<kTest>(base + S::kOffQ + s * S::kTileBytes + hh * (128 * 128), &map_q, (h * a.group + g0 + i / sp.per_head) * HD + 64 * hh,
+                        tma_load_2d<kTest>(base + S::kOffQ + s * S::kTileBytes + hh * (128 * 128), &map_q, (h * a.group + g0 + i / sp.per_head) * hd + 64 * hh,
                                            q_begin + sp.t_lo + i % sp.per_head * 128, q_full(s));
                 }
             }
@@ -692,7 +698,8 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                     asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
                     const uint32_t qbase = base + S::kOffQ + s * S::kTileBytes;
 #pragma unroll
-                    for (int kk = 0; kk < HD / 16; ++kk) {
+                    for (int kk = 0; kk < HD / 16; ++kk) {              // (a copy of a head's queries may hold the next one's behind them)
+                        if (!kExact && kk >= hd / 16) break;
                         const uint64_t dk = umma_desc(base + (kk / 4) * (128 * 128)) + 2 * (kk % 4);
                         const uint64_t dq = umma_desc(qbase + (kk / 4) * (128 * 128)) + 2 * (kk % 4);
                         umma_ss(tmem + 128 * buf, dk, dq, idesc, kk > 0 ? 1u : 0u);
@@ -721,11 +728,12 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
             // ---- the tile's keys (all products of the turn before are complete: this warp has seen the last one's barrier)
 #pragma unroll
             for (int m = 0; m < HD / 16; ++m) {
-                const int id = r + 128 * m, key = id / (HD / 16), piece = id % (HD / 16);
+                if (!kExact && m >= hd / 16) break;
+                const int id = r + 128 * m, key = id / (hd / 16), piece = id - key * (hd / 16);
                 const int j = kt * 2 + key / 64;
                 uint4 u = make_uint4(0, 0, 0, 0);
                 if (j * kPageTokens < start + q_len)
-                    u = *reinterpret_cast<const uint4*>(kv.k + (size_t)table[j] * kv.k_stride + ((size_t)h * kPageTokens + key % 64) * HD + piece * 16);
+                    u = *reinterpret_cast<const uint4*>(kv.k + (size_t)table[j] * kv.k_stride + ((size_t)h * kPageTokens + key % 64) * hd + piece * 16);
                 uint32_t o[8];
                 bf16_of_codes(u.x, o[0], o[1]);
                 bf16_of_codes(u.y, o[2], o[3]);
@@ -814,16 +822,16 @@ e4m3_weights_sum_kernel(const PromptArgs a, const E4M3Pages kv, const float* __r
     kv.weights[page * kv.weight_stride + (size_t)h * kPageTokens + row % kPageTokens] += sum;
 }
 
-template <int HD, bool kTest>
+template <int HD, bool kExact, bool kTest>
 int launch_weights(const PromptArgs& a, const E4M3Pages& kv, const CUtensorMap& map_q, int B, int max_kv_len, float* parts, cudaStream_t stream) {
     static bool configured = false;
     if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(e4m3_weights_kernel<HD, kTest>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightShape<HD>::kSmemBytes);
+        const cudaError_t e = cudaFuncSetAttribute(e4m3_weights_kernel<HD, kExact, kTest>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightShape<HD>::kSmemBytes);
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
     const int part_rows = (max_kv_len + 127) / 128 * 128;
-    const int st = launch_behind(e4m3_weights_kernel<HD, kTest>, dim3(part_rows / 128, a.n_heads, B), dim3(kWeightThreads),
+    const int st = launch_behind(e4m3_weights_kernel<HD, kExact, kTest>, dim3(part_rows / 128, a.n_heads, B), dim3(kWeightThreads),
                                   (size_t)WeightShape<HD>::kSmemBytes, stream, map_q, a, kv, parts, part_rows);
     if (st != 0) return st;
     return launch_behind(e4m3_weights_sum_kernel, dim3((part_rows + 255) / 256, kv.n_kv, B), dim3(256), 0, stream, a, kv, (const float*)parts, part_rows);
@@ -847,7 +855,7 @@ GTG_API int gtg_attention_e4m3_tcgen05(const void* q, int ldq, void* out, int ld
     float* weights = kv.weights;
     if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || window < 0 || max_kv_len <= 0 || (weights && !scratch)) return kErrBadArgument;
     if (n_heads > 65535) return kErrUnsupported;
-    if ((hd != 64 && hd != 128) || ldq % 8 || ldo % 8 || (uintptr_t)q % 16 || (uintptr_t)out % 16) return kErrUnsupported;
+    if (hd % 16 || hd > 128 || ldq % 8 || ldo % 8 || (uintptr_t)q % 16 || (uintptr_t)out % 16) return kErrUnsupported;
     if (B > 65535 || ((long long)max_q_len * (n_heads / n_kv) + BQ - 1) / BQ > 65535) return kErrUnsupported;
     PromptArgs a = {};
     a.q = (const bf16*)q; a.ldq = ldq; a.out = (bf16*)out; a.ldo = ldo;
@@ -856,14 +864,17 @@ GTG_API int gtg_attention_e4m3_tcgen05(const void* q, int ldq, void* out, int ld
     a.stats = weights ? (float2*)scratch : nullptr;
     float* parts = scratch + (weights ? 2 * (size_t)N * n_heads : 0);
     const bool test = g_test_waits;
-    const int st = hd == 64 ? (test ? launch<64, true>(a, kv, B, max_q_len, stream) : launch<64, false>(a, kv, B, max_q_len, stream))
-                            : (test ? launch<128, true>(a, kv, B, max_q_len, stream) : launch<128, false>(a, kv, B, max_q_len, stream));
+#define GTG_LAUNCH(WHAT, HD, EXACT, ...) (test ? WHAT<HD, EXACT, true>(__VA_ARGS__) : WHAT<HD, EXACT, false>(__VA_ARGS__))
+#define GTG_BY_SIZE(WHAT, ...) (hd == 64 ? GTG_LAUNCH(WHAT, 64, true, __VA_ARGS__) : hd == 128 ? GTG_LAUNCH(WHAT, 128, true, __VA_ARGS__) \
+                                : hd < 64 ? GTG_LAUNCH(WHAT, 64, false, __VA_ARGS__) : GTG_LAUNCH(WHAT, 128, false, __VA_ARGS__))
+    const int st = GTG_BY_SIZE(launch, a, kv, B, max_q_len, stream);
     if (st != 0 || !weights) return st;
     CUtensorMap map_q;
     const int mt = make_map(&map_q, q, N, n_heads * hd, ldq, 128);
     if (mt != 0) return mt;
-    return hd == 64 ? (test ? launch_weights<64, true>(a, kv, map_q, B, max_kv_len, parts, stream) : launch_weights<64, false>(a, kv, map_q, B, max_kv_len, parts, stream))
-                    : (test ? launch_weights<128, true>(a, kv, map_q, B, max_kv_len, parts, stream) : launch_weights<128, false>(a, kv, map_q, B, max_kv_len, parts, stream));
+    return GTG_BY_SIZE(launch_weights, a, kv, map_q, B, max_kv_len, parts, stream);
+#undef GTG_BY_SIZE
+#undef GTG_LAUNCH
 }
 
 // For the test of the give-up path: while set, launches take the kTest form, in which the conversion's warps never say that a

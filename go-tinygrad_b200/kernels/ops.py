@@ -1779,7 +1779,7 @@ E4M3_FEW_QUERIES = 32         # tokens of a step times the heads of a group, up 
 
 def _e4m3_prompt_form(dt: int, max_q_len: int, n_heads: int, n_kv: int, hd: int) -> bool:
     """Whether the tcgen05 form serves (if rows of q and out also start on 16-byte boundaries)."""
-    return dt == 1 and (hd == 64 or hd == 128) and max_q_len * (n_heads // n_kv) > E4M3_FEW_QUERIES
+    return dt == 1 and hd % 16 == 0 and hd <= 128 and max_q_len * (n_heads // n_kv) > E4M3_FEW_QUERIES
 
 
 def _e4m3_prompt_scratch(n_seqs: int, n_tokens: int, n_heads: int, kv, max_kv_len: int) -> int:
