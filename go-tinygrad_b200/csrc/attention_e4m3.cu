@@ -5,7 +5,7 @@
 // the query heads of its key/value head.
 //
 //   few_queries:      bfloat16, heads of up to 128 channels in steps of 16, few queries a sequence (attention_e4m3_few.cuh);
-//   attention_rows:   any head size and type, one block per (token, query head); scores, softmax and sums in float.
+//   attention_rows:   any head size and type, a block or several per (token, query head); scores, softmax and sums in float.
 //   row_weights:      the weights, once every row's maximum and sum are known: a block per (cache page, head, sequence).
 #include "attention_e4m3_few.cuh"
 
@@ -16,12 +16,13 @@ constexpr int kRowThreads = 128;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kMaxChannels = 256;
 
-// 32 rows at a time a warp: a lane scores one row and then adds up the channels lane, lane + 32, ... of all 32.
+// 32 rows at a time a warp: a lane scores one row and then adds up the channels lane, lane + 32, ... of all 32.  Few tokens over
+// long sequences are cut into `splits` blocks each, whose parts (maximum, sum, outputs) rows_join_kernel joins in their order.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
 attention_rows_kernel(const T* __restrict__ q, int ldq, T* __restrict__ out, int ldo, const E4M3Pages kv, const int* __restrict__ cu_seqlens,
                       const int* __restrict__ slots, const int* __restrict__ start_pos, int B, int n_heads, float scale, int window,
-                      float2* __restrict__ stats) {
+                      float2* __restrict__ stats, float* __restrict__ parts) {
     chain_release();
     chain_wait();
     __shared__ float qs[kMaxChannels];
@@ -45,7 +46,7 @@ attention_rows_kernel(const T* __restrict__ q, int ldq, T* __restrict__ out, int
     float o[kMaxChannels / 32];
 #pragma unroll
     for (int i = 0; i < kMaxChannels / 32; ++i) o[i] = 0.f;
-    for (int c = first / 32 + warp; c * 32 <= row; c += kRowWarps) {
+    for (int c = first / 32 + blockIdx.z * kRowWarps + warp; c * 32 <= row; c += kRowWarps * gridDim.z) {
         const size_t page = table[c / (kPageTokens / 32)];
         const int t0 = c % (kPageTokens / 32) * 32, t = t0 + lane, j = c * 32 + lane;
         const float k_scale = kv.scales[page * kv.scale_stride + h], v_scale = kv.scales[page * kv.scale_stride + kv.n_kv + h];
@@ -115,12 +116,36 @@ attention_rows_kernel(const T* __restrict__ q, int ldq, T* __restrict__ out, int
     const float M_use = M == -INFINITY ? 0.f : M;
     float f[kRowWarps], L = 0.f;
     for (int w = 0; w < kRowWarps; ++w) { f[w] = expf(wm[w] - M_use); L += f[w] * wl[w]; }
+    float* part = gridDim.z > 1 ? parts + (((size_t)token * n_heads + head) * gridDim.z + blockIdx.z) * (hd + 2) : nullptr;
+    if (part && tid == 0) { part[0] = M; part[1] = L; }
     for (int d = tid; d < hd; d += kRowThreads) {
         float acc = 0.f;
         for (int w = 0; w < kRowWarps; ++w) acc += f[w] * wo[w][d];
+        if (part) part[2 + d] = acc;
+        else out[(size_t)token * ldo + head * hd + d] = from_f32<T>(acc / L);
+    }
+    if (stats && !part && tid == 0) stats[(size_t)token * n_heads + head] = make_float2(M_use * kLog2e, L);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads)
+rows_join_kernel(const float* __restrict__ parts, int splits, T* __restrict__ out, int ldo, const int* __restrict__ cu_seqlens, int B, int n_heads,
+                 int hd, float2* __restrict__ stats) {
+    chain_release();
+    chain_wait();
+    const int token = blockIdx.x, head = blockIdx.y;
+    if (token < cu_seqlens[0] || token >= cu_seqlens[B]) return;
+    const float* part = parts + ((size_t)token * n_heads + head) * splits * (hd + 2);
+    float M = -INFINITY, L = 0.f;
+    for (int s = 0; s < splits; ++s) M = fmaxf(M, part[(size_t)s * (hd + 2)]);
+    const float M_use = M == -INFINITY ? 0.f : M;
+    for (int s = 0; s < splits; ++s) L += expf(part[(size_t)s * (hd + 2)] - M_use) * part[(size_t)s * (hd + 2) + 1];
+    for (int d = threadIdx.x; d < hd; d += kRowThreads) {
+        float acc = 0.f;
+        for (int s = 0; s < splits; ++s) acc += expf(part[(size_t)s * (hd + 2)] - M_use) * part[(size_t)s * (hd + 2) + 2 + d];
         out[(size_t)token * ldo + head * hd + d] = from_f32<T>(acc / L);
     }
-    if (stats && tid == 0) stats[(size_t)token * n_heads + head] = make_float2(M_use * kLog2e, L);
+    if (stats && threadIdx.x == 0) stats[(size_t)token * n_heads + head] = make_float2(M_use * kLog2e, L);
 }
 
 // A block per (page of the sequence, key/value head, sequence): 64 rows by two halves of the (query, head) pairs that may
@@ -189,12 +214,27 @@ int launch_row_weights(const void* q, int ldq, const E4M3Pages& kv, const int* c
                           (const T*)q, ldq, kv, cu_seqlens, slots, start_pos, n_heads, scale, window, stats);
 }
 
+// Blocks a (token, query head) has: as many as make four a multiprocessor, of 512 rows and more (float, 8 heads of 64 over 16,000 rows:
+// 20 us where one block each took 194; over 1,100: 14.2 and 17.8).
+int rows_splits(int N, int n_heads, int max_kv_len, int window) {
+    const long long seen = window > 0 ? std::min(window, max_kv_len) : max_kv_len;
+    return (int)std::max(1LL, std::min(4LL * 148 / ((long long)N * n_heads), seen / 512));
+}
+long long rows_floats(int N, int n_heads, int hd, int splits, bool weigh) {
+    return (weigh ? 2LL * N * n_heads : 0) + (splits > 1 ? (long long)N * n_heads * splits * (hd + 2) : 0);
+}
+
 template <typename T>
 int launch_rows(const void* q, int ldq, void* out, int ldo, const E4M3Pages& kv, const int* cu_seqlens, const int* slots, const int* start_pos,
                 int B, int max_kv_len, int N, int n_heads, float scale, int window, float* scratch, cudaStream_t stream) {
     float2* stats = kv.weights ? (float2*)scratch : nullptr;
-    const int st = launch_chained(attention_rows_kernel<T>, dim3(N, n_heads), dim3(kRowThreads), 0, stream, (const T*)q, ldq, (T*)out, ldo, kv,
-                                  cu_seqlens, slots, start_pos, B, n_heads, scale, window, stats);
+    const int splits = rows_splits(N, n_heads, max_kv_len, window);
+    float* parts = splits > 1 ? scratch + (kv.weights ? 2LL * N * n_heads : 0) : nullptr;
+    int st = launch_chained(attention_rows_kernel<T>, dim3(N, n_heads, splits), dim3(kRowThreads), 0, stream, (const T*)q, ldq, (T*)out, ldo, kv,
+                            cu_seqlens, slots, start_pos, B, n_heads, scale, window, stats, parts);
+    if (st == 0 && splits > 1)
+        st = launch_behind(rows_join_kernel<T>, dim3(N, n_heads), dim3(kRowThreads), 0, stream, (const float*)parts, splits, (T*)out, ldo, cu_seqlens, B,
+                           n_heads, kv.hd, stats);
     if (st != 0 || !kv.weights) return st;
     return launch_row_weights<T>(q, ldq, kv, cu_seqlens, slots, start_pos, B, max_kv_len, n_heads, scale, window, stats, stream);
 }
@@ -209,9 +249,9 @@ static FewPlan few_plan(int B, int max_q_len, int n_heads, int n_kv, int hd, int
 // Floats of scratch that gtg_attention_e4m3 needs for the same numbers.
 GTG_API long long gtg_attention_e4m3_scratch_floats(int dtype, int B, int N, int max_q_len, int n_heads, int n_kv, int hd, int max_kv_len,
                                                     long long total_kv_len, int window, int weigh) {
-    (void)total_kv_len; (void)window;
+    (void)total_kv_len;
     if (B <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || max_q_len <= 0 || max_kv_len <= 0) return 0;
-    const long long rows = weigh ? 2LL * N * n_heads : 0;
+    const long long rows = rows_floats(N, n_heads, hd, rows_splits(std::max(N, 1), n_heads, max_kv_len, window), weigh != 0);
     if (few_takes(dtype, max_q_len, n_heads, n_kv, hd))
         return std::max(few_plan(B, max_q_len, n_heads, n_kv, hd, max_kv_len, weigh).floats(), rows);
     return rows;
@@ -239,7 +279,7 @@ GTG_API int gtg_attention_e4m3(int dtype, const void* q, int ldq, void* out, int
         switch (hd) { GTG_FEW(16) GTG_FEW(32) GTG_FEW(48) GTG_FEW(64) GTG_FEW(80) GTG_FEW(96) GTG_FEW(112) GTG_FEW(128) }
 #undef GTG_FEW
     }
-    if (weights && !scratch) return kErrBadArgument;
+    if (rows_floats(N, n_heads, hd, rows_splits(N, n_heads, max_kv_len, window), weights != nullptr) && !scratch) return kErrBadArgument;
     if (dtype == 0) return launch_rows<float>(q, ldq, out, ldo, kv, cu_seqlens, slots, start_pos, B, max_kv_len, N, n_heads, scale, window, scratch, stream);
     return launch_rows<bf16>(q, ldq, out, ldo, kv, cu_seqlens, slots, start_pos, B, max_kv_len, N, n_heads, scale, window, scratch, stream);
 }

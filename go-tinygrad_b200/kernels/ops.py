@@ -1800,10 +1800,12 @@ def attention_e4m3_scratch_floats(dtype: torch.dtype, n_seqs: int, n_tokens: int
                                   total_kv_len: int = 0, window: Optional[int] = None) -> int:
     """Floats of scratch `attention_e4m3` needs for the same arguments (0: none)."""
     window = kv.window if window is None else window
+    prompt = 0
     if _e4m3_prompt_form(0 if dtype == torch.float32 else 1, max_q_len, n_heads, kv.n_kv_heads, kv.head_dim):
-        return _e4m3_prompt_scratch(n_seqs, n_tokens, n_heads, kv, int(max_kv_len))
-    return _e4m3_few_scratch(kv.k.get_device(), 0 if dtype == torch.float32 else 1, n_seqs, n_tokens, int(max_q_len), n_heads,
-                             kv.n_kv_heads, kv.head_dim, int(max_kv_len), int(total_kv_len), int(window or 0), 1 if kv.weights is not None else 0)
+        prompt = _e4m3_prompt_scratch(n_seqs, n_tokens, n_heads, kv, int(max_kv_len))     # if its rows allow it; else what follows
+    return max(prompt, _e4m3_few_scratch(kv.k.get_device(), 0 if dtype == torch.float32 else 1, n_seqs, n_tokens, int(max_q_len), n_heads,
+                                         kv.n_kv_heads, kv.head_dim, int(max_kv_len), int(total_kv_len), int(window or 0),
+                                         1 if kv.weights is not None else 0))
 
 
 def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Tensor, slots: torch.Tensor, start_pos: torch.Tensor, max_q_len: int,
@@ -1837,7 +1839,9 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
     if N == 0 or B == 0:
         return
     _need_gpu(q, "attention_e4m3")
-    prompt = _e4m3_prompt_form(dt, max_q_len, n_heads, kv.n_kv_heads, hd)
+    # (the tcgen05 form copies rows of q by their 16 bytes)
+    prompt = (_e4m3_prompt_form(dt, max_q_len, n_heads, kv.n_kv_heads, hd)
+              and not (q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16))
     if prompt:
         need = _e4m3_prompt_scratch(B, N, n_heads, kv, int(max_kv_len))
     else:
@@ -1849,7 +1853,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
         elif (scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < need or scratch.data_ptr() % 16
               or scratch.device != q.device):
             raise KernelError(f"attention_e4m3: scratch needs {need} contiguous floats on a 16-byte boundary of the cache's device")
-    if prompt and not (q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16):
+    if prompt:
         _check(_fn("gtg_attention_e4m3_tcgen05")(q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv.address(), cu_seqlens.data_ptr(),
                                                  slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), N, n_heads, float(scale),
                                                  int(window or 0), scratch.data_ptr() if need else None, _stream()), "attention_e4m3")
