@@ -15,6 +15,7 @@
 // largest v of the block's pages, and O 2^w / l the result.  Where v_j is so far below w that P_j could be 0 while its probability is
 // not (a block of zeros among others, for one), v_j counts as w - 96 and the codes are made smaller for it.
 // M is raised only when a step's sum of P exceeds 2^15, so P, times 2^7 besides, stays below half's largest number.
+// Where that makes fewer blocks than multiprocessors, several share a pair of tiles' pages and leave their results to a joining kernel.
 // What bounds it is the softmax: its exponentials alone are 1,024 cycles of the 2,500 that a step of both tiles takes, its wait for
 // scores 400 to 540, their products 800.  Measured on a B200: 2,048 tokens, 32 heads of 64: 56 us; 512 tokens behind 7,680,
 // 2 sequences, 8 kv heads of 128 under 32: 165 us, 0.83 of what the same kernel for a bfloat16 cache takes in the second case and
@@ -33,6 +34,7 @@ constexpr int BK = kPageTokens;                          // rows of the cache a 
 // saw every answer hundreds of cycles late: 3,600 cycles a page where the softmax takes 1,900.
 constexpr int kKeyWarps = 2, kValueWarps = 2, kScoreWarp = 12, kOutputWarp = 14;
 constexpr int kThreads = 512;
+constexpr int kLeastSteps = 8;                           // of a block, where several share a tile pair's
 constexpr int kTmemCols = 512, kTileCols = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPShift = 7.0f, kMostSum = 32768.0f;
@@ -63,6 +65,9 @@ struct PromptArgs {
     float scale;
     int window;
     float2* stats;               // [token][head]: what a score (in powers of two) is compared with, and the sum; or null
+    int splits;                  // blocks that share a tile pair's pages
+    float* part_o;               // [token][head][split][channel]: their results, where there are several,
+    float2* part_stats;          // [token][head][split]: and statistics; a sum of 0 where the split saw no row
 };
 
 __device__ __forceinline__ void store_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -161,7 +166,8 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     using S = Shape<HD>;
     extern __shared__ __align__(1024) unsigned char smem[];
     const int h = blockIdx.x, b = blockIdx.y, hd = kExact ? HD : kv.hd;
-    const int row_begin = (gridDim.z - 1 - blockIdx.z) * 2 * BQ;
+    const int place = gridDim.z - 1 - blockIdx.z, split = place % a.splits;
+    const int row_begin = place / a.splits * 2 * BQ;
     const int q_begin = a.cu_seqlens[b];
     const int q_len = a.cu_seqlens[b + 1] - q_begin;
     const int n_rows = q_len * a.group;
@@ -195,9 +201,23 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     const int n_tiles = n_rows - row_begin > BQ ? 2 : 1;
     const int first_at = start + row_begin / a.group;            // cache row of the block's first query, and of its last
     const int last_at = start + (min(row_begin + 2 * BQ, n_rows) - 1) / a.group;
-    const int j_lo = (a.window > 0 ? max(0, first_at - a.window + 1) : 0) / kPageTokens;
-    const int steps_last = last_at / kPageTokens - j_lo + 1;     // of the last tile; an earlier one may see less
-    const int steps_first = n_tiles == 2 ? (start + (row_begin + BQ - 1) / a.group) / kPageTokens - j_lo + 1 : steps_last;
+    int j_lo = (a.window > 0 ? max(0, first_at - a.window + 1) : 0) / kPageTokens;
+    int steps_last = last_at / kPageTokens - j_lo + 1;           // of the last tile; an earlier one may see less
+    int steps_first = n_tiles == 2 ? (start + (row_begin + BQ - 1) / a.group) / kPageTokens - j_lo + 1 : steps_last;
+    if (a.splits > 1) {                                          // this block's share of them
+        const int share = max(kLeastSteps, (steps_last + a.splits - 1) / a.splits);
+        j_lo += split * share;
+        steps_first = min(max(steps_first - split * share, 0), share);
+        steps_last = min(steps_last - split * share, share);
+        if (steps_last <= 0) {                                   // nothing left for it
+            chain_wait();
+            if (threadIdx.x < 2 * BQ && row_begin + (int)threadIdx.x < n_rows) {
+                const int row = row_begin + threadIdx.x;
+                a.part_stats[((size_t)(q_begin + row / a.group) * a.n_heads + h * a.group + row % a.group) * a.splits + split] = make_float2(0.f, 0.f);
+            }
+            return;
+        }
+    }
     auto page_not_whole = [&](int j) {                           // a page that not every query of the block sees whole
         return j * kPageTokens + kPageTokens - 1 > first_at || (a.window > 0 && j * kPageTokens <= last_at - a.window);
     };
@@ -519,15 +539,20 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full(tt, i));
         }
-        if (ok) ok = all_wait(pv_done(tt, n_steps - 1), phase(n_steps - 1));
+        if (ok && n_steps > 0) ok = all_wait(pv_done(tt, n_steps - 1), phase(n_steps - 1));
         if (ok) {
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
             const float inv = 1.0f / l_run, unit = __uint_as_float(__float_as_uint(v_least) + ((uint32_t)kMostApart << 23));    // 2^w
-            if (a.stats && real) a.stats[(size_t)(q_begin + token) * a.n_heads + head] = make_float2(m_run == -INFINITY ? 0.f : m_run - (float)((int)(__float_as_uint(unit) >> 23) - 127) - kPShift, l_run);
+            const float2 stat = make_float2(m_run == -INFINITY ? 0.f : m_run - (float)((int)(__float_as_uint(unit) >> 23) - 127) - kPShift, l_run);
+            const size_t at = (size_t)(q_begin + token) * a.n_heads + head;
+            const bool in_parts = a.splits > 1;
+            if (real && in_parts) a.part_stats[at * a.splits + split] = stat;
+            else if (real && a.stats) a.stats[at] = stat;
+            float* part = in_parts ? a.part_o + (at * a.splits + split) * hd : nullptr;
             bf16* dst = a.out + (size_t)(q_begin + token) * a.ldo + (size_t)head * hd;
             const bool odd = *odd_flag != 0;
 #pragma unroll 1
-            for (int c = 0; 32 * c < hd; ++c) {
+            for (int c = 0; 32 * c < hd && n_steps > 0; ++c) {
                 tmem_ld32(tile_at + S::kColO + 32 * c, sv);
                 asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
                 if (odd && real) {
@@ -542,7 +567,16 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                                 if ((kExact || 32 * c + d < hd) && (vp[d * kPageTokens + row] & 0x7f) == 0x7f) sv[d] = 0x7fc00000u;
                     }
                 }
-                if (real) {
+                if (real && in_parts) {
+#pragma unroll
+                    for (int piece = 0; piece < 8; ++piece) {
+                        if (!kExact && 32 * c + 4 * piece >= hd) break;
+                        float o4[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o4[x] = __uint_as_float(sv[4 * piece + x]) * inv * unit;
+                        *reinterpret_cast<float4*>(part + 32 * c + 4 * piece) = make_float4(o4[0], o4[1], o4[2], o4[3]);
+                    }
+                } else if (real) {
 #pragma unroll
                     for (int piece = 0; piece < 4; ++piece) {
                         if (!kExact && 32 * c + 8 * piece >= hd) break;
@@ -566,6 +600,39 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     }
 }
 
+// Joins the blocks that shared a tile pair's pages: their results, each with the mass 2^x l that its statistics say.
+__global__ void __launch_bounds__(256)
+e4m3_prompt_join_kernel(const PromptArgs a, int B, int N, int hd) {
+    chain_release();
+    chain_wait();
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int lanes = hd / 4, d = (int)(id % lanes) * 4;         // four channels a thread
+    const long long row = id / lanes;
+    const int token = (int)(row / a.n_heads), head = (int)(row % a.n_heads);
+    if (token >= N || token < a.cu_seqlens[0] || token >= a.cu_seqlens[B]) return;
+    const float2* stats = a.part_stats + row * a.splits;
+    const float* o = a.part_o + row * a.splits * hd + d;
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; ++s)
+        if (stats[s].y != 0.f) top = fmaxf(top, stats[s].x + log2f(stats[s].y));
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float mass = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 st = stats[s];
+        const float4 v = *reinterpret_cast<const float4*>(o + (size_t)s * hd);
+        if (st.y == 0.f) continue;
+        const float f = fast_exp2(st.x + log2f(st.y) - top);
+        mass += f;
+        acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+    }
+    const float inv = 1.0f / mass;
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(a.out + (size_t)token * a.ldo + (size_t)head * hd + d) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    if (a.stats && d == 0) a.stats[row] = make_float2(top, mass);
+}
+
 template <int HD, bool kExact, bool kTest>
 int launch(const PromptArgs& a, const E4M3Pages& kv, int B, int max_q_len, cudaStream_t stream) {
     static bool configured = false;
@@ -575,7 +642,7 @@ int launch(const PromptArgs& a, const E4M3Pages& kv, int B, int max_q_len, cudaS
         configured = true;
     }
     const long long rows = (long long)max_q_len * a.group;
-    return launch_chained(attention_e4m3_prompt_kernel<HD, kExact, kTest>, dim3(kv.n_kv, B, (unsigned)((rows + 2 * BQ - 1) / (2 * BQ))), dim3(kThreads),
+    return launch_chained(attention_e4m3_prompt_kernel<HD, kExact, kTest>, dim3(kv.n_kv, B, (unsigned)((rows + 2 * BQ - 1) / (2 * BQ) * a.splits)), dim3(kThreads),
                           (size_t)Shape<HD>::kSmemBytes, stream, a, kv);
 }
 // ============================================================== gathered weights of prompts and chunks
@@ -848,26 +915,33 @@ GTG_API int gtg_attention_e4m3_tcgen05_status() {
 // scratch for that: 2 N n_heads floats and n_heads B times max_kv_len rounded up to 128.
 GTG_API int gtg_attention_e4m3_tcgen05(const void* q, int ldq, void* out, int ldo, const E4M3Pages* pages, const int* cu_seqlens,
                                        const int* slots, const int* start_pos, int B, int max_q_len, int max_kv_len, int N, int n_heads,
-                                       float scale, int window, float* scratch, cudaStream_t stream) {
+                                       float scale, int window, int splits, float* scratch, cudaStream_t stream) {
     if (B <= 0 || max_q_len <= 0 || N <= 0) return 0;
     const E4M3Pages kv = *pages;
     const int n_kv = kv.n_kv, hd = kv.hd;
     float* weights = kv.weights;
-    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || window < 0 || max_kv_len <= 0 || (weights && !scratch)) return kErrBadArgument;
+    if (n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || window < 0 || max_kv_len <= 0 || splits < 1 || ((weights || splits > 1) && !scratch)) return kErrBadArgument;
     if (n_heads > 65535) return kErrUnsupported;
     if (hd % 16 || hd > 128 || ldq % 8 || ldo % 8 || (uintptr_t)q % 16 || (uintptr_t)out % 16) return kErrUnsupported;
-    if (B > 65535 || ((long long)max_q_len * (n_heads / n_kv) + BQ - 1) / BQ > 65535) return kErrUnsupported;
+    if (B > 65535 || ((long long)max_q_len * (n_heads / n_kv) + BQ - 1) / BQ > 65535 / splits) return kErrUnsupported;
     PromptArgs a = {};
     a.q = (const bf16*)q; a.ldq = ldq; a.out = (bf16*)out; a.ldo = ldo;
     a.cu_seqlens = cu_seqlens; a.slots = slots; a.start_pos = start_pos;
     a.n_heads = n_heads; a.group = n_heads / n_kv; a.scale = scale; a.window = window;
-    a.stats = weights ? (float2*)scratch : nullptr;
-    float* parts = scratch + (weights ? 2 * (size_t)N * n_heads : 0);
+    // scratch: results and statistics of splits, statistics, weights by head
+    const size_t rows = (size_t)N * n_heads;
+    a.splits = splits;
+    a.part_o = scratch;
+    a.part_stats = (float2*)(scratch + (splits > 1 ? rows * splits * hd : 0));
+    a.stats = weights ? a.part_stats + (splits > 1 ? rows * splits : 0) : nullptr;
+    float* parts = weights ? (float*)(a.stats + rows) : nullptr;
     const bool test = g_test_waits;
 #define GTG_LAUNCH(WHAT, HD, EXACT, ...) (test ? WHAT<HD, EXACT, true>(__VA_ARGS__) : WHAT<HD, EXACT, false>(__VA_ARGS__))
 #define GTG_BY_SIZE(WHAT, ...) (hd == 64 ? GTG_LAUNCH(WHAT, 64, true, __VA_ARGS__) : hd == 128 ? GTG_LAUNCH(WHAT, 128, true, __VA_ARGS__) \
                                 : hd < 64 ? GTG_LAUNCH(WHAT, 64, false, __VA_ARGS__) : GTG_LAUNCH(WHAT, 128, false, __VA_ARGS__))
-    const int st = GTG_BY_SIZE(launch, a, kv, B, max_q_len, stream);
+    int st = GTG_BY_SIZE(launch, a, kv, B, max_q_len, stream);
+    if (st == 0 && splits > 1)
+        st = launch_behind(e4m3_prompt_join_kernel, dim3((unsigned)((rows * (hd / 4) + 255) / 256)), dim3(256), 0, stream, a, B, N, hd);
     if (st != 0 || !weights) return st;
     CUtensorMap map_q;
     const int mt = make_map(&map_q, q, N, n_heads * hd, ldq, 128);

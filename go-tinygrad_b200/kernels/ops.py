@@ -138,7 +138,7 @@ _SIGNATURES = {
     "gtg_kv_evict_e4m3": ("kv_e4m3", [_I, _P, _L, _L, _L, _L, _P, _P, _I, _I, _I, _I, _P, _P]),
     "gtg_attention_e4m3_scratch_floats": ("attention_e4m3", [_I, _I, _I, _I, _I, _I, _I, _I, _L, _I, _I]),
     "gtg_attention_e4m3": ("attention_e4m3", [_I, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _L, _I, _I, _F, _I, _P, _P]),
-    "gtg_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", [_P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _P, _P]),
+    "gtg_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", [_P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P]),
     "gtg_attention_e4m3_tcgen05_status": ("attention_e4m3_tcgen05", []),
     "gtg_attention_e4m3_tcgen05_test_hooks": ("attention_e4m3_tcgen05", [_I]),
     "gtg_argmax": ("sampling", [_P, _I, _I, _I, _P, _P]),
@@ -1782,11 +1782,21 @@ def _e4m3_prompt_form(dt: int, max_q_len: int, n_heads: int, n_kv: int, hd: int)
     return dt == 1 and hd % 16 == 0 and hd <= 128 and max_q_len * (n_heads // n_kv) > E4M3_FEW_QUERIES
 
 
-def _e4m3_prompt_scratch(n_seqs: int, n_tokens: int, n_heads: int, kv, max_kv_len: int) -> int:
-    """Statistics a query, and the weights of each head's block, which are added up in the heads' order."""
+def _e4m3_prompt_splits(n_seqs: int, max_q_len: int, n_heads: int, n_kv: int, max_kv_len: int, window: int) -> int:
+    """Blocks that share the pages of 256 query rows: what fills the multiprocessors, each with 8 pages or more.  (32 heads over 8 key
+    heads: 512 tokens of 128 channels behind 7,680 take 104 us with two, 168 with one; 64 tokens of 64 behind 15,000 47 and 274.)"""
+    blocks = n_seqs * n_kv * ((max_q_len * (n_heads // n_kv) + 255) // 256)
+    pages = (min(max_kv_len, window + max_q_len) if window else max_kv_len) // 64
+    return max(1, min(148 // max(blocks, 1), pages // 8, 32))
+
+
+def _e4m3_prompt_scratch(n_seqs: int, n_tokens: int, n_heads: int, kv, max_kv_len: int, splits: int) -> int:
+    """Results and statistics of the blocks that share pages; where weights are gathered, statistics a query, and the weights of
+    each head's block, which are added up in the heads' order."""
+    parts = n_heads * n_tokens * splits * (kv.head_dim + 2) if splits > 1 else 0
     if kv.weights is None:
-        return 0
-    return n_heads * (2 * n_tokens + n_seqs * ((max_kv_len + 127) // 128 * 128))
+        return parts
+    return parts + n_heads * (2 * n_tokens + n_seqs * ((max_kv_len + 127) // 128 * 128))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1802,7 +1812,8 @@ def attention_e4m3_scratch_floats(dtype: torch.dtype, n_seqs: int, n_tokens: int
     window = kv.window if window is None else window
     prompt = 0
     if _e4m3_prompt_form(0 if dtype == torch.float32 else 1, max_q_len, n_heads, kv.n_kv_heads, kv.head_dim):
-        prompt = _e4m3_prompt_scratch(n_seqs, n_tokens, n_heads, kv, int(max_kv_len))     # if its rows allow it; else what follows
+        splits = _e4m3_prompt_splits(n_seqs, int(max_q_len), n_heads, kv.n_kv_heads, int(max_kv_len), int(window or 0))
+        prompt = _e4m3_prompt_scratch(n_seqs, n_tokens, n_heads, kv, int(max_kv_len), splits)         # if its rows allow it; else what follows
     return max(prompt, _e4m3_few_scratch(kv.k.get_device(), 0 if dtype == torch.float32 else 1, n_seqs, n_tokens, int(max_q_len), n_heads,
                                          kv.n_kv_heads, kv.head_dim, int(max_kv_len), int(total_kv_len), int(window or 0),
                                          1 if kv.weights is not None else 0))
@@ -1843,7 +1854,8 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
     prompt = (_e4m3_prompt_form(dt, max_q_len, n_heads, kv.n_kv_heads, hd)
               and not (q.stride(0) % 8 or out.stride(0) % 8 or q.data_ptr() % 16 or out.data_ptr() % 16))
     if prompt:
-        need = _e4m3_prompt_scratch(B, N, n_heads, kv, int(max_kv_len))
+        splits = _e4m3_prompt_splits(B, int(max_q_len), n_heads, kv.n_kv_heads, int(max_kv_len), int(window or 0))
+        need = _e4m3_prompt_scratch(B, N, n_heads, kv, int(max_kv_len), splits)
     else:
         need = _e4m3_few_scratch(q.get_device(), dt, B, N, int(max_q_len), n_heads, kv.n_kv_heads, hd, int(max_kv_len), int(total_kv_len),
                                  int(window or 0), 1 if kv.weights is not None else 0)
@@ -1856,7 +1868,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
     if prompt:
         _check(_fn("gtg_attention_e4m3_tcgen05")(q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv.address(), cu_seqlens.data_ptr(),
                                                  slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), N, n_heads, float(scale),
-                                                 int(window or 0), scratch.data_ptr() if need else None, _stream()), "attention_e4m3")
+                                                 int(window or 0), splits, scratch.data_ptr() if need else None, _stream()), "attention_e4m3")
         return
     _check(_fn("gtg_attention_e4m3")(dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv.address(), cu_seqlens.data_ptr(),
                                      slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), int(total_kv_len), N, n_heads,

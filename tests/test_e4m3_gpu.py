@@ -300,7 +300,9 @@ PROMPTS = [
     ([1, 2, 3], [1, 2, 3], 4, 2, 64), ([300, 64, 129, 5], [300, 64, 1, 2], 4, 4, 64), ([200, 333], [190, 33], 8, 2, 128), ([150, 64, 9], [0, 60, 9], 4, 1, 64),
     ([700], [700], 2, 1, 128), ([513, 100], [257, 100], 6, 2, 64), ([90, 70], [40, 70], 3, 1, 48), ([130, 40], [130, 7], 4, 2, 16), ([100], [100], 10, 2, 96),
     ([260], [200], 7, 1, 112), ([129], [128], 5, 5, 80), ([140, 64], [129, 64], 6, 3, 32), ([70, 70], [3, 70], 2, 1, 20), ([100], [65], 2, 2, 256),
-    ([1300], [16], 16, 2, 64), ([900, 333], [2, 5], 8, 8, 128)]
+    ([1300], [16], 16, 2, 64), ([900, 333], [2, 5], 8, 8, 128),
+    # long rows that several blocks share, beside sequences that have few or none
+    ([2600, 300, 64, 1500], [150, 300, 1, 0], 8, 2, 64), ([3000], [40], 4, 1, 128), ([2100], [700], 2, 1, 80), ([5000, 1100], [33, 600], 1, 1, 64)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -407,7 +409,7 @@ def test_queries_as_large_as_their_type_holds(dtype, new):
 @pytest.mark.parametrize("hd", [64, 128, 48])
 @pytest.mark.parametrize("new", [1, 70, 330])
 @pytest.mark.parametrize("small", [0.0, 2.0 ** -90])
-@pytest.mark.parametrize("order", [(0, 1, 1, 0, 1, 0), (1, 0, 0, 1, 0, 1)])
+@pytest.mark.parametrize("order", [(0, 1, 1, 0, 1, 0), (1, 0, 0, 1, 0, 1), (1,) * 16 + (0,) * 20])
 def test_blocks_of_zeros_have_their_share_of_the_probability(dtype, hd, new, small, order):
     """Blocks of values that are zero, or next to it, among others, with keys of their own or zero too: their scales are as small
     as scales get, their probabilities are not.  Bound: attention_case's, each channel's sizes summed."""
@@ -434,6 +436,14 @@ def test_blocks_of_zeros_have_their_share_of_the_probability(dtype, hd, new, sma
     total = p.gathered[0][0] + gathered
     bound = gathered * (2 * rel + new * heads * 2.0 ** -24) + total * 2.0 ** -23 + 1e-30
     assert (np.abs(p.read_weights(0, 0, n) - total) <= bound).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 32])
+@pytest.mark.parametrize("window", [1, 64, 700, 1500])
+def test_windows_over_long_rows(hd, window):
+    """Blocks that share a sequence's pages, of which some queries see none."""
+    worst, _ = attention_case(BF16, [2400, 1900], [300, 1900], 2, 1, hd, window=window)
+    assert worst <= 1, worst
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
