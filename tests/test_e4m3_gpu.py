@@ -446,6 +446,14 @@ def test_windows_over_long_rows(hd, window):
     assert worst <= 1, worst
 
 
+@pytest.mark.parametrize("window", [0, 3, 70])
+@pytest.mark.parametrize("held,new,heads,n_kv,hd", [([400, 1, 130], [400, 1, 100], 8, 2, 64), ([900], [500], 6, 6, 48), ([300, 64], [300, 64], 7, 1, 112),
+                                                    ([333, 20], [332, 0], 24, 8, 16)])
+def test_many_rows_in_float(window, held, new, heads, n_kv, hd):
+    worst, worst_w = attention_case(F32, held, new, heads, n_kv, hd, window=window, weights=not window, past_end=3)
+    assert worst <= 1 and worst_w <= 1, (worst, worst_w)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("longest", [1, 3, 40])
 def test_many_sequences_some_without_new_tokens(dtype, longest):
@@ -492,11 +500,12 @@ def test_a_query_that_is_not_a_number_shows_in_the_weights(dtype, hd, new):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("hd", [64, 128, 48, 20])
-@pytest.mark.parametrize("new,window", [(2, 0), (5, 0), (60, 0), (130, 0), (3, 40), (100, 40)])
-def test_nan_values_spoil_the_queries_that_see_their_rows(dtype, hd, new, window):
+@pytest.mark.parametrize("new,window,held", [(2, 0, 200), (5, 0, 200), (60, 0, 200), (130, 0, 200), (3, 40, 200), (100, 40, 200), (700, 0, 900),
+                                             (700, 40, 900)])
+def test_nan_values_spoil_the_queries_that_see_their_rows(dtype, hd, new, window, held):
     """One channel of one value row is NaN: queries before it are untouched, those at or behind it have NaN in that channel of
     its head (until it is behind the window), and nowhere else."""
-    held, row, channel = 200, 199 - new // 2, 11
+    row, channel = held - 1 - new // 2, 11
     p = Pages([held], 2, hd, seed=18)
     p.v.view(torch.uint8)[p.pages[0][row // 64], 1, channel, row % 64] = NAN
     q = torch.randn(new, 4 * hd, device=DEV).to(dtype)
