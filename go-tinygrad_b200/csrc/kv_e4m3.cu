@@ -270,8 +270,8 @@ template <int HD> struct Move {
 
 template <int PLANE> __device__ __forceinline__ void plane_sync() { asm volatile("bar.sync %0, %1;\n" ::"n"(1 + PLANE), "n"(kPlaneThreads) : "memory"); }
 
-// 16 codes times a power of two each word's pair shares: x[e] is codes 2 e, 2 e + 1, r[e] the factors (in half: clamped to what
-// half holds, beyond which codes are all zero, or all become zero).
+// Two codes times a power of two each, as halves (the factors clamped to what half holds, beyond which codes are all zero, or
+// all become zero).
 __device__ __forceinline__ __half2 times_ratio(uint32_t two_codes, float a, float b) {
     const uint32_t h = e4m3_pair_f16(two_codes);
     const float lo = 5.9604645e-8f, hi = 32768.f;
