@@ -839,28 +839,39 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                 const int hi = (int)min(past, 128LL);
                 const bool whole = __all_sync(full, lo == 0 && hi == 128);
                 const float* yt = y + 128 * buf;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                uint64_t sum[2] = {0, 0};
+                auto add_up = [&](auto masked) {
+                    const uint64_t f2 = two(f, f);
 #pragma unroll 1
-                for (int c = 0; c < 128; c += 32) {
-                    uint32_t sv[32];
-                    tmem_ld32(tmem + 128 * buf + lane_off + c, sv);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+                    for (int c = 0; c < 128; c += 32) {
+                        uint32_t sv[32];
+                        tmem_ld32(tmem + 128 * buf + lane_off + c, sv);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 s4 = *reinterpret_cast<const float4*>(yt + c + e);
-                        const float ys[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 y4 = *reinterpret_cast<const float4*>(yt + c + e);
+                            const uint64_t x[2] = {fma2(two(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), f2, two(y4.x, y4.y)),
+                                                   fma2(two(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])), f2, two(y4.z, y4.w))};
                             // (no probability is above 1: the bound is for scores so large that their roundings are powers of two)
-                            const float p = fast_exp2(min_or_nan(fmaf(__uint_as_float(sv[e + x]), f, ys[x]), 0.f));
-                            sum[x] += whole || (c + e + x >= lo && c + e + x < hi) ? p : 0.f;
+                            float p[4] = {fast_exp2(min_or_nan(first_of(x[0]), 0.f)), fast_exp2(min_or_nan(second_of(x[0]), 0.f)),
+                                          fast_exp2(min_or_nan(first_of(x[1]), 0.f)), fast_exp2(min_or_nan(second_of(x[1]), 0.f))};
+                            if constexpr (decltype(masked)::value) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (c + e + i < lo || c + e + i >= hi) p[i] = 0.f;
+                            }
+                            sum[0] = add2(sum[0], two(p[0], p[1]));
+                            sum[1] = add2(sum[1], two(p[2], p[3]));
                         }
                     }
-                }
+                };
+                if (whole) add_up(std::false_type());
+                else add_up(std::true_type());
                 asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_free(buf));
-                total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                sum[0] = add2(sum[0], sum[1]);
+                total += first_of(sum[0]) + second_of(sum[0]);
             }
             if (ok && in_parts) *part = total;
             else if (ok && there) kv.weights[page * kv.weight_stride + (size_t)h * kPageTokens + row % kPageTokens] += total;
