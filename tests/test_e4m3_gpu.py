@@ -600,6 +600,48 @@ def test_rows_of_any_stride(hd, new):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 48])
+@pytest.mark.parametrize("new", [[1, 1, 1], [70, 2, 64]])
+def test_kernels_that_begin_early(dtype, hd, new):
+    """Steps over the layers of a model, kernels chained (each may begin while the one before it drains) and recorded into a graph, and
+    once more one after the other: the same bits everywhere.  The layers share q and the scratch, so what begins too early shows."""
+    layers = [Pages([3000 - m, 1200 - m, 300 - m], 2, hd, seed=70 + i, weights=True, dropped=[0, 5, 9], room=400) for i, m in enumerate((3, 60, 128, 7))]
+    heads, steps, n = 8, 3, sum(new)
+    qkv = [torch.randn(n, (heads + 4) * hd, device=DEV).to(dtype) for _ in layers]
+    q, cu = torch.empty(n, heads * hd, dtype=dtype, device=DEV), cut(new)
+    views = [p.view() for p in layers]
+    starts = [[ints([h + g + m * t for h, g, m in zip(p.held, p.gone, new)]) for t in range(steps)] for p in layers]
+    need = max(ops.attention_e4m3_scratch_floats(dtype, 3, n, max(new), heads, v, 3300) for v in views)
+    scratch = torch.empty(max(need, 4), device=DEV)
+
+    def run(outs):
+        for t in range(steps):
+            for i, (p, v) in enumerate(zip(layers, views)):
+                ops.kv_store_e4m3(qkv[i], None, heads, 2, v, cu, ints_of[i], starts[i][t], max(new), q)
+                ops.attention_e4m3(q, outs[t][i], v, cu, ints_of[i], starts[i][t], max(new), heads, hd ** -0.5, max_kv_len=3300, scratch=scratch)
+    ints_of = [ints(p.slots) for p in layers]
+    before = [[x.clone() for x in (p.k.view(torch.uint8), p.v.view(torch.uint8), p.scales, p.weights)] for p in layers]
+    results = []
+    for chained in (False, True, True):
+        for p, b in zip(layers, before):
+            for x, y in zip((p.k.view(torch.uint8), p.v.view(torch.uint8), p.scales, p.weights), b):
+                x.copy_(y)
+        outs = [[torch.zeros_like(q) for _ in layers] for _ in range(steps)]
+        if not chained:
+            run(outs)
+        else:
+            with ops.chained_launches():
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    run(outs)
+                g.replay()
+        torch.cuda.synchronize()
+        results.append([x.clone() for row in outs for x in row] + [x.clone() for p in layers for x in (p.k.view(torch.uint8), p.v.view(torch.uint8), p.scales, p.weights)])
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("new", [1, 100])
 def test_pages_further_than_32_bits_count(dtype, new):
     """The same sequence in a small cache and at the end of one of 4.4 GB: attention, a step's store and an eviction agree bit by bit."""
