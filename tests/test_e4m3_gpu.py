@@ -811,6 +811,19 @@ def test_evict_by_weights_of_all_kinds(weights_of):
     evict_case([700, 130], 129, 30, 2, 64, entries=1, weights_of=weights_of)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 48, 20])
+@pytest.mark.parametrize("budget,recent,heavy", [(100, 20, [(10, 50), (900, 935), (1500, 1505)]), (130, 0, [(640, 641), (1000, 1100), (2400, 2429)]),
+                                                  (64, 1, [(2490, 2499)]), (300, 300, []), (200, 10, [(i, i + 1) for i in range(0, 2500, 13)])])
+def test_evict_over_pages_of_which_nothing_stays(hd, budget, recent, heavy):
+    """Rows that stay lie in few pages, far apart, or one or two in every page."""
+    def weights_of(rng, n):
+        w = rng.random(n).astype(np.float32)
+        for lo, hi in heavy:
+            w[lo: min(hi, n)] += 10
+        return w
+    evict_case([2500, 1300, 60], budget, recent, 2, hd, entries=1, weights_of=weights_of)
+
+
 @pytest.mark.parametrize("hd", [64, 20])
 def test_evict_leaves_sequences_longer_than_it_was_told_of(hd):
     p = Pages([300, 200], 2, hd, seed=31, weights=True, dropped=[0, 0])
