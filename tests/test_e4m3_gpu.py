@@ -641,6 +641,29 @@ def test_kernels_that_begin_early(dtype, hd, new):
         assert all(torch.equal(a, b) for a, b in zip(results[0], other))
 
 
+@pytest.mark.parametrize("new", [1, 4])
+def test_a_table_too_wide_to_count_its_steps_in_32_bits(new):
+    """Rows of the block table 2^27 entries apart: such a step takes the general kernel, scratch as for any."""
+    p = Pages([700, 90], 8, 64, seed=63, weights=True)
+    wide = torch.zeros(p.table.shape[0], 1 << 27, dtype=torch.int32, device=DEV)
+    wide[:, : p.table.shape[1]] = p.table
+    q = torch.randn(2 * new, 16 * 64, device=DEV).bfloat16()
+    before, outs, weights = p.weights.clone(), [], []
+    for table in (p.table, wide[:, : p.table.shape[1]]):
+        p.weights.copy_(before)
+        view, out = E4M3KVView(p.k, p.v, p.scales, table, weights=p.weights), torch.empty_like(q)
+        ops.attention_e4m3(q, out, view, cut([new, new]), ints(p.slots), ints([700 - new, 90 - new]), new, 16, 0.125, max_kv_len=700)
+        outs.append(out.double())
+        weights.append(p.weights.double())
+    # each within half a step (2^-8) and the products' roundings of the same value
+    assert ((outs[0] - outs[1]).abs() <= outs[0].abs() * 2.0 ** -7 + 2.0 ** -9).all()
+    # as attention_case has it for each of the two, the largest sum of sizes taken from the norms
+    longest = max(np.linalg.norm(r[0].values(), axis=1).max() for rows in p.rows for r in rows)
+    delta = 68 * 2.0 ** -23 * q.double().reshape(-1, 64).norm(dim=1).max().item() * longest * 0.125
+    rel = 2 * (2 * (2 * delta + 2.0 ** -21 + 700 * 2.0 ** -24) + 2 * new * 2.0 ** -24) + 2.0 ** -22
+    assert ((weights[0] - weights[1]).abs() <= rel * weights[0].abs()).all()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("new", [1, 100])
 def test_pages_further_than_32_bits_count(dtype, new):
