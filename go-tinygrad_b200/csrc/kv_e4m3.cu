@@ -270,17 +270,29 @@ template <int HD> struct Move {
 
 template <int PLANE> __device__ __forceinline__ void plane_sync() { asm volatile("bar.sync %0, %1;\n" ::"n"(1 + PLANE), "n"(kPlaneThreads) : "memory"); }
 
-// Two codes times a power of two each, as halves (the factors clamped to what half holds, beyond which codes are all zero, or
-// all become zero).
+// Two codes times a power of two each, as halves.  Below 2^-24, half's least, every code becomes zero all the same.  Above 2^17 every
+// code is zero: that factor takes the smallest, 2^-9, to 2^8, and 2^18 would take it beyond the 448 that the new scale was made
+// for.  Half holds powers up to 2^15: where a factor is FAR above that, the rest is multiplied in a second time.  (Asked once a tile:
+// asked at every word, the large eviction named below took 287 us instead of 276.)
+constexpr float kLeastHalf = 5.9604645e-8f, kMostHalf = 32768.f;
+template <bool FAR>
 __device__ __forceinline__ __half2 times_ratio(uint32_t two_codes, float a, float b) {
     const uint32_t h = e4m3_pair_f16(two_codes);
-    const float lo = 5.9604645e-8f, hi = 32768.f;
-    return __hmul2(*reinterpret_cast<const __half2*>(&h), __floats2half2_rn(fminf(fmaxf(a, lo), hi), fminf(fmaxf(b, lo), hi)));
+    __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h),
+                        __floats2half2_rn(fminf(fmaxf(a, kLeastHalf), kMostHalf), fminf(fmaxf(b, kLeastHalf), kMostHalf)));
+    if constexpr (FAR)
+        x = __hmul2(x, __floats2half2_rn(fminf(fmaxf(a * (1.f / kMostHalf), 1.f), 4.f), fminf(fmaxf(b * (1.f / kMostHalf), 1.f), 4.f)));
+    return x;
 }
 __device__ __forceinline__ uint32_t pair_codes(__half2 x) {
     unsigned short r;
     asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;\n" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&x)));
     return r;
+}
+// Four codes times a power of two each.
+template <bool FAR>
+__device__ __forceinline__ uint32_t times_ratios(uint32_t w, float a, float b, float c, float d) {
+    return pair_codes(times_ratio<FAR>(w, a, b)) | pair_codes(times_ratio<FAR>(w >> 16, c, d)) << 16;
 }
 // Each byte's |code| + 1, or 0 for NaN: the even bytes of a word and the odd ones, as 16-bit numbers that maxima are taken of.
 __device__ __forceinline__ uint32_t even_sizes(uint32_t w) { return ((w & 0x007f007fu) + 0x00010001u) & 0x007f007fu; }
@@ -464,10 +476,12 @@ kv_evict_move_kernel(const E4M3Pages pages, const EvictStrides strides, int* __r
                 if (id / (HD / 16) >= rows) continue;
                 uint32_t word[4] = {mine[m].x, mine[m].y, mine[m].z, mine[m].w};
                 const float ratio = was[m] * inverse;
-                if (ratio != 1.f) {
+                if (ratio > kMostHalf) {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        word[x] = pair_codes(times_ratio(word[x], ratio, ratio)) | pair_codes(times_ratio(word[x] >> 16, ratio, ratio)) << 16;
+                    for (int x = 0; x < 4; ++x) word[x] = times_ratios<true>(word[x], ratio, ratio, ratio, ratio);
+                } else if (ratio != 1.f) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) word[x] = times_ratios<false>(word[x], ratio, ratio, ratio, ratio);
                 }
                 *reinterpret_cast<uint4*>(at + id * 16) = make_uint4(word[0], word[1], word[2], word[3]);
             }
@@ -546,12 +560,18 @@ kv_evict_move_kernel(const E4M3Pages pages, const EvictStrides strides, int* __r
                                  fmaxf(size_value(even >> 16) * was[2], size_value(odd >> 16) * was[3]));
         const float scale = e4m3_needed_scale(block_most(most, to, plane_sync<1>)), inverse = pow2_inverse(scale);
         const bool same = was[0] == scale && was[1] == scale && was[2] == scale && was[3] == scale;
+        if (fmaxf(fmaxf(was[0], was[1]), fmaxf(was[2], was[3])) * inverse > kMostHalf) {
+#pragma unroll
+            for (int i = 0; i < CHANNELS; ++i)
+                word[i] = times_ratios<true>(word[i], was[0] * inverse, was[1] * inverse, was[2] * inverse, was[3] * inverse);
+        } else if (!same) {
+#pragma unroll
+            for (int i = 0; i < CHANNELS; ++i)
+                word[i] = times_ratios<false>(word[i], was[0] * inverse, was[1] * inverse, was[2] * inverse, was[3] * inverse);
+        }
         uint8_t* at = vc + (size_t)page_id[to] * pages.v_stride + r0;
 #pragma unroll
         for (int i = 0; i < CHANNELS; ++i) {
-            if (!same)
-                word[i] = pair_codes(times_ratio(word[i], was[0] * inverse, was[1] * inverse)) |
-                          pair_codes(times_ratio(word[i] >> 16, was[2] * inverse, was[3] * inverse)) << 16;
             uint8_t* row = at + (t / 16 + APART * i) * kPageTokens;
             if (r0 + 4 <= rows) *reinterpret_cast<uint32_t*>(row) = word[i];
             else
@@ -655,7 +675,7 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, b
 __device__ __forceinline__ uint32_t rescaled_bytes(uint32_t w, int n, float ratio) {
     if (n <= 0) return w;
     const uint32_t mask = n >= 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
-    const uint32_t r = pair_codes(times_ratio(w, ratio, ratio)) | pair_codes(times_ratio(w >> 16, ratio, ratio)) << 16;
+    const uint32_t r = times_ratios<false>(w, ratio, ratio, ratio, ratio);      // (a scale only grows here)
     return (r & mask) | (w & ~mask);
 }
 
