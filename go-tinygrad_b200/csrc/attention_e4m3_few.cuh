@@ -756,8 +756,8 @@ FewPlan few_plan_for(int B, int max_q_len, int n_heads, int n_kv, int max_kv_len
 
 template <int HD, int NT>
 int launch_few_tiles(const FewArgs& a, const E4M3Pages& kv, cudaStream_t stream) {
-    const int st = launch_chained(few_queries_kernel<HD, NT>, dim3(a.workers / kFewWarps), dim3(kFewThreads), Few<HD>::RING,
-                                  stream, a, kv);
+    const int st = launch_early(a.chained != 0, few_queries_kernel<HD, NT>, dim3(a.workers / kFewWarps), dim3(kFewThreads), Few<HD>::RING,
+                                stream, a, kv);
     if (st != 0) return st;
     const int join = (a.columns + Join<HD>::columns_each(a.columns) - 1) / Join<HD>::columns_each(a.columns);
     // no more blocks than run at once: each begins with the same few reads, and a second turn would wait for them again

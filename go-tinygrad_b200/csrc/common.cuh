@@ -134,9 +134,11 @@ __device__ __forceinline__ void chain_release() { asm volatile("griddepcontrol.l
 static int g_chained_launch = 0;
 GTG_API void gtg_set_chained_launch(int on) { g_chained_launch = on ? 1 : 0; }
 
+// With `early` the kernel may begin before the one before it is complete.  (The switch is the caller's: whoever launches several
+// kernels in a call reads it once and says so here, since another thread may turn it meanwhile.)
 template <typename... Params, typename... Args>
-static inline int launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
-                                 cudaStream_t stream, Args... args) {
+static inline int launch_early(bool early, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
+                               cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -146,9 +148,14 @@ static inline int launch_chained(void (*kernel)(Params...), dim3 grid, dim3 bloc
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = g_chained_launch ? 1 : 0;
+    cfg.numAttrs = early ? 1 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
     return e != cudaSuccess ? (int)e : launch_status();
+}
+template <typename... Params, typename... Args>
+static inline int launch_chained(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
+                                 cudaStream_t stream, Args... args) {
+    return launch_early(g_chained_launch != 0, kernel, grid, block, smem, stream, args...);
 }
 
 // The same for a grid of thread-block clusters of `cluster_x` blocks along x.

@@ -37,11 +37,7 @@ constexpr int kLeastExponent = -126;
 // whether the caller chains its kernels or not, and waits for it itself (chain_wait).
 template <typename... Params, typename... Args>
 static inline int launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
-    const int chained = g_chained_launch;
-    g_chained_launch = 1;
-    const int st = launch_chained(kernel, grid, block, smem, stream, args...);
-    g_chained_launch = chained;
-    return st;
+    return launch_early(true, kernel, grid, block, smem, stream, args...);
 }
 
 __device__ __forceinline__ bool finite_f32(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
