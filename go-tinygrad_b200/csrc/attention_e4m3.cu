@@ -207,9 +207,11 @@ row_weights_kernel(const T* __restrict__ q, int ldq, const E4M3Pages kv, const i
 template <typename T>
 int launch_row_weights(const void* q, int ldq, const E4M3Pages& kv, const int* cu_seqlens, const int* slots, const int* start_pos, int B,
                        int max_kv_len, int n_heads, float scale, int window, const float2* stats, cudaStream_t stream) {
-    const size_t smem = ((size_t)kPageTokens * (kv.hd + 1) + 8 * (size_t)kv.hd) * sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(row_weights_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
+    auto bytes = [](int hd) { return ((size_t)kPageTokens * (hd + 1) + 8 * (size_t)hd) * sizeof(float); };
+    const size_t smem = bytes(kv.hd);
+    static bool allowed[kMaxDevices] = {};
+    const int set = allow_shared((const void*)row_weights_kernel<T>, bytes(kMaxChannels), allowed);
+    if (set != 0) return set;
     return launch_behind(row_weights_kernel<T>, dim3((max_kv_len + kPageTokens - 1) / kPageTokens, kv.n_kv, B), dim3(kRowThreads), smem, stream,
                           (const T*)q, ldq, kv, cu_seqlens, slots, start_pos, n_heads, scale, window, stats);
 }

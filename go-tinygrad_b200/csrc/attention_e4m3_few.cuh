@@ -723,9 +723,9 @@ struct FewPlan {
 // Warps of this kernel that the current device runs at once (asked once a device).
 template <int HD, int NT>
 int few_workers() {
-    static int cached[64] = {};
+    static int cached[kMaxDevices] = {};
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kFewWarps;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return kFewWarps;
     if (cached[dev] == 0) {
         int blocks = 0, sms = 0;
         if (cudaFuncSetAttribute(few_queries_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<HD>::RING) != cudaSuccess ||

@@ -635,12 +635,9 @@ e4m3_prompt_join_kernel(const PromptArgs a, int B, int N, int hd) {
 
 template <int HD, bool kExact, bool kTest>
 int launch(const PromptArgs& a, const E4M3Pages& kv, int B, int max_q_len, cudaStream_t stream) {
-    static bool configured = false;
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(attention_e4m3_prompt_kernel<HD, kExact, kTest>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::kSmemBytes);
-        if (e != cudaSuccess) return (int)e;
-        configured = true;
-    }
+    static bool allowed[kMaxDevices] = {};
+    const int set = allow_shared((const void*)attention_e4m3_prompt_kernel<HD, kExact, kTest>, Shape<HD>::kSmemBytes, allowed);
+    if (set != 0) return set;
     const long long rows = (long long)max_q_len * a.group;
     return launch_chained(attention_e4m3_prompt_kernel<HD, kExact, kTest>, dim3(kv.n_kv, B, (unsigned)((rows + 2 * BQ - 1) / (2 * BQ) * a.splits)), dim3(kThreads),
                           (size_t)Shape<HD>::kSmemBytes, stream, a, kv);
@@ -902,12 +899,9 @@ e4m3_weights_sum_kernel(const PromptArgs a, const E4M3Pages kv, const float* __r
 
 template <int HD, bool kExact, bool kTest>
 int launch_weights(const PromptArgs& a, const E4M3Pages& kv, const CUtensorMap& map_q, int B, int max_kv_len, float* parts, cudaStream_t stream) {
-    static bool configured = false;
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(e4m3_weights_kernel<HD, kExact, kTest>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightShape<HD>::kSmemBytes);
-        if (e != cudaSuccess) return (int)e;
-        configured = true;
-    }
+    static bool allowed[kMaxDevices] = {};
+    const int set = allow_shared((const void*)e4m3_weights_kernel<HD, kExact, kTest>, WeightShape<HD>::kSmemBytes, allowed);
+    if (set != 0) return set;
     const int part_rows = (max_kv_len + 127) / 128 * 128;
     const int st = launch_behind(e4m3_weights_kernel<HD, kExact, kTest>, dim3(part_rows / 128, a.n_heads, B), dim3(kWeightThreads),
                                   (size_t)WeightShape<HD>::kSmemBytes, stream, map_q, a, kv, parts, part_rows);

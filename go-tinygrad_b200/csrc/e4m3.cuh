@@ -40,6 +40,21 @@ static inline int launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block
     return launch_early(true, kernel, grid, block, smem, stream, args...);
 }
 
+// Lets `kernel` take up to `bytes` of shared memory on the current device, asked for once a device: the permission is the device's, and
+// a size that differed by call could be lowered by another thread between here and the launch.  done: the kernel's own, one a device.
+constexpr int kMaxDevices = 64;
+static inline int allow_shared(const void* kernel, size_t bytes, bool (&done)[kMaxDevices]) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    const bool counted = dev >= 0 && dev < kMaxDevices;
+    if (counted && done[dev]) return 0;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) return (int)e;
+    if (counted) done[dev] = true;
+    return 0;
+}
+
 __device__ __forceinline__ bool finite_f32(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 __device__ __forceinline__ float min_or_nan(float a, float b) {

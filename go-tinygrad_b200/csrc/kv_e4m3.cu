@@ -582,6 +582,7 @@ kv_evict_move_kernel(const E4M3Pages pages, const EvictStrides strides, int* __r
     cp_async_wait<0>();
 }
 
+constexpr size_t kMoveBytes = 200 * 1024;   // what that kernel takes at most; longer sequences take the general one
 size_t move_bytes(int hd, int max_length, int budget) {
     const size_t max_pages = (max_length + kPageTokens - 1) / kPageTokens;
     return kStaged * (size_t)hd * kPageTokens + max_pages * kPageTokens * 4 + (size_t)(budget + 63) / 64 * 64 * 4 + max_pages * 12;
@@ -590,12 +591,9 @@ template <int HD>
 int launch_move(const E4M3Pages& pages, const EvictStrides& strides, int* dropped, const int* slots, const int* lengths, int max_length, int budget,
                 int recent, int* kept, int B, int entries, cudaStream_t stream) {
     const size_t smem = move_bytes(HD, max_length, budget);
-    static size_t configured = 48 * 1024 - 4096;
-    if (smem > configured) {
-        const cudaError_t e = cudaFuncSetAttribute(kv_evict_move_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return (int)e;
-        configured = smem;
-    }
+    static bool allowed[kMaxDevices] = {};
+    const int st = allow_shared((const void*)kv_evict_move_kernel<HD>, kMoveBytes, allowed);
+    if (st != 0) return st;
     kv_evict_move_kernel<HD><<<dim3(pages.n_kv, B, entries), kMoveThreads, smem, stream>>>(pages, strides, dropped, slots, lengths, max_length, budget,
                                                                                           recent, kept);
     return launch_status();
@@ -927,7 +925,7 @@ GTG_API int gtg_kv_evict_e4m3(int entries, const E4M3Pages* first, long long k_e
     if (smem > 40 * 1024) return kErrUnsupported;
     const EvictStrides strides = {k_entry, v_entry, scale_entry, weight_entry};
     // sequences whose weights fit in shared memory, heads of a multiple of 16 channels; else the general form
-    if (hd % 16 == 0 && hd <= 128 && move_bytes(hd, max_length, budget) <= 200 * 1024) {
+    if (hd % 16 == 0 && hd <= 128 && move_bytes(hd, max_length, budget) <= kMoveBytes) {
 #define GTG_MOVE(HD) case HD: return launch_move<HD>(pages, strides, dropped, slots, lengths, max_length, budget, recent, kept, B, entries, stream);
         switch (hd) { GTG_MOVE(16) GTG_MOVE(32) GTG_MOVE(48) GTG_MOVE(64) GTG_MOVE(80) GTG_MOVE(96) GTG_MOVE(112) GTG_MOVE(128) }
 #undef GTG_MOVE
