@@ -646,7 +646,9 @@ int launch(const PromptArgs& a, const E4M3Pages& kv, int B, int max_q_len, cudaS
 // weight_j += sum over the queries that see row j, of all heads of the group, of 2^(score - x) / l, x and l the query's
 // statistics that the attention left.  The products again, the other way round: one block per (128 rows of the cache, query
 // head, sequence), the rows as the tile's rows, so that a thread owns a row and its sum:
-//   K      converted once to bfloat16 (exact) into shared memory, S = K Q^T by tcgen05.mma 128 x 128 x head size;
+//   K      converted once to bfloat16 into shared memory, S = K Q^T by tcgen05.mma 128 x 128 x head size.  Not the codes but the keys
+//          they stand for, 2^-32 of them (exact: bfloat16 has float's range): queries come as they are, and the codes' products with
+//          the largest of them, before the key scale makes them small, left float's range;
 //   Q      128 tokens of one head at a time by tensor copies through a ring, as they are (bfloat16);
 //   sums   four warps, S from tensor memory, 1 / l folded into the exponent: one multiply-add, one exponential and one add a
 //          score.  The exponentials bound it (16 a cycle).
@@ -662,11 +664,16 @@ template <int HD> struct WeightShape {
     static constexpr int kSmemBytes = kOffBar + 256;
 };
 
-// Four codes as four bfloat16.
-__device__ __forceinline__ void bf16_of_codes(uint32_t w, uint32_t& lo, uint32_t& hi) {
+// What a block's codes are multiplied with there: 2^-32 times its scale 2^k, and 2^-100 at least, so that codes of 2^-9 are still
+// normal numbers.
+__device__ __forceinline__ float key_factor(float k_scale) {
+    return __int_as_float(max((int)(__float_as_uint(k_scale) & 0x7f800000u) - (32 << 23), 27 << 23));
+}
+// Four codes times a power of two as four bfloat16.
+__device__ __forceinline__ void bf16_of_codes(uint32_t w, float times, uint32_t& lo, uint32_t& hi) {
     const uint32_t a = e4m3_pair_f16(w), b = e4m3_pair_f16(w >> 16);
     const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
-    const __nv_bfloat162 p = __floats2bfloat162_rn(x.x, x.y), r = __floats2bfloat162_rn(y.x, y.y);
+    const __nv_bfloat162 p = __floats2bfloat162_rn(x.x * times, x.y * times), r = __floats2bfloat162_rn(y.x * times, y.y * times);
     lo = *reinterpret_cast<const uint32_t*>(&p);
     hi = *reinterpret_cast<const uint32_t*>(&r);
 }
@@ -796,13 +803,17 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                 const int id = r + 128 * m, key = id / (hd / 16), piece = id - key * (hd / 16);
                 const int j = kt * 2 + key / 64;
                 uint4 u = make_uint4(0, 0, 0, 0);
-                if (j * kPageTokens < start + q_len)
-                    u = *reinterpret_cast<const uint4*>(kv.k + (size_t)table[j] * kv.k_stride + ((size_t)h * kPageTokens + key % 64) * hd + piece * 16);
+                float times = 0.f;
+                if (j * kPageTokens < start + q_len) {
+                    const size_t page = table[j];
+                    u = *reinterpret_cast<const uint4*>(kv.k + page * kv.k_stride + ((size_t)h * kPageTokens + key % 64) * hd + piece * 16);
+                    times = key_factor(kv.scales[page * kv.scale_stride + h]);
+                }
                 uint32_t o[8];
-                bf16_of_codes(u.x, o[0], o[1]);
-                bf16_of_codes(u.y, o[2], o[3]);
-                bf16_of_codes(u.z, o[4], o[5]);
-                bf16_of_codes(u.w, o[6], o[7]);
+                bf16_of_codes(u.x, times, o[0], o[1]);
+                bf16_of_codes(u.y, times, o[2], o[3]);
+                bf16_of_codes(u.z, times, o[4], o[5]);
+                bf16_of_codes(u.w, times, o[6], o[7]);
                 const uint32_t at = base + (piece / 4) * (128 * 128) + key * 128;
                 store_shared16(at + (((piece % 4 * 2) ^ (key & 7)) << 4), o[0], o[1], o[2], o[3]);
                 store_shared16(at + (((piece % 4 * 2 + 1) ^ (key & 7)) << 4), o[4], o[5], o[6], o[7]);
@@ -811,12 +822,13 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
             __syncwarp();
             if (lane == 0) mbar_arrive(k_full);
             const size_t page = there ? table[row / kPageTokens] : 0;
-            const float f = there ? a.scale * kLog2e * kv.scales[page * kv.scale_stride + h] : 0.f;
+            const float k_scale = there ? kv.scales[page * kv.scale_stride + h] : 0.f;
+            const float f = a.scale * kLog2e * (k_scale * pow2_inverse(key_factor(k_scale)));
             auto statistic = [&](int i) {                        // of tile i's column r: what takes a score to its probability's exponent
                 const int token = sp.t_lo + i % sp.per_head * 128 + r;
                 if (i >= tiles || token >= sp.t_hi) return 0.f;
                 const float2 st = a.stats[(size_t)(q_begin + token) * a.n_heads + h * a.group + g0 + i / sp.per_head];
-                return -(st.x + log2f(st.y));
+                return score_slack(st.x) - (st.x + log2f(st.y));
             };
             float mine = statistic(0), total = 0.f;
             for (int i = 0; i < tiles; ++i, ++n) {
@@ -849,7 +861,7 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                             const float4 y4 = *reinterpret_cast<const float4*>(yt + c + e);
                             const uint64_t x[2] = {fma2(two(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), f2, two(y4.x, y4.y)),
                                                    fma2(two(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])), f2, two(y4.z, y4.w))};
-                            // (no probability is above 1: the bound is for scores so large that their roundings are powers of two)
+                            // (no probability is above 1: the bound is for scores that lie within their roundings of the maximum)
                             float p[4] = {fast_exp2(min_or_nan(first_of(x[0]), 0.f)), fast_exp2(min_or_nan(second_of(x[0]), 0.f)),
                                           fast_exp2(min_or_nan(first_of(x[1]), 0.f)), fast_exp2(min_or_nan(second_of(x[1]), 0.f))};
                             if constexpr (decltype(masked)::value) {
