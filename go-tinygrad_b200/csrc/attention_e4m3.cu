@@ -124,7 +124,7 @@ attention_rows_kernel(const T* __restrict__ q, int ldq, T* __restrict__ out, int
         if (part) part[2 + d] = acc;
         else out[(size_t)token * ldo + head * hd + d] = from_f32<T>(acc / L);
     }
-    if (stats && !part && tid == 0) stats[(size_t)token * n_heads + head] = make_float2(M_use * kLog2e, L);
+    if (stats && !part && tid == 0) stats[(size_t)token * n_heads + head] = make_float2(M_use, L);
 }
 
 template <typename T>
@@ -145,7 +145,7 @@ rows_join_kernel(const float* __restrict__ parts, int splits, T* __restrict__ ou
         for (int s = 0; s < splits; ++s) acc += expf(part[(size_t)s * (hd + 2)] - M_use) * part[(size_t)s * (hd + 2) + 2 + d];
         out[(size_t)token * ldo + head * hd + d] = from_f32<T>(acc / L);
     }
-    if (stats && threadIdx.x == 0) stats[(size_t)token * n_heads + head] = make_float2(M_use * kLog2e, L);
+    if (stats && threadIdx.x == 0) stats[(size_t)token * n_heads + head] = make_float2(M_use, L);
 }
 
 // A block per (page of the sequence, key/value head, sequence): 64 rows by two halves of the (query, head) pairs that may
@@ -190,9 +190,9 @@ row_weights_kernel(const T* __restrict__ q, int ldq, const E4M3Pages kv, const i
             for (int i = part; i < here; i += 2) {
                 const int at = start + from + (p0 + i) / group;
                 if (row > at || (window > 0 && row <= at - window)) continue;
-                float s = 0.f;
+                float s = 0.f;                                                  // the very score that the attention took its maximum of
                 for (int d = 0; d < hd; ++d) s = fmaf(qs[i * hd + d], ks[t * ld + d], s);
-                sum += exp2f(min_or_nan(fmaf(s * k_scale, kUp * kLog2e, -st[i].x), 0.f)) / st[i].y;
+                sum += expf(s * k_scale * kUp - st[i].x) / st[i].y;
             }
         }
         if (part) half_sum[t] = sum;

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from go_tinygrad_b200.kernels import ops
-from test_e4m3_gpu import BF16, DEV, Pages, cut, ints
+from test_e4m3_gpu import BF16, DEV, F32, Pages, cut, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +59,10 @@ def test_prompts(hd, size, key_size, new, held, loose):
     """Scores of up to 2^90 out of queries that leave float's range when they are multiplied with codes; `loose`: rows that the plan has
     no room for."""
     one_row_a_query(BF16, hd, new, held, size, key_size, loose=loose)
+
+
+@pytest.mark.parametrize("dtype,hd", [(F32, 64), (F32, 128), (F32, 48), (F32, 20), (BF16, 20)])
+@pytest.mark.parametrize("size,key_size", LARGE)
+@pytest.mark.parametrize("new,held,loose", [(1, 200, False), (1, 1500, False), (70, 200, False), (40, 1500, False), (5, 900, True)])
+def test_any_head_size_and_type(dtype, hd, size, key_size, new, held, loose):
+    one_row_a_query(dtype, hd, new, held, size, key_size, loose=loose)
