@@ -694,7 +694,7 @@ few_join_kernel(const FewArgs a, const E4M3Pages kv, int join_blocks) {
                 const bf16* qr = a.q + (size_t)(span.first + c / a.group) * a.ldq + (size_t)(h * a.group + c % a.group) * HD;
                 float s = 0.f;
                 for (int d = 0; d < HD; ++d) s = fmaf(__bfloat162float(qr[d]) * kDown, e4m3_value(kr[d]), s);
-                sum += exp2_fast(s * k_scale * kUp - top[c] + kPShift) * inverse[c];
+                sum += exp2_fast(min_or_nan(s * k_scale * kUp - top[c] + score_slack(top[c]), 0.f) + kPShift) * inverse[c];
             }
         }
         kv.weights[page * kv.weight_stride + h * kPageTokens + t] += sum;

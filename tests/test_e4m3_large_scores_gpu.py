@@ -66,3 +66,11 @@ def test_prompts(hd, size, key_size, new, held, loose):
 @pytest.mark.parametrize("new,held,loose", [(1, 200, False), (1, 1500, False), (70, 200, False), (40, 1500, False), (5, 900, True)])
 def test_any_head_size_and_type(dtype, hd, size, key_size, new, held, loose):
     one_row_a_query(dtype, hd, new, held, size, key_size, loose=loose)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 48, 16])
+@pytest.mark.parametrize("size,key_size", LARGE)
+@pytest.mark.parametrize("new,held,loose", [(1, 200, False), (5, 900, False), (1, 900, True), (5, 900, True), (16, 2000, True)])
+def test_few_queries(hd, size, key_size, new, held, loose):
+    """`loose`: rows whose scores the plan has no room to keep, which are computed once more."""
+    one_row_a_query(BF16, hd, new, held, size, key_size, loose=loose)
