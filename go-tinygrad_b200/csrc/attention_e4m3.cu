@@ -250,8 +250,7 @@ static FewPlan few_plan(int B, int max_q_len, int n_heads, int n_kv, int hd, int
 
 // Floats of scratch that gtg_attention_e4m3 needs for the same numbers.
 GTG_API long long gtg_attention_e4m3_scratch_floats(int dtype, int B, int N, int max_q_len, int n_heads, int n_kv, int hd, int max_kv_len,
-                                                    long long total_kv_len, int window, int weigh) {
-    (void)total_kv_len;
+                                                    int window, int weigh) {
     if (B <= 0 || n_kv <= 0 || n_heads <= 0 || n_heads % n_kv || max_q_len <= 0 || max_kv_len <= 0) return 0;
     const long long rows = rows_floats(N, n_heads, hd, rows_splits(std::max(N, 1), n_heads, max_kv_len, window), weigh != 0);
     if (few_takes(dtype, max_q_len, n_heads, n_kv, hd))
@@ -259,11 +258,11 @@ GTG_API long long gtg_attention_e4m3_scratch_floats(int dtype, int B, int N, int
     return rows;
 }
 
-// dtype: of q and out (0 float, 1 bfloat16).  max_kv_len: rows of the longest sequence after this step; total_kv_len: of all
-// (0: not known); they decide how the work is cut and how many blocks look for weights.
+// dtype: of q and out (0 float, 1 bfloat16).  max_kv_len: rows of the longest sequence after this step; it decides how the work is cut
+// and how many blocks look for weights.
 GTG_API int gtg_attention_e4m3(int dtype, const void* q, int ldq, void* out, int ldo, const E4M3Pages* pages, const int* cu_seqlens,
-                               const int* slots, const int* start_pos, int B, int max_q_len, int max_kv_len, long long total_kv_len, int N,
-                               int n_heads, float scale, int window, float* scratch, cudaStream_t stream) {
+                               const int* slots, const int* start_pos, int B, int max_q_len, int max_kv_len, int N, int n_heads,
+                               float scale, int window, float* scratch, cudaStream_t stream) {
     if (B <= 0 || N <= 0 || max_q_len <= 0) return 0;
     const E4M3Pages kv = *pages;
     const int n_kv = kv.n_kv, hd = kv.hd;

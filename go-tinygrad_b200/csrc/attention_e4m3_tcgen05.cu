@@ -928,8 +928,9 @@ GTG_API int gtg_attention_e4m3_tcgen05_status() {
     return v;
 }
 
-// Heads of 64 or 128 channels, bfloat16 rows of q and out on 16-byte boundaries.  weights (or null) gather what the rows get;
-// scratch for that: 2 N n_heads floats and n_heads B times max_kv_len rounded up to 128.
+// Heads of a multiple of 16 channels up to 128; bfloat16 rows of q and out on 16-byte boundaries.  splits: blocks that share the pages of
+// 256 query rows.  scratch, in floats, on a 16-byte boundary: with several splits N n_heads splits (hd + 2); where the pages have
+// weights, which then gather what their rows get, 2 N n_heads and n_heads B times max_kv_len rounded up to 128 more; else null.
 GTG_API int gtg_attention_e4m3_tcgen05(const void* q, int ldq, void* out, int ldo, const E4M3Pages* pages, const int* cu_seqlens,
                                        const int* slots, const int* start_pos, int B, int max_q_len, int max_kv_len, int N, int n_heads,
                                        float scale, int window, int splits, float* scratch, cudaStream_t stream) {

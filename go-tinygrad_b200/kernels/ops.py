@@ -136,8 +136,8 @@ _SIGNATURES = {
                                                             _I, _I, _I, _I, _I, _F, _I, _I, _P, _F, _I, _P, _P]),
     "gtg_kv_store_e4m3": ("kv_e4m3", [_I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P, _I, _P]),
     "gtg_kv_evict_e4m3": ("kv_e4m3", [_I, _P, _L, _L, _L, _L, _P, _P, _I, _I, _I, _I, _P, _P]),
-    "gtg_attention_e4m3_scratch_floats": ("attention_e4m3", [_I, _I, _I, _I, _I, _I, _I, _I, _L, _I, _I]),
-    "gtg_attention_e4m3": ("attention_e4m3", [_I, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _L, _I, _I, _F, _I, _P, _P]),
+    "gtg_attention_e4m3_scratch_floats": ("attention_e4m3", [_I, _I, _I, _I, _I, _I, _I, _I, _I, _I]),
+    "gtg_attention_e4m3": ("attention_e4m3", [_I, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _P, _P]),
     "gtg_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", [_P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P]),
     "gtg_attention_e4m3_tcgen05_status": ("attention_e4m3_tcgen05", []),
     "gtg_attention_e4m3_tcgen05_test_hooks": ("attention_e4m3_tcgen05", [_I]),
@@ -1801,21 +1801,21 @@ def _e4m3_prompt_scratch(n_seqs: int, n_tokens: int, n_heads: int, kv, max_kv_le
 
 @functools.lru_cache(maxsize=1024)
 def _e4m3_few_scratch(device: int, dt: int, n_seqs: int, n_tokens: int, max_q_len: int, n_heads: int, n_kv: int, hd: int, max_kv_len: int,
-                      total_kv_len: int, window: int, weigh: int) -> int:
+                      window: int, weigh: int) -> int:
     """Floats for these sizes on the current device, number `device` (-1: none): a call of the library that says so is not made twice."""
-    return int(_fn("gtg_attention_e4m3_scratch_floats")(dt, n_seqs, n_tokens, max_q_len, n_heads, n_kv, hd, max_kv_len, total_kv_len, window, weigh))
+    return int(_fn("gtg_attention_e4m3_scratch_floats")(dt, n_seqs, n_tokens, max_q_len, n_heads, n_kv, hd, max_kv_len, window, weigh))
 
 
 def attention_e4m3_scratch_floats(dtype: torch.dtype, n_seqs: int, n_tokens: int, max_q_len: int, n_heads: int, kv, max_kv_len: int,
                                   total_kv_len: int = 0, window: Optional[int] = None) -> int:
-    """Floats of scratch `attention_e4m3` needs for the same arguments (0: none)."""
+    """Floats of scratch `attention_e4m3` needs for the same arguments (0: none; `total_kv_len` changes nothing)."""
     window = kv.window if window is None else window
     prompt = 0
     if _e4m3_prompt_form(0 if dtype == torch.float32 else 1, max_q_len, n_heads, kv.n_kv_heads, kv.head_dim):
         splits = _e4m3_prompt_splits(n_seqs, int(max_q_len), n_heads, kv.n_kv_heads, int(max_kv_len), int(window or 0))
         prompt = _e4m3_prompt_scratch(n_seqs, n_tokens, n_heads, kv, int(max_kv_len), splits)         # if its rows allow it; else what follows
     return max(prompt, _e4m3_few_scratch(kv.k.get_device(), 0 if dtype == torch.float32 else 1, n_seqs, n_tokens, int(max_q_len), n_heads,
-                                         kv.n_kv_heads, kv.head_dim, int(max_kv_len), int(total_kv_len), int(window or 0),
+                                         kv.n_kv_heads, kv.head_dim, int(max_kv_len), int(window or 0),
                                          1 if kv.weights is not None else 0))
 
 
@@ -1826,8 +1826,9 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
     between: q [N, n_heads * head_dim] rotated, its keys and values in the cache (`kv_store_e4m3`), out like q (float32 or
     bfloat16).  Sequence b owns q's rows cu_seqlens[b]..cu_seqlens[b+1] (`max_q_len` of them at most) at positions start_pos[b], ...;
     a query sees the rows at and before its own, the last `window` of them where a window is given (default: the view's).
-    `max_kv_len`: rows of the longest sequence after this step; `total_kv_len`: of all (0: not known).  Both decide only how the work
-    is cut: a sequence that has outgrown them is still computed right.  Where the view gathers weights, every row's grows by the
+    `max_kv_len`: rows of the longest sequence after this step.  It decides only how the work is cut: a sequence that has outgrown it
+    is still computed right.  `total_kv_len`, rows of all sequences, is taken as the other attention calls take it and decides
+    nothing: the kernels count the rows themselves.  Where the view gathers weights, every row's grows by the
     sum of its probabilities over the step's queries and the heads that share it (no two of the step's sequences may share a page
     then).  Rows of q and out behind the last sequence are left alone.  `scratch`: float32, at least `attention_e4m3_scratch_floats` (None: taken from the allocator)."""
     _rows2d(q, "attention_e4m3: q")
@@ -1857,7 +1858,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
         splits = _e4m3_prompt_splits(B, int(max_q_len), n_heads, kv.n_kv_heads, int(max_kv_len), int(window or 0))
         need = _e4m3_prompt_scratch(B, N, n_heads, kv, int(max_kv_len), splits)
     else:
-        need = _e4m3_few_scratch(q.get_device(), dt, B, N, int(max_q_len), n_heads, kv.n_kv_heads, hd, int(max_kv_len), int(total_kv_len),
+        need = _e4m3_few_scratch(q.get_device(), dt, B, N, int(max_q_len), n_heads, kv.n_kv_heads, hd, int(max_kv_len),
                                  int(window or 0), 1 if kv.weights is not None else 0)
     if need:
         if scratch is None:
@@ -1871,8 +1872,8 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
                                                  int(window or 0), splits, scratch.data_ptr() if need else None, _stream()), "attention_e4m3")
         return
     _check(_fn("gtg_attention_e4m3")(dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), kv.address(), cu_seqlens.data_ptr(),
-                                     slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), int(total_kv_len), N, n_heads,
-                                     float(scale), int(window or 0), _ptr(scratch) if need else None, _stream()), "attention_e4m3")
+                                     slots.data_ptr(), start_pos.data_ptr(), B, int(max_q_len), int(max_kv_len), N, n_heads, float(scale),
+                                     int(window or 0), _ptr(scratch) if need else None, _stream()), "attention_e4m3")
 
 
 def kv_evict_e4m3(storage, slots: torch.Tensor, lengths: torch.Tensor, max_length: int, budget: int, recent: int,
