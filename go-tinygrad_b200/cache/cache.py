@@ -263,8 +263,6 @@ class _KVGroup:
             self.storage = torch.zeros((n_entries, n_pages, request.planes, request.n_kv_heads, PAGE_TOKENS,
                                         request.head_dim), dtype=dtype, device=device)
         self.table_host = torch.zeros((n_slots, pages_per_seq), dtype=torch.int32)
-        if device.type == "cuda":
-            self.table_host = self.table_host.pin_memory()
         self.table = torch.zeros((n_slots, pages_per_seq), dtype=torch.int32, device=device)
         self.pages_of: Dict[int, List[int]] = {}     # slot -> its pages by index; -1: given back (slid out of the window)
         self.dirty: set = set()
@@ -339,6 +337,7 @@ class Cache:
         self.slots = SlotTable(self.n_slots)
         self._length = [0] * self.n_slots
         self._dropped = [0] * self.n_slots
+        self._flushed: Optional[Tuple[object, object]] = None      # stream of the last copy of block-table rows, and an event behind it
         # what users of the cache keep with it and want gone when it goes (the generation
         # loop: its recorded decode steps); the cache itself never looks inside
         self.attachments: Dict[str, object] = {}
@@ -525,7 +524,7 @@ class Cache:
         if not slots:
             return []
         self.flush_tables()
-        both = torch.tensor([list(slots), held], dtype=torch.int32).to(self.device)
+        both = self._sent(torch.tensor([list(slots), held], dtype=torch.int32))
         kept = [ops.kv_evict_e4m3(grp.e4m3, both[0], both[1], max(held), budget, recent) for grp in self.groups]
         pages = (budget + PAGE_TOKENS - 1) // PAGE_TOKENS
         for slot, rows in zip(slots, held):
@@ -546,11 +545,29 @@ class Cache:
                 self.evict(due)
 
     def flush_tables(self) -> None:
-        """Copy block-table rows that changed on the host to the device."""
+        """Copy block-table rows that changed on the host to the device, on the current stream; what was copied on another stream before
+        is there for this one's next kernels too."""
+        stream = torch.cuda.current_stream(self.device) if self.device.type == "cuda" else None
+        if self._flushed is not None and self._flushed[0] != stream:
+            stream.wait_event(self._flushed[1])
+        changed = False
         for grp in self.groups:
             for slot in sorted(grp.dirty):
-                grp.table[slot].copy_(grp.table_host[slot])
+                grp.table[slot].copy_(self._staged(grp.table_host[slot]), non_blocking=True)
+                changed = True
             grp.dirty.clear()
+        if changed and stream is not None:
+            self._flushed = (stream, stream.record_event())
+
+    def _staged(self, host: torch.Tensor) -> torch.Tensor:
+        """What `host` holds now, where a copy to the device does not stop the host: page-locked memory of its own, which PyTorch hands
+        out again only once copies from it are done, so `host` may change meanwhile."""
+        if self.device.type != "cuda":
+            return host
+        return torch.empty(host.shape, dtype=host.dtype, pin_memory=True).copy_(host)
+
+    def _sent(self, host: torch.Tensor) -> torch.Tensor:
+        return self._staged(host).to(self.device, non_blocking=True)
 
     # ------------------------------------------------------------ accounting
     def tokens_held(self) -> int:

@@ -1,5 +1,5 @@
 """Steps of whole models over the 8-bit cache: a looped design whose values are its keys, with state beside the cache; layers that
-see a window and give pages back."""
+see a window and give pages back; steps on the device that do not stop the host."""
 import numpy as np
 import pytest
 import torch
@@ -8,6 +8,7 @@ import go_tinygrad_b200 as lib
 import plain_e4m3 as plain
 from conftest import make_prompts
 from go_tinygrad_b200.cache import KeepRule
+from go_tinygrad_b200.engine.decode import DecodeBatch
 from test_e4m3_gpu import BF16, DEV, F32, HALF_STEP
 from test_ropovik_gpu import CONFIG_P
 
@@ -178,3 +179,64 @@ def test_layers_that_see_a_window_give_pages_back(model_folders, name, dtype, wi
         checked_step(model, cache, entries, dtype, None, window=window)
     assert [cache.length(s) for s in slots] == [356, 167]
     assert cache.free_pages()[0] >= free - 2 * ((window + 63) // 64 + 1)          # what two windows touch is all that is held
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_device_steps_do_not_stop_the_host(model_folders, dtype):
+    """Steps that feed back their own tokens, across evictions and into pages taken anew: no call waits for the device."""
+    model = lib.Model.load(model_folders["A"], dtype=dtype, device="cuda")
+    keep = KeepRule(64, 16, slack=20)
+    prompts = make_prompts("A", [70, 5, 60], seed=8)
+
+    def run(watched):
+        cache = model.new_cache(64 * 16, 3, kv_format="e4m3", keep=keep)
+        slots = [cache.open_sequence() for _ in prompts]
+        lib.step(model, cache, [lib.StepEntry(s, p, []) for s, p in zip(slots, prompts)])
+        batch = DecodeBatch(model, cache, slots, [0, 1, 2], lib.Sampler())
+        tokens = [batch.step_host([5, 6, 7], [1, 1, 1])]
+        picked = [torch.empty_like(batch.sampled) for _ in range(60)]
+        for t in picked[:3]:                               # the step is recorded
+            batch.step_device()
+            t.copy_(batch.sampled)
+        batch.reserve_ahead(60)
+        torch.cuda.synchronize()
+        mode = torch.cuda.get_sync_debug_mode()
+        evictions, evict = [], cache.evict
+        cache.evict = lambda which, *a, **kw: (evictions.append(list(which)), evict(which, *a, **kw))[1]
+        try:
+            if watched:
+                torch.cuda.set_sync_debug_mode("error")
+            for t in picked[3:]:
+                batch.step_device()
+                t.copy_(batch.sampled)
+        finally:
+            torch.cuda.set_sync_debug_mode(mode)
+            del cache.evict
+        assert len(evictions) >= 4 and all(cache.held(s) < keep.most for s in slots)
+        return tokens + [t.tolist() for t in picked]
+    assert run(True) == run(False)
+
+
+@pytest.mark.parametrize("kv_format", [None, "e4m3"])
+def test_block_tables_copied_on_another_stream(model_folders, kv_format):
+    """Pages taken for two sequences, whose rows one stream's step copies for both; the other's step, on a stream of its own, waits for
+    the copy and for nothing else."""
+    model = lib.Model.load(model_folders["A"], dtype="float32", device="cuda")
+    prompts = make_prompts("A", [130, 90], seed=11)
+    want = [lib.step(model, c, [lib.StepEntry(c.open_sequence(), p, [len(p) - 1])]) for p in prompts for c in [model.new_cache(64 * 8, 2, kv_format=kv_format)]]
+    for _ in range(3):
+        cache = model.new_cache(64 * 8, 2, kv_format=kv_format)
+        slots = [cache.open_sequence() for _ in prompts]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in prompts]
+        cache.reserve_many([(s, len(p)) for s, p in zip(slots, prompts)])
+        with torch.cuda.stream(streams[0]):
+            torch.cuda._sleep(20_000_000)                  # the copy waits behind this
+            cache.flush_tables()
+        got = []
+        for stream, s, p in zip(streams[::-1], slots[::-1], prompts[::-1]):
+            with torch.cuda.stream(stream):
+                got.append(lib.step(model, cache, [lib.StepEntry(s, p, [len(p) - 1])]))
+            stream.synchronize()                           # (a model's steps share its workspace)
+        for a, b in zip(got[::-1], want):
+            assert torch.equal(a, b)
