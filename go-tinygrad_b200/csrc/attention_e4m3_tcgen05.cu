@@ -171,7 +171,10 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     const int q_begin = a.cu_seqlens[b];
     const int q_len = a.cu_seqlens[b + 1] - q_begin;
     const int n_rows = q_len * a.group;
-    if (row_begin >= n_rows) return;                             // before any barrier or tensor memory
+    if (row_begin >= n_rows) {                                   // before any barrier or tensor memory
+        if (blockIdx.x + blockIdx.y + blockIdx.z == 0) chain_wait();     // (one block waits whatever there is to do, so that a grid
+        return;                                                  // of nothing is not complete before the kernel it stands behind)
+    }
     const uint32_t base = smem_addr(smem);
     if (base & 1023u) {
         if (threadIdx.x == 0) atomicExch(&g_status, 2);
@@ -690,7 +693,10 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
     const int q_len = a.cu_seqlens[b + 1] - q_begin;
     const int slot = a.slots[b];
     const int start = a.start_pos[b] - (kv.dropped ? kv.dropped[slot] : 0);
-    if (q_len <= 0 || (int)blockIdx.x * 128 >= start + q_len) return;
+    if (q_len <= 0 || (int)blockIdx.x * 128 >= start + q_len) {
+        if (blockIdx.x + blockIdx.y + blockIdx.z == 0) chain_wait();     // as above
+        return;
+    }
     const uint32_t base = smem_addr(smem);
     if (base & 1023u) {
         if (threadIdx.x == 0) atomicExch(&g_status, 2);

@@ -1,4 +1,4 @@
-"""Calls of the 8-bit cache from two threads at once, each on a stream and a cache of its own."""
+"""Calls of the 8-bit cache from two threads at once, each on a stream and a cache of its own, and the order of chained kernels."""
 import threading
 
 import pytest
@@ -62,3 +62,28 @@ def test_two_threads(dtype, new):
         assert len(got[i]) == 25 * n
         for at, x in enumerate(got[i]):
             assert torch.equal(x, want[i][at % n]), (i, at)
+
+
+@pytest.mark.parametrize("weights", [False, True])
+def test_a_prompt_step_of_no_tokens_keeps_the_order(weights):
+    """Chained kernels: rotation of many rows that are nobody's, attention of sequences that bring nothing, and a second rotation into
+    the last of those rows, which must come last."""
+    heads, hd, n = 32, 128, 6000
+    p = Pages([300, 70], 2, hd, seed=4, weights=weights)
+    nothing = ints([0, 0, 0])
+    first, second = torch.randn(n, heads * hd, device=DEV).bfloat16(), torch.randn(8, heads * hd, device=DEV).bfloat16()
+    qkv = torch.cat([first, torch.zeros(n, 4 * hd, device=DEV).bfloat16()], 1)
+    other = torch.cat([second, torch.zeros(8, 4 * hd, device=DEV).bfloat16()], 1)
+    before = [x.clone() for x in (p.k.view(torch.uint8), p.v.view(torch.uint8), p.scales)]
+    kv, slots, start, out = p.view(), ints(p.slots), ints([300, 70]), torch.full((n, heads * hd), 7.0, device=DEV).bfloat16()
+    q = torch.empty(n, heads * hd, dtype=BF16, device=DEV)
+    with ops.chained_launches():
+        for _ in range(20):
+            q.zero_()
+            ops.kv_store_e4m3(qkv, None, heads, 2, kv, nothing, slots, start, 200, q)
+            ops.attention_e4m3(q, out, kv, nothing, slots, start, 200, heads, 0.1, max_kv_len=300)
+            ops.kv_store_e4m3(other, None, heads, 2, kv, nothing, slots, start, 200, q[n - 8:])
+            assert torch.equal(q[: n - 8], first[: n - 8]) and torch.equal(q[n - 8:], second)
+    assert (out == 7.0).all() and all(torch.equal(a, b) for a, b in zip(before, (p.k.view(torch.uint8), p.v.view(torch.uint8), p.scales)))
+    if weights:
+        assert (p.read_weights(0, 0, 300).astype("float32") == p.gathered[0][0].astype("float32")).all()
