@@ -803,23 +803,29 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                 continue;
             }
             // ---- the tile's keys (all products of the turn before are complete: this warp has seen the last one's barrier)
+            const bool both = (kt * 2 + 1) * kPageTokens < start + q_len;                       // the tile's second page exists too
+            const size_t pages[2] = {(size_t)table[kt * 2], both ? (size_t)table[kt * 2 + 1] : 0};
+            const float k_scales[2] = {kv.scales[pages[0] * kv.scale_stride + h], both ? kv.scales[pages[1] * kv.scale_stride + h] : 0.f};
+            uint4 u[HD / 16];
+#pragma unroll
+            for (int m = 0; m < HD / 16; ++m) {                  // (all asked for before the first is waited for)
+                u[m] = make_uint4(0, 0, 0, 0);
+                if (!kExact && m >= hd / 16) continue;
+                const int id = r + 128 * m, key = id / (hd / 16), piece = id - key * (hd / 16);
+                if (key < kPageTokens || both)
+                    u[m] = *reinterpret_cast<const uint4*>(kv.k + (key < kPageTokens ? pages[0] : pages[1]) * kv.k_stride +
+                                                           ((size_t)h * kPageTokens + key % 64) * hd + piece * 16);
+            }
+            const float times[2] = {key_factor(k_scales[0]), key_factor(k_scales[1])};
 #pragma unroll
             for (int m = 0; m < HD / 16; ++m) {
                 if (!kExact && m >= hd / 16) break;
                 const int id = r + 128 * m, key = id / (hd / 16), piece = id - key * (hd / 16);
-                const int j = kt * 2 + key / 64;
-                uint4 u = make_uint4(0, 0, 0, 0);
-                float times = 0.f;
-                if (j * kPageTokens < start + q_len) {
-                    const size_t page = table[j];
-                    u = *reinterpret_cast<const uint4*>(kv.k + page * kv.k_stride + ((size_t)h * kPageTokens + key % 64) * hd + piece * 16);
-                    times = key_factor(kv.scales[page * kv.scale_stride + h]);
-                }
                 uint32_t o[8];
-                bf16_of_codes(u.x, times, o[0], o[1]);
-                bf16_of_codes(u.y, times, o[2], o[3]);
-                bf16_of_codes(u.z, times, o[4], o[5]);
-                bf16_of_codes(u.w, times, o[6], o[7]);
+                bf16_of_codes(u[m].x, key < kPageTokens ? times[0] : times[1], o[0], o[1]);
+                bf16_of_codes(u[m].y, key < kPageTokens ? times[0] : times[1], o[2], o[3]);
+                bf16_of_codes(u[m].z, key < kPageTokens ? times[0] : times[1], o[4], o[5]);
+                bf16_of_codes(u[m].w, key < kPageTokens ? times[0] : times[1], o[6], o[7]);
                 const uint32_t at = base + (piece / 4) * (128 * 128) + key * 128;
                 store_shared16(at + (((piece % 4 * 2) ^ (key & 7)) << 4), o[0], o[1], o[2], o[3]);
                 store_shared16(at + (((piece % 4 * 2 + 1) ^ (key & 7)) << 4), o[4], o[5], o[6], o[7]);
@@ -827,9 +833,9 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(k_full);
-            const size_t page = there ? table[row / kPageTokens] : 0;
-            const float k_scale = there ? kv.scales[page * kv.scale_stride + h] : 0.f;
-            const float f = a.scale * kLog2e * (k_scale * pow2_inverse(key_factor(k_scale)));
+            const size_t page = r < kPageTokens ? pages[0] : pages[1];
+            const float k_scale = r < kPageTokens ? k_scales[0] : k_scales[1];
+            const float f = there ? a.scale * kLog2e * (k_scale * pow2_inverse(key_factor(k_scale))) : 0.f;
             auto statistic = [&](int i) {                        // of tile i's column r: what takes a score to its probability's exponent
                 const int token = sp.t_lo + i % sp.per_head * 128 + r;
                 if (i >= tiles || token >= sp.t_hi) return 0.f;
