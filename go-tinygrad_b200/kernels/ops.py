@@ -1685,7 +1685,7 @@ def attention_decode_bf16(q, out, kv, slots, positions, n_heads: int, scale: flo
 
 
 # ------------------------------------------------------------ the 8-bit key/value cache
-E4M3_MAX_CHANNELS = 256       # of a head
+E4M3_MAX_CHANNELS = 256       # of a head that the attention takes
 
 
 def _need_e4m3(kv, what: str, q, slots, start_pos, cu_seqlens) -> None:
@@ -1839,6 +1839,8 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kv, cu_seqlens: torch.Ten
         raise KernelError("attention_e4m3: q and out must be [N, n_heads * head_dim] of one dtype")
     if out.get_device() != q.get_device():
         raise KernelError("attention_e4m3: out must be on the cache's device")
+    if hd > E4M3_MAX_CHANNELS:
+        raise KernelError(f"attention_e4m3: takes heads of up to {E4M3_MAX_CHANNELS} channels, not {hd}")
     if n_heads <= 0 or n_heads % kv.n_kv_heads:
         raise KernelError(f"attention_e4m3: {n_heads} query heads cannot share {kv.n_kv_heads} key/value heads")
     if N and (max_q_len < 1 or max_kv_len < 1):

@@ -232,7 +232,7 @@ class GQAttention(Mixer):
             return [KVRequest(self.n_kv, 2 * self.head_dim, self.cache_window, value_dim=self.value_dim)]
         if self.general:
             return [KVRequest(self.n_kv, self.head_dim, self.cache_window, value_dim=self.value_dim, chunk=self.chunk)]
-        return [KVRequest(self.n_kv, self.head_dim, self.cache_window, e4m3=not self.rows_route)]
+        return [KVRequest(self.n_kv, self.head_dim, self.cache_window, e4m3=not self.rows_route and self.head_dim <= ops.E4M3_MAX_CHANNELS)]
 
     def load(self, tensors: Mapping[str, torch.Tensor], rt: Runtime) -> None:
         parts = [tensors[self.names["q"]]]

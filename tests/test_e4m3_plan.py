@@ -47,3 +47,24 @@ def test_steps_that_differ_in_all_rows_only_ask_once(monkeypatch):
         assert len(asked) == 2
     finally:
         ops._e4m3_few_scratch.cache_clear()
+
+
+def test_heads_that_the_attention_does_not_take():
+    """A model with larger heads is refused when its cache is made, not in its first step; at the limit it is served."""
+    from conftest import TINY_A
+    from go_tinygrad_b200.config.registry import find_architecture
+    from go_tinygrad_b200.engine.model import Model
+    from go_tinygrad_b200.kernels import KernelError
+    from go_tinygrad_b200.parts.base import Runtime
+    arch = find_architecture(TINY_A)
+    for dim in (256, 258, 320):
+        model = Model(arch.plan(arch.read_config(dict(TINY_A, head_dim=dim))), Runtime(torch.device("cpu"), torch.bfloat16))
+        assert all(h.kv.head_dim == dim for h in model.new_cache(128, 1).handles)
+        if dim <= ops.E4M3_MAX_CHANNELS:
+            assert all(h.kv.format == "e4m3" for h in model.new_cache(128, 1, kv_format="e4m3").handles)
+        else:
+            with pytest.raises(ValueError, match="entry 0 asks for keys and values that its mixer does not read"):
+                model.new_cache(128, 1, kv_format="e4m3")
+    q, one = torch.zeros(1, 4 * 272), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(KernelError, match="up to 256 channels, not 272"):
+        ops.attention_e4m3(q, torch.zeros_like(q), view(dim=272), torch.tensor([0, 1], dtype=torch.int32), one, one, 1, 4, 0.1, max_kv_len=1)
