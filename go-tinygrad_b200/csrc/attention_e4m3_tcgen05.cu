@@ -16,9 +16,10 @@
 // not (a block of zeros among others, for one), v_j counts as w - 96 and the codes are made smaller for it.
 // M is raised only when a step's sum of P exceeds 2^15, so P, times 2^7 besides, stays below half's largest number.
 // Where that makes fewer blocks than multiprocessors, several share a pair of tiles' pages and leave their results to a joining kernel.
-// What bounds it is the softmax: its exponentials alone are 1,024 cycles of the 2,500 that a step of both tiles takes, its wait for
-// scores 400 to 540, their products 800.  Measured on a B200: 2,048 tokens, 32 heads of 64: 56 us; 512 tokens behind 7,680,
-// 2 sequences, 8 kv heads of 128 under 32: 165 us, 0.83 of what the same kernel for a bfloat16 cache takes in the second case and
+// No one unit bounds it: of the 2,500 cycles that a step of both tiles takes, the exponentials fill 1,024 (over a whole call their unit is
+// 32 to 42 % busy) and the products 660 (64 channels) to 1,350 (128); the rest is warps waiting for one another's results, 400 to 540
+// of it the softmax's for its scores.  Measured on a B200: 2,048 tokens, 32 heads of 64: 55 us; 512 tokens behind 7,680,
+// 2 sequences, 8 kv heads of 128 under 32: 168 us, 0.84 of what the same kernel for a bfloat16 cache takes in the second case and
 // 1.2 of it in the first, where the blocks' begins count.  Steps on the way there, in the second case: 128 rows a block, two threads
 // a row 257; issuing from warps of their own 180; codes straight to registers instead of through shared memory 177; two
 // threads a row again, with 24 warps, 195.  Every wait is bounded (status word as in the products).
@@ -654,7 +655,8 @@ int launch(const PromptArgs& a, const E4M3Pages& kv, int B, int max_q_len, cudaS
 //          the largest of them, before the key scale makes them small, left float's range;
 //   Q      128 tokens of one head at a time by tensor copies through a ring, as they are (bfloat16);
 //   sums   four warps, S from tensor memory, 1 / l folded into the exponent: one multiply-add, one exponential and one add a
-//          score.  The exponentials bound it (16 a cycle).
+//          score.  No unit is full (exponentials 39 % of theirs, issue slots 41 %): a sub-partition has one such warp a block, two
+//          in all, which reads 32 columns, waits for them, and adds.
 // A block a head of the group leaves its sums beside the others', and a second kernel adds them in the heads' order (a block for
 // all heads: one block's 48 tiles were the time of all, 95 us of 147 for prompts of 200 to 1,500 tokens).  So a weight does
 // not depend on what else runs.

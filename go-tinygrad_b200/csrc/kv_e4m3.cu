@@ -257,9 +257,10 @@ kv_evict_kernel(const E4M3Pages pages, const EvictStrides strides, int* __restri
 // their way while a tile is worked on (what a tile overwrites no later one reads).  The rows of the values are innermost, so
 // a value tile is gathered out of whole pages in shared memory, each copied there once: a thread has the same four rows of
 // the tile in several channels, and a word of four codes comes out of the four words that hold them by three byte permutations.
-// What bounds it is instructions: 24 entries x 3 sequences of 2,000 rows x 32 heads of 64 take 337 us on a B200, their 875 MB
-// would take 136.  Eight warps, each with twice the channels that sixteen have, because much of a tile's work is the same for
-// all its channels (sixteen: 440 us; eight cost 2 us of 17 where there are fewer blocks than multiprocessors).
+// What bounds it is instructions: 24 entries x 3 sequences of 2,000 rows x 32 heads of 64 take 256 us on a B200 with 71 % of the issue
+// slots busy; the 680 MB that reach memory (blocks of which nothing moves are left alone) would take 106.  Eight warps, each with
+// twice the channels that sixteen have, because much of a tile's work is the same for all its channels (an earlier form: 440 us with
+// sixteen, 337 with eight; eight cost 2 us of 17 where there are fewer blocks than multiprocessors).
 constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32, kPlaneThreads = kMoveThreads / 2;
 constexpr int kStaged = 4;                 // value pages in shared memory: two that a tile is gathered from, two on their way
 template <int HD> struct Move {
