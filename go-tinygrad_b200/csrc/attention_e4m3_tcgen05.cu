@@ -14,7 +14,9 @@
 // maximum of x, P_j = 2^(x_j - M) and O = sum P_j code_j.  The sum is l = sum P_j 2^(w - v_j) = sum 2^(score_j - M + w), w the
 // largest v of the block's pages, and O 2^w / l the result.  Where v_j is so far below w that P_j could be 0 while its probability is
 // not (a block of zeros among others, for one), v_j counts as w - 96 and the codes are made smaller for it.
-// M is raised only when a step's sum of P exceeds 2^15, so P, times 2^7 besides, stays below half's largest number.
+// M is raised only when a step's sum of P exceeds 2^15, so P, times 2^7 besides, stays below half's largest number.  From |M| = 2^20 on
+// M's own rounding counts, and v_j would get lost in it: M is also kept as the score and the v that it came of, and scores, rounded
+// as that one was, are compared with it apart from the v.  So rows of one score have one probability, however large it is.
 // Where that makes fewer blocks than multiprocessors, several share a pair of tiles' pages and leave their results to a joining kernel.
 // No one unit bounds it: of the 2,500 cycles that a step of both tiles takes, the exponentials fill 1,024 (over a whole call their unit is
 // 32 to 42 % busy) and the products 660 (64 channels) to 1,350 (128); the rest is warps waiting for one another's results, 400 to 540
@@ -45,7 +47,7 @@ constexpr int kMostApart = 96;                           // powers of two that a
 // take no more than that part.
 template <int HD> struct Shape {
     static constexpr int kQBytes = BQ * HD * 2, kTileBytes = BK * HD * 2;
-    static constexpr int kOffK = 2 * kQBytes, kOffV = kOffK + 2 * kTileBytes, kOffBar = kOffV + 2 * kTileBytes;
+    static constexpr int kOffK = 2 * kQBytes, kOffV = kOffK + 2 * kTileBytes, kOffM = kOffV + 2 * kTileBytes, kOffBar = kOffM + 2 * BQ * 8;
     static constexpr int kSmemBytes = kOffBar + 256;
     static constexpr int kColO = BK, kColP = BK + HD;    // of a tile's tensor memory: S, O, two of P
     static_assert(BK + HD + BK <= kTileCols, "tensor memory");
@@ -65,10 +67,10 @@ struct PromptArgs {
     int n_heads, group;
     float scale;
     int window;
-    float2* stats;               // [token][head]: what a score (in powers of two) is compared with, and the sum; or null
+    float2* stats;               // [token][head]: s, M's score, and c, or null: a row's probability is 2^(score - s + c)
     int splits;                  // blocks that share a tile pair's pages
     float* part_o;               // [token][head][split][channel]: their results, where there are several,
-    float2* part_stats;          // [token][head][split]: and statistics; a sum of 0 where the split saw no row
+    float2* part_stats;          // [token][head][split]: and statistics; s is -infinity where the split saw no row
 };
 
 __device__ __forceinline__ void store_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -217,7 +219,7 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
             chain_wait();
             if (threadIdx.x < 2 * BQ && row_begin + (int)threadIdx.x < n_rows) {
                 const int row = row_begin + threadIdx.x;
-                a.part_stats[((size_t)(q_begin + row / a.group) * a.n_heads + h * a.group + row % a.group) * a.splits + split] = make_float2(0.f, 0.f);
+                a.part_stats[((size_t)(q_begin + row / a.group) * a.n_heads + h * a.group + row % a.group) * a.splits + split] = make_float2(-INFINITY, 0.f);
             }
             return;
         }
@@ -441,6 +443,9 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
         // scales, 32 steps at a time: lane l has those of step (i / 32 * 32 + l)
         float k_scales = 0.f, v_scales = 1.f;
         float m_run = -INFINITY, l_run = 0.f;
+        // what M is the sum of, score and v: touched only where M is raised or large, so not kept in registers (5 us of 170 there)
+        float2* made_of = reinterpret_cast<float2*>(smem + S::kOffM) + tt * BQ + r;
+        *made_of = make_float2(-INFINITY, 0.f);
         uint32_t sv[BK];
         bool ok = true;
         for (int i = 0; i < n_steps; ++i) {
@@ -495,20 +500,23 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                 }
                 sum = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
             };
-            const bool fresh = __any_sync(full, m_run == -INFINITY);
-            if (!fresh) exponentials(sl, add - m_run + kPShift);
-            if (fresh || __any_sync(full, first_of(sum) + second_of(sum) > kMostSum)) {
+            const bool careful = __any_sync(full, fabsf(m_run) > kLargeScore);       // (-infinity: a row that has seen nothing)
+            if (!careful) exponentials(sl, add - m_run + kPShift);
+            if (careful || __any_sync(full, first_of(sum) + second_of(sum) > kMostSum)) {
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < BK; c += 8)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sv[c + e]), __uint_as_float(sv[c + 4 + e]));
-                const float m_step = fmaf(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), sl, add);
-                const bool raise = m_step > m_run;
+                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), m_step = fmaf(top, sl, add), score = __fmul_rn(top, sl);
+                const bool apart = fabsf(m_run) > kLargeScore || fabsf(m_step) > kLargeScore;
+                float up = m_step - m_run;                        // how much larger this step's is
+                if (apart) up = (score - made_of->x) + (add - made_of->y);
                 float corr = 1.0f;
-                if (raise) {
-                    corr = fast_exp2(m_run - m_step);             // 0 for a row that has seen nothing
+                if (up > 0.f) {
+                    corr = fast_exp2(-up);                        // 0 for a row that has seen nothing
                     m_run = m_step;
+                    *made_of = make_float2(score, add);
                     l_run *= corr;
                 }
                 if (i > 0) {                                      // O may only be touched between products
@@ -527,10 +535,10 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
                 }
                 const float m_use = m_run == -INFINITY ? 0.f : m_run;
                 float mult = sl, shift = add - m_use + kPShift;
-                if (__any_sync(full, fabsf(m_use) > 4194304.0f)) {
-                    // M's own rounding is a quarter and more here: take it from scores rounded as it was, which leaves 0 for its row
+                if (__any_sync(full, fabsf(m_use) > kLargeScore)) {
+                    const float from = made_of->x == -INFINITY ? 0.f : made_of->x, apart_by = add - made_of->y;
 #pragma unroll
-                    for (int c = 0; c < BK; ++c) sv[c] = __float_as_uint(fmaf(__uint_as_float(sv[c]), sl, add) - m_use);
+                    for (int c = 0; c < BK; ++c) sv[c] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(sv[c]), sl), from) + apart_by);
                     mult = 1.0f;
                     shift = kPShift;
                 }
@@ -547,7 +555,8 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
         if (ok) {
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::);
             const float inv = 1.0f / l_run, unit = __uint_as_float(__float_as_uint(v_least) + ((uint32_t)kMostApart << 23));    // 2^w
-            const float2 stat = make_float2(m_run == -INFINITY ? 0.f : m_run - (float)((int)(__float_as_uint(unit) >> 23) - 127) - kPShift, l_run);
+            // P = 2^(score - s + v_j - v + 7), v that of M, and the probability is P 2^(w - v_j) / l
+            const float2 stat = make_float2(made_of->x, (float)((int)(__float_as_uint(unit) >> 23) - 127) + kPShift - made_of->y - log2f(l_run));
             const size_t at = (size_t)(q_begin + token) * a.n_heads + head;
             const bool in_parts = a.splits > 1;
             if (real && in_parts) a.part_stats[at * a.splits + split] = stat;
@@ -604,7 +613,8 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
     }
 }
 
-// Joins the blocks that shared a tile pair's pages: their results, each with the mass 2^x l that its statistics say.
+// Joins the blocks that shared a tile pair's pages: their results, each with the mass 2^(s - c) that its statistics say, relative to
+// the largest.  s and c are subtracted apart: next to a large s c would be lost.
 __global__ void __launch_bounds__(256)
 e4m3_prompt_join_kernel(const PromptArgs a, int B, int N, int hd) {
     chain_release();
@@ -616,17 +626,19 @@ e4m3_prompt_join_kernel(const PromptArgs a, int B, int N, int hd) {
     if (token >= N || token < a.cu_seqlens[0] || token >= a.cu_seqlens[B]) return;
     const float2* stats = a.part_stats + row * a.splits;
     const float* o = a.part_o + row * a.splits * hd + d;
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s)
-        if (stats[s].y != 0.f) top = fmaxf(top, stats[s].x + log2f(stats[s].y));
+    float2 top = make_float2(-INFINITY, 0.f);
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 st = stats[s];
+        if (st.x != -INFINITY && !(st.x - st.y <= top.x - top.y)) top = st;
+    }
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float mass = 0.f;
 #pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
         const float2 st = stats[s];
         const float4 v = *reinterpret_cast<const float4*>(o + (size_t)s * hd);
-        if (st.y == 0.f) continue;
-        const float f = fast_exp2(st.x + log2f(st.y) - top);
+        if (st.x == -INFINITY) continue;
+        const float f = fast_exp2(min_or_nan((st.x - top.x) - (st.y - top.y), 64.f));     // (above 0 only as far as the choice was rounded)
         mass += f;
         acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
     }
@@ -634,7 +646,7 @@ e4m3_prompt_join_kernel(const PromptArgs a, int B, int N, int hd) {
     const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
     *reinterpret_cast<uint2*>(a.out + (size_t)token * a.ldo + (size_t)head * hd + d) =
         make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-    if (a.stats && d == 0) a.stats[row] = make_float2(top, mass);
+    if (a.stats && d == 0) a.stats[row] = make_float2(top.x, top.y - log2f(mass));
 }
 
 template <int HD, bool kExact, bool kTest>
@@ -647,16 +659,17 @@ int launch(const PromptArgs& a, const E4M3Pages& kv, int B, int max_q_len, cudaS
                           (size_t)Shape<HD>::kSmemBytes, stream, a, kv);
 }
 // ============================================================== gathered weights of prompts and chunks
-// weight_j += sum over the queries that see row j, of all heads of the group, of 2^(score - x) / l, x and l the query's
+// weight_j += sum over the queries that see row j, of all heads of the group, of 2^(score - s + c), s and c the query's
 // statistics that the attention left.  The products again, the other way round: one block per (128 rows of the cache, query
 // head, sequence), the rows as the tile's rows, so that a thread owns a row and its sum:
 //   K      converted once to bfloat16 into shared memory, S = K Q^T by tcgen05.mma 128 x 128 x head size.  Not the codes but the keys
 //          they stand for, 2^-32 of them (exact: bfloat16 has float's range): queries come as they are, and the codes' products with
 //          the largest of them, before the key scale makes them small, left float's range;
 //   Q      128 tokens of one head at a time by tensor copies through a ring, as they are (bfloat16);
-//   sums   four warps, S from tensor memory, 1 / l folded into the exponent: one multiply-add, one exponential and one add a
-//          score.  No unit is full (exponentials 39 % of theirs, issue slots 41 %): a sub-partition has one such warp a block, two
-//          in all, which reads 32 columns, waits for them, and adds.
+//   sums   four warps, S from tensor memory, c - s one number a query: one multiply-add, one exponential and one add a
+//          score.  Tiles with a query whose |s| is large take a form of their own, in which a score that may be s is s (score_slack).
+//          No unit is full (exponentials 39 % of theirs, issue slots 41 %):
+//          a sub-partition has one such warp a block, two in all, which reads 32 columns, waits for them, and adds.
 // A block a head of the group leaves its sums beside the others', and a second kernel adds them in the heads' order (a block for
 // all heads: one block's 48 tiles were the time of all, 95 us of 147 for prompts of 200 to 1,500 tokens).  So a weight does
 // not depend on what else runs.
@@ -665,7 +678,7 @@ constexpr int kWeightThreads = 192;                      // sums 0-3, copies 4, 
 template <int HD> struct WeightShape {
     static constexpr int kStages = HD == 64 ? 3 : 2;
     static constexpr int kTileBytes = 128 * HD * 2;      // 128 rows of keys, or of queries
-    static constexpr int kOffQ = kTileBytes, kOffY = kOffQ + kStages * kTileBytes, kOffBar = kOffY + 2 * 128 * 4;
+    static constexpr int kOffQ = kTileBytes, kOffY = kOffQ + kStages * kTileBytes, kOffC = kOffY + 2 * 128 * 4, kOffBar = kOffC + 2 * 128 * 8;
     static constexpr int kSmemBytes = kOffBar + 256;
 };
 
@@ -713,12 +726,13 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
     auto y_full = [&](int s) { return bars + 88u + 8u * s; };
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + S::kOffBar + 128);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kOffBar + 136);
+    volatile int* large_tile = reinterpret_cast<volatile int*>(smem + S::kOffBar + 144);     // by buffer: 1 + the last tile with a large |s|
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int* table = kv.block_table + (size_t)slot * kv.table_stride;
     if (threadIdx.x == 0) {
         mbar_init(k_full, 4);
         for (int s = 0; s < S::kStages; ++s) { mbar_init(q_full(s), 1); mbar_init(q_free(s), 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(s_full(s), 1); mbar_init(s_free(s), 4); mbar_init(y_full(s), 4); }
+        for (int s = 0; s < 2; ++s) { mbar_init(s_full(s), 1); mbar_init(s_free(s), 4); mbar_init(y_full(s), 4); large_tile[s] = 0; }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::);
     }
@@ -791,7 +805,8 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
     } else {
         const unsigned full = 0xffffffffu;
         const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
-        float* y = reinterpret_cast<float*>(smem + S::kOffY);
+        float* y = reinterpret_cast<float*>(smem + S::kOffY);                           // by buffer and column: c - s,
+        float2* apart = reinterpret_cast<float2*>(smem + S::kOffC);                     // and s and c
         const int r = threadIdx.x;                               // row of the tile; also a column of the next tile's statistics
         bool ok = true;
         for (int kt = blockIdx.x; kt * 128 < start + q_len && ok; kt += gridDim.x) {
@@ -838,16 +853,18 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
             const size_t page = r < kPageTokens ? pages[0] : pages[1];
             const float k_scale = r < kPageTokens ? k_scales[0] : k_scales[1];
             const float f = there ? a.scale * kLog2e * (k_scale * pow2_inverse(key_factor(k_scale))) : 0.f;
-            auto statistic = [&](int i) {                        // of tile i's column r: what takes a score to its probability's exponent
+            auto statistic = [&](int i) {                        // of tile i's column r
                 const int token = sp.t_lo + i % sp.per_head * 128 + r;
-                if (i >= tiles || token >= sp.t_hi) return 0.f;
-                const float2 st = a.stats[(size_t)(q_begin + token) * a.n_heads + h * a.group + g0 + i / sp.per_head];
-                return score_slack(st.x) - (st.x + log2f(st.y));
+                if (i >= tiles || token >= sp.t_hi) return make_float2(0.f, 0.f);
+                return a.stats[(size_t)(q_begin + token) * a.n_heads + h * a.group + g0 + i / sp.per_head];
             };
-            float mine = statistic(0), total = 0.f;
+            float2 mine = statistic(0);
+            float total = 0.f;
             for (int i = 0; i < tiles; ++i, ++n) {
                 const int buf = n & 1;
-                y[128 * buf + r] = mine;
+                y[128 * buf + r] = mine.y - mine.x;
+                apart[128 * buf + r] = mine;
+                if (fabsf(mine.x) > kLargeScore) large_tile[buf] = n + 1;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(y_full(buf));
                 mine = statistic(i + 1);
@@ -862,8 +879,9 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                 const int hi = (int)min(past, 128LL);
                 const bool whole = __all_sync(full, lo == 0 && hi == 128);
                 const float* yt = y + 128 * buf;
+                const float4* at = reinterpret_cast<const float4*>(apart + 128 * buf);
                 uint64_t sum[2] = {0, 0};
-                auto add_up = [&](auto masked) {
+                auto add_up = [&](auto masked, auto large) {
                     const uint64_t f2 = two(f, f);
 #pragma unroll 1
                     for (int c = 0; c < 128; c += 32) {
@@ -873,9 +891,18 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
 #pragma unroll
                         for (int e = 0; e < 32; e += 4) {
                             const float4 y4 = *reinterpret_cast<const float4*>(yt + c + e);
-                            const uint64_t x[2] = {fma2(two(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), f2, two(y4.x, y4.y)),
-                                                   fma2(two(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])), f2, two(y4.z, y4.w))};
-                            // (no probability is above 1: the bound is for scores that lie within their roundings of the maximum)
+                            uint64_t x[2] = {fma2(two(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), f2, two(y4.x, y4.y)),
+                                             fma2(two(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])), f2, two(y4.z, y4.w))};
+                            if constexpr (decltype(large)::value) {
+                                auto exponent = [&](uint32_t score, float s, float own) {
+                                    const float d = fmaf(__uint_as_float(score), f, -s);
+                                    return own + (fabsf(d) <= score_slack(s) ? 0.f : d);
+                                };
+                                const float4 a = at[(c + e) / 2], b = at[(c + e) / 2 + 1];
+                                x[0] = two(exponent(sv[e], a.x, a.y), exponent(sv[e + 1], a.z, a.w));
+                                x[1] = two(exponent(sv[e + 2], b.x, b.y), exponent(sv[e + 3], b.z, b.w));
+                            }
+                            // (no probability is above 1: the bound is for what scores' roundings leave)
                             float p[4] = {fast_exp2(min_or_nan(first_of(x[0]), 0.f)), fast_exp2(min_or_nan(second_of(x[0]), 0.f)),
                                           fast_exp2(min_or_nan(first_of(x[1]), 0.f)), fast_exp2(min_or_nan(second_of(x[1]), 0.f))};
                             if constexpr (decltype(masked)::value) {
@@ -888,8 +915,9 @@ e4m3_weights_kernel(const __grid_constant__ CUtensorMap map_q, const PromptArgs 
                         }
                     }
                 };
-                if (whole) add_up(std::false_type());
-                else add_up(std::true_type());
+                if (large_tile[buf] == n + 1) add_up(std::true_type(), std::true_type());
+                else if (whole) add_up(std::false_type(), std::false_type());
+                else add_up(std::true_type(), std::false_type());
                 asm volatile("tcgen05.fence::before_thread_sync;\n" ::);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_free(buf));

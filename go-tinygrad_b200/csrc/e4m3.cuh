@@ -66,8 +66,9 @@ __device__ __forceinline__ float min_or_nan(float a, float b) {
 // Where a score is computed once more, by other instructions than those that found its query's maximum `top` (both in powers of two),
 // the two are apart by their sums' roundings.  From 2^20 on these are units: the winning row could come out at any probability
 // between 0 and 1, and so what lies within this much of the maximum counts as the maximum.  Sums of 128 products agree to a few
-// of the 64 steps of 2^-23 that this is; rows that lie nearer than that in truth are not told apart by float scores at all.
-__device__ __forceinline__ float score_slack(float top) { return fabsf(top) > 1048576.f ? fabsf(top) * 7.62939453125e-6f : 0.f; }
+// of the 64 steps of 2^-23 that this is; which of two rows that lie nearer is the larger, float scores cannot say.
+constexpr float kLargeScore = 1048576.f;
+__device__ __forceinline__ float score_slack(float top) { return fabsf(top) > kLargeScore ? fabsf(top) * 7.62939453125e-6f : 0.f; }
 
 // The least power of two 2^k, k >= -126, with most <= 448 * 2^k, for finite most >= 0: 448 = 1.75 * 2^8, so k is the
 // exponent less 8, one more where the mantissa exceeds 1.75.

@@ -3,8 +3,9 @@ import numpy as np
 import pytest
 import torch
 
+import plain_e4m3 as plain
 from go_tinygrad_b200.kernels import ops
-from test_e4m3_gpu import BF16, DEV, F32, Pages, cut, ints
+from test_e4m3_gpu import BF16, DEV, F32, HALF_STEP, Pages, cut, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +75,59 @@ def test_any_head_size_and_type(dtype, hd, size, key_size, new, held, loose):
 def test_few_queries(hd, size, key_size, new, held, loose):
     """`loose`: rows whose scores the plan has no room to keep, which are computed once more."""
     one_row_a_query(BF16, hd, new, held, size, key_size, loose=loose)
+
+
+def equal_rows(dtype, hd, new, held, size, key_size, sign, heads=2, loose=False, seed=8):
+    """Rows of one key among rows of another, whose scores are far below: the first share each query's probability evenly, however
+    large the score they have in common is, and the result is the mean of their values."""
+    rng = np.random.default_rng(seed)
+    p = Pages([held], 1, hd, seed=seed, weights=True)
+    k, v = p.rows[0][0]
+    k.codes, k.scales, v.codes, v.scales = np.zeros((0, hd)), [], np.zeros((0, hd)), []
+    low, high = np.sort(rng.uniform(1, 3, 2))
+    if sign < 0:
+        low, high = -high, -low                            # the larger score is the one nearer to zero
+    direction = rng.choice([-1.0, 1.0], hd) * rng.choice([1.0, 0.5, 0.25], hd)
+    wins = rng.random(held) < 0.7
+    wins[: held - new + 1: 5] = True
+    wins[0] = True
+    k.append(np.where(wins[:, None], high, low) * direction * key_size)
+    values = rng.standard_normal((held, hd))
+    values[::64] = 3.5                                     # a block has the least scale for that, or, with a larger value, the next
+    v.append(values)
+    p.gathered[0][0][:] = 0.0
+    p.write(0)
+    scale = hd ** -0.5
+    q = torch.from_numpy(np.tile(direction * size, (new, heads)) * rng.choice([1.0, 0.5], (new, 1))).to(dtype).to(DEV)
+    qs = q.double().cpu().numpy().reshape(new, heads, hd)
+    out = torch.empty_like(q)
+    ops.attention_e4m3(q, out, p.view(), cut([new]), ints(p.slots), ints([held - new]), new, heads, scale, max_kv_len=held // 3 if loose else held)
+    want, gathered = plain.attend(qs, k.values(), v.values(), held - new, scale)
+    spread = (np.abs(qs.reshape(-1, hd)) @ np.abs(k.values()).T).max() * scale
+    got = out.double().cpu().numpy().reshape(want.shape)
+    # the tied scores come out alike, whatever their roundings are; a probability is rounded to 11 bits, a result to its type
+    bound = np.abs(v.values()).max() * (2.0 ** -11 + held * 2.0 ** -24) + np.abs(want) * HALF_STEP[dtype] * (1 + 2.0 ** -7)
+    assert (np.abs(got - want) <= bound).all(), (np.abs(got - want) / bound).max()
+    off = 2 * (hd + 4) * 2.0 ** -23 * spread
+    rel = 2.0 ** -18 + held * 2.0 ** -22 + (2 * off if spread < 2.0 ** 17 else 0.0)
+    added = p.read_weights(0, 0, held)
+    assert (np.abs(added - gathered) <= gathered * rel + 2.0 ** -40).all(), (added.sum(), gathered.sum(), (np.abs(added - gathered) / (gathered + 1e-30)).max())
+
+
+TIED = [(2.0 ** 127, 2.0 ** -40), (2.0 ** 60, 2.0 ** -20), (2.0 ** 20, 2.0 ** 60), (2.0 ** 20, 2.0 ** 3), (2.0 ** 20, 2.0 ** -1), (2.0 ** 9, 1.0)]
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("hd", [64, 128, 48])
+@pytest.mark.parametrize("size,key_size", TIED)
+@pytest.mark.parametrize("new,held,loose", [(70, 200, False), (40, 1500, False), (300, 700, False), (70, 900, True)])
+def test_prompts_share_evenly(sign, hd, size, key_size, new, held, loose):
+    equal_rows(BF16, hd, new, held, size, key_size, sign, loose=loose)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype,hd", [(F32, 64), (F32, 20), (BF16, 20), (BF16, 64), (BF16, 128)])
+@pytest.mark.parametrize("size,key_size", TIED)
+@pytest.mark.parametrize("new,held,loose", [(1, 200, False), (5, 900, False), (5, 900, True), (1, 1500, False)])
+def test_few_tokens_share_evenly(sign, dtype, hd, size, key_size, new, held, loose):
+    equal_rows(dtype, hd, new, held, size, key_size, sign, loose=loose)
