@@ -217,7 +217,7 @@ int launch_row_weights(const void* q, int ldq, const E4M3Pages& kv, const int* c
 }
 
 // Blocks a (token, query head) has: as many as make four a multiprocessor, of 512 rows and more (float, 8 heads of 64 over 16,000 rows:
-// 19.5 us where one block each takes 190; over 1,100: 13.8 and 17.3).
+// 19.5 us where one block each takes 190; over 1,100: 13.9 and 17.6).
 int rows_splits(int N, int n_heads, int max_kv_len, int window) {
     const long long seen = window > 0 ? std::min(window, max_kv_len) : max_kv_len;
     return (int)std::max(1LL, std::min(4LL * 148 / ((long long)N * n_heads), seen / 512));

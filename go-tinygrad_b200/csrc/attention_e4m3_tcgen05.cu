@@ -20,8 +20,8 @@
 // Where that makes fewer blocks than multiprocessors, several share a pair of tiles' pages and leave their results to a joining kernel.
 // No one unit bounds it: of the 2,500 cycles that a step of both tiles takes, the exponentials fill 1,024 (over a whole call their unit is
 // 32 to 42 % busy) and the products 660 (64 channels) to 1,350 (128); the rest is warps waiting for one another's results, 400 to 540
-// of it the softmax's for its scores.  Measured on a B200: 2,048 tokens, 32 heads of 64: 55 us; 512 tokens behind 7,680,
-// 2 sequences, 8 kv heads of 128 under 32: 168 us, 0.84 of what the same kernel for a bfloat16 cache takes in the second case and
+// of it the softmax's for its scores.  Measured on a B200: 2,048 tokens, 32 heads of 64: 54.5 us; 512 tokens behind 7,680,
+// 2 sequences, 8 kv heads of 128 under 32: 166 us, 0.83 of what the same kernel for a bfloat16 cache takes in the second case and
 // 1.2 of it in the first, where the blocks' begins count.  Steps on the way there, in the second case: 128 rows a block, two threads
 // a row 257; issuing from warps of their own 180; codes straight to registers instead of through shared memory 177; two
 // threads a row again, with 24 warps, 195.  Every wait is bounded (status word as in the products).
@@ -443,8 +443,10 @@ attention_e4m3_prompt_kernel(const PromptArgs a, const E4M3Pages kv) {
         // scales, 32 steps at a time: lane l has those of step (i / 32 * 32 + l)
         float k_scales = 0.f, v_scales = 1.f;
         float m_run = -INFINITY, l_run = 0.f;
-        // what M is the sum of, score and v: touched only where M is raised or large, so not kept in registers (5 us of 170 there)
-        float2* made_of = reinterpret_cast<float2*>(smem + S::kOffM) + tt * BQ + r;
+        // What M is the sum of, score and v, touched only where M is raised or large.  In registers where there is room (prompt of
+        // 2,048 tokens, 32 heads of 64: 54.4 us, else 55.9), else in shared memory (chunks of 512, 128 channels: 166 us, else 175).
+        float2 registers;
+        float2* made_of = HD == 64 ? &registers : reinterpret_cast<float2*>(smem + S::kOffM) + tt * BQ + r;
         *made_of = make_float2(-INFINITY, 0.f);
         uint32_t sv[BK];
         bool ok = true;
@@ -668,7 +670,7 @@ int launch(const PromptArgs& a, const E4M3Pages& kv, int B, int max_q_len, cudaS
 //   Q      128 tokens of one head at a time by tensor copies through a ring, as they are (bfloat16);
 //   sums   four warps, S from tensor memory, c - s one number a query: one multiply-add, one exponential and one add a
 //          score.  Tiles with a query whose |s| is large take a form of their own, in which a score that may be s is s (score_slack).
-//          No unit is full (exponentials 39 % of theirs, issue slots 41 %):
+//          No unit is full (exponentials 42 % of theirs, issue slots 43 %):
 //          a sub-partition has one such warp a block, two in all, which reads 32 columns, waits for them, and adds.
 // A block a head of the group leaves its sums beside the others', and a second kernel adds them in the heads' order (a block for
 // all heads: one block's 48 tiles were the time of all, 95 us of 147 for prompts of 200 to 1,500 tokens).  So a weight does

@@ -1784,7 +1784,7 @@ def _e4m3_prompt_form(dt: int, max_q_len: int, n_heads: int, n_kv: int, hd: int)
 
 def _e4m3_prompt_splits(n_seqs: int, max_q_len: int, n_heads: int, n_kv: int, max_kv_len: int, window: int) -> int:
     """Blocks that share the pages of 256 query rows: what fills the multiprocessors, each with 8 pages or more.  (32 heads over 8 key
-    heads: 512 tokens of 128 channels behind 7,680 take 100 us with two, 161 with one; 64 tokens of 64 behind 15,000 46 and 270.)"""
+    heads: 512 tokens of 128 channels behind 7,680 take 98 us with two, 161 with one; 64 tokens of 64 behind 15,000 40 and 272.)"""
     blocks = n_seqs * n_kv * ((max_q_len * (n_heads // n_kv) + 255) // 256)
     pages = (min(max_kv_len, window + max_q_len) if window else max_kv_len) // 64
     return max(1, min(148 // max(blocks, 1), pages // 8, 32))
